@@ -395,6 +395,74 @@ int32_t k2t_attn_decode_noalloc(k2t_ctx *ctx, int32_t bits, const float *d_q, in
                                 const void *d_vs, int32_t cap, int32_t seq, int32_t window, int32_t sink_tokens,
                                 float attn_scale, float *d_out);
 
+/* ---- several continuations of one prompt ----------------------------------- */
+
+/* No counterparts in the reference, whose sessions decode one sequence: a batch of rows (beams,
+ * samples) that continue n_seq prompts, `beams` rows each, row r of sequence r / beams.  A
+ * sequence's prompt is one cache that its rows share; what a row adds is a cache of its own.
+ *
+ * A batched KV cache in k2t_kv_store's formats: `cap` slots per (row, KV head), slot
+ * (row * n_kv_heads + head) * cap + position; kq / vq: int8 [slot][hd] or NF4 nibbles
+ * [slot][hd/2], 16-byte aligned; ks / vs: f32 [slot] or BF16 [slot][hd/64], aligned to one
+ * slot's scales.  len: no row holds more positions (0 .. cap); d_len: a device int32 per row
+ * with what it holds, read when the kernels run and taken as within 0 .. len, or NULL: len. */
+typedef struct k2t_kv_rows {
+    void *kq, *ks, *vq, *vs;
+    const int32_t *d_len;
+    int32_t cap, len;
+} k2t_kv_rows;
+
+/* Quantizes K and V heads into a batched cache as k2t_kv_store does (same bytes): token t < ntok
+ * of row b is d_k + (b * ntok + t) * row_stride floats, n_kv_heads post-RoPE heads back to back
+ * (d_v likewise: both may point into qkv rows), and goes to position d_pos[b] + t.  d_counts
+ * (nullable): row b has min(ntok, d_counts[b]) tokens.  Positions outside 0 .. cap - 1 are not
+ * written; nothing else in the cache changes.  kv->len and d_len are not used. */
+int32_t k2t_kv_append(k2t_ctx *ctx, int32_t bits, const float *d_k, const float *d_v, size_t row_stride,
+                      int32_t batch, int32_t ntok, int32_t n_kv_heads, int32_t head_dim, const int32_t *d_pos,
+                      const int32_t *d_counts, const k2t_kv_rows *kv);
+/* The same positions read back: code * scale, ifwht64 per 64-block, as fp32 heads in
+ * k2t_kv_append's layout.  Tokens that it would not have written are left as they were. */
+int32_t k2t_kv_load(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, int32_t batch, int32_t ntok,
+                    int32_t n_kv_heads, int32_t head_dim, const int32_t *d_pos, const int32_t *d_counts, float *d_k,
+                    float *d_v, size_t row_stride);
+/* Rearranges row caches in place to the beams that were chosen: every row r takes the positions
+ * below its source's length from row d_parents[r], all rows at once; positions at or behind that
+ * length keep their bytes, and lengths (kv->d_len) are not changed.  The cache holds n_layers
+ * blocks of n_seq * beams rows; a parent outside its row's sequence leaves the row as it was.
+ * beams <= 64. */
+int32_t k2t_kv_reorder(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const int32_t *d_parents,
+                       int32_t n_layers, int32_t n_seq, int32_t beams, int32_t n_kv_heads, int32_t head_dim);
+/* Attention of one token of every row: k2t_attn_decode (int8 queries, same scores and softmax)
+ * over its sequence's prefix rows followed by its own tail.  d_q: row r's n_heads post-RoPE
+ * query heads at d_q + r * q_stride floats; prefix: a cache of n_seq rows, tail: of n_seq * beams
+ * rows (either may be NULL); d_out [n_seq * beams][n_heads][hd].  A row with no positions gets
+ * zeros.  d_ws: device workspace of at least k2t_attn_shared_workspace bytes, 16-byte aligned,
+ * of this call alone while it runs; it needs no initial value.  Allocates nothing, asynchronous,
+ * and may be captured (the lengths are read at every replay). */
+int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_stride, int32_t n_seq, int32_t beams,
+                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const k2t_kv_rows *prefix,
+                        const k2t_kv_rows *tail, float attn_scale, float *d_out, void *d_ws, size_t ws_bytes);
+/* Its workspace for caches of up to prefix_len and tail_len positions (their `len`). */
+int32_t k2t_attn_shared_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, int32_t n_heads, int32_t n_kv_heads,
+                                  int32_t head_dim, int32_t prefix_len, int32_t tail_len, size_t *bytes);
+/* Beam search's choice: the k best continuations of every sequence over its `beams` rows and
+ * the vocabulary.  Row r's logits are d_logits + r * row_stride, its score so far is d_scores[r]
+ * (-inf: the row is not in use); the candidate (r, token) scores d_scores[r] + log softmax(logits
+ * of r)[token], summed in 64 bits.  A logit of NaN counts as -inf, +inf as the largest float;
+ * scores of -inf or NaN are no candidates.  d_done[r] != 0 (nullable; needs eos >= 0): the row has
+ * ended, its one candidate is (r, eos) at its score.  Best first; equal scores: the lower row,
+ * then the higher logit, then the lower token.  d_out_* [n_seq][k]: score, token, row of the
+ * batch (what k2t_kv_reorder takes), and (nullable) done = the row had ended or token == eos
+ * (eos -1: none).  Where a sequence has fewer candidates the rest get score -inf, token max(eos,
+ * 0), its first row, and done 1.  With k == beams the outputs may be the input scores and done
+ * flags.  beams <= 64, k <= 128.  d_ws as in k2t_attn_shared. */
+int32_t k2t_beam_select(k2t_ctx *ctx, const float *d_logits, int32_t vocab, size_t row_stride, const float *d_scores,
+                        const int32_t *d_done, int32_t n_seq, int32_t beams, int32_t k, int32_t eos,
+                        float *d_out_scores, int32_t *d_out_tokens, int32_t *d_out_parents, int32_t *d_out_done,
+                        void *d_ws, size_t ws_bytes);
+int32_t k2t_beam_select_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, int32_t vocab, int32_t k,
+                                  size_t *bytes);
+
 /* ---- sparse-MoE experts (.k2tm shards) ------------------------------------- */
 
 /* K2tmShardHeader (moe_800b.rs:792-854): page 0 of a .k2tm shard ("K2TM800B_V1\0", then

@@ -114,6 +114,13 @@ SIGNATURES = {
     "k2t_stream_read_probe": (I32, [VP, VP, SZ, VP]),
     "k2t_expf_host": (C.c_float, [C.c_float]),
     "k2t_expf_device": (I32, [VP, VP, VP, SZ]),
+    "k2t_kv_append": (I32, [VP, I32, VP, VP, SZ, I32, I32, I32, I32, VP, VP, VP]),
+    "k2t_kv_load": (I32, [VP, I32, VP, I32, I32, I32, I32, VP, VP, VP, VP, SZ]),
+    "k2t_kv_reorder": (I32, [VP, I32, VP, VP, I32, I32, I32, I32, I32]),
+    "k2t_attn_shared": (I32, [VP, I32, VP, SZ, I32, I32, I32, I32, I32, VP, VP, C.c_float, VP, VP, SZ]),
+    "k2t_attn_shared_workspace": (I32, [VP, I32, I32, I32, I32, I32, I32, I32, C.POINTER(SZ)]),
+    "k2t_beam_select": (I32, [VP, VP, I32, SZ, VP, VP, I32, I32, I32, I32, VP, VP, VP, VP, VP, SZ]),
+    "k2t_beam_select_workspace": (I32, [VP, I32, I32, I32, I32, C.POINTER(SZ)]),
     "k2t_attn_decode_noalloc": (I32, [VP, I32, VP, I32, I32, I32, VP, VP, VP, VP, I32, I32, I32, I32, C.c_float,
                                       VP]),
 }
@@ -140,6 +147,16 @@ class K2tmLayout(C.Structure):
     """k2t_k2tm_layout (NfExpertByteLayout offsets)."""
     _fields_ = [(n, C.c_int64) for n in ("gu_codebook_off", "dn_codebook_off", "gu_pair_off", "gu_pair_bytes",
                                          "dn_pair_off", "dn_pair_bytes", "aligned_expert_bytes")]
+
+
+class KVRows(C.Structure):
+    """k2t_kv_rows: a batched KV cache, cap slots per (row, KV head), in k2t_kv_store's formats.
+    len: no row holds more positions (default cap); d_len: int32 tensor, what each row holds."""
+    _fields_ = [("kq", VP), ("ks", VP), ("vq", VP), ("vs", VP), ("d_len", VP), ("cap", I32), ("len", I32)]
+
+    def __init__(self, kq, ks, vq, vs, cap, len=None, d_len=None):
+        super().__init__(_p(kq), _p(ks), _p(vq), _p(vs), _p(d_len), cap, cap if len is None else len)
+        self._keep = (kq, ks, vq, vs, d_len)
 
 
 def k2tm_read_header(page):
@@ -189,6 +206,15 @@ def _p(t):
     if isinstance(t, int):
         return t
     return t.data_ptr()
+
+
+def _ref(s):
+    """Address of a ctypes structure (or None)."""
+    return None if s is None else C.addressof(s)
+
+
+def _nbytes(t):
+    return 0 if t is None else t.numel() * t.element_size()
 
 
 def _host(a):
@@ -309,6 +335,45 @@ class Ctx:
         check(lib().k2t_moe_ffn(self.h, bank.h, shard_layer, _p(router_w), _p(router_bias), top_k,
                                 int(bool(norm_topk_prob)), scoring, _p(hidden), _p(post_norm), float(eps),
                                 _p(route_ids), _p(route_weights)))
+
+    # -- several continuations of one prompt
+    def kv_append(self, bits, k, v, row_stride, batch, ntok, n_kv_heads, head_dim, pos, kv, counts=None):
+        """k2t_kv_append: K / V heads of batch x ntok tokens -> positions pos[row] + t of a KVRows."""
+        check(lib().k2t_kv_append(self.h, bits, _p(k), _p(v), row_stride, batch, ntok, n_kv_heads, head_dim, _p(pos),
+                                  _p(counts), _ref(kv)))
+
+    def kv_load(self, bits, kv, batch, ntok, n_kv_heads, head_dim, pos, k, v, row_stride, counts=None):
+        """k2t_kv_load: the same positions read back as fp32 heads."""
+        check(lib().k2t_kv_load(self.h, bits, _ref(kv), batch, ntok, n_kv_heads, head_dim, _p(pos), _p(counts), _p(k),
+                                _p(v), row_stride))
+
+    def kv_reorder(self, bits, kv, parents, n_layers, n_seq, beams, n_kv_heads, head_dim):
+        """k2t_kv_reorder: every row takes its parent row's positions, in place."""
+        check(lib().k2t_kv_reorder(self.h, bits, _ref(kv), _p(parents), n_layers, n_seq, beams, n_kv_heads, head_dim))
+
+    def attn_shared(self, bits, q, q_stride, n_seq, beams, n_heads, n_kv_heads, head_dim, prefix, tail, attn_scale,
+                    out, ws):
+        """k2t_attn_shared: one token of every row over its sequence's prefix and its own tail; ws:
+        uint8 tensor of attn_shared_workspace bytes."""
+        check(lib().k2t_attn_shared(self.h, bits, _p(q), q_stride, n_seq, beams, n_heads, n_kv_heads, head_dim,
+                                    _ref(prefix), _ref(tail), attn_scale, _p(out), _p(ws), _nbytes(ws)))
+
+    def attn_shared_workspace(self, n_seq, beams, n_heads, n_kv_heads, head_dim, prefix_len, tail_len):
+        n = SZ()
+        check(lib().k2t_attn_shared_workspace(self.h, n_seq, beams, n_heads, n_kv_heads, head_dim, prefix_len,
+                                              tail_len, C.byref(n)))
+        return n.value
+
+    def beam_select(self, logits, vocab, row_stride, scores, done, n_seq, beams, k, eos, out_scores, out_tokens,
+                    out_parents, out_done, ws):
+        """k2t_beam_select: the k best (row, token) of every sequence; done / out_done may be None."""
+        check(lib().k2t_beam_select(self.h, _p(logits), vocab, row_stride, _p(scores), _p(done), n_seq, beams, k, eos,
+                                    _p(out_scores), _p(out_tokens), _p(out_parents), _p(out_done), _p(ws), _nbytes(ws)))
+
+    def beam_select_workspace(self, n_seq, beams, vocab, k):
+        n = SZ()
+        check(lib().k2t_beam_select_workspace(self.h, n_seq, beams, vocab, k, C.byref(n)))
+        return n.value
 
     def gemv_chunk_dots(self, m, xq, xsum, dots):
         check(lib().k2t_gemv_chunk_dots(self.h, m.h, _p(xq), _p(xsum), _p(dots)))

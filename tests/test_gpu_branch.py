@@ -1,0 +1,390 @@
+"""Several continuations of one prompt: the batched Hadamard cache (k2t_kv_append, k2t_kv_load,
+k2t_kv_reorder), attention over a shared prefix (k2t_attn_shared) and beam search's choice
+(k2t_beam_select), against 64-bit references (branch_ref) and the one-sequence operators."""
+
+import numpy as np
+import pytest
+import torch
+
+import branch_ref as R
+import k2t
+
+pytestmark = pytest.mark.gpu
+
+
+def dev(a):
+    a = np.ascontiguousarray(a)
+    return torch.from_numpy(a.view(np.int16) if a.dtype == np.uint16 else a).cuda()
+
+
+def host(t, like):
+    return t.cpu().numpy().view(like.dtype)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def rows_of(cache, cap, length=None, d_len=None):
+    t = [dev(a) for a in cache]
+    return t, k2t.KVRows(*t, cap=cap, len=length, d_len=d_len)
+
+
+def workspace(n):
+    return torch.full((n,), 0x7F, dtype=torch.uint8, device="cuda")
+
+
+# ---------------------------------------------------------------- append, load
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch,ntok,nkv,cap", [(1, 1, 1, 1), (3, 5, 2, 9), (2, 70, 3, 71), (5, 1, 4, 3)])
+def test_append_writes_kv_stores_bytes_and_load_reads_them(gpu_ctx, bits, hd, batch, ntok, nkv, cap):
+    print(f"kv_append bits={bits} hd={hd} batch={batch} ntok={ntok} nkv={nkv} cap={cap}", flush=True)
+    rng = np.random.default_rng(bits * hd + ntok)
+    width = 2 * nkv * hd + hd + 4  # a q head in front, padding behind
+    x = (rng.standard_normal((batch * ntok, width)) * rng.uniform(0.01, 4, (batch * ntok, 1))).astype(np.float32)
+    x[0, hd:2 * hd] = 0.0  # a zero head
+    pos = rng.integers(-2, cap + 1, batch).astype(np.int32)
+    counts = rng.integers(0, ntok + 2, batch).astype(np.int32)
+    pos[0], counts[0] = 0, ntok
+    want = R.new_cache(bits, batch, nkv, cap, hd)
+    (kq, ks, vq, vs), kv = rows_of(want, cap)
+    dx = dev(x)
+    at = dx.data_ptr() + 4 * hd
+    gpu_ctx.kv_append(bits, at, at + 4 * nkv * hd, width, batch, ntok, nkv, hd, dev(pos), kv, counts=dev(counts))
+    got_k = torch.full((batch * ntok, nkv * hd + 8), 3.25, device="cuda")
+    got_v = got_k.clone()
+    gpu_ctx.kv_load(bits, kv, batch, ntok, nkv, hd, dev(pos), got_k, got_v, nkv * hd + 8, counts=dev(counts))
+    gpu_ctx.sync()
+    load = [np.full((batch * ntok, nkv * hd + 8), 3.25) for _ in range(2)]
+    tol = [np.zeros_like(a) for a in load]
+    for b in range(batch):
+        for t in range(min(ntok, counts[b])):
+            p = pos[b] + t
+            if not 0 <= p < cap:
+                continue
+            for h in range(nkv):
+                for w in range(2):
+                    o = hd + (w * nkv + h) * hd
+                    q, s = R.store(bits, x[b * ntok + t, o:o + hd])
+                    want[2 * w][b, h, p], want[2 * w + 1][b, h, p] = q, s
+                    v = R.values(bits, want[2 * w][b, h, p], want[2 * w + 1][b, h, p])
+                    load[w][b * ntok + t, h * hd:(h + 1) * hd] = R.unrotate(v)
+                    # code * scale, then six sums and a division by 8: 7 roundings of a block's sum
+                    tol[w][b * ntok + t, h * hd:(h + 1) * hd] = 7.5 * R.U * R.block_sums(np.abs(v)) / 8
+    for g, w in zip((kq, ks, vq, vs), want):
+        assert np.array_equal(host(g, w).view(np.uint8), w.view(np.uint8))
+    for g, w, t in zip((got_k, got_v), load, tol):
+        assert (np.abs(g.cpu().numpy() - w) <= t).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_append_equals_kv_store(gpu_ctx, bits):
+    rng = np.random.default_rng(5)
+    hd, n = 128, 33
+    x = dev(rng.standard_normal((n, 2 * hd)).astype(np.float32))
+    a, kv = rows_of(R.new_cache(bits, 1, 1, n, hd), n)
+    gpu_ctx.kv_append(bits, x, x.data_ptr() + 4 * hd, 2 * hd, 1, n, 1, hd, ints([0]), kv)
+    b, _ = rows_of(R.new_cache(bits, 1, 1, n, hd), n)
+    gpu_ctx.kv_store(bits, x[:, :hd].contiguous(), n, hd, b[0], b[1])
+    gpu_ctx.kv_store(bits, x[:, hd:].contiguous(), n, hd, b[2], b[3])
+    gpu_ctx.sync()
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_append_offsets_past_32_bits(gpu_ctx):
+    """A cache of 2^20 positions x 40 heads of 128 bytes (5 GiB): the last head's last slot."""
+    hd, nkv, cap = 128, 40, 1 << 20
+    q = torch.zeros(nkv * cap, hd, dtype=torch.int8, device="cuda")
+    s = torch.zeros(nkv * cap, device="cuda")
+    kv = k2t.KVRows(q, s, q, s, cap=cap)  # (K and V alike, so one buffer serves for both)
+    x = torch.randn(1, nkv * hd, device="cuda")
+    gpu_ctx.kv_append(8, x, x, nkv * hd, 1, 1, nkv, hd, ints([cap - 1]), kv)
+    y = torch.zeros_like(x)
+    gpu_ctx.kv_load(8, kv, 1, 1, nkv, hd, ints([cap - 1]), y, torch.zeros_like(x), nkv * hd)
+    gpu_ctx.sync()
+    rq, rs = R.store(8, x[0, -hd:].cpu().numpy())
+    assert np.array_equal(q[-1].cpu().numpy(), rq) and float(s[-1]) == float(rs)
+    # half a code step of each head's scale, per rotated element: 8 in all after the rotation
+    assert float((x - y).abs().max()) <= 64 / 8 * 0.51 * float(s.max())
+    assert int((q != 0).any(1).sum()) == nkv
+
+
+# ---------------------------------------------------------------- reorder
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("layers,n_seq,beams,nkv,cap,length", [(1, 1, 2, 1, 5, 5), (2, 3, 4, 2, 33, 30), (1, 2, 13, 3, 70, 1),
+                                                               (3, 1, 31, 1, 20, 19), (1, 1, 64, 2, 300, 290)])
+def test_reorder_moves_rows_in_place(gpu_ctx, bits, hd, layers, n_seq, beams, nkv, cap, length):
+    print(f"kv_reorder bits={bits} hd={hd} {layers} {n_seq} {beams} {nkv} {cap} {length}", flush=True)
+    rng = np.random.default_rng(beams + hd)
+    rows = n_seq * beams
+    cache = R.new_cache(bits, layers * rows, nkv, cap, hd, rng)
+    lens = rng.integers(0, length + 1, rows).astype(np.int32)
+    lens[rng.integers(rows)] = length
+    parents = np.concatenate([s * beams + rng.integers(0, beams, beams) for s in range(n_seq)]).astype(np.int32)
+    parents[0] = rows if rows < 2 else -5  # a parent outside its sequence
+    if n_seq > 1:
+        parents[-1] = 0  # another sequence's row
+    want = []
+    for a in cache:
+        a = a.reshape((layers, rows) + a.shape[1:])
+        new = a.copy()
+        for r in range(rows):
+            p = parents[r]
+            if p // beams == r // beams and 0 <= p < rows:
+                new[:, r, :, :lens[p]] = a[:, p, :, :lens[p]]
+        want.append(new)
+    t, kv = rows_of(cache, cap, length, dev(lens))
+    gpu_ctx.kv_reorder(bits, kv, dev(parents), layers, n_seq, beams, nkv, hd)
+    gpu_ctx.sync()
+    for g, w in zip(t, want):
+        assert np.array_equal(host(g, w).reshape(-1), w.reshape(-1))
+
+
+# ---------------------------------------------------------------- attention
+ATTN = [
+    # n_seq, beams, nq, nkv, prefix, tail
+    (1, 1, 1, 1, 1, 0), (1, 1, 4, 4, 0, 1), (1, 4, 9, 3, 45, 7), (2, 3, 8, 2, 63, 65), (1, 5, 4, 4, 257, 31),
+    (1, 17, 8, 1, 130, 3), (3, 2, 24, 2, 513, 20), (1, 33, 4, 2, 1000, 33), (1, 1, 16, 1, 700, 300), (1, 64, 2, 1, 31, 2),
+]
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("n_seq,beams,nq,nkv,prefix,tail", ATTN)
+def test_attention_over_prefix_and_tail(gpu_ctx, bits, hd, n_seq, beams, nq, nkv, prefix, tail):
+    print(f"attn_shared bits={bits} hd={hd} {n_seq} {beams} {nq} {nkv} {prefix} {tail}", flush=True)
+    rng = np.random.default_rng(prefix + tail + hd + bits)
+    rows, pcap, tcap = n_seq * beams, max(prefix, 1) + 3, max(tail, 1) + 2
+    pre, tl = R.new_cache(bits, n_seq, nkv, pcap, hd, rng), R.new_cache(bits, rows, nkv, tcap, hd, rng)
+    plen = rng.integers(prefix // 2, prefix + 1, n_seq).astype(np.int32)
+    tlen = rng.integers(0, tail + 1, rows).astype(np.int32)
+    plen[0], tlen[-1] = prefix, tail
+    for c, n in ((pre, plen), (tl, tlen)):  # what lies behind a row's positions is never used
+        for r in range(len(n)):
+            if bits == 8:
+                c[1][r, :, n[r]:] = np.nan
+                c[3][r, :, n[r]:] = np.inf
+            else:
+                c[1][r, :, n[r]:] = 0x7FC0
+                c[3][r, :, n[r]:] = 0x7F80
+    width = nq * hd + 4
+    q = (2 * rng.standard_normal((rows, width))).astype(np.float32)
+    scale = hd ** -0.5
+    out = torch.full((rows, nq, hd), float("nan"), device="cuda")
+    _, p = rows_of(pre, pcap, prefix, dev(plen))
+    _, t = rows_of(tl, tcap, tail, dev(tlen))
+    ws = workspace(gpu_ctx.attn_shared_workspace(n_seq, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(bits, dev(q), width, n_seq, beams, nq, nkv, hd, p, t, scale, out, ws)
+    gpu_ctx.sync()
+    want, bound = R.attention(bits, q[:, :nq * hd].reshape(rows, nq, hd), pre, tl, plen, tlen, beams, nq, nkv, hd, scale)
+    err = np.abs(out.cpu().numpy() - want)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+def test_attention_without_positions_prefix_or_tail(gpu_ctx, bits, hd):
+    """Rows that hold nothing get zeros; a missing cache is one of no positions; lengths beyond
+    `len` or below zero count as `len` and zero."""
+    rng = np.random.default_rng(hd)
+    beams, nq, nkv = 3, 4, 2
+    pre, tl = R.new_cache(bits, 1, nkv, 40, hd, rng), R.new_cache(bits, beams, nkv, 9, hd, rng)
+    q = rng.standard_normal((beams, nq * hd)).astype(np.float32)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, 40, 9))
+    none = R.new_cache(bits, beams, nkv, 1, hd, rng)
+    for p_len, t_len in (([0], [0, 4, -3]), ([99], [99, 2, 9]), (None, [1, 0, 5]), ([17], None)):
+        _, p = rows_of(pre, 40, 40, ints(p_len) if p_len else None)
+        _, t = rows_of(tl, 9, 8, ints(t_len) if t_len else None)
+        out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+        gpu_ctx.attn_shared(bits, dev(q), nq * hd, 1, beams, nq, nkv, hd, p if p_len else None, t if t_len else None,
+                            0.125, out, ws)
+        gpu_ctx.sync()
+        a = np.clip(p_len or [0], 0, 40)
+        b = np.clip(t_len or [0, 0, 0], 0, 8)
+        want, bound = R.attention(bits, q.reshape(beams, nq, hd), pre, tl if t_len else none, a, b, beams, nq, nkv, hd, 0.125)
+        err = np.abs(out.cpu().numpy() - want)
+        assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_weights_far_apart_and_scales_of_any_size(gpu_ctx, bits):
+    """One position takes all the weight, wherever it lies; V scales from 1e-12 to 1e12."""
+    rng = np.random.default_rng(bits)
+    beams, nq, nkv, hd, prefix, tail = 2, 2, 1, 64, 300, 40
+    for spot in (0, 31, 32, 255, 256, 299, 300, 339):
+        pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+        size = np.float32(10.0 ** rng.uniform(-12, 12))
+        for c in (pre, tl):
+            if bits == 8:
+                c[3][:] = c[3] * size
+            else:
+                c[3][:] = ((R.bf16(c[3]) * size).view(np.uint32) >> 16).astype(np.uint16)
+        q = (30 * rng.standard_normal((beams, nq, hd))).astype(np.float32)
+        for r in range(beams):
+            c, row, pos = (pre, 0, spot) if spot < prefix else (tl, r, spot - prefix)
+            if bits == 8:  # the position's K head is the query's own codes
+                import oracle as O
+                c[0][row, 0, pos], c[1][row, 0, pos] = O.kv_quant_head(q[r, 0])[0], 0.05
+        out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+        _, p = rows_of(pre, prefix)
+        _, t = rows_of(tl, tail)
+        ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+        gpu_ctx.attn_shared(bits, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, t, 0.125, out, ws)
+        gpu_ctx.sync()
+        want, bound = R.attention(bits, q, pre, tl, [prefix], [tail] * beams, beams, nq, nkv, hd, 0.125)
+        err = np.abs(out.cpu().numpy() - want)
+        assert (err <= bound).all(), (spot, float((err / bound).max()))
+
+
+def test_attention_agrees_with_attn_decode(gpu_ctx):
+    """A row's output is the one-sequence operator's over its prefix and tail laid end to end."""
+    rng = np.random.default_rng(11)
+    beams, nq, nkv, hd, prefix, tail = 4, 8, 2, 128, 900, 61
+    pre, tl = R.new_cache(8, 1, nkv, prefix, hd, rng), R.new_cache(8, beams, nkv, tail, hd, rng)
+    q = (2 * rng.standard_normal((beams, nq, hd))).astype(np.float32)
+    out = torch.empty((beams, nq, hd), device="cuda")
+    _, p = rows_of(pre, prefix)
+    _, t = rows_of(tl, tail)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(8, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, t, hd ** -0.5, out, ws)
+    _, bound = R.attention(8, q, pre, tl, [prefix], [tail] * beams, beams, nq, nkv, hd, hd ** -0.5)
+    for r in range(beams):
+        c = [dev(np.concatenate((a[0], b[r]), 1)) for a, b in zip(pre, tl)]
+        one = torch.empty((nq, hd), device="cuda")
+        gpu_ctx.attn_decode(8, dev(q[r]), nq, nkv, hd, *c, prefix + tail, prefix + tail, hd ** -0.5, one)
+        # both are within the bound of the exact value
+        assert (np.abs(out[r].cpu().numpy() - one.cpu().numpy()) <= 2 * bound[r]).all()
+
+
+def test_attention_past_32_bit_offsets(gpu_ctx):
+    """A prefix of 2^21 positions in a cache of 20 heads of 128 bytes (5 GiB), of which only the last
+    100 positions matter: their scores are far above the others'."""
+    hd, nkv, cap, beams = 128, 20, 1 << 21, 2
+    kq = torch.zeros(nkv * cap, hd, dtype=torch.int8, device="cuda")
+    ks = torch.full((nkv * cap,), 0.05, device="cuda")
+    rng = np.random.default_rng(3)
+    tail = R.new_cache(8, 1, nkv, 100, hd, rng)
+    q = (4 * rng.standard_normal((beams, nkv, hd))).astype(np.float32)
+    import oracle as O
+    for h in range(nkv):
+        code = O.kv_quant_head(q[0, h])[0].astype(np.int64)
+        tail[0][0, h] = np.clip(code + rng.integers(-20, 21, (100, hd)), -127, 127)
+        tail[1][0, h] = 0.05
+        at = slice((h + 1) * cap - 100, (h + 1) * cap)
+        kq[at], ks[at] = dev(tail[0][0, h]), dev(tail[1][0, h])
+    q[1] = q[0]
+    p = k2t.KVRows(kq, ks, kq, ks, cap=cap)  # (V is K)
+    out = torch.empty((beams, nkv, hd), device="cuda")
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nkv, nkv, hd, cap, 0))
+    gpu_ctx.attn_shared(8, dev(q.reshape(beams, -1)), nkv * hd, 1, beams, nkv, nkv, hd, p, None, 1.0, out, ws)
+    gpu_ctx.sync()
+    tail[2], tail[3] = tail[0], tail[1]
+    none = R.new_cache(8, 1, nkv, 1, hd, rng)
+    both = [np.repeat(a, beams, 0) for a in tail]
+    want, bound = R.attention(8, q, none, both, [0], [100] * beams, beams, nkv, nkv, hd, 1.0)
+    err = np.abs(out.cpu().numpy() - want)
+    assert (err <= 2 * bound).all(), float((err / bound).max())
+
+
+# ---------------------------------------------------------------- select
+def run_select(ctx, logits, scores, done, n_seq, beams, k, eos, stride=None):
+    v = logits.shape[1]
+    wide = np.full((logits.shape[0], stride or v), 1e30, np.float32)
+    wide[:, :v] = logits
+    n = (n_seq, k)
+    o = [torch.full(n, -7, dtype=d, device="cuda") for d in (torch.float32, torch.int32, torch.int32, torch.int32)]
+    ws = workspace(ctx.beam_select_workspace(n_seq, beams, v, k))
+    ctx.beam_select(dev(wide), v, wide.shape[1], dev(scores), None if done is None else dev(done), n_seq, beams, k, eos,
+                    *o, ws)
+    ctx.sync()
+    return [t.cpu().numpy() for t in o]
+
+
+# exp is off by 4 units, a sum of 4096 in lanes, waves and slices by 40 roundings: the logarithm by
+# less than 2^-18; the score is then rounded once
+def score_tol(s):
+    return np.where(np.isfinite(s), np.abs(s) * R.U, 0) + 2.0 ** -18
+
+
+@pytest.mark.parametrize("n_seq,beams,vocab,k", [(1, 1, 1, 1), (1, 1, 7, 9), (1, 4, 8192, 4), (3, 2, 1001, 128), (2, 8, 4097, 16),
+                                                 (1, 64, 515, 128), (1, 5, 49152, 10), (2, 3, 20000, 1)])
+@pytest.mark.parametrize("with_done", [False, True])
+def test_select_matches_the_reference(gpu_ctx, n_seq, beams, vocab, k, with_done):
+    print(f"beam_select {n_seq} {beams} {vocab} {k} done={with_done}", flush=True)
+    rng = np.random.default_rng(vocab + k)
+    rows = n_seq * beams
+    logits = (3 * rng.standard_normal((rows, vocab))).astype(np.float32)
+    scores = rng.uniform(-9, -1, rows).astype(np.float32)
+    eos = min(3, vocab - 1)
+    done = (rng.random(rows) < 0.4).astype(np.int32) if with_done else None
+    if beams > 2:
+        scores[1] = -np.inf  # a row not in use, whose logits mean nothing
+        logits[1] = np.nan
+    ws, wt, wp, wd, gap = R.select(logits, scores, done, n_seq, beams, k, eos)
+    assert gap > 2.0 ** -15, "inputs too near a tie to be told apart"
+    s, t, p, d = run_select(gpu_ctx, logits, scores, done, n_seq, beams, k, eos, stride=vocab + 5)
+    assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(d, wd)
+    assert np.array_equal(np.isinf(s), np.isinf(ws)) and (np.abs(s - ws)[np.isfinite(ws)] <= score_tol(ws)[np.isfinite(ws)]).all()
+
+
+def test_select_ties_masks_and_odd_values(gpu_ctx):
+    """Equal logits and equal rows (the lower token, the lower row first), -inf and NaN logits, rows
+    of the lowest value, +inf, a row with nothing, few candidates."""
+    v, k = 5000, 12
+    base = np.zeros((6, v), np.float32)
+    base[1] = base[0]  # two equal rows of equal logits
+    base[2] = np.finfo(np.float32).min  # a mask of the lowest value everywhere
+    base[3] = -np.inf
+    base[3, [4999, 17, 4096]] = [1.0, 1.0, np.nan]
+    base[4] = -np.inf
+    base[5, 4321] = np.inf
+    base[5, 7] = -0.0
+    cases = [([-1, -1, -20, -20, -20, -20], 6), ([-9, -9, -1, -9, -9, -9], 6), ([-np.inf] * 3 + [-2, -1, -np.inf], 6),
+             ([-50, -50, -50, -50, -50, 0], 6), ([np.nan, -np.inf, -np.inf, 0, 0, -np.inf], 6)]
+    for scores, beams in cases:
+        sc = np.array(scores, np.float32)
+        ws, wt, wp, wd, _ = R.select(base, sc, None, 1, beams, k, 17)
+        s, t, p, d = run_select(gpu_ctx, base, sc, None, 1, beams, k, 17)
+        assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(d, wd), scores
+        w32 = ws.astype(np.float32)
+        fin = np.isfinite(w32)
+        assert np.array_equal(s[~fin], w32[~fin]) and (np.abs(s - ws)[fin] <= score_tol(ws)[fin]).all(), scores
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "blocks", "equal"])
+def test_select_of_ordered_logits(gpu_ctx, order):
+    """The k best all in one place, or all equal: the same choice however the slices are cut."""
+    v, k = 9000, 100
+    x = np.arange(v, dtype=np.float32) / 64
+    if order == "falling":
+        x = x[::-1].copy()
+    elif order == "blocks":
+        x = (np.arange(v) % 64 // 4).astype(np.float32)
+    elif order == "equal":
+        x[:] = 2.5
+    logits, scores = np.stack((x, x, x)), np.array([-3, -2, -2], np.float32)
+    ws, wt, wp, wd, _ = R.select(logits, scores, None, 1, 3, k, -1)
+    s, t, p, d = run_select(gpu_ctx, logits, scores, None, 1, 3, k, -1)
+    assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(d, wd)
+    assert (np.abs(s - ws) <= score_tol(ws)).all()
+
+
+def test_select_in_place_and_without_flags(gpu_ctx):
+    """k == beams: the scores and done flags are replaced in place; done flags may be left out."""
+    rng = np.random.default_rng(9)
+    n, beams, v = 3, 4, 700
+    logits = rng.standard_normal((n * beams, v)).astype(np.float32)
+    scores, done = rng.uniform(-5, 0, n * beams).astype(np.float32), (rng.random(n * beams) < 0.3).astype(np.int32)
+    ws, wt, wp, wd, gap = R.select(logits, scores, done, n, beams, beams, 1)
+    assert gap > 2.0 ** -15
+    ds, dd = dev(scores), dev(done)
+    tok, par = ints([0] * n * beams), ints([0] * n * beams)
+    w = workspace(gpu_ctx.beam_select_workspace(n, beams, v, beams))
+    gpu_ctx.beam_select(dev(logits), v, v, ds, dd, n, beams, beams, 1, ds, tok, par, dd, w)
+    gpu_ctx.sync()
+    assert np.array_equal(tok.cpu().numpy(), wt.reshape(-1)) and np.array_equal(par.cpu().numpy(), wp.reshape(-1))
+    assert np.array_equal(dd.cpu().numpy(), wd.reshape(-1))
+    assert (np.abs(ds.cpu().numpy() - ws.reshape(-1)) <= score_tol(ws.reshape(-1))).all()
+    gpu_ctx.beam_select(dev(logits), v, v, dev(scores), None, n, beams, beams, -1, ds, tok, par, None, w)
+    gpu_ctx.sync()
+    _, wt, wp, _, _ = R.select(logits, scores, None, n, beams, beams, -1)
+    assert np.array_equal(tok.cpu().numpy(), wt.reshape(-1)) and np.array_equal(par.cpu().numpy(), wp.reshape(-1))
