@@ -11,6 +11,8 @@ namespace k2t {
 
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 struct RowsArgs {
     const float *k, *v;
     float *ko, *vo;
@@ -203,11 +205,11 @@ void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const in
     const int piece = beams > 32 ? 8 : 16;
     A.code_blocks = (int)(((size_t)kv.len * (A.code_bytes / piece) + 255) / 256);
     const dim3 grid((unsigned)(2 * (size_t)n_layers * n_seq * nkv), (unsigned)(A.code_blocks + (kv.len + 255) / 256));
-    if (beams <= 4) hipLaunchKernelGGL((kv_reorder_kernel<4, uint4>), grid, dim3(256), 0, st, A);
-    else if (beams <= 8) hipLaunchKernelGGL((kv_reorder_kernel<8, uint4>), grid, dim3(256), 0, st, A);
-    else if (beams <= 16) hipLaunchKernelGGL((kv_reorder_kernel<16, uint4>), grid, dim3(256), 0, st, A);
-    else if (beams <= 32) hipLaunchKernelGGL((kv_reorder_kernel<32, uint4>), grid, dim3(256), 0, st, A);
-    else hipLaunchKernelGGL((kv_reorder_kernel<64, uint2>), grid, dim3(256), 0, st, A);
+    if (beams <= 4) hipLaunchKernelGGL((kv_reorder_kernel<4, u32x4>), grid, dim3(256), 0, st, A);
+    else if (beams <= 8) hipLaunchKernelGGL((kv_reorder_kernel<8, u32x4>), grid, dim3(256), 0, st, A);
+    else if (beams <= 16) hipLaunchKernelGGL((kv_reorder_kernel<16, u32x4>), grid, dim3(256), 0, st, A);
+    else if (beams <= 32) hipLaunchKernelGGL((kv_reorder_kernel<32, u32x4>), grid, dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((kv_reorder_kernel<64, u32x2>), grid, dim3(256), 0, st, A);
     hip_check(hipGetLastError(), "kv_reorder launch");
 }
 
