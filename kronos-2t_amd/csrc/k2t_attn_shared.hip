@@ -16,9 +16,11 @@ namespace {
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kWaves = 4, kTile = 32;  // waves of a workgroup; positions of a wave's tile
+// A running maximum is raised once a score passes it by more than this (in powers of two): raising it
+// rescales the outputs, and some column of a tile would nearly always ask for it.
+constexpr float kSlack = 6.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct SharedArgs {
@@ -39,86 +41,85 @@ __device__ __forceinline__ int row_len(const k2t_kv_rows &kv, int row) {
     return kv.d_len ? max(0, min(kv.d_len[row], kv.len)) : kv.len;
 }
 
-// A wave's tile of 32 positions as its lanes load it (li = lane % 16, lg = lane / 16).
-// K: rows 16 j + li, the 16 (NF4: 8) bytes lg of every 64-block.  V: positions 16 j + 4 lg + i, the
-// HD / 16 bytes li of the row (NF4: two bytes of every block).  Scales: positions 16 j + 4 lg + i.
+// A wave's tile of 32 positions as its lanes load it (li = lane % 16, lg = lane / 16), in two halves
+// that are dead at different times.  K: rows 16 j + li, the 16 (NF4: 8) bytes lg of every 64-block,
+// and the scales of positions 16 j + 4 lg + i.  V: those positions, the HD / 16 bytes li of the row
+// (NF4: two bytes of every block).
 template <int HD, int BITS>
-struct Tile {
-    static constexpr int NB = HD / 64, KW = BITS == 8 ? 4 : 2, VW = BITS == 8 ? HD / 64 : NB;
-    static constexpr int SN = BITS == 8 ? 1 : NB;  // scales per position
+struct TileK {
+    static constexpr int NB = HD / 64, KW = BITS == 8 ? 4 : 2, SN = BITS == 8 ? 1 : NB;
     uint32_t k[2][NB][KW];
-    uint32_t v[2][4][VW];
-    float ks[2][4][SN], vs[2][4][SN];
+    uint32_t ks[2][4], vs[2][4];  // float, or the slot's BF16 scales (block 0 low)
+
+    static __device__ __forceinline__ float scale(uint32_t w, int n) {
+        return __uint_as_float(BITS == 8 ? w : n ? w & 0xFFFF0000u : w << 16);
+    }
+};
+template <int HD, int BITS>
+struct TileV {
+    uint32_t v[2][4][HD / 64];
 };
 
-template <int HD, int BITS, bool PARTIAL>
-__device__ __forceinline__ void load_tile(Tile<HD, BITS> &T, const k2t_kv_rows &kv, size_t base, int t0, int t1,
-                                          uint32_t li, uint32_t lg) {
+// The tile whose first position has slot `slot`; n positions of it exist (rows behind them repeat the
+// last).  Addresses are a wave-uniform pointer and a small offset per lane.
+template <int HD, int BITS>
+__device__ __forceinline__ void load_k(TileK<HD, BITS> &T, const k2t_kv_rows &kv, size_t slot, int n, uint32_t li,
+                                       uint32_t lg) {
     constexpr int NB = HD / 64, RB = BITS == 8 ? HD : HD / 2;
-    const auto clamp = [&](int t) { return PARTIAL ? min(t, t1 - 1) : t; };
-    const uint8_t *kq = (const uint8_t *)kv.kq + base * RB, *vq = (const uint8_t *)kv.vq + base * RB;
+    const auto at = [&](uint32_t p) { return min(p, (uint32_t)n - 1u); };
+    const uint8_t *kq = (const uint8_t *)kv.kq + slot * RB;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        const uint8_t *row = kq + (size_t)clamp(t0 + 16 * j + (int)li) * RB;
+        const uint32_t row = at(16u * j + li) * RB;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             if constexpr (BITS == 8) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(row + 64 * b + 16 * lg);
+                const uint4 w = *reinterpret_cast<const uint4 *>(kq + (row + 64 * b + 16 * lg));
                 T.k[j][b][0] = w.x;
                 T.k[j][b][1] = w.y;
                 T.k[j][b][2] = w.z;
                 T.k[j][b][3] = w.w;
             } else {
-                const uint2 w = *reinterpret_cast<const uint2 *>(row + 32 * b + 8 * lg);
+                const uint2 w = *reinterpret_cast<const uint2 *>(kq + (row + 32 * b + 8 * lg));
                 T.k[j][b][0] = w.x;
                 T.k[j][b][1] = w.y;
             }
         }
-        const int p0 = t0 + 16 * j + 4 * (int)lg;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint8_t *vr = vq + (size_t)clamp(p0 + i) * RB;
-            if constexpr (BITS == 8) {
-                if constexpr (HD == 128) {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(vr + 8 * li);
-                    T.v[j][i][0] = w.x;
-                    T.v[j][i][1] = w.y;
-                } else {
-                    T.v[j][i][0] = *reinterpret_cast<const uint32_t *>(vr + 4 * li);
-                }
+            const uint32_t p = at(16u * j + 4u * lg + i);
+            if constexpr (BITS == 8 || NB == 2) {
+                T.ks[j][i] = ((const uint32_t *)kv.ks + slot)[p];
+                T.vs[j][i] = ((const uint32_t *)kv.vs + slot)[p];
             } else {
-#pragma unroll
-                for (int b = 0; b < NB; b++) T.v[j][i][b] = *reinterpret_cast<const uint16_t *>(vr + 32 * b + 2 * li);
+                T.ks[j][i] = ((const uint16_t *)kv.ks + slot)[p];
+                T.vs[j][i] = ((const uint16_t *)kv.vs + slot)[p];
             }
-        }
-        if constexpr (BITS == 8) {
-            const float *ks = (const float *)kv.ks + base, *vs = (const float *)kv.vs + base;
-            if constexpr (PARTIAL) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    T.ks[j][i][0] = ks[clamp(p0 + i)];
-                    T.vs[j][i][0] = vs[clamp(p0 + i)];
-                }
-            } else {
-                const f4u a = *reinterpret_cast<const f4u *>(ks + p0), b = *reinterpret_cast<const f4u *>(vs + p0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    T.ks[j][i][0] = a[i];
-                    T.vs[j][i][0] = b[i];
-                }
-            }
-        } else {
-            const uint16_t *ks = (const uint16_t *)kv.ks + base * NB, *vs = (const uint16_t *)kv.vs + base * NB;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const size_t at = (size_t)clamp(p0 + i) * NB + b;
-                    T.ks[j][i][b] = __uint_as_float((uint32_t)ks[at] << 16);
-                    T.vs[j][i][b] = __uint_as_float((uint32_t)vs[at] << 16);
-                }
         }
     }
+}
+template <int HD, int BITS>
+__device__ __forceinline__ void load_v(TileV<HD, BITS> &T, const k2t_kv_rows &kv, size_t slot, int n, uint32_t li,
+                                       uint32_t lg) {
+    constexpr int RB = BITS == 8 ? HD : HD / 2;
+    const uint8_t *vq = (const uint8_t *)kv.vq + slot * RB;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t p = 16u * j + 4u * lg + i, row = min(p, (uint32_t)n - 1u) * RB;
+            if constexpr (BITS == 8 && HD == 128) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(vq + (row + 8 * li));
+                T.v[j][i][0] = w.x;
+                T.v[j][i][1] = w.y;
+            } else if constexpr (BITS == 8) {
+                T.v[j][i][0] = *reinterpret_cast<const uint32_t *>(vq + (row + 4 * li));
+            } else {
+#pragma unroll
+                for (int b = 0; b < HD / 64; b++)
+                    T.v[j][i][b] = *reinterpret_cast<const uint16_t *>(vq + (row + 32 * b + 2 * li));
+            }
+        }
 }
 
 // The NF4 KV codebook's tables (nf4_xor_tables).
@@ -160,142 +161,141 @@ __device__ __forceinline__ void v_halves(const uint32_t w0, const uint32_t w1, c
     }
 }
 
+// A position's four V values of one word: int8 as they are; NF4 from four nibbles, in the order 0, 2,
+// 1, 3 of the byte pair.
+template <int BITS>
+__device__ __forceinline__ uint32_t v_word(uint32_t w, const Nf4 &c) {
+    if constexpr (BITS == 8) return w;
+    return nf4_xlut((w & 0x0F0Fu) | ((w & 0xF0F0u) << 12), c.t0, c.t1, c.u0, c.u1);
+}
+
 // Two floats as f16 pairs hi + lo: x = hi + lo within 2^-21 |x|.
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    typedef __fp16 v2hh __attribute__((ext_vector_type(2)));
-    const v2hh h = __builtin_amdgcn_cvt_pkrtz(x0, x1);
-    const v2hh l = __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.0f, x0), fmaf((float)h[1], -1.0f, x1));
-    hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, l);
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    float r0, r1;  // x - hi, exact: one mixed-precision fma each (the compiler converts and subtracts)
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(x1));
+#else
+    r0 = x0;
+    r1 = x1;
+#endif
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
 }
 
 // What a wave carries from tile to tile for NQ tiles of 16 columns: lane li is a column.
+// The factor c = 2^(135 - cexp) brings the largest V scale to 2^8 .. 2^9, so that the weights' f16
+// pieces neither overflow (a weight is at most 2^kSlack) nor lose bits.
 template <int HD, int NQ>
 struct State {
-    v4f o[NQ][HD / 16];  // output tile b of column li, times 2^c
+    v4f o[NQ][HD / 16];  // output tile b of column li, times c
     float m[NQ], l[NQ];  // running maximum (powers of two); this lane's share of the sum
-    uint32_t cexp;       // exponent of the V scales' common factor c (biased), 0: none yet
+    uint32_t cexp;       // exponent (biased) of the largest V scale seen, which sets the factor c; 0: none yet
+
+    __device__ __forceinline__ void clear() {
+        cexp = 0;
+#pragma unroll
+        for (int a = 0; a < NQ; a++) {
+            m[a] = -INFINITY;
+            l[a] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < HD / 16; b++) o[a][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    __device__ __forceinline__ float back() const { return cexp ? __uint_as_float((cexp - 8u) << 23) : 0.0f; }  // 1 / c
 };
 
-template <int HD, int BITS, int NQ, bool PARTIAL>
-__device__ __forceinline__ void step(State<HD, NQ> &S, const Tile<HD, BITS> &T, const v4i (&qb)[NQ][HD / 64],
-                                     const float (&qas)[NQ], const Nf4 &cb, int t0, int t1, uint32_t lg) {
-    constexpr int NB = HD / 64, DB = HD / 16, SN = Tile<HD, BITS>::SN;
-    // V scales times a power of two that brings the largest seen to 2^13 .. 2^14, so that the weights'
-    // f16 pieces neither overflow nor lose bits; it changes when a larger one comes
-    float vmax = 0.0f;
+// Scores of 16 positions x 16 columns, 64-block b of NB: int8 sums the blocks' dots, which are exact,
+// and scales them once; NF4 scales every block's.  s: lane (lg, li) positions 4 lg + i, column li.
+template <int BITS, int NB, typename Scale>
+__device__ __forceinline__ void scores(const v4i (&kf)[NB], const v4i (&qb)[NB], Scale ks, float (&s)[4]) {
+    v4i d = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        if (BITS == 4 && b) d = v4i{0, 0, 0, 0};
+        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[b], qb[b], d, 0, 0, 0);
+        if (BITS == 8 && b + 1 < NB) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            s[i] = BITS == 4 && b ? fmaf((float)d[i], ks(i, b), s[i]) : (float)d[i] * ks(i, 0);
+    }
+}
+
+// Weights of a tile from its scores: t = dots * K scales of positions 16 j + 4 lg + i of the columns
+// li, n of the tile's 32 exist; vs = V scales.  Leaves pairs of weights times V scale times c as hi and
+// lo pieces.  Maxima and c change in one place, off the usual path.
+template <int HD, int NQ, int SN>
+__device__ __forceinline__ void weights(State<HD, NQ> &S, float (&t)[NQ][2][4], const float (&qas)[NQ], float (&vs)[2][4][SN],
+                                        int n, uint32_t lg, uint32_t (&ph)[NQ][SN][4], uint32_t (&pl)[NQ][SN][4]) {
+    float vmax = 0.0f, top[NQ];
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int n = 0; n < SN; n++) vmax = fmaxf(vmax, fabsf(T.vs[j][i][n]));
+            for (int k = 0; k < SN; k++) vmax = fmaxf(vmax, fabsf(vs[j][i][k]));
     const uint32_t e_lane = __float_as_uint(vmax) >> 23;
-    if (__any(e_lane > S.cexp)) {
-        uint32_t e = e_lane;
-        e = max(e, (uint32_t)xor_lane((int)e, 16));
-        e = max(e, (uint32_t)xor_lane((int)e, 32));
-        e = max(max(e, S.cexp), 27u);  // (scales below 2^-100 share its factor)
-        if (S.cexp) {
-            const float down = ldexpf(1.0f, (int)S.cexp - (int)e);
-#pragma unroll
-            for (int a = 0; a < NQ; a++)
-#pragma unroll
-                for (int b = 0; b < DB; b++) S.o[a][b] = S.o[a][b] * down;
-        }
-        S.cexp = e;
-    }
-    const float c = __uint_as_float((267u - S.cexp) << 23);
-    uint32_t ph[NQ][SN][4], pl[NQ][SN][4];  // weights: pairs of positions, hi and lo pieces
+    bool news = e_lane > S.cexp;
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
-        float s[2][4];
+        top[a] = fmaxf(fmaxf(fmaxf(t[a][0][0], t[a][0][1]), fmaxf(t[a][0][2], t[a][0][3])),
+                       fmaxf(fmaxf(t[a][1][0], t[a][1][1]), fmaxf(t[a][1][2], t[a][1][3])));
+        top[a] *= qas[a];  // (qas >= 0: the largest t is the largest score)
+        news |= top[a] > S.m[a] + kSlack;
+    }
+    if (__any(news)) {
+        uint32_t e = max(e_lane, (uint32_t)xor_lane((int)e_lane, 16));
+        e = max(e, (uint32_t)xor_lane((int)e, 32));
+        e = max(max(e, S.cexp), 27u);  // (scales below 2^-100 share its factor)
+        const float down = S.cexp ? ldexpf(1.0f, (int)S.cexp - (int)e) : 1.0f;
+        S.cexp = e;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            if constexpr (BITS == 8) {
-                v4i d = {0, 0, 0, 0};
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k_operand<BITS>(T.k[j][b], cb), qb[a][b], d, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[j][i] = (float)d[i] * T.ks[j][i][0];
-            } else {
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const v4i z = {0, 0, 0, 0};
-                    const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k_operand<BITS>(T.k[j][b], cb), qb[a][b], z, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        s[j][i] = b == 0 ? (float)d[i] * T.ks[j][i][0] : fmaf((float)d[i], T.ks[j][i][b], s[j][i]);
-                }
-            }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[j][i] = s[j][i] * qas[a];
-                if (PARTIAL && t0 + 16 * j + 4 * (int)lg + i >= t1) s[j][i] = -INFINITY;
-                top = fmaxf(top, s[j][i]);
-            }
-        if (__any(top > S.m[a])) {
-            top = fmaxf(top, xor_lane(top, 16));
-            top = fmaxf(top, xor_lane(top, 32));
-            const float mn = fmaxf(S.m[a], top);
-            const float corr = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
+        for (int a = 0; a < NQ; a++) {
+            float mn = fmaxf(top[a], xor_lane(top[a], 16));
+            mn = fmaxf(mn, xor_lane(mn, 32));
+            mn = mn > S.m[a] + kSlack ? mn : S.m[a];
+            const float corr = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
             S.m[a] = mn;
             S.l[a] *= corr;
 #pragma unroll
-            for (int b = 0; b < DB; b++) S.o[a][b] = S.o[a][b] * corr;
+            for (int b = 0; b < HD / 16; b++) S.o[a][b] = S.o[a][b] * (corr * down);
         }
+    }
+    const float c = __uint_as_float((262u - S.cexp) << 23);
+#pragma unroll
+    for (int a = 0; a < NQ; a++) {
         const float m = S.m[a] == -INFINITY ? 0.0f : S.m[a];
-        float p[2][4];
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                p[j][i] = __builtin_amdgcn_exp2f(s[j][i] - m);
-                S.l[a] += p[j][i];
-            }
+            for (int i = 0; i < 4; i++) t[a][j][i] = __builtin_amdgcn_exp2f(fmaf(t[a][j][i], qas[a], -m));
+    }
+    if (n < kTile) {  // positions behind the last one repeat it: they weigh nothing
 #pragma unroll
-        for (int n = 0; n < SN; n++)
+        for (int a = 0; a < NQ; a++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (16 * j + 4 * (int)lg + i >= n) t[a][j][i] = 0.0f;
+    }
+#pragma unroll
+    for (int a = 0; a < NQ; a++) {
+        S.l[a] += ((t[a][0][0] + t[a][0][1]) + (t[a][0][2] + t[a][0][3])) + ((t[a][1][0] + t[a][1][1]) + (t[a][1][2] + t[a][1][3]));
+#pragma unroll
+        for (int k = 0; k < SN; k++)
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2)
-                    split2(p[j][i] * (T.vs[j][i][n] * c), p[j][i + 1] * (T.vs[j][i + 1][n] * c), ph[a][n][2 * j + i / 2],
-                           pl[a][n][2 * j + i / 2]);
+                    split2(t[a][j][i] * (vs[j][i][k] * c), t[a][j][i + 1] * (vs[j][i + 1][k] * c), ph[a][k][2 * j + i / 2],
+                           pl[a][k][2 * j + i / 2]);
     }
-    // o^T += V^T w^T, four output tiles (one 4-byte word of V per position) at a time
-#pragma unroll
-    for (int g = 0; g < DB / 4; g++) {
-        uint32_t h[2][4][2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                w[i] = T.v[j][i][g];
-                if constexpr (BITS == 4)  // nibbles in the order 0, 2, 1, 3 of the byte pair
-                    w[i] = nf4_xlut((w[i] & 0x0F0Fu) | ((w[i] & 0xF0F0u) << 12), cb.t0, cb.t1, cb.u0, cb.u1);
-            }
-            v_halves(w[0], w[1], w[2], w[3], h[j]);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const v8h va = __builtin_bit_cast(v8h, make_uint4(h[0][t][0], h[0][t][1], h[1][t][0], h[1][t][1]));
-#pragma unroll
-            for (int a = 0; a < NQ; a++) {
-                constexpr int last = SN - 1;
-                const int n = g < last ? g : last;
-                const v8h lo = __builtin_bit_cast(v8h, make_uint4(pl[a][n][0], pl[a][n][1], pl[a][n][2], pl[a][n][3]));
-                const v8h hi = __builtin_bit_cast(v8h, make_uint4(ph[a][n][0], ph[a][n][1], ph[a][n][2], ph[a][n][3]));
-                S.o[a][4 * g + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, lo, S.o[a][4 * g + t], 0, 0, 0);
-                S.o[a][4 * g + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, hi, S.o[a][4 * g + t], 0, 0, 0);
-            }
-        }
-    }
+}
+
+// o += V^T w^T over 32 positions for one tile of output and 16 columns.
+__device__ __forceinline__ v4f add_tile(v8h va, const uint32_t (&w)[4], v4f o) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(va, __builtin_bit_cast(v8h, make_uint4(w[0], w[1], w[2], w[3])), o, 0, 0, 0);
 }
 
 // Dimension of row x (0 .. 15) of output tile b.
@@ -307,233 +307,499 @@ __device__ __forceinline__ int out_dim(int b, int x) {
     return 64 * (b >> 2) + 32 * (y >> 4) + 16 * hi + (y & 15);
 }
 
-template <int HD>
-struct Shared {
-    __align__(16) int8_t qi[32][HD + 16];
-    float qas[32];
-    float wm[kWaves][16], wl[kWaves][16];
-    __align__(16) float wo[kWaves][16][HD + 4];
+// What an item works on: columns col0 .. col0 + n - 1, column x being head head0 + x % group of row
+// row0 + x / group, over len[0] positions of one cache from slot[0] on, then len[1] of another.
+struct Item {
+    k2t_kv_rows kv[2];
+    size_t slot[2];
+    int len[2];
+    int row0, head0, col0, n, part;
 };
 
-// One item: `cols` columns (q heads of rows) from col0 on, 16 NQ at most, over positions [t0, t1) of
-// one cache row.  Column x is head head0 + x % group of row row0 + x / group.
-template <int HD, int BITS, int NQ>
-__device__ __forceinline__ void item(const SharedArgs &A, Shared<HD> &sh, const k2t_kv_rows &kv, size_t base, int t0, int t1,
-                                     int row0, int head0, int col0, int cols, int part) {
-    constexpr int NB = HD / 64, DB = HD / 16;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, li = lane & 15u, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
-    const int n = min(16 * NQ, cols - col0);  // columns of this item
-    // queries: sixteen lanes per 64-block, rotated and quantized with one scale per head
+template <int HD, int COLS>
+struct Queries {
+    __align__(16) int8_t q[COLS][HD + 16];
+    float qas[COLS];
+};
+
+// One 64-block of a query head by sixteen lanes (four elements each), rotated and quantized with one
+// scale per head as k2t_kv_store's int8 heads; block b of NB, the blocks of a head in neighbouring
+// groups of lanes.  All lanes take part.
+struct Quant4 {
+    uint32_t w;  // four codes
+    float qas;   // scale of the head's scores, in powers of two
+};
+template <int NB>
+__device__ __forceinline__ Quant4 quantize_block(float4 f, uint64_t mask, uint32_t li, float attn_scale) {
+    float v[4] = {f.x, f.y, f.z, f.w};
+    const uint32_t sb = (uint32_t)(mask >> (4u * li)) & 0xFu;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = flip_sign(v[j], (sb >> j) & 1u) * 0.125f;
+    butterflies_slice4(v, li);
+    float mx = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    mx = fmaxf(mx, xchg1(mx));
+    mx = fmaxf(mx, xchg2(mx));
+    mx = fmaxf(mx, xchg4(mx));
+    mx = fmaxf(mx, xchg8(mx));
+    if (NB > 1) mx = fmaxf(mx, xor_lane(mx, 16));
+    const bool tiny = mx <= FLT_EPSILON;
+    const float inv = 127.0f / mx;
+    Quant4 r{0u, tiny ? 0.0f : ((mx / 127.0f) * attn_scale) * kLog2e};
+#pragma unroll
+    for (int j = 0; j < 4; j++) r.w |= (tiny ? 0u : (uint32_t)(int)rintf(v[j] * inv) & 0xFFu) << (8 * j);
+    return r;
+}
+
+// The item's queries (columns behind the last repeat it) into LDS.
+template <int HD, int COLS>
+__device__ __forceinline__ void quantize_queries(const SharedArgs &A, const Item &I, Queries<HD, COLS> &Q) {
+    constexpr int NB = HD / 64, kTurns = (COLS * NB + 4 * kWaves - 1) / (4 * kWaves);
+    const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    float4 f[kTurns];  // every load in flight at once
+#pragma unroll
+    for (int k = 0; k < kTurns; k++) {
+        const int u = 4 * (wave + kWaves * k) + (int)lg, c = I.col0 + min(u / NB, I.n - 1);
+        f[k] = *reinterpret_cast<const float4 *>(A.q + (size_t)(I.row0 + c / A.group) * A.q_stride +
+                                                 (size_t)(I.head0 + c % A.group) * HD + 64 * (u % NB) + 4 * li);
+    }
     uint64_t mask[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) mask[b] = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
-    for (int u = 4 * wave; u < 16 * NQ * NB; u += 4 * kWaves) {
-        const int x = (u + (int)lg) / NB, b = (u + (int)lg) % NB;
-        const int c = col0 + min(x, n - 1);
-        const float *src = A.q + (size_t)(row0 + c / A.group) * A.q_stride + (size_t)(head0 + c % A.group) * HD;
-        const float4 f = *reinterpret_cast<const float4 *>(src + 64 * b + 4 * li);
-        float v[4] = {f.x, f.y, f.z, f.w};
-        const uint32_t sb = (uint32_t)((NB > 1 && b ? mask[NB - 1] : mask[0]) >> (4u * li)) & 0xFu;
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = flip_sign(v[j], (sb >> j) & 1u) * 0.125f;
-        butterflies_slice4(v, li);
-        float mx = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-        mx = fmaxf(mx, xchg1(mx));
-        mx = fmaxf(mx, xchg2(mx));
-        mx = fmaxf(mx, xchg4(mx));
-        mx = fmaxf(mx, xchg8(mx));
-        if (NB > 1) mx = fmaxf(mx, xor_lane(mx, 16));
-        const bool tiny = mx <= FLT_EPSILON;
-        const float inv = 127.0f / mx;
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) w |= (tiny ? 0u : (uint32_t)(int)rintf(v[j] * inv) & 0xFFu) << (8 * j);
-        *reinterpret_cast<uint32_t *>(&sh.qi[x][64 * b + 4 * li]) = w;
-        if (li == 0 && b == 0) sh.qas[x] = tiny ? 0.0f : ((mx / 127.0f) * A.attn_scale) * kLog2e;
+    for (int k = 0; k < kTurns; k++) {
+        const int u = 4 * (wave + kWaves * k) + (int)lg, x = u / NB, b = u % NB;
+        const Quant4 r = quantize_block<NB>(f[k], NB > 1 && b ? mask[NB - 1] : mask[0], li, A.attn_scale);
+        if (x >= COLS) continue;
+        *reinterpret_cast<uint32_t *>(&Q.q[x][64 * b + 4 * li]) = r.w;
+        if (li == 0 && b == 0) Q.qas[x] = r.qas;
     }
     __syncthreads();
-    v4i qb[NQ][NB];
-    float qas[NQ];
+}
+
+// The score MFMA's B operand of 16 columns, lane li's codes at r, in the K operand's element order.
+template <int HD, int BITS>
+__device__ __forceinline__ void query_operand(const int8_t *r, uint32_t lg, v4i (&qb)[HD / 64]) {
 #pragma unroll
-    for (int a = 0; a < NQ; a++) {
-        const int8_t *r = sh.qi[16 * a + li];
-        qas[a] = sh.qas[16 * a + li];
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            if constexpr (BITS == 8) {
-                const int4 w = *reinterpret_cast<const int4 *>(r + 64 * b + 16 * lg);
-                qb[a][b] = v4i{w.x, w.y, w.z, w.w};
-            } else {
-                const int e = 64 * b + 32 * (int)(lg >> 1) + 8 * (int)(lg & 1u);
-                const int2 x = *reinterpret_cast<const int2 *>(r + e), y = *reinterpret_cast<const int2 *>(r + e + 16);
-                qb[a][b] = v4i{x.x, x.y, y.x, y.y};
-            }
-        }
-    }
-    Nf4 cb{};
-    if constexpr (BITS == 4) nf4_xor_tables(kNf4Cb0, kNf4Cb1, kNf4Cb2, kNf4Cb3, cb.t0, cb.t1, cb.u0, cb.u1);
-    State<HD, NQ> S;
-    S.cexp = 0;
-#pragma unroll
-    for (int a = 0; a < NQ; a++) {
-        S.m[a] = -INFINITY;
-        S.l[a] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < DB; b++) S.o[a][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    for (int t = t0 + kTile * wave; t < t1; t += kTile * kWaves) {
-        Tile<HD, BITS> T;
-        if (t + kTile <= t1) {
-            load_tile<HD, BITS, false>(T, kv, base, t, t1, li, lg);
-            step<HD, BITS, NQ, false>(S, T, qb, qas, cb, t, t1, lg);
+    for (int b = 0; b < HD / 64; b++) {
+        if constexpr (BITS == 8) {
+            const int4 w = *reinterpret_cast<const int4 *>(r + 64 * b + 16 * lg);
+            qb[b] = v4i{w.x, w.y, w.z, w.w};
         } else {
-            load_tile<HD, BITS, true>(T, kv, base, t, t1, li, lg);
-            step<HD, BITS, NQ, true>(S, T, qb, qas, cb, t, t1, lg);
+            const int e = 64 * b + 32 * (int)(lg >> 1) + 8 * (int)(lg & 1u);
+            const int2 u = *reinterpret_cast<const int2 *>(r + e), w = *reinterpret_cast<const int2 *>(r + e + 16);
+            qb[b] = v4i{u.x, u.y, w.x, w.y};
         }
     }
-    // the waves' results joined in wave order, one tile of columns at a time
-    const float back = S.cexp ? __uint_as_float((S.cexp - 13u) << 23) : 0.0f;  // 1 / c
+}
+// The waves' results, added in wave order, 16 columns at a time: a part for the merge, or (WHOLE) the
+// output itself.
+template <int HD>
+struct Join {
+    float m[kWaves][16], l[kWaves][16];
+    uint64_t mask[HD / 64];  // Hadamard signs (WHOLE)
+    __align__(16) float o[kWaves][16][HD + 4];
+};
+template <int HD, int BITS, int NQ, bool WHOLE>
+__device__ __forceinline__ void join(const SharedArgs &A, const Item &I, const State<HD, NQ> &S, Join<HD> &J) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, li = lane & 15u, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const float back = S.back();
+    if constexpr (WHOLE) {
+#pragma unroll
+        for (int b = 0; b < HD / 64; b++) {
+            const uint64_t mask = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
+            if (tid == 0) J.mask[b] = mask;
+        }
+    }
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
-        if (16 * a >= n) break;
+        if (16 * a >= I.n) break;
         float l = S.l[a];
         l += xor_lane(l, 16);
         l += xor_lane(l, 32);
         if (lg == 0) {
-            sh.wm[wave][li] = S.m[a];
-            sh.wl[wave][li] = l;
+            J.m[wave][li] = S.m[a];
+            J.l[wave][li] = l;
         }
 #pragma unroll
-        for (int b = 0; b < DB; b++)
+        for (int b = 0; b < HD / 16; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) sh.wo[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * back;
+            for (int i = 0; i < 4; i++) J.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * back;
         __syncthreads();
         const int x = (int)(tid >> 4), sl = (int)(tid & 15u);  // column, sixteenth of its dimensions
-        float M = -INFINITY;
+        if (16 * a + x < I.n) {
+            float M = -INFINITY, L = 0.0f, e[kWaves];
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) M = fmaxf(M, sh.wm[w][x]);
-        float e[kWaves], L = 0.0f;
+            for (int w = 0; w < kWaves; w++) M = fmaxf(M, J.m[w][x]);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            e[w] = sh.wm[w][x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh.wm[w][x] - M);
-            L = fmaf(sh.wl[w][x], e[w], L);
-        }
-        if (16 * a + x < n) {
-            const int c = col0 + 16 * a + x;
-            const size_t at = ((size_t)(row0 + c / A.group) * A.nq + head0 + c % A.group) * (A.np + A.nt) + part;
+            for (int w = 0; w < kWaves; w++) {
+                e[w] = J.m[w][x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(J.m[w][x] - M);
+                L = fmaf(J.l[w][x], e[w], L);
+            }
+            const int c = I.col0 + 16 * a + x;
+            const size_t pair = (size_t)(I.row0 + c / A.group) * A.nq + I.head0 + c % A.group;
+            const size_t at = WHOLE ? pair : pair * (A.np + A.nt) + I.part;
 #pragma unroll
             for (int d = 0; d < HD; d += 64) {
                 float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kWaves; w++) {
-                    const float4 v = *reinterpret_cast<const float4 *>(&sh.wo[w][x][d + 4 * sl]);
+                    const float4 v = *reinterpret_cast<const float4 *>(&J.o[w][x][d + 4 * sl]);
                     r.x = fmaf(v.x, e[w], r.x);
                     r.y = fmaf(v.y, e[w], r.y);
                     r.z = fmaf(v.z, e[w], r.z);
                     r.w = fmaf(v.w, e[w], r.w);
                 }
-                *reinterpret_cast<float4 *>(A.part + at * HD + d + 4 * sl) = r;
+                if constexpr (WHOLE) {
+                    // ifwht64 with four elements on each of sixteen lanes (those of a column take part together)
+                    const float inv = 1.0f / L;
+                    float v[4] = {r.x * inv, r.y * inv, r.z * inv, r.w * inv};
+                    butterflies_slice4(v, (uint32_t)sl);
+                    const uint32_t sb = (uint32_t)(J.mask[d / 64] >> (4 * sl)) & 0xFu;
+                    r = make_float4(flip_sign(v[0] * 0.125f, sb & 1u), flip_sign(v[1] * 0.125f, (sb >> 1) & 1u),
+                                    flip_sign(v[2] * 0.125f, (sb >> 2) & 1u), flip_sign(v[3] * 0.125f, sb >> 3));
+                }
+                *reinterpret_cast<float4 *>((WHOLE ? A.out : A.part) + at * HD + d + 4 * sl) = r;
             }
-            if (sl == 0) A.stat[at] = make_float2(M, L);
+            if (!WHOLE && sl == 0) A.stat[at] = make_float2(M, L);
         }
         __syncthreads();
     }
 }
 
-template <int HD, int BITS>
+// An item's columns (16 NQ at most): each wave takes every fourth tile of 32 positions.  The next tile's K is
+// loaded as soon as this one's scores are taken, the next V once this one's products are under way.
+template <int HD, int NQ>
+struct Shared {
+    Queries<HD, 16 * NQ> q;
+    Join<HD> j;
+};
+template <int HD, int BITS, int NQ, bool WHOLE>
+__device__ __forceinline__ void attend(const SharedArgs &A, const Item &I, Shared<HD, NQ> &sh) {
+    constexpr int NB = HD / 64, DB = HD / 16, SN = TileK<HD, BITS>::SN;
+    const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    Nf4 cb{};
+    if constexpr (BITS == 4) nf4_xor_tables(kNf4Cb0, kNf4Cb1, kNf4Cb2, kNf4Cb3, cb.t0, cb.t1, cb.u0, cb.u1);
+    TileK<HD, BITS> K;
+    TileV<HD, BITS> V;
+    const int first = (I.len[0] + kTile - 1) / kTile, tiles = first + (I.len[1] + kTile - 1) / kTile;
+    // (loads behind the last tile repeat it: issued without a branch, so that a wait for the older ones
+    // can leave the newer ones in flight)
+    const auto place = [&](int i, const k2t_kv_rows *&kv, size_t &slot, int &n) {
+        const int k = i < first ? 0 : 1, at = kTile * (k ? i - first : i);
+        kv = &I.kv[k];
+        slot = I.slot[k] + at;
+        n = I.len[k] - at;
+    };
+    const auto next_k = [&](int i) {
+        const k2t_kv_rows *kv;
+        size_t slot;
+        int n;
+        place(min(i, tiles - 1), kv, slot, n);
+        load_k(K, *kv, slot, n, li, lg);
+    };
+    const auto next_v = [&](int i) {
+        const k2t_kv_rows *kv;
+        size_t slot;
+        int n;
+        place(min(i, tiles - 1), kv, slot, n);
+        load_v(V, *kv, slot, n, li, lg);
+    };
+    next_k(wave);
+    next_v(wave);
+    quantize_queries(A, I, sh.q);
+    v4i qb[NQ][NB];
+    float qas[NQ];
+#pragma unroll
+    for (int a = 0; a < NQ; a++) {
+        qas[a] = sh.q.qas[16 * a + li];
+        query_operand<HD, BITS>(sh.q.q[16 * a + li], lg, qb[a]);
+    }
+    State<HD, NQ> S;
+    S.clear();
+    for (int i = wave; i < tiles; i += kWaves) {
+        const int left = i < first ? I.len[0] - kTile * i : I.len[1] - kTile * (i - first);
+        float s[NQ][2][4], vs[2][4][SN];
+        v4i kf[2][NB];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) kf[j][b] = k_operand<BITS>(K.k[j][b], cb);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int a = 0; a < NQ; a++)
+                scores<BITS>(kf[j], qb[a], [&](int i, int n) { return K.scale(K.ks[j][i], n); }, s[a][j]);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int n = 0; n < SN; n++) vs[j][i][n] = K.scale(K.vs[j][i], n);
+        // (behind the last use, so that the same registers take the load: a copy of them would wait for it)
+        __builtin_amdgcn_sched_barrier(0);
+        next_k(i + kWaves);
+        uint32_t ph[NQ][SN][4], pl[NQ][SN][4];
+        weights<HD, NQ, SN>(S, s, qas, vs, left, lg, ph, pl);
+        // four output tiles (one 4-byte word of V per position) at a time
+#pragma unroll
+        for (int g = 0; g < DB / 4; g++) {
+            uint32_t h[2][4][2];
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                v_halves(v_word<BITS>(V.v[j][0][g], cb), v_word<BITS>(V.v[j][1][g], cb), v_word<BITS>(V.v[j][2][g], cb),
+                         v_word<BITS>(V.v[j][3][g], cb), h[j]);
+            if (g + 1 == DB / 4) {
+                __builtin_amdgcn_sched_barrier(0);
+                next_v(i + kWaves);
+            }
+            // the small pieces of all four tiles, then the large ones: no product waits for the one before
+            constexpr int kBlocks = SN - 1;  // (NF4 blocks have weights of their own)
+            v8h va[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                va[u] = __builtin_bit_cast(v8h, make_uint4(h[0][u][0], h[0][u][1], h[1][u][0], h[1][u][1]));
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int a = 0; a < NQ; a++) S.o[a][4 * g + u] = add_tile(va[u], pl[a][g & kBlocks], S.o[a][4 * g + u]);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int a = 0; a < NQ; a++) S.o[a][4 * g + u] = add_tile(va[u], ph[a][g & kBlocks], S.o[a][4 * g + u]);
+        }
+    }
+    join<HD, BITS, NQ, WHOLE>(A, I, S, sh.j);
+}
+
+template <int HD, int BITS, int NQ>
 __global__ __launch_bounds__(64 * kWaves, 2) void shared_part_kernel(SharedArgs A) {
-    __shared__ Shared<HD> sh;
+    __shared__ union U {
+        Shared<HD, NQ> prefix;
+        Shared<HD, 1> tail;
+        __device__ U() {}
+    } sh;
     const int id = (int)blockIdx.x;
+    Item I;
     if (id < A.pre_items) {
         // A unit's column groups read the same K / V: they get ids congruent mod 8, one XCD's.
         const int slot = id >> 3, unit = (id & 7) + 8 * (slot / A.pgroups), cg = slot % A.pgroups;
         if (unit >= A.units) return;
-        const int part = unit % A.np, sk = unit / A.np, head = sk % A.nkv, seq = sk / A.nkv;
-        const int t0 = part * A.plen, t1 = min(row_len(A.pre, seq), t0 + A.plen);
-        if (t0 >= t1) return;
-        item<HD, BITS, 2>(A, sh, A.pre, ((size_t)seq * A.nkv + head) * A.pre.cap, t0, t1, seq * A.beams, head * A.group,
-                          32 * cg, A.beams * A.group, part);
+        const int sk = unit / A.np, head = sk % A.nkv, seq = sk / A.nkv;
+        I.part = unit % A.np;
+        const int t0 = I.part * A.plen;
+        I.kv[0] = I.kv[1] = A.pre;
+        I.slot[0] = I.slot[1] = ((size_t)seq * A.nkv + head) * A.pre.cap + t0;
+        I.len[0] = min(row_len(A.pre, seq) - t0, A.plen);
+        I.len[1] = 0;
+        if (I.len[0] <= 0) return;
+        I.row0 = seq * A.beams;
+        I.head0 = head * A.group;
+        I.col0 = 16 * NQ * cg;
+        I.n = min(16 * NQ, A.beams * A.group - I.col0);
+        attend<HD, BITS, NQ, false>(A, I, sh.prefix);
         return;
     }
     int t = id - A.pre_items;
     const int cg = t % A.tgroups;
     t /= A.tgroups;
-    const int part = t % A.nt;
+    I.part = t % A.nt;
     t /= A.nt;
     const int head = t % A.nkv, row = t / A.nkv;
-    const int t0 = part * A.tlen, t1 = min(row_len(A.tail, row), t0 + A.tlen);
-    if (t0 >= t1) return;
-    item<HD, BITS, 1>(A, sh, A.tail, ((size_t)row * A.nkv + head) * A.tail.cap, t0, t1, row, head * A.group, 16 * cg, A.group,
-                      A.np + part);
+    const int t0 = I.part * A.tlen;
+    I.kv[0] = I.kv[1] = A.tail;
+    I.slot[0] = I.slot[1] = ((size_t)row * A.nkv + head) * A.tail.cap + t0;
+    I.len[0] = min(row_len(A.tail, row) - t0, A.tlen);
+    I.len[1] = 0;
+    if (I.len[0] <= 0) return;
+    I.part += A.np;
+    I.row0 = row;
+    I.head0 = head * A.group;
+    I.col0 = 16 * cg;
+    I.n = min(16, A.group - I.col0);
+    attend<HD, BITS, 1, false>(A, I, sh.tail);
 }
 
-// One wave per (head, row): the parts that hold positions, in order, and ifwht64.
-template <int HD>
-__global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs A) {
-    const uint32_t lane = threadIdx.x;
-    const int head = blockIdx.x, row = blockIdx.y, n = A.np + A.nt;
+// Few positions: one workgroup per (row, KV head, 16 q heads) takes the prefix and the tail and writes
+// the output; the prefix is read once per row, by so few bytes that a second launch costs more.
+template <int HD, int BITS>
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_whole_kernel(SharedArgs A) {
+    __shared__ Shared<HD, 1> sh;
+    int t = (int)blockIdx.x;
+    const int cg = t % A.tgroups;
+    t /= A.tgroups;
+    const int head = t % A.nkv, row = t / A.nkv, seq = row / A.beams;
+    Item I;
+    I.kv[0] = A.pre;
+    I.kv[1] = A.tail;
+    I.slot[0] = ((size_t)seq * A.nkv + head) * A.pre.cap;
+    I.slot[1] = ((size_t)row * A.nkv + head) * A.tail.cap;
+    I.len[0] = A.pre.cap ? row_len(A.pre, seq) : 0;
+    I.len[1] = A.tail.cap ? row_len(A.tail, row) : 0;
+    I.row0 = row;
+    I.head0 = head * A.group;
+    I.col0 = 16 * cg;
+    I.n = min(16, A.group - I.col0);
+    I.part = 0;
+    if (I.len[0] + I.len[1] == 0) {
+        float *out = A.out + ((size_t)row * A.nq + I.head0 + I.col0) * HD;
+        for (int i = (int)threadIdx.x; i < I.n * HD; i += 64 * kWaves) out[i] = 0.0f;
+        return;
+    }
+    attend<HD, BITS, 1, true>(A, I, sh);
+}
+
+// One (head, row) per WAVES waves: its parts' maxima and sums one per lane, then the outputs of every
+// WAVES-th part, eight or sixteen loads in flight, joined in wave order, and ifwht64.  Parts that hold no
+// positions were not written and count nothing.
+template <int HD, int WAVES>
+__global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs A, int pairs) {
+    constexpr int E = HD / 64, kAhead = WAVES > 1 ? 8 : 16;  // values per lane; loads in flight
+    __shared__ float sum[WAVES > 1 ? WAVES : 1][HD];
+    const uint32_t lane = threadIdx.x & 63u;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int pair = WAVES == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x, w0 = WAVES == 1 ? 0 : wave;
+    if (pair >= pairs) return;
+    const int row = pair / A.nq, n = A.np + A.nt;
+    const size_t at = (size_t)pair * n;
     const int np = A.np ? (row_len(A.pre, row / A.beams) + A.plen - 1) / A.plen : 0;
     const int nt = A.nt ? (row_len(A.tail, row) + A.tlen - 1) / A.tlen : 0;
-    const size_t at = ((size_t)row * A.nq + head) * n;
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int i = 0; i < np + nt; i++) {
-        const size_t p = at + (i < np ? i : A.np + i - np);
-        const float2 st = A.stat[p];
-        const float mn = fmaxf(m, st.x), a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float b = __builtin_amdgcn_exp2f(st.x - mn);
-        l = fmaf(l, a, st.y * b);
-        o0 = fmaf(o0, a, A.part[p * HD + lane] * b);
-        if (HD > 64) o1 = fmaf(o1, a, A.part[p * HD + HD - 64 + lane] * b);
+    float m = -INFINITY, l = 0.0f, o[E] = {};
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const int mine = i0 + (int)lane, cnt = min(64, n - i0);
+        float v[kAhead][E];
+        const auto load = [&](int j0) {
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) {
+                const float *p = A.part + (at + i0 + min(j0 + u * WAVES, cnt - 1)) * HD + E * lane;
+                if constexpr (E == 2) {
+                    const float2 f = *reinterpret_cast<const float2 *>(p);
+                    v[u][0] = f.x;
+                    v[u][1] = f.y;
+                } else {
+                    v[u][0] = *p;
+                }
+            }
+        };
+        const float2 st = A.stat[at + min(mine, n - 1)];
+        load(w0);
+        const bool live = mine < n && (mine < A.np ? mine < np : mine - A.np < nt);
+        const float mn = fmaxf(m, wave_max_f(live ? st.x : -INFINITY));
+        if (mn == -INFINITY) continue;
+        const float e = live ? __builtin_amdgcn_exp2f(st.x - mn) : 0.0f, corr = __builtin_amdgcn_exp2f(m - mn);
+        l = fmaf(l, corr, wave_sum_f(live ? st.y * e : 0.0f));
+#pragma unroll
+        for (int k = 0; k < E; k++) o[k] *= corr;
         m = mn;
+        for (int j0 = w0; j0 < cnt; j0 += kAhead * WAVES) {
+            if (j0 > w0) load(j0);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) {
+                const int j = j0 + u * WAVES;
+                const float w = j < cnt ? lane_val(e, j) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < E; k++) o[k] = w != 0.0f ? fmaf(v[u][k], w, o[k]) : o[k];
+            }
+        }
     }
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int k = 0; k < E; k++) sum[wave][E * lane + k] = o[k];
+        __syncthreads();
+        if (wave >= E) return;
+    }
+    // one 64-block per wave or turn, one element per lane
     const float inv = np + nt == 0 ? 0.0f : 1.0f / l;
-    float *out = A.out + ((size_t)row * A.nq + head) * HD;
-    out[lane] = ifwht_lane(o0 * inv, 0, lane);
-    if (HD > 64) out[64 + lane] = ifwht_lane(o1 * inv, 1, lane);
+    float *out = A.out + (size_t)pair * HD;
+    if constexpr (WAVES > 1) {
+        float r = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) r += sum[w][64 * wave + lane];
+        out[64 * wave + lane] = ifwht_lane(r * inv, wave, lane);
+    } else {
+        // (a lane's two neighbouring elements of HD = 128 to one element of each block)
+#pragma unroll
+        for (int b = 0; b < E; b++) {
+            float r = o[0];
+            if constexpr (E == 2) {
+                const int from = 32 * b + (int)(lane >> 1);
+                const float r0 = __shfl(o[0], from, kWave), r1 = __shfl(o[E - 1], from, kWave);
+                r = (lane & 1u) ? r1 : r0;
+            }
+            out[64 * b + lane] = ifwht_lane(r * inv, b, lane);
+        }
+    }
 }
 
-// How the positions are cut into parts: enough workgroups for two on every CU, a tile per wave at
-// least.
+// shared_whole_kernel up to this many positions, times its rounds of four workgroups per CU.  Measured
+// on both sides (8 rows x 32 heads x 64: 320 positions 6.7 us and 8.6 in two launches, 620 8.3 and 8.8,
+// 1220 11.9 and 9.8; 64 rows, two rounds, 320 positions 17.7 and 15.8).
+constexpr size_t kWholeMax = 600;
+// Prefix items of two tiles of columns from this many (tile of columns, 32 positions) steps on: fewer
+// instructions per step, but half the workgroups (32 / 4 heads x 128, 12000 positions: 32 rows, 24000
+// steps, 28.0 us and 30.9 with one tile; 16 rows, 12000 steps, 23.2 and 21.2).
+constexpr size_t kTwoTiles = 18000;
+
+// How the work is cut.  nq: the prefix items' column tiles; parts so that there are about two
+// workgroups for every CU, of a tile for every wave at least.
 struct Plan {
-    int np, plen, pgroups, nt, tlen, tgroups;
+    int nq, np, plen, pgroups, nt, tlen, tgroups;
+    bool whole;  // shared_whole_kernel
 };
 Plan plan_of(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_len) {
-    const int group = s.nq / s.nkv, least = kTile * kWaves;
+    const int group = s.nq / s.nkv, cols = s.beams * group, least = kTile * kWaves;
     Plan P{};
-    P.pgroups = (s.beams * group + 31) / 32;
     P.tgroups = (group + 15) / 16;
-    const auto cut = [&](int len, int items, int &n, int &each) {
+    const size_t cus = (size_t)std::max(1, ctx->num_cus), wholes = (size_t)s.n_seq * s.beams * s.nkv * P.tgroups;
+    P.whole = ((size_t)prefix_len + tail_len) * ((wholes + 4 * cus - 1) / (4 * cus)) <= kWholeMax;
+    if (P.whole) return P;
+    const size_t steps = (size_t)s.n_seq * s.nkv * ((cols + 15) / 16) * (prefix_len / kTile);
+    P.nq = steps >= kTwoTiles ? 2 : 1;
+    P.pgroups = (cols + 16 * P.nq - 1) / (16 * P.nq);
+    const auto cut = [&](int len, size_t items, int &n, int &each) {
         if (len == 0) return;
-        const int want = std::max(1, 2 * std::max(1, ctx->num_cus) / std::max(1, items));
+        const int want = (int)std::max<size_t>(1, 2 * cus / std::max<size_t>(1, items));
         each = ((len + want - 1) / want + least - 1) / least * least;
         n = (len + each - 1) / each;
     };
-    cut(prefix_len, s.n_seq * s.nkv * P.pgroups, P.np, P.plen);
-    cut(tail_len, s.n_seq * s.beams * s.nkv * P.tgroups, P.nt, P.tlen);
+    cut(prefix_len, (size_t)s.n_seq * s.nkv * P.pgroups, P.np, P.plen);
+    cut(tail_len, (size_t)s.n_seq * s.beams * s.nkv * P.tgroups, P.nt, P.tlen);
     return P;
 }
 size_t part_slots(const SharedShape &s, const Plan &P) { return (size_t)s.n_seq * s.beams * s.nq * (P.np + P.nt); }
 
+template <int HD, int BITS>
+void launch_parts(hipStream_t st, const SharedArgs &A, const Plan &P, size_t items) {
+    const dim3 grid((unsigned)items), block(64 * kWaves);
+    if (P.nq == 2) hipLaunchKernelGGL((shared_part_kernel<HD, BITS, 2>), grid, block, 0, st, A);
+    else hipLaunchKernelGGL((shared_part_kernel<HD, BITS, 1>), grid, block, 0, st, A);
+    hip_check(hipGetLastError(), "attn_shared launch");
+}
+
 template <int HD>
-void launch_shared(hipStream_t st, int bits, const SharedArgs &A, const SharedShape &s, size_t items) {
-    const int rows = s.n_seq * s.beams;
-    if (items) {
-        if (bits == 8)
-            hipLaunchKernelGGL((shared_part_kernel<HD, 8>), dim3((unsigned)items), dim3(64 * kWaves), 0, st, A);
-        else
-            hipLaunchKernelGGL((shared_part_kernel<HD, 4>), dim3((unsigned)items), dim3(64 * kWaves), 0, st, A);
+void launch_shared(hipStream_t st, int bits, const SharedArgs &A, const SharedShape &s, const Plan &P, size_t items) {
+    const int pairs = s.n_seq * s.beams * s.nq;
+    if (P.whole) {
+        const dim3 grid((unsigned)((size_t)s.n_seq * s.beams * s.nkv * P.tgroups));
+        if (bits == 8) hipLaunchKernelGGL((shared_whole_kernel<HD, 8>), grid, dim3(64 * kWaves), 0, st, A);
+        else hipLaunchKernelGGL((shared_whole_kernel<HD, 4>), grid, dim3(64 * kWaves), 0, st, A);
         hip_check(hipGetLastError(), "attn_shared launch");
+        return;
     }
-    hipLaunchKernelGGL(shared_merge_kernel<HD>, dim3(s.nq, rows), dim3(64), 0, st, A);
+    if (items && bits == 8) launch_parts<HD, 8>(st, A, P, items);
+    if (items && bits == 4) launch_parts<HD, 4>(st, A, P, items);
+    if (A.np + A.nt > 16) hipLaunchKernelGGL((shared_merge_kernel<HD, 4>), dim3(pairs), dim3(256), 0, st, A, pairs);
+    else hipLaunchKernelGGL((shared_merge_kernel<HD, 1>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs);
     hip_check(hipGetLastError(), "attn_shared merge launch");
 }
 
 }  // namespace
 
 size_t attn_shared_ws_bytes(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_len) {
-    const size_t slots = part_slots(s, plan_of(ctx, s, prefix_len, tail_len));
-    return std::max<size_t>(16, slots * (s.hd * sizeof(float) + sizeof(float2)));
+    const Plan P = plan_of(ctx, s, prefix_len, tail_len);
+    return std::max<size_t>(16, part_slots(s, P) * (s.hd * sizeof(float) + sizeof(float2)));
 }
 
 void launch_attn_shared(k2t_ctx *ctx, hipStream_t st, int bits, const float *q, size_t q_stride, const SharedShape &s,
@@ -563,8 +829,8 @@ void launch_attn_shared(k2t_ctx *ctx, hipStream_t st, int bits, const float *q, 
     if (pre + tails > (size_t)1 << 23) throw Error(K2T_E_ARG, "too many rows, heads and positions in one call");
     A.units = (int)units;
     A.pre_items = P.np ? (int)pre : 0;
-    if (s.hd == 128) launch_shared<128>(st, bits, A, s, A.pre_items + tails);
-    else launch_shared<64>(st, bits, A, s, A.pre_items + tails);
+    if (s.hd == 128) launch_shared<128>(st, bits, A, s, P, A.pre_items + tails);
+    else launch_shared<64>(st, bits, A, s, P, A.pre_items + tails);
 }
 
 }  // namespace k2t

@@ -145,7 +145,7 @@ def test_reorder_moves_rows_in_place(gpu_ctx, bits, hd, layers, n_seq, beams, nk
 ATTN = [
     # n_seq, beams, nq, nkv, prefix, tail
     (1, 1, 1, 1, 1, 0), (1, 1, 4, 4, 0, 1), (1, 4, 9, 3, 45, 7), (2, 3, 8, 2, 63, 65), (1, 5, 4, 4, 257, 31),
-    (1, 17, 8, 1, 130, 3), (3, 2, 24, 2, 513, 20), (1, 33, 4, 2, 1000, 33), (1, 1, 16, 1, 700, 300), (1, 64, 2, 1, 31, 2),
+    (1, 17, 8, 1, 130, 3), (3, 2, 24, 2, 513, 20), (1, 3, 2, 1, 9000, 5), (2, 40, 4, 4, 700, 2), (1, 2, 40, 2, 600, 150), (1, 33, 4, 2, 1000, 33), (1, 1, 16, 1, 700, 300), (1, 64, 2, 1, 31, 2),
 ]
 
 
@@ -179,6 +179,27 @@ def test_attention_over_prefix_and_tail(gpu_ctx, bits, hd, n_seq, beams, nq, nkv
     want, bound = R.attention(bits, q[:, :nq * hd].reshape(rows, nq, hd), pre, tl, plen, tlen, beams, nq, nkv, hd, scale)
     err = np.abs(out.cpu().numpy() - want)
     assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+def test_attention_of_many_rows(gpu_ctx, bits, hd):
+    """Enough rows and positions for the prefix items of two tiles of columns (18304 steps); the last
+    item holds one tile."""
+    rng = np.random.default_rng(hd + bits)
+    beams, nq, nkv, prefix, tail = 61, 32, 8, 4600, 3
+    pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+    q = (2 * rng.standard_normal((beams, nq, hd))).astype(np.float32)
+    out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+    _, p = rows_of(pre, prefix)
+    _, t = rows_of(tl, tail)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(bits, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, t, hd ** -0.5, out, ws)
+    gpu_ctx.sync()
+    rows = [0, 1, 30, 59, 60]  # (the reference of a few rows)
+    want, bound = R.attention(bits, q[rows], pre, [a[rows] for a in tl], [prefix], [tail] * 5, 5, nq, nkv, hd, hd ** -0.5)
+    err = np.abs(out.cpu().numpy()[rows] - want)
+    assert (err <= bound).all(), float((err / bound).max())
+    assert torch.isfinite(out).all()
 
 
 @pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
