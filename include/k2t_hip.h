@@ -455,7 +455,7 @@ int32_t k2t_attn_shared_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, in
  * batch (what k2t_kv_reorder takes), and (nullable) done = the row had ended or token == eos
  * (eos -1: none).  Where a sequence has fewer candidates the rest get score -inf, token max(eos,
  * 0), its first row, and done 1.  With k == beams the outputs may be the input scores and done
- * flags.  beams <= 64, k <= 128.  d_ws as in k2t_attn_shared. */
+ * flags.  vocab <= 262144, beams <= 64, k <= 128.  d_ws as in k2t_attn_shared. */
 int32_t k2t_beam_select(k2t_ctx *ctx, const float *d_logits, int32_t vocab, size_t row_stride, const float *d_scores,
                         const int32_t *d_done, int32_t n_seq, int32_t beams, int32_t k, int32_t eos,
                         float *d_out_scores, int32_t *d_out_tokens, int32_t *d_out_parents, int32_t *d_out_done,

@@ -75,7 +75,7 @@ def test_select():
     n = C.c_size_t()
     assert call("k2t_beam_select_workspace", CTX, 2, 4, 1000, 8, C.byref(n)) == 0 and n.value >= 16
     good = [CTX, P, 1000, 1000, P, P, 2, 4, 8, 5, P, P, P, P, P, n.value]
-    refused("k2t_beam_select", good, [{0: None}, {1: None}, {2: 0}, {3: 999}, {4: None}, {6: -1}, {7: 0}, {7: 65}, {8: 0},
+    refused("k2t_beam_select", good, [{0: None}, {1: None}, {2: 0}, {2: 262145, 3: 262145}, {3: 999}, {4: None}, {6: -1}, {7: 0}, {7: 65}, {8: 0},
                                       {8: 129}, {9: -2}, {9: 1000}, {9: -1}, {10: None}, {11: None}, {12: None}, {14: None},
                                       {14: P + 8}, {15: n.value - 1}, {6: 20000}])
     refused("k2t_beam_select_workspace", [CTX, 2, 4, 1000, 8, C.byref(n)], [{0: None}, {2: 65}, {3: 0}, {4: 0}, {5: None}])
