@@ -17,65 +17,201 @@ struct RowsArgs {
     const float *k, *v;
     float *ko, *vo;
     size_t row_stride;
-    int ntok, nkv, hd, bits;
+    int ntok, nkv;
     const int *pos, *counts;
     k2t_kv_rows kv;
     size_t row0;  // first cache row
-    size_t units;  // heads of the call: batch * ntok * 2 * nkv
+    uint32_t units;  // 64-blocks of a row's tokens: ntok * 2 * nkv * (hd / 64)
 };
 
-// Head `u` of a call: token (row, t), K or V, KV head; its cache slot, or false where the token does
-// not exist or its position lies outside the cache.
-struct HeadAt {
+// The kernels below give every 64-block of a head to sixteen lanes, four consecutive elements each
+// (butterflies_slice4: the bits of kv_store_kernel's one element per lane); the blocks of a head are
+// neighbours.  Grid y: the row of the call.
+//
+// Block `u` of a row: token t, K or V, KV head; the head's place in the call and its cache slot.  False
+// where the token does not exist or its position lies outside the cache.
+struct BlockAt {
     size_t in, slot;
-    int is_v;
+    int is_v, b;
 };
-__device__ __forceinline__ bool head_at(const RowsArgs &A, size_t u, HeadAt &h) {
-    const int hv = (int)(u % (2u * A.nkv));
-    const size_t tok = u / (2u * A.nkv);
-    const int row = (int)(tok / A.ntok), t = (int)(tok % A.ntok);
-    h.is_v = hv >= A.nkv;
-    const int head = h.is_v ? hv - A.nkv : hv;
-    if (A.counts && t >= A.counts[row]) return false;
+template <int NB>
+__device__ __forceinline__ bool block_at(const RowsArgs &A, uint32_t u, BlockAt &h) {
+    const uint32_t heads = 2u * (uint32_t)A.nkv, hu = u / NB, t = hu / heads, hv = hu - t * heads;
+    const int row = (int)blockIdx.y;
+    h.b = (int)(u % NB);
+    h.is_v = hv >= (uint32_t)A.nkv;
+    const uint32_t head = h.is_v ? hv - A.nkv : hv;
     const long long p = (long long)A.pos[row] + t;
-    if (p < 0 || p >= A.kv.cap) return false;
-    h.in = tok * A.row_stride + (size_t)head * A.hd;
+    h.in = ((size_t)row * A.ntok + t) * A.row_stride + (size_t)head * (64 * NB) + 64 * h.b;
     h.slot = ((A.row0 + row) * A.nkv + head) * (size_t)A.kv.cap + (size_t)p;
-    return true;
+    return u < A.units && (!A.counts || (int)t < A.counts[row]) && p >= 0 && p < A.kv.cap;
 }
 
-// One wave per head, one element (of each 64-block) per lane: kv_store_kernel's arithmetic.
+// Magnitude place p (0 .. 7) of the nearest codebook value, and nf4_nearest_idx from it (three levels of
+// comparisons; a NaN takes the last place there as well).
+__device__ __forceinline__ uint32_t nf4_place(float y) {
+    const float a = fabsf(y);
+    const bool c1 = !(a < 51.0f), c2 = !(a < (c1 ? 85.5f : 24.5f));
+    const bool c3 = !(a < (c1 ? (c2 ? 111.5f : 66.5f) : (c2 ? 37.5f : 12.0f)));
+    return (c1 ? 4u : 0u) + (c2 ? 2u : 0u) + (c3 ? 1u : 0u);
+}
+__device__ __forceinline__ uint32_t nf4_index(float y) {
+    const uint32_t p = nf4_place(y);
+    return y >= 0.0f ? 8u + p : 7u - p;
+}
+// The nearest codebook value itself.
+__device__ __forceinline__ float nf4_nearest(float y) {
+    const float m = (float)__builtin_amdgcn_perm(kNf4Cb3, kNf4Cb2, nf4_place(y) | 0x0C0C0C00u);
+    return y >= 0.0f ? m : -m;
+}
+
+__device__ __forceinline__ float group_max(float v) {  // of sixteen lanes
+    v = fmaxf(v, xchg1(v));
+    v = fmaxf(v, xchg2(v));
+    v = fmaxf(v, xchg4(v));
+    return fmaxf(v, xchg8(v));
+}
+
+// Heads quantized into the cache: kv_store_kernel's arithmetic and bytes.
+// NF4: the block's scale is num / den with num summed in element order, 64 dependent additions: a wave
+// puts the terms of 4 TURNS blocks in LDS and as many lanes add one block each.
+template <int NB, int BITS, int TURNS>
 __global__ __launch_bounds__(256) void kv_append_kernel(RowsArgs A) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    HeadAt h;
-    if (u >= A.units || !head_at(A, u, h)) return;
-    const float *x = (h.is_v ? A.v : A.k) + h.in;
-    const int nb = A.hd / 64;
-    const float r0 = fwht_lane(x[lane], 0, lane);
-    const float r1 = nb > 1 ? fwht_lane(x[64 + lane], 1, lane) : 0.0f;
-    kv_store_head(r0, r1, nb, lane, A.bits, A.hd, h.slot, (int8_t *)(h.is_v ? A.kv.vq : A.kv.kq),
-                  (float *)(h.is_v ? A.kv.vs : A.kv.ks));
+    __shared__ __align__(16) float term[BITS == 4 ? 4 : 1][BITS == 4 ? 4 * TURNS : 1][68];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, sl = lane & 15u, lg = lane >> 4, wave = tid >> 6;
+    uint64_t mask[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) mask[b] = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
+    BlockAt at[TURNS];
+    bool live[TURNS];
+    float v[TURNS][4];
+#pragma unroll
+    for (int k = 0; k < TURNS; k++) {
+        live[k] = block_at<NB>(A, (blockIdx.x * TURNS + k) * 16u + 4u * wave + lg, at[k]);
+        const float4 f = live[k] ? *reinterpret_cast<const float4 *>((at[k].is_v ? A.v : A.k) + at[k].in + 4 * sl)
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[k][0] = f.x;
+        v[k][1] = f.y;
+        v[k][2] = f.z;
+        v[k][3] = f.w;
+    }
+#pragma unroll
+    for (int k = 0; k < TURNS; k++) {
+        const uint32_t sb = (uint32_t)((NB > 1 && at[k].b ? mask[NB - 1] : mask[0]) >> (4u * sl)) & 0xFu;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[k][j] = flip_sign(v[k][j], (sb >> j) & 1u) * 0.125f;
+        butterflies_slice4(v[k], sl);
+    }
+    if constexpr (BITS == 8) {
+#pragma unroll
+        for (int k = 0; k < TURNS; k++) {
+            float mx = group_max(fmaxf(fmaxf(fabsf(v[k][0]), fabsf(v[k][1])), fmaxf(fabsf(v[k][2]), fabsf(v[k][3]))));
+            if (NB > 1) mx = fmaxf(mx, xor_lane(mx, 16));
+            const bool tiny = mx <= FLT_EPSILON;
+            const float inv = 127.0f / mx;
+            uint32_t w = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) w |= (tiny ? 0u : (uint32_t)(int)rintf(v[k][j] * inv) & 0xFFu) << (8 * j);
+            if (!live[k]) continue;
+            int8_t *q = (int8_t *)(at[k].is_v ? A.kv.vq : A.kv.kq) + at[k].slot * (64 * NB) + 64 * at[k].b;
+            *reinterpret_cast<uint32_t *>(q + 4 * sl) = w;
+            if (sl == 0 && at[k].b == 0) ((float *)(at[k].is_v ? A.kv.vs : A.kv.ks))[at[k].slot] = tiny ? 0.0f : mx / 127.0f;
+        }
+    } else {
+        float mx[TURNS], den[TURNS], num[TURNS];
+#pragma unroll
+        for (int k = 0; k < TURNS; k++) {
+            mx[k] = group_max(fmaxf(fmaxf(fabsf(v[k][0]), fabsf(v[k][1])), fmaxf(fabsf(v[k][2]), fabsf(v[k][3]))));
+            const float inv0 = 127.0f / mx[k];
+            float4 t;
+            float c[4], cc = 0.0f;  // (squares of codes: whole numbers below 2^24, any order)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                c[j] = nf4_nearest(v[k][j] * inv0);
+                cc += c[j] * c[j];
+            }
+            t = make_float4(v[k][0] * c[0], v[k][1] * c[1], v[k][2] * c[2], v[k][3] * c[3]);
+            *reinterpret_cast<float4 *>(&term[wave][4 * k + lg][4 * sl]) = t;
+            cc += xchg1(cc);
+            cc += xchg2(cc);
+            cc += xchg4(cc);
+            den[k] = cc + xchg8(cc);
+        }
+        __builtin_amdgcn_wave_barrier();
+        float sum = 0.0f;
+        const float *mine = term[wave][lane % (4 * TURNS)];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float4 t = *reinterpret_cast<const float4 *>(mine + 4 * i);
+            sum += t.x;
+            sum += t.y;
+            sum += t.z;
+            sum += t.w;
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < TURNS; k++) num[k] = __shfl(sum, 4 * k + (int)lg, kWave);
+#pragma unroll
+        for (int k = 0; k < TURNS; k++) {
+            const float s_ref = (den[k] > 1e-12f && num[k] > 0.0f) ? num[k] / den[k] : mx[k] / 127.0f;
+            const bool none = mx[k] < 1e-30f;
+            const uint16_t sb = none ? 0 : f32_to_bf16_rne(s_ref);
+            const float s_fin = __uint_as_float((uint32_t)sb << 16);
+            const float inv = s_fin > 1e-30f ? 1.0f / s_fin : 0.0f;
+            uint32_t w = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) w |= (none ? 8u : nf4_index(v[k][j] * inv)) << (8 * j);
+            // byte h * 16 + i: element h * 32 + i low, h * 32 + 16 + i high, four slices further on
+            const uint32_t hi = (uint32_t)xchg4((int)w);
+            if (!live[k]) continue;
+            uint8_t *q = (uint8_t *)(at[k].is_v ? A.kv.vq : A.kv.kq) + at[k].slot * (32 * NB) + 32 * at[k].b;
+            if ((sl & 4u) == 0) *reinterpret_cast<uint32_t *>(q + 16 * (sl >> 3) + 4 * (sl & 3u)) = w | (hi << 4);
+            if (sl == 0) ((uint16_t *)(at[k].is_v ? A.kv.vs : A.kv.ks))[at[k].slot * NB + at[k].b] = sb;
+        }
+    }
 }
 
+// The same positions read back: code * scale and ifwht64.
+template <int NB, int BITS, int TURNS>
 __global__ __launch_bounds__(256) void kv_load_kernel(RowsArgs A) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    HeadAt h;
-    if (u >= A.units || !head_at(A, u, h)) return;
-    float *y = (h.is_v ? A.vo : A.ko) + h.in;
-    const void *q = h.is_v ? A.kv.vq : A.kv.kq, *s = h.is_v ? A.kv.vs : A.kv.ks;
-    for (int b = 0; b < A.hd / 64; b++) {
-        float v;
-        if (A.bits == 8) {
-            v = (float)((const int8_t *)q)[h.slot * A.hd + 64 * b + lane] * ((const float *)s)[h.slot];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, sl = lane & 15u, lg = lane >> 4, wave = tid >> 6;
+    uint64_t mask[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) mask[b] = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
+    BlockAt at[TURNS];
+    bool live[TURNS];
+    uint32_t w[TURNS];
+    float scale[TURNS];
+#pragma unroll
+    for (int k = 0; k < TURNS; k++) {
+        live[k] = block_at<NB>(A, (blockIdx.x * TURNS + k) * 16u + 4u * wave + lg, at[k]);
+        w[k] = 0;
+        scale[k] = 0.0f;
+        if (!live[k]) continue;
+        const void *q = at[k].is_v ? A.kv.vq : A.kv.kq, *s = at[k].is_v ? A.kv.vs : A.kv.ks;
+        if constexpr (BITS == 8) {
+            w[k] = *reinterpret_cast<const uint32_t *>((const int8_t *)q + at[k].slot * (64 * NB) + 64 * at[k].b + 4 * sl);
+            scale[k] = ((const float *)s)[at[k].slot];
         } else {
-            // byte h * 16 + i: element h * 32 + i low, h * 32 + 16 + i high
-            const uint8_t w = ((const uint8_t *)q)[h.slot * (A.hd / 2) + 32 * b + 16 * (lane >> 5) + (lane & 15u)];
-            const uint16_t sb = ((const uint16_t *)s)[h.slot * (A.hd / 64) + b];
-            v = (float)nf4_cb_value((lane & 16u) ? w >> 4 : w & 15) * __uint_as_float((uint32_t)sb << 16);
+            w[k] = *reinterpret_cast<const uint32_t *>((const uint8_t *)q + at[k].slot * (32 * NB) + 32 * at[k].b +
+                                                       16 * (sl >> 3) + 4 * (sl & 3u));
+            scale[k] = __uint_as_float((uint32_t)((const uint16_t *)s)[at[k].slot * NB + at[k].b] << 16);
         }
-        y[64 * b + lane] = ifwht_lane(v, b, lane);
+    }
+    uint32_t t0, t1, u0, u1;
+    nf4_xor_tables(kNf4Cb0, kNf4Cb1, kNf4Cb2, kNf4Cb3, t0, t1, u0, u1);
+#pragma unroll
+    for (int k = 0; k < TURNS; k++) {
+        if constexpr (BITS == 4) w[k] = nf4_xlut(((sl & 4u) ? w[k] >> 4 : w[k]) & 0x0F0F0F0Fu, t0, t1, u0, u1);
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = (float)(int8_t)((w[k] >> (8 * j)) & 0xFFu) * scale[k];
+        butterflies_slice4(v, sl);
+        const uint32_t sb = (uint32_t)((NB > 1 && at[k].b ? mask[NB - 1] : mask[0]) >> (4u * sl)) & 0xFu;
+        if (!live[k]) continue;
+        *reinterpret_cast<float4 *>((at[k].is_v ? A.vo : A.ko) + at[k].in + 4 * sl) =
+            make_float4(flip_sign(v[0] * 0.125f, sb & 1u), flip_sign(v[1] * 0.125f, (sb >> 1) & 1u),
+                        flip_sign(v[2] * 0.125f, (sb >> 2) & 1u), flip_sign(v[3] * 0.125f, sb >> 3));
     }
 }
 
@@ -137,20 +273,44 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs A) {
         move_column<uint16_t, NB>((uint16_t *)s + slot0 + pos, slots, par, A.beams, lens, pos);
 }
 
-RowsArgs rows_args(const k2t_kv_rows &kv, int bits, size_t row_stride, int batch, int ntok, int nkv, int hd,
-                   const int *pos, const int *counts, int layer) {
+RowsArgs rows_args(const k2t_kv_rows &kv, size_t row_stride, int batch, int ntok, int nkv, int hd, const int *pos,
+                   const int *counts, int layer) {
     RowsArgs A{};
     A.row_stride = row_stride;
     A.ntok = ntok;
     A.nkv = nkv;
-    A.hd = hd;
-    A.bits = bits;
     A.pos = pos;
     A.counts = counts;
     A.kv = kv;
     A.row0 = (size_t)layer * batch;
-    A.units = (size_t)batch * ntok * 2 * nkv;
+    A.units = (uint32_t)((size_t)ntok * 2 * nkv * (hd / 64));
     return A;
+}
+
+// Two blocks per sixteen lanes from this many on, where every SIMD has its waves anyway (8 x 1024
+// tokens, 8 heads x 128, 262144 blocks: int8 append 23.3 us and 25.1 with one, load 19.9 and 22.0; 515
+// tokens, 32 heads x 64, 32960 blocks: 4.9 and 4.4).
+constexpr size_t kManyBlocks = 1 << 16;
+
+template <int NB, int BITS, bool LOAD>
+void launch_rows(hipStream_t st, const RowsArgs &A, int batch) {
+    const bool many = (size_t)A.units * batch >= kManyBlocks;
+    const dim3 grid((A.units + (many ? 31 : 15)) / (many ? 32 : 16), (unsigned)batch), block(256);
+    if constexpr (LOAD) {
+        if (many) hipLaunchKernelGGL((kv_load_kernel<NB, BITS, 2>), grid, block, 0, st, A);
+        else hipLaunchKernelGGL((kv_load_kernel<NB, BITS, 1>), grid, block, 0, st, A);
+    } else {
+        if (many) hipLaunchKernelGGL((kv_append_kernel<NB, BITS, 2>), grid, block, 0, st, A);
+        else hipLaunchKernelGGL((kv_append_kernel<NB, BITS, 1>), grid, block, 0, st, A);
+    }
+    hip_check(hipGetLastError(), LOAD ? "kv_load launch" : "kv_append launch");
+}
+template <bool LOAD>
+void launch_rows_of(hipStream_t st, int bits, int hd, const RowsArgs &A, int batch) {
+    if (bits == 8 && hd == 64) launch_rows<1, 8, LOAD>(st, A, batch);
+    else if (bits == 8) launch_rows<2, 8, LOAD>(st, A, batch);
+    else if (hd == 64) launch_rows<1, 4, LOAD>(st, A, batch);
+    else launch_rows<2, 4, LOAD>(st, A, batch);
 }
 
 bool heads_aligned(const float *k, const float *v) {
@@ -160,7 +320,7 @@ bool heads_aligned(const float *k, const float *v) {
 void check_heads_call(k2t_ctx *ctx, int bits, int batch, int ntok, int nkv, int hd, size_t row_stride,
                       const void *d_pos, const k2t_kv_rows *kv) {
     branch_arg(ctx != nullptr && kv != nullptr, "NULL argument");
-    branch_arg(batch >= 0 && ntok >= 0 && nkv > 0, "negative batch or ntok, or no KV heads");
+    branch_arg(batch >= 0 && batch <= 65535 && ntok >= 0 && nkv > 0, "batch must be 0 .. 65535, ntok >= 0, n_kv_heads > 0");
     check_kv_rows(kv, bits, hd);
     branch_arg((size_t)batch * ntok * nkv <= (size_t)1 << 24, "more than 2^24 heads in one call");
     branch_arg(row_stride >= (size_t)nkv * hd && row_stride % 4 == 0,
@@ -184,18 +344,10 @@ void check_kv_rows(const k2t_kv_rows *kv, int bits, int hd) {
 
 void launch_kv_append(hipStream_t st, int bits, const float *k, const float *v, size_t row_stride, int batch, int ntok,
                       int nkv, int hd, const int *pos, const int *counts, const k2t_kv_rows &kv, int layer) {
-    RowsArgs A = rows_args(kv, bits, row_stride, batch, ntok, nkv, hd, pos, counts, layer);
+    RowsArgs A = rows_args(kv, row_stride, batch, ntok, nkv, hd, pos, counts, layer);
     A.k = k;
     A.v = v;
-    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)((A.units + 3) / 4)), dim3(256), 0, st, A);
-    hip_check(hipGetLastError(), "kv_append launch");
-}
-
-static void launch_kv_load(hipStream_t st, RowsArgs A, float *k, float *v) {
-    A.ko = k;
-    A.vo = v;
-    hipLaunchKernelGGL(kv_load_kernel, dim3((unsigned)((A.units + 3) / 4)), dim3(256), 0, st, A);
-    hip_check(hipGetLastError(), "kv_load launch");
+    launch_rows_of<false>(st, bits, hd, A, batch);
 }
 
 void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const int *parents, int n_layers, int n_seq,
@@ -242,9 +394,10 @@ int32_t k2t_kv_load(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, int32_t b
         branch_arg(d_k && d_v, "NULL argument");
         branch_arg(heads_aligned(d_k, d_v), "d_k and d_v must be 16-byte aligned");
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
-        launch_kv_load(ctx->stream,
-                       rows_args(*kv, bits, row_stride, batch, ntok, n_kv_heads, head_dim, d_pos, d_counts, 0), d_k,
-                       d_v);
+        RowsArgs A = rows_args(*kv, row_stride, batch, ntok, n_kv_heads, head_dim, d_pos, d_counts, 0);
+        A.ko = d_k;
+        A.vo = d_v;
+        launch_rows_of<true>(ctx->stream, bits, head_dim, A, batch);
     });
 }
 

@@ -92,6 +92,44 @@ def test_append_equals_kv_store(gpu_ctx, bits):
     assert all(torch.equal(u, v) for u, v in zip(a, b))
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_append_and_load_of_many_tokens(gpu_ctx, bits, hd):
+    """Enough blocks for two per group of lanes, ragged rows: append against k2t_kv_store's bytes, load
+    against append's."""
+    g = torch.Generator(device="cuda").manual_seed(hd + bits)
+    batch, ntok, nkv = 3, 701, 2048 // hd
+    x = torch.randn(batch * ntok, 2 * nkv * hd, generator=g, device="cuda")
+    counts, pos, cap = [701, 350, 699], [0, 3, 2], 704
+    want, _ = rows_of(R.new_cache(bits, batch, nkv, cap, hd), cap)
+    a, kv = rows_of(R.new_cache(bits, batch, nkv, cap, hd), cap)
+    q, s = (torch.empty((batch * ntok * nkv,) + t.shape[3:], dtype=t.dtype, device="cuda") for t in want[:2])
+    for w in range(2):
+        heads = x[:, w * nkv * hd:(w + 1) * nkv * hd].contiguous()
+        gpu_ctx.kv_store(bits, heads, batch * ntok * nkv, hd, q, s)
+        gpu_ctx.sync()
+        for b in range(batch):
+            for got, t in ((q, want[2 * w]), (s, want[2 * w + 1])):
+                rows = got.view((batch, ntok, nkv) + t.shape[3:])[b, :counts[b]].transpose(0, 1)
+                t[b, :, pos[b]:pos[b] + counts[b]] = rows
+    at = x.data_ptr()
+    gpu_ctx.kv_append(bits, at, at + 4 * nkv * hd, 2 * nkv * hd, batch, ntok, nkv, hd, ints(pos), kv, counts=ints(counts))
+    y = torch.full_like(x, 9.0)
+    gpu_ctx.kv_load(bits, kv, batch, ntok, nkv, hd, ints(pos), y.data_ptr(), y.data_ptr() + 4 * nkv * hd, 2 * nkv * hd,
+                    counts=ints(counts))
+    gpu_ctx.sync()
+    assert all(torch.equal(u, v) for u, v in zip(a, want))
+    for b in range(batch):
+        rows = y.view(batch, ntok, 2, nkv, hd)[b]
+        assert bool((rows[counts[b]:] == 9.0).all())
+        for w in range(2):
+            n = counts[b]
+            vals = R.values(bits, host(a[2 * w][b, :, pos[b]:pos[b] + n], np.zeros(0, np.int8 if bits == 8 else np.uint8)),
+                            host(a[2 * w + 1][b, :, pos[b]:pos[b] + n], np.zeros(0, np.float32 if bits == 8 else np.uint16)))
+            err = np.abs(rows[:n, w].cpu().numpy().transpose(1, 0, 2) - R.unrotate(vals))
+            assert (err <= 7.5 * R.U * R.block_sums(np.abs(vals)) / 8).all()
+
+
 def test_append_offsets_past_32_bits(gpu_ctx):
     """A cache of 2^20 positions x 40 heads of 128 bytes (5 GiB): the last head's last slot."""
     hd, nkv, cap = 128, 40, 1 << 20
