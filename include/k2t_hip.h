@@ -358,6 +358,17 @@ int32_t k2t_model_prefill(k2t_model *m, const int32_t *tokens, int32_t n, float 
  * n_steps decode steps whose next token is the argmax of the logits, chosen on the
  * device.  tokens_out (nullable) receives the n_steps argmax tokens. */
 int32_t k2t_model_generate(k2t_model *m, int32_t first_token, int32_t n_steps, int32_t *tokens_out);
+/* Beam search (no counterpart in the reference, which decodes greedily or samples): feeds
+ * first_token, then chooses n_steps times the n_beams best continuations by the sum of their log
+ * probabilities (k2t_beam_select; ties there).  tokens_out [n_beams][n_steps] and scores_out [n_beams],
+ * best first; eos (-1: none) ends a beam, whose score then stays and whose further tokens are eos.  The
+ * beams share the model's cache (k2t_attn_shared) and have tails of their own; afterwards the cache and
+ * the position are those of the best one, as k2t_model_generate leaves its own: everything fed but the
+ * last token (from an eos on nothing).  Fast mode, full cache (int8 or NF4), n_beams <= 64 and <= the
+ * model's max_batch, vocabulary <= 262144.  With one beam it decodes greedily.  The buffers (tails of
+ * n_steps positions for every layer and beam, logits) stay with the model. */
+int32_t k2t_model_beam_search(k2t_model *m, int32_t first_token, int32_t n_beams, int32_t n_steps, int32_t eos,
+                              int32_t *tokens_out, float *scores_out);
 /* Device pointer of the last logits (valid after a step; read after k2t_model_sync). */
 int32_t k2t_model_logits(k2t_model *m, const float **d_logits);
 int32_t k2t_model_sync(k2t_model *m);

@@ -384,7 +384,8 @@ void check_select(k2t_ctx *ctx, int n_seq, int beams, int vocab, int k) {
     branch_arg(beams >= 1 && beams <= kMaxBeams, "beams must be 1 .. 64");
     branch_arg(k >= 1 && k <= kMaxPicks, "k must be 1 .. 128");
     branch_arg(n_seq >= 0 && (size_t)n_seq * beams <= 65535, "n_seq * beams must be 0 .. 65535");
-    branch_arg(vocab >= 1 && vocab <= 64 * kSlice, "vocab must be 1 .. 262144");
+    static_assert(kMaxSelectVocab == 64 * kSlice, "a lane per slice");
+    branch_arg(vocab >= 1 && vocab <= kMaxSelectVocab, "vocab must be 1 .. 262144");
 }
 
 }  // namespace

@@ -8,7 +8,7 @@
 
 namespace k2t {
 
-constexpr int kMaxBeams = 64, kMaxPicks = 128;
+constexpr int kMaxBeams = 64, kMaxPicks = 128, kMaxSelectVocab = 262144;
 
 inline void branch_arg(bool ok, const char *msg) {
     if (!ok) throw Error(K2T_E_ARG, msg);

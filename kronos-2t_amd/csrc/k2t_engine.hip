@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/k2t_hip.h"
+#include "k2t_branch.h"
 #include "k2t_decode_mk.h"
 #include "k2t_internal.h"
 #include "k2t_moe.h"
@@ -36,6 +37,9 @@ void launch_embed(hipStream_t st, const k2t_mat *m, const int *tokens, int ntok,
 void launch_kv_synthetic(hipStream_t st, int8_t *kq, int8_t *vq, float *ks, float *vs, int layers_kv, int cap,
                          int n_pos, int hd, int bits, uint64_t seed);
 void launch_kv_store(hipStream_t st, const float *heads, int n, int hd, int bits, int8_t *qbuf, float *sbuf);
+void launch_beam_post(hipStream_t st, float *qkv, const float *bias, const float *qn, const float *kn, float eps,
+                      const float *rope, const int *pos_dev, int pos0, int nq, int nkv, int hd, int rows, int bits,
+                      const k2t_kv_rows &tail);
 void launch_embed_rows(hipStream_t st, const void *rows, bool bf16, const int *tokens, int ntok, int d, float *out);
 void launch_advance_pos(hipStream_t st, int *pos, int n);
 void launch_argmax(hipStream_t st, const float *x, int n, int *out_idx);
@@ -281,6 +285,16 @@ struct k2t_model {
     int mk_head_off = 0;  // first workgroup of the persistent kernel's lm_head phase
     int mk_nsp = 1;       // attention spans per q head in the persistent kernel
     unsigned long long *mk_terms = nullptr;  // exact-order variant: epilogue operands per workgroup
+    // beam search: the rows' tail caches (beam_cap slots per row and KV head, every layer), their logits,
+    // and the choices of every step; grown on demand
+    std::vector<void *> beam_allocs;
+    int beam_rows = 0, beam_cap = 0;
+    size_t beam_ws_bytes = 0;
+    k2t_kv_rows beam_tail{};
+    float *beam_logits = nullptr, *beam_scores = nullptr;
+    int *beam_done = nullptr, *beam_pos = nullptr;
+    int *beam_tokens = nullptr, *beam_parents = nullptr;  // [step][row]
+    void *beam_ws = nullptr;
 };
 
 namespace {
@@ -419,11 +433,19 @@ ActTiles act_tiles_for(const k2t_model *m, const k2t_mat *w, int ntok) {
     return m->ctx->mfma == 1 && gemm_mfma_supported(w, ntok) ? ActTiles{m->xt, m->st, m->ut} : ActTiles{};
 }
 
+// A step of beam search: one token of every row, at position prefix + tail - 1 (device copy: m->beam_pos).
+struct BeamStep {
+    const int *tokens;
+    int prefix, tail;  // positions a row attends to: its own of this step included
+};
+
 // One forward pass over `ntok` tokens already in m->tokens, positions pos..pos+ntok-1.
 // Logits (of the last token) go to m->logits; the device position advances by ntok.
+// With `beam` the tokens are rows that continue the model's cache, each with a tail cache; every row's
+// logits go to m->beam_logits, and the model's cache and position stay as they are.
 // ctx_bound: the position after the batch's last token when the host knows it (prefill;
 // never a captured step, whose position moves between replays), else 0.
-void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0) {
+void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0, const BeamStep *beam = nullptr) {
     if (m->exact) {
         forward_exact(m, ntok, with_logits);
         return;
@@ -434,13 +456,14 @@ void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0) {
     const int hd = c.head_dim, nq = c.n_heads, nkv = c.n_kv_heads, d = c.hidden, inter = c.intermediate;
     const float attn_scale = 1.0f / sqrtf((float)hd);
     const int nsplit = attn_max_splits(m->ring.window > 0 ? std::min(c.max_seq, m->ring.window) : c.max_seq);
+    const int *tokens = beam ? beam->tokens : m->tokens;
     if (m->embed_kind == K2T_EMBED_F32 || m->embed_kind == K2T_EMBED_BF16)
-        launch_embed_rows(st, m->embed_rows, m->embed_kind == K2T_EMBED_BF16, m->tokens, ntok, c.hidden, m->hidden);
+        launch_embed_rows(st, m->embed_rows, m->embed_kind == K2T_EMBED_BF16, tokens, ntok, c.hidden, m->hidden);
     else
-        launch_embed(st, m->embed_kind == K2T_EMBED_NF4 ? m->embed_mat : m->head, m->tokens, ntok, m->hidden);
+        launch_embed(st, m->embed_kind == K2T_EMBED_NF4 ? m->embed_mat : m->head, tokens, ntok, m->hidden);
     // One token: the RMSNorm / SwiGLU + FWHT + int8 activations are built inside the GEMVs
     // (each wave for its own chunks); batches use the standalone kernels.  Same codes.
-    const bool fused = ntok == 1;
+    const bool fused = ntok == 1 && !beam;
     for (int l = 0; l < c.n_layers; l++) {
         const auto &L = m->layers[l];
         bool qkv_posted = false;
@@ -450,7 +473,7 @@ void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0) {
             const ActTiles tq = act_tiles_for(m, L.qkv, ntok);
             launch_rmsnorm_act(st, ctx->signs, m->hidden, L.in_norm, c.rms_eps, d, ntok, m->xq, m->xs, m->xsum, tq);
             // head size 64 with producer tiles: qkv_post's work as the GEMV's epilogue
-            qkv_posted = hd == 64 && tq.xt &&
+            qkv_posted = hd == 64 && tq.xt && !beam &&
                          launch_gemm_mfma_qkv(ctx, L.qkv, tq, ntok, m->qkv, (size_t)(nq + 2 * nkv) * hd,
                                               QkvPostDev{L.bias, L.q_norm, L.k_norm, m->rope, c.rms_eps, m->pos_dev,
                                                          nq, nkv, l, m->ring, m->kq, m->vq, m->ks, m->vs});
@@ -461,16 +484,34 @@ void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0) {
         // One token: qkv_post's work runs inside the attention kernel.  A batch stores every
         // token's K / V first (a later token of the batch attends to them).
         AttnPost post{};
-        if (ntok == 1) {
+        if (beam) {
+            const size_t slots = (size_t)l * ntok * nkv * m->beam_cap;
+            k2t_kv_rows tail = kv_rows_at(m->beam_tail, m->ring.bits, hd, slots), prefix{};
+            launch_beam_post(st, m->qkv, L.bias, L.q_norm, L.k_norm, c.rms_eps, m->rope, m->beam_pos, beam->prefix, nq, nkv,
+                             hd, ntok, m->ring.bits, tail);
+            tail.len = beam->tail;
+            prefix.kq = m->kq;
+            prefix.ks = m->ks;
+            prefix.vq = m->vq;
+            prefix.vs = m->vs;
+            prefix = kv_rows_at(prefix, m->ring.bits, hd, (size_t)l * nkv * m->ring.cap);
+            prefix.cap = m->ring.cap;
+            prefix.len = beam->prefix;
+            launch_attn_shared(ctx, st, m->ring.bits, m->qkv, (size_t)(nq + 2 * nkv) * hd, SharedShape{1, ntok, nq, nkv, hd},
+                               prefix, tail, attn_scale, m->attn_f, m->beam_ws);
+            launch_act_quant(ctx, m->attn_f, nullptr, nullptr, nq * hd, ntok, m->xq, m->xs, m->xsum);
+        } else if (ntok == 1) {
             post = AttnPost{1, L.bias, L.q_norm, L.k_norm, m->rope, c.rms_eps};
         } else if (!qkv_posted) {
             launch_qkv_post(st, m->qkv, L.bias, L.q_norm, L.k_norm, c.rms_eps, m->rope, m->pos_dev, nq, nkv, hd, ntok,
                             l, m->ring, m->kq, m->vq, m->ks, m->vs, false);
         }
-        const ActTiles to = act_tiles_for(m, L.o, ntok);  // (none for one token: the grouped kernel writes none)
-        launch_attention(st, m->qkv, (nq + 2 * nkv) * hd, m->kq, m->vq, m->ks, m->vs, post, m->pos_dev, l, nq, nkv,
-                         hd, m->ring, attn_scale, nsplit, ntok, m->attn_part, nullptr, m->xq, m->xs, m->xsum,
-                         SpanWork{m->attn_words, m->attn_cnt, m->err_dev, ctx->num_cus}, ctx_bound, to, ctx->mfma != 0);
+        // (none for one token: the grouped kernel writes none)
+        const ActTiles to = beam ? ActTiles{} : act_tiles_for(m, L.o, ntok);
+        if (!beam)
+            launch_attention(st, m->qkv, (nq + 2 * nkv) * hd, m->kq, m->vq, m->ks, m->vs, post, m->pos_dev, l, nq, nkv,
+                             hd, m->ring, attn_scale, nsplit, ntok, m->attn_part, nullptr, m->xq, m->xs, m->xsum,
+                             SpanWork{m->attn_words, m->attn_cnt, m->err_dev, ctx->num_cus}, ctx_bound, to, ctx->mfma != 0);
         launch_gemv_ex(ctx, L.o, m->xq, m->xs, m->xsum, ntok, m->hidden, d, true, 0, to);
         if (L.has_moe) {
             // each token has its own routes (forward_layer_single); a batch groups its tokens
@@ -504,6 +545,12 @@ void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0) {
                 launch_gemv_ex(ctx, L.down, m->xq, m->xs, m->xsum, ntok, m->hidden, d, true, 0, td);
             }
         }
+    }
+    if (beam) {
+        launch_rmsnorm_act(st, ctx->signs, m->hidden, m->final_norm, c.rms_eps, d, ntok, m->xq, m->xs, m->xsum);
+        launch_gemv_ex(ctx, m->head, m->xq, m->xs, m->xsum, ntok, m->beam_logits, c.vocab, false);
+        launch_advance_pos(st, m->beam_pos, 1);
+        return;
     }
     if (with_logits) {
         const float *last = m->hidden + (size_t)(ntok - 1) * d;
@@ -774,6 +821,118 @@ void decode_step(k2t_model *m, bool pk, int token, int *next) {
     hip_check(hipGraphLaunch(m->graph, m->stream), "graph launch");
 }
 
+void free_beams(k2t_model *m) {
+    for (void *p : m->beam_allocs) (void)hipFree(p);
+    m->beam_allocs.clear();
+    m->beam_rows = m->beam_cap = 0;
+    m->beam_ws_bytes = 0;
+}
+
+// Buffers of a search over `rows` rows and n_steps choices, from `prefix` cached positions on.  They grow
+// (what is there is given back first) and stay with the model.
+void ensure_beams(k2t_model *m, int rows, int n_steps, int prefix) {
+    const k2t_model_config &c = m->cfg;
+    const SharedShape shape{1, rows, c.n_heads, c.n_kv_heads, c.head_dim};
+    size_t ws = std::max(beam_select_ws_bytes(1, rows, c.vocab, rows), beam_select_ws_bytes(1, 1, c.vocab, rows));
+    for (int t = 1; t < n_steps; t++) ws = std::max(ws, attn_shared_ws_bytes(m->ctx, shape, prefix, t));
+    if (rows == m->beam_rows && n_steps <= m->beam_cap && ws <= m->beam_ws_bytes) return;
+    hip_check(hipStreamSynchronize(m->stream), "beam workspace sync");
+    free_beams(m);
+    const auto get = [&](size_t bytes) {
+        void *p = nullptr;
+        const hipError_t e = hipMalloc(&p, bytes);
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            free_beams(m);
+            throw Error(K2T_E_NOMEM, std::string("hipMalloc failed: ") + hipGetErrorString(e));
+        }
+        m->beam_allocs.push_back(p);
+        return p;
+    };
+    const size_t slots = (size_t)c.n_layers * rows * c.n_kv_heads * n_steps;
+    m->beam_tail = k2t_kv_rows{};
+    m->beam_tail.kq = get(slots * c.head_dim);
+    m->beam_tail.vq = get(slots * c.head_dim);
+    m->beam_tail.ks = get(slots * sizeof(float));
+    m->beam_tail.vs = get(slots * sizeof(float));
+    m->beam_tail.cap = n_steps;
+    m->beam_logits = (float *)get((size_t)rows * c.vocab * sizeof(float));
+    m->beam_scores = (float *)get((size_t)rows * sizeof(float));
+    m->beam_done = (int *)get((size_t)rows * sizeof(int));
+    m->beam_pos = (int *)get(sizeof(int));
+    m->beam_tokens = (int *)get((size_t)n_steps * rows * sizeof(int));
+    m->beam_parents = (int *)get((size_t)n_steps * rows * sizeof(int));
+    m->beam_ws = get(ws);
+    m->beam_ws_bytes = ws;
+    m->beam_rows = rows;
+    m->beam_cap = n_steps;
+}
+
+// The search: the model's step for first_token, then a choice per step over the rows.  Returns the
+// choices (token and parent row of every step), the last scores and the rows' done flags.
+void beam_search(k2t_model *m, int first_token, int rows, int n_steps, int eos, std::vector<int> &tokens,
+                 std::vector<int> &parents, std::vector<float> &scores) {
+    const k2t_model_config &c = m->cfg;
+    hipStream_t st = m->stream;
+    const int prefix = m->pos + 1, bits = m->ring.bits;
+    ensure_beams(m, rows, n_steps, prefix);
+    decode_step(m, persistent_at(m, m->pos), first_token, nullptr);
+    StreamSwap sw(m);
+    launch_store_int(st, m->beam_pos, prefix);
+    hip_check(hipMemsetAsync(m->beam_scores, 0, sizeof(float), st), "score clear");
+    hip_check(hipMemsetAsync(m->beam_done, 0, sizeof(int), st), "done clear");
+    int *done = eos >= 0 ? m->beam_done : nullptr;
+    launch_beam_select(st, m->logits, c.vocab, c.vocab, m->beam_scores, done, 1, 1, rows, eos, m->beam_scores,
+                       m->beam_tokens, m->beam_parents, done, m->beam_ws);
+    for (int t = 1; t < n_steps; t++) {
+        int *tok = m->beam_tokens + (size_t)t * rows, *par = m->beam_parents + (size_t)t * rows;
+        const BeamStep step{tok - rows, prefix, t};
+        forward(m, rows, true, 0, &step);
+        launch_beam_select(st, m->beam_logits, c.vocab, c.vocab, m->beam_scores, done, 1, rows, rows, eos, m->beam_scores,
+                           tok, par, done, m->beam_ws);
+        k2t_kv_rows tail = m->beam_tail;
+        tail.len = t;
+        if (rows > 1) launch_kv_reorder(st, bits, tail, par, c.n_layers, 1, rows, c.n_kv_heads, c.head_dim);
+    }
+    const size_t n = (size_t)n_steps * rows;
+    tokens.resize(n);
+    parents.resize(n);
+    scores.resize(rows);
+    hip_check(hipMemcpyAsync(tokens.data(), m->beam_tokens, n * sizeof(int), hipMemcpyDeviceToHost, st), "tokens download");
+    hip_check(hipMemcpyAsync(parents.data(), m->beam_parents, n * sizeof(int), hipMemcpyDeviceToHost, st), "parents download");
+    hip_check(hipMemcpyAsync(scores.data(), m->beam_scores, rows * sizeof(float), hipMemcpyDeviceToHost, st),
+              "scores download");
+    hip_check(hipStreamSynchronize(st), "sync");
+}
+
+// The first `n` tail positions of row 0 (the best one) join the model's cache behind `prefix`.
+void adopt_best(k2t_model *m, int prefix, int n) {
+    const k2t_model_config &c = m->cfg;
+    const int bits = m->ring.bits, hd = c.head_dim;
+    const size_t code = bits == 8 ? hd : hd / 2, scale = bits == 8 ? 4 : hd / 32;
+    for (int l = 0; l < c.n_layers && n > 0; l++) {
+        const k2t_kv_rows from = kv_rows_at(m->beam_tail, bits, hd, (size_t)l * m->beam_rows * c.n_kv_heads * m->beam_cap);
+        k2t_kv_rows to{};
+        to.kq = m->kq;
+        to.ks = m->ks;
+        to.vq = m->vq;
+        to.vs = m->vs;
+        to = kv_rows_at(to, bits, hd, (size_t)l * c.n_kv_heads * m->ring.cap + prefix);
+        const auto copy = [&](void *dst, const void *src, size_t slot) {
+            hip_check(hipMemcpy2DAsync(dst, m->ring.cap * slot, src, m->beam_cap * slot, n * slot, c.n_kv_heads,
+                                       hipMemcpyDeviceToDevice, m->stream),
+                      "tail copy");
+        };
+        copy(to.kq, from.kq, code);
+        copy(to.vq, from.vq, code);
+        copy(to.ks, from.ks, scale);
+        copy(to.vs, from.vs, scale);
+    }
+    launch_store_int(m->stream, m->pos_dev, prefix + n);
+    hip_check(hipStreamSynchronize(m->stream), "sync");
+    m->pos = prefix + n;
+}
+
 }  // namespace
 
 namespace k2t {
@@ -878,6 +1037,7 @@ void k2t_model_destroy(k2t_model *m) {
     if (m->stream) (void)hipStreamSynchronize(m->stream);
     if (m->graph) (void)hipGraphExecDestroy(m->graph);
     for (void *p : m->allocs) (void)hipFree(p);
+    free_beams(m);
     for (k2t_mat *x : m->owned) k2t_mat_destroy(x);
     if (m->stream) (void)hipStreamDestroy(m->stream);
     delete m;
@@ -1262,6 +1422,40 @@ int32_t k2t_model_generate(k2t_model *m, int32_t first_token, int32_t n_steps, i
             (void)hipFree(dev_out);
             m->allocs.pop_back();
         }
+        check_mk_error(m);
+    });
+}
+
+int32_t k2t_model_beam_search(k2t_model *m, int32_t first_token, int32_t n_beams, int32_t n_steps, int32_t eos,
+                              int32_t *tokens_out, float *scores_out) {
+    return mguard([&] {
+        arg(m && tokens_out && scores_out, "NULL argument");
+        check_ready(m);
+        arg(n_beams >= 1 && n_beams <= kMaxBeams, "n_beams must be 1 .. 64");
+        arg(n_beams <= m->max_batch, "more beams than the model's max batch");
+        arg(n_steps >= 1, "n_steps < 1");
+        arg(m->cfg.vocab <= kMaxSelectVocab, "beam search takes vocabularies up to 262144");
+        arg(eos >= -1 && eos < m->cfg.vocab, "eos must be -1 (none) or a token");
+        arg(first_token >= 0 && first_token < m->cfg.vocab, "token out of range");
+        arg(n_steps <= m->cfg.max_seq - m->pos, "generation exceeds max_seq");
+        arg(!m->exact, "beam search runs in fast mode only");
+        arg(m->ring.window == 0, "beam search needs the full KV cache (no sliding window)");
+        hip_check(hipSetDevice(m->ctx->device), "hipSetDevice");
+        std::vector<int> tokens, parents;
+        std::vector<float> scores;
+        const int prefix = m->pos + 1;
+        beam_search(m, first_token, n_beams, n_steps, eos, tokens, parents, scores);
+        for (int b = 0; b < n_beams; b++) {
+            scores_out[b] = scores[b];
+            for (int t = n_steps - 1, row = b; t >= 0; t--) {
+                tokens_out[(size_t)b * n_steps + t] = tokens[(size_t)t * n_beams + row];
+                row = parents[(size_t)t * n_beams + row];
+            }
+        }
+        int fed = n_steps - 1;  // what generate feeds: all but the last token, and nothing from an eos on
+        for (int t = 0; t < fed && eos >= 0; t++)
+            if (tokens_out[t] == eos) fed = t;
+        adopt_best(m, prefix, fed);
         check_mk_error(m);
     });
 }

@@ -215,6 +215,32 @@ __global__ __launch_bounds__(256) void kv_load_kernel(RowsArgs A) {
     }
 }
 
+// A step's qkv rows of the engine's beam search: qkv_post_kernel with every row at position *pos_dev and
+// K / V into the row's tail, at position *pos_dev - pos0.
+__global__ __launch_bounds__(64) void beam_post_kernel(float *__restrict__ qkv, const float *__restrict__ bias,
+                                                       const float *__restrict__ qn, const float *__restrict__ kn,
+                                                       float eps, const float *__restrict__ rope,
+                                                       const int *__restrict__ pos_dev, int pos0, int nq, int nkv, int hd,
+                                                       int bits, k2t_kv_rows tail) {
+    const uint32_t lane = threadIdx.x;
+    const int head = blockIdx.x, row = blockIdx.y, nb = hd / 64, pos = pos_dev[0];
+    float *h = qkv + ((size_t)row * (nq + 2 * nkv) + head) * hd;
+    float v0, v1;
+    head_post(h, head, nq, nkv, hd, bias, qn, kn, eps, rope, pos, lane, v0, v1);
+    if (head < nq) {
+        h[lane] = v0;
+        if (nb > 1) h[64 + lane] = v1;
+        return;
+    }
+    const bool is_k = head < nq + nkv;
+    const int kvh = is_k ? head - nq : head - nq - nkv, t = pos - pos0;
+    if (t < 0 || t >= tail.cap) return;
+    const float r0 = fwht_lane(v0, 0, lane);
+    const float r1 = nb > 1 ? fwht_lane(v1, 1, lane) : 0.0f;
+    kv_store_head(r0, r1, nb, lane, bits, hd, ((size_t)row * nkv + kvh) * tail.cap + t,
+                  (int8_t *)(is_k ? tail.kq : tail.vq), (float *)(is_k ? tail.ks : tail.vs));
+}
+
 // Rows of one (layer, sequence, KV head, K or V) rearranged in place.  A thread owns one column (the
 // same T-sized piece of every row): it reads the column of every row that moves from its source row
 // before it writes any, so no other thread or buffer is involved.
@@ -348,6 +374,14 @@ void launch_kv_append(hipStream_t st, int bits, const float *k, const float *v, 
     A.k = k;
     A.v = v;
     launch_rows_of<false>(st, bits, hd, A, batch);
+}
+
+void launch_beam_post(hipStream_t st, float *qkv, const float *bias, const float *qn, const float *kn, float eps,
+                      const float *rope, const int *pos_dev, int pos0, int nq, int nkv, int hd, int rows, int bits,
+                      const k2t_kv_rows &tail) {
+    hipLaunchKernelGGL(beam_post_kernel, dim3(nq + 2 * nkv, rows), dim3(64), 0, st, qkv, bias, qn, kn, eps, rope, pos_dev,
+                       pos0, nq, nkv, hd, bits, tail);
+    hip_check(hipGetLastError(), "beam_post launch");
 }
 
 void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const int *parents, int n_layers, int n_seq,

@@ -84,6 +84,7 @@ SIGNATURES = {
     "k2t_model_decode": (I32, [VP, I32, VP]),
     "k2t_model_prefill": (I32, [VP, VP, I32, VP]),
     "k2t_model_generate": (I32, [VP, I32, I32, VP]),
+    "k2t_model_beam_search": (I32, [VP, I32, I32, I32, I32, VP, VP]),
     "k2t_model_logits": (I32, [VP, C.POINTER(VP)]),
     "k2t_model_sync": (I32, [VP]),
     "k2t_model_set_embedding": (I32, [VP, I32, VP, VP]),
@@ -653,6 +654,15 @@ class Model:
         check(lib().k2t_model_generate(self.h, int(first_token), int(n_steps),
                                        None if out is None else out.ctypes.data_as(VP)))
         return None if out is None else out[:n_steps]
+
+    def beam_search(self, first_token, n_beams, n_steps, eos=-1):
+        """k2t_model_beam_search: (tokens int32 [n_beams][n_steps], scores float32 [n_beams]), best first."""
+        import numpy as np
+        tokens = np.empty((max(n_beams, 1), max(n_steps, 1)), np.int32)
+        scores = np.empty(max(n_beams, 1), np.float32)
+        check(lib().k2t_model_beam_search(self.h, int(first_token), int(n_beams), int(n_steps), int(eos),
+                                          tokens.ctypes.data_as(VP), scores.ctypes.data_as(VP)))
+        return tokens, scores
 
     def sync(self):
         check(lib().k2t_model_sync(self.h))
