@@ -1,12 +1,20 @@
-// Beam search's choice over the rows of a sequence and the vocabulary (k2t_beam_select), in two
-// launches: every slice of 4096 logits leaves its maximum, its sum of exponentials and its k best,
-// sorted; one workgroup per sequence adds a row's slices up, merges their lists, and merges the rows'.
+// Beam search's choice over the rows of a sequence and the vocabulary (k2t_beam_select): the k largest of
+// score[r] + (x[r][t] - max x[r]) - log sum_t exp(x[r][t] - max x[r]), in two launches.  Every slice of 4096
+// logits leaves its maximum, its sum of exponentials and its k best, sorted; one workgroup per sequence
+// adds a row's slices up, and chooses among the entries of all rows' lists.
 //
 // A slice is read once into registers.  Its k best are among the elements that reach a bound: each of
-// the four waves finds the (k/4)-th largest of its 64 threads' maxima (bit by bit, counting lanes by
-// ballot), and at least k elements reach the smallest of the four; in random logits few more do.  They
-// are sorted by counting, for each, the larger ones.  Everything that orders is a unique key, so the
-// result depends on no timing.
+// the four waves finds a bound that k/4 of its 64 threads' maxima reach, and at least k elements reach
+// the smallest of the four; in random logits few more do.  They are sorted by counting, for each, the
+// larger ones.  Everything that orders is a unique key, so the result depends on no timing.
+//
+// What bounds it: the logits have to be read once (12.6 MB at 8 sequences of 8 rows of 49152: 2.4 us), but
+// both kernels take longer than their bytes, the first for its instructions (some 25 per logit on 3
+// waves per SIMD: 6.0 us there, 8.3 us before exp came down to one v_exp_f32 and keys were only made
+// for what reaches the bound), the second for chains of dependent steps on one CU (5.8 us there; 6.8 us
+// for 16 rows of 151936, k 32).  Both: 8.9 us for one sequence of 4 rows of 8192, 13.6 us and 15.6 us.
+// Slices of 4096 give 48 rows and up a workgroup per CU; the alternative of fewer, larger ones leaves
+// CUs idle in a single sequence.
 #include <float.h>
 #include <math.h>
 
@@ -39,21 +47,44 @@ struct SelArgs {
     const float *scores;
     const int *done;
     float2 *stat;              // [row][slice]: maximum, sum of exp(x - maximum)
-    unsigned long long *keys;  // [row][slice][k], best first, 0 behind the last
-    unsigned long long *far;   // [row][k], and tokens: a row's picks behind those that LDS holds
-    int *far_token;
+    unsigned long long *keys;  // [row][k][slice], best first, 0 behind the last
     float *o_scores;
     int *o_tokens, *o_parents, *o_done;
 };
 
-// The r-th largest of a wave's keys (`ord` the logit's order, 0 for none, `token` unique), as the
-// smallest key that reaches it; 0 where fewer than r lanes have one.
+// Largest of a wave's values (DPP row shifts and broadcasts: no LDS round trip), in every lane.
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+    const auto up = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false));  // row_shr:1
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false));  // row_shr:2
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false));  // row_shr:4
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false));  // row_shr:8
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));  // row_bcast:15
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast:31
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// Up to this many a bound is found maximum by maximum, beyond by bits: 10.2 us against 10.9 us for 4 rows
+// of 8192 (k 4: 1 and 2 maxima), 15.1 us against 15.5 us for 8 sequences (k 16: 1 of them here).
+constexpr int kFewMaxima = 3;
+
+// A bound that at least r of a wave's keys reach (`ord` the logit's order, 0 for none, `token` unique)
+// and hardly any other; 0 where fewer than r lanes have one.
 __device__ __forceinline__ unsigned long long wave_kth(uint32_t ord, uint32_t token, int r) {
     uint32_t t = 0;
+    if (r <= kFewMaxima) {  // maximum by maximum
+        while (true) {
+            t = wave_max_u(ord);
+            r -= __popcll(__ballot(ord == t));
+            if (r <= 0 || t == 0) return (unsigned long long)t << 32;
+            ord = ord == t ? 0 : ord;
+        }
+    }
 #pragma unroll
     for (int bit = 31; bit >= 0; bit--) {
         const uint32_t c = t | (1u << bit);
-        if (__popcll(__ballot(ord >= c)) >= r) t = c;
+        const int n = __popcll(__ballot(ord >= c));
+        if (n >= r) t = c;
+        if (n == r) return (unsigned long long)t << 32;  // (nearly always within a dozen bits)
     }
     if (t == 0) return 0;
     // equal logits at the bound: only the lowest tokens of them are needed
@@ -69,33 +100,50 @@ __device__ __forceinline__ unsigned long long wave_kth(uint32_t ord, uint32_t to
     return ((unsigned long long)t << 32) | (0xFFFFFFFFu - low);
 }
 
+// Position of this lane among the lanes that `yes`.
+__device__ __forceinline__ int lane_rank(unsigned long long yes) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(yes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)yes, 0u));
+}
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // (rows start at any float)
+
 // One slice of one row: its maximum, its sum of exponentials and its k best logits.
 __global__ __launch_bounds__(kSelThreads) void select_slice_kernel(SelArgs A) {
     constexpr int kSelWaves = kSelThreads / 64;
     __shared__ unsigned long long list[kSlice];
-    __shared__ unsigned long long bound[kSelWaves];
+    __shared__ unsigned long long wave_top[kSelWaves];
+    __shared__ uint32_t bound[kSelWaves];
     __shared__ float redf[2 * kSelWaves];
     __shared__ int count;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6;
     const int slice = blockIdx.x, row = blockIdx.y;
     const float *x = A.logits + (size_t)row * A.row_stride;
-    const uint32_t first = (uint32_t)slice * kSlice + tid;  // this thread's tokens: first + 256 j
+    // a thread's tokens: four in a row, 1024 apart; in a slice that the vocabulary ends in 256 apart, so
+    // that what there is goes to all threads
+    const bool whole = (slice + 1) * kSlice <= A.vocab;
+    const int first = slice * kSlice + (whole ? 4 : 1) * (int)tid, step = whole ? 1 : kSelThreads;
+    const auto token_of = [&](int i) { return first + i / 4 * (4 * kSelThreads) + i % 4 * step; };
     float v[kSelPer];
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < kSelPer; j++) v[j] = x[min((int)first + j * kSelThreads, A.vocab - 1)];
-    float mx = -INFINITY;
-    uint32_t at = 0;
-#pragma unroll
-    for (int j = 0; j < kSelPer; j++) {
-        const bool none = v[j] != v[j] || (int)first + j * kSelThreads >= A.vocab;
-        v[j] = none ? -INFINITY : fminf(v[j], FLT_MAX);
-        if (v[j] > mx) {  // (the lowest token of equal ones)
-            mx = v[j];
-            at = first + j * kSelThreads;
+        for (int j = 0; j < kSelPer; j += 4) {
+            const f32x4u w = *reinterpret_cast<const f32x4u *>(x + token_of(j));
+            for (int e = 0; e < 4; e++) v[j + e] = w[e];
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSelPer; i++) v[i] = x[min(token_of(i), A.vocab - 1)];
+#pragma unroll
+        for (int i = 0; i < kSelPer; i++) v[i] = token_of(i) < A.vocab ? v[i] : -INFINITY;
     }
-    const unsigned long long best = mx > -INFINITY ? logit_key(mx, at) : 0;
-    const unsigned long long kth = wave_kth((uint32_t)(best >> 32), at, (A.k + kSelWaves - 1) / kSelWaves);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kSelPer; i++) {
+        v[i] = fminf(fmaxf(v[i], -INFINITY), FLT_MAX);  // (the larger of NaN and -inf is -inf)
+        mx = fmaxf(mx, v[i]);
+    }
+    const uint32_t best = mx > -INFINITY ? (uint32_t)(logit_key(mx, 0) >> 32) : 0u;
+    const uint32_t kth = (uint32_t)(wave_kth(best, tid, (A.k + kSelWaves - 1) / kSelWaves) >> 32);
     mx = wave_max_f(mx);
     if (tid == 0) count = 0;
     if (lane == 0) {
@@ -103,52 +151,74 @@ __global__ __launch_bounds__(kSelThreads) void select_slice_kernel(SelArgs A) {
         redf[wv] = mx;
     }
     __syncthreads();
-    unsigned long long b = bound[0];
+    uint32_t least = bound[0];
     mx = redf[0];
 #pragma unroll
     for (int w = 1; w < kSelWaves; w++) {
-        b = bound[w] < b ? bound[w] : b;
+        least = min(least, bound[w]);
         mx = fmaxf(mx, redf[w]);
     }
+    // (a wave without enough maxima: every logit but -inf)
+    const float pass = least ? key_logit((unsigned long long)least << 32) : -FLT_MAX;
+    // exp by v_exp_f32: the product's rounding is 2^-24 of an exponent, which is small where the term is not
+    const float from = mx > -INFINITY ? mx : 0.0f;
     float sum = 0.0f;
+    unsigned long long yes[kSelPer];
+    int mine = 0;
 #pragma unroll
-    for (int j = 0; j < kSelPer; j++) {
-        if (v[j] == -INFINITY) continue;
-        sum += expf(v[j] - mx);
-        const unsigned long long key = logit_key(v[j], first + j * kSelThreads);
-        if (key >= b) list[atomicAdd(&count, 1)] = key;  // (their order does not matter: sorted below)
+    for (int i = 0; i < kSelPer; i++) {
+        sum += __builtin_amdgcn_exp2f((v[i] - from) * 1.4426950408889634f);
+        yes[i] = __ballot(v[i] >= pass);
+        mine += __popcll(yes[i]);
+    }
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&count, mine);  // (their order does not matter: sorted below)
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (int i = 0; i < kSelPer; i++) {
+        if (yes[i] == 0) continue;
+        if ((yes[i] >> lane) & 1) list[at + lane_rank(yes[i])] = logit_key(v[i], (uint32_t)token_of(i));
+        at += __popcll(yes[i]);
     }
     sum = wave_sum_f(sum);
     if (lane == 0) redf[kSelWaves + wv] = sum;
     __syncthreads();
-    const size_t out = (size_t)row * A.slices + slice;
     if (tid == 0) {
         sum = 0.0f;
         for (int w = 0; w < kSelWaves; w++) sum += redf[kSelWaves + w];
-        A.stat[out] = make_float2(mx, sum);
+        A.stat[(size_t)row * A.slices + slice] = make_float2(mx, sum);
     }
+    unsigned long long *keys = A.keys + (size_t)row * A.k * A.slices + slice;
     const int n = count;
-    for (int c = (int)tid; c < n; c += kSelThreads) {
-        const unsigned long long mine = list[c];
-        int rank = 0;
+    for (int c = n + (int)tid; c < A.k; c += kSelThreads) keys[(size_t)c * A.slices] = 0;
+    if (n <= kSlice / 4) {
+        for (int c = (int)tid; c < n; c += kSelThreads) {
+            const unsigned long long key = list[c];
+            int rank = 0;
 #pragma unroll 8
-        for (int i = 0; i < n; i++) rank += list[i] > mine ? 1 : 0;
-        if (rank < A.k) A.keys[out * A.k + rank] = mine;
+            for (int i = 0; i < n; i++) rank += list[i] > key ? 1 : 0;
+            if (rank < A.k) keys[(size_t)rank * A.slices] = key;
+        }
+        return;
     }
-    for (int c = n + (int)tid; c < A.k; c += kSelThreads) A.keys[out * A.k + c] = 0;
+    // equal logits by the hundred: one by one
+    unsigned long long last = ~0ull;
+    for (int r = 0; r < A.k; r++) {
+        unsigned long long top = 0;
+        for (int c = (int)tid; c < n; c += kSelThreads) top = list[c] < last && list[c] > top ? list[c] : top;
+        for (int m = 32; m >= 1; m >>= 1) {
+            const unsigned long long other = __shfl_xor(top, m, kWave);
+            top = other > top ? other : top;
+        }
+        if (lane == 0) wave_top[wv] = top;
+        __syncthreads();
+        last = wave_top[0];
+        for (int w = 1; w < kSelWaves; w++) last = wave_top[w] > last ? wave_top[w] : last;
+        if (tid == 0) keys[(size_t)r * A.slices] = last;
+        __syncthreads();
+    }
 }
 
-// Largest of a wave's values (DPP row shifts and broadcasts: no LDS round trip), in every lane.
-__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
-    const auto up = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false));  // row_shr:1
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false));  // row_shr:2
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false));  // row_shr:4
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false));  // row_shr:8
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));  // row_bcast:15
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast:31
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
 // The lane with the largest key (the lowest of equal ones); -1 where every key is 0.
 __device__ __forceinline__ int wave_best(unsigned long long key) {
     const uint32_t hi = (uint32_t)(key >> 32), top = wave_max_u(hi);
@@ -171,10 +241,9 @@ __device__ __forceinline__ double key_score(unsigned long long k) {
 }
 
 constexpr int kMergeWaves = 16;
-constexpr int kHeads = 8;       // entries of each list read at once
-constexpr int kListLds = 512;   // keys of a row that a wave can sort in LDS
-constexpr int kPickLds = 2048;  // picks of a sequence's rows that LDS holds
-constexpr int kPoolLds = 2048;  // picks that the last sort takes
+constexpr int kHeads = 8;      // entries of each list read at once
+constexpr int kCands = 14336;  // candidates of a sequence that LDS holds
+constexpr int kPool = 1024;    // candidates that the sort takes
 
 // Depth and count for a bound over `lists` sorted lists: `count` lists whose entry at `depth` reaches
 // the bound hold k entries that do.
@@ -182,192 +251,195 @@ struct Cut {
     int depth, count;
 };
 __device__ __forceinline__ Cut cut_of(int lists, int k) {
-    const int deep = min(k, (2 * k + lists - 1) / lists);
+    const int deep = min(k, (3 * k + 2 * lists - 1) / (2 * lists));  // (half as many again pass in random logits)
     return Cut{deep - 1, (k + deep - 1) / deep};
 }
-// Position of this lane among the lanes that `yes`, and their number.
-__device__ __forceinline__ int lane_rank(unsigned long long yes) {
-    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(yes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)yes, 0u));
+// A candidate of row b of the sequence: among equal scores the larger of these goes first (the lower
+// row, then the higher logit, then the lower token).
+__device__ __forceinline__ unsigned long long cand_of(int b, unsigned long long key) {
+    return ((unsigned long long)(kMaxBeams - 1 - b) << 50) | ((key >> 32) << 18) | (key & 0x3FFFFu);
 }
+__device__ __forceinline__ int cand_row(unsigned long long c) { return kMaxBeams - 1 - (int)(c >> 50); }
+__device__ __forceinline__ int cand_token(unsigned long long c) { return 0x3FFFF - (int)(c & 0x3FFFFu); }
+__device__ __forceinline__ float cand_logit(unsigned long long c) { return key_logit((c >> 18) << 32); }
 
-// One sequence.  Waves merge rows' lists, a list per lane: the entries that reach a bound (cut_of) are
-// sorted by counting the larger ones.  Other waves add up the rows' sums meanwhile.  Then the rows'
-// picks are merged, a row per lane, the same way.  Where more reach a bound than LDS holds (the best
-// logits all in a few slices) the lists are merged step by step: the lane with the largest head gives
-// the next one and moves on.
-// What bounds it is latency: a handful of dependent reads and counts, not bytes.
+// One sequence.  Waves go through rows' lists, a list per lane, for the entries that reach a bound
+// (cut_of), while other waves add up the rows' sums.  All rows' entries are then candidates like a
+// slice's elements: a bound from each wave's share of them, and those that reach the smallest are
+// sorted by counting the better ones, the counting shared out over the waves.  Where more reach a
+// row's bound than its share of LDS (the best logits all in a few slices) its k best are taken one by
+// one, and likewise the sequence's where more reach the last bound than the sort takes.
+// What bounds it is latency and the issue rate of one CU: no bytes to speak of.
 __global__ __launch_bounds__(64 * kMergeWaves) void select_merge_kernel(SelArgs A) {
-    __shared__ union {
-        unsigned long long list[kMergeWaves][kListLds];
-        struct {
-            unsigned long long key[kPoolLds];
-            uint32_t from[kPoolLds];  // row of the sequence << 8 | place among its picks
-        } pool;
-    } sh;
-    __shared__ unsigned long long pick[kPickLds];  // logit keys, then score keys
-    __shared__ int pick_token[kPickLds];
+    __shared__ unsigned long long cand[kCands];
+    __shared__ ulonglong2 pool[kPool];  // score key, candidate
+    __shared__ int pool_rank[kPool];
     __shared__ double row_lse[kMaxBeams];
     __shared__ float row_top[kMaxBeams], row_score[kMaxBeams];
-    __shared__ int picks[kMaxBeams], ended[kMaxBeams];
-    __shared__ int pool_n;
+    __shared__ int ended[kMaxBeams];
+    __shared__ uint32_t wave_bound[kMergeWaves];
+    __shared__ ulonglong2 wave_top[kMergeWaves];
+    __shared__ int cands, pool_n;
+    static_assert(kCands / kMaxBeams >= kMaxPicks, "every row's share holds its k best");
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const int seq = blockIdx.x, row0 = seq * A.beams, S = A.slices, k = A.k;
-    const int depth = min(k, kPickLds / A.beams);
+    const int share = kCands / A.beams;
     const bool mine = (int)lane < S;
+    if (tid == 0) cands = pool_n = 0;
+    __syncthreads();
     for (int task = wave; task < 2 * A.beams; task += kMergeWaves) {
         const int b = task < A.beams ? task : task - A.beams, row = row0 + b;
         const size_t base = (size_t)row * S;
         if (task >= A.beams) {
             const float2 st = mine ? A.stat[base + lane] : make_float2(-INFINITY, 0.0f);
-            const float score = A.scores[row];
             const float top = wave_max_f(st.x);
             // (in 64 bits: scores of different rows are told apart by the sum's last bits)
-            double sum = st.x > -INFINITY ? (double)st.y * exp((double)st.x - (double)top) : 0.0;
+            double sum = st.x > -INFINITY ? (double)st.y * (double)expf(st.x - top) : 0.0;
             for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, kWave);
             if (lane == 0) {
                 row_top[b] = top;
                 row_lse[b] = log(sum);
-                row_score[b] = score;
             }
             continue;
         }
-        const unsigned long long *list = A.keys + (base + min((int)lane, S - 1)) * k;
+        const unsigned long long *list = A.keys + base * k + min((int)lane, S - 1);  // its entry j: list[j * S]
         const Cut cut = cut_of(S, k);
         const float score = A.scores[row];
         const bool over = A.done && A.done[row] != 0;
-        unsigned long long deep = list[cut.depth];
+        unsigned long long deep = list[cut.depth * S];
         unsigned long long head[kHeads];  // (nearly always all that reaches the bound)
 #pragma unroll
-        for (int j = 0; j < kHeads; j++) head[j] = list[min(j, k - 1)];
+        for (int j = 0; j < kHeads; j++) head[j] = list[min(j, k - 1) * S];
 #pragma unroll
         for (int j = 0; j < kHeads; j++) head[j] = mine && j < k ? head[j] : 0;
         deep = mine ? deep : 0;
         const unsigned long long bound = wave_kth((uint32_t)(deep >> 32), key_token(deep), cut.count);
+        const auto reach = [&](unsigned long long key) { return __ballot(key != 0 && key >= bound); };
         int found = 0;
-        const auto keep = [&](unsigned long long key) {
-            const unsigned long long yes = __ballot(key != 0 && key >= bound);
-            const int at = found + lane_rank(yes);
-            if (((yes >> lane) & 1) && at < kListLds) sh.list[wave][at] = key;
-            found += __popcll(yes);
-            return yes != 0;
-        };
 #pragma unroll
-        for (int j = 0; j < kHeads; j++) keep(head[j]);
-        if (__ballot(head[kHeads - 1] != 0 && head[kHeads - 1] >= bound))
-            for (int j = kHeads; j < k; j++)
-                if (!keep(mine ? list[j] : 0)) break;
-        const auto put = [&](int n, unsigned long long key) {
-            if (n < depth) pick[b * depth + n] = key;
-            else A.far[(size_t)row * k + n] = key;
-        };
-        int n = min(found, k);
-        if (found <= kListLds) {
-            for (int c = (int)lane; c < found; c += 64) {
-                const unsigned long long key = sh.list[wave][c];
-                int rank = 0;
-#pragma unroll 8
-                for (int i = 0; i < found; i++) rank += sh.list[wave][i] > key ? 1 : 0;
-                if (rank < k) put(rank, key);
-            }
+        for (int j = 0; j < kHeads; j++) found += __popcll(reach(head[j]));
+        const bool longer = reach(head[kHeads - 1]) != 0;
+        for (int j = kHeads; longer && j < k; j++) {
+            const unsigned long long yes = reach(mine ? list[j * S] : 0);
+            found += __popcll(yes);
+            if (!yes) break;
+        }
+        int n = found <= share ? found : k;
+        if (!(score > -INFINITY)) n = 0;
+        else if (over) n = 1;
+        int at = 0;
+        if (lane == 0) {
+            at = atomicAdd(&cands, n);  // (their order does not matter)
+            row_score[b] = score;
+            ended[b] = over;
+        }
+        at = __builtin_amdgcn_readfirstlane(at);
+        if (n == 0) continue;
+        if (over) {
+            if (lane == 0) cand[at] = cand_of(b, logit_key(0.0f, (uint32_t)A.eos));
+        } else if (n == found) {
+            const auto keep = [&](unsigned long long key) {
+                const unsigned long long yes = reach(key);
+                if ((yes >> lane) & 1) cand[at + lane_rank(yes)] = cand_of(b, key);
+                at += __popcll(yes);
+                return yes != 0;
+            };
+#pragma unroll
+            for (int j = 0; j < kHeads; j++) keep(head[j]);
+            for (int j = kHeads; longer && j < k; j++)
+                if (!keep(mine ? list[j * S] : 0)) break;
         } else {
-            int at = 0;
+            int next = 0;
             unsigned long long cur = head[0];
-            for (n = 0; n < k; n++) {
-                const int who = wave_best(cur);
-                if (who < 0) break;
-                if ((int)lane == who) {
-                    put(n, cur);
-                    at++;
-                    cur = at < k ? list[at] : 0;
+            for (int i = 0; i < k; i++) {
+                if ((int)lane == wave_best(cur)) {
+                    cand[at + i] = cand_of(b, cur);
+                    next++;
+                    cur = next < k ? list[next * S] : 0;
                 }
             }
         }
-        if (!(score > -INFINITY)) n = 0;
-        else if (over) n = 1;
-        if (lane == 0) {
-            picks[b] = n;
-            ended[b] = over;
-        }
     }
     __syncthreads();
-    // logit keys to score keys (never 0) and tokens
-    const auto scored = [&](int b, unsigned long long key) {
+    const int total = cands;
+    const auto score_of = [&](unsigned long long c) {  // (never 0)
+        const int b = cand_row(c);
         if (ended[b]) return score_key((double)row_score[b]);
-        return score_key((double)row_score[b] + (((double)key_logit(key) - (double)row_top[b]) - row_lse[b]));
+        return score_key((double)row_score[b] + (((double)cand_logit(c) - (double)row_top[b]) - row_lse[b]));
     };
-    for (int i = (int)tid; i < A.beams * k; i += 64 * kMergeWaves) {
-        const int b = i / k, n = i % k;
-        if (n >= picks[b]) continue;
-        if (n < depth) {
-            const unsigned long long key = pick[b * depth + n];
-            pick[b * depth + n] = scored(b, key);
-            pick_token[b * depth + n] = ended[b] ? A.eos : (int)key_token(key);
-        } else {
-            const size_t at = (size_t)(row0 + b) * k + n;
-            const unsigned long long key = A.far[at];
-            A.far[at] = scored(b, key);
-            A.far_token[at] = (int)key_token(key);
-        }
-    }
-    __syncthreads();
-    const auto score_at = [&](int b, int i) {
-        if (i < depth) return ld_lds(&pick[b * depth + i]);
-        return ld_global(A.far + (size_t)(row0 + b) * k + i);
-    };
-    const auto give = [&](int n, unsigned long long key, int b, int i) {
-        const int token = i < depth ? ld_lds(&pick_token[b * depth + i]) : ld_global(A.far_token + (size_t)(row0 + b) * k + i);
+    const auto give = [&](int n, unsigned long long score, unsigned long long c) {
         const size_t out = (size_t)seq * k + n;
-        A.o_scores[out] = (float)key_score(key);
+        const int b = cand_row(c), token = cand_token(c);
+        A.o_scores[out] = (float)key_score(score);
         A.o_tokens[out] = token;
         A.o_parents[out] = row0 + b;
         if (A.o_done) A.o_done[out] = ended[b] || token == A.eos;
     };
-    if (wave == 0) {
-        const int held = (int)lane < A.beams ? picks[lane] : 0;
-        const Cut cut = cut_of(A.beams, k);
-        // (a bound on the upper half of the key: a few more pass)
-        const uint32_t deep = cut.depth < held ? (uint32_t)(score_at((int)lane, cut.depth) >> 32) : 0u;
-        const unsigned long long bound = wave_kth(deep, lane, cut.count) & 0xFFFFFFFF00000000ull;
-        int found = 0;
-        for (int j = 0; j < k; j++) {
-            const unsigned long long key = j < held ? score_at((int)lane, j) : 0;
-            const unsigned long long yes = __ballot(key != 0 && key >= bound);
-            if (!yes) break;
-            const int at = found + lane_rank(yes);
-            if (((yes >> lane) & 1) && at < kPoolLds) {
-                sh.pool.key[at] = key;
-                sh.pool.from[at] = (lane << 8) | (uint32_t)j;
-            }
-            found += __popcll(yes);
-        }
-        if (lane == 0) pool_n = found;
-        if (found > kPoolLds) {
-            int at = 0;
-            unsigned long long key = held > 0 ? score_at((int)lane, 0) : 0;
-            for (int n = 0; n < k; n++) {
-                const int who = wave_best(key);  // (equal scores: the lower lane, so the lower row)
-                if (who < 0) break;
-                if ((int)lane == who) {
-                    give(n, key, who, at);
-                    at++;
-                    key = at < held ? score_at(who, at) : 0;
-                }
-            }
-        }
+    // Every wave's share has some of every row's; (rotated: not all lanes on one bank)
+    const int first = (int)(lane * kMergeWaves + ((lane + (uint32_t)wave) & (kMergeWaves - 1)));
+    unsigned long long c0 = 0, s0 = 0;
+    if (first < total) {
+        c0 = cand[first];
+        s0 = score_of(c0);
     }
+    uint32_t best = (uint32_t)(s0 >> 32);
+    for (int i = first + 64 * kMergeWaves; i < total; i += 64 * kMergeWaves)
+        best = max(best, (uint32_t)(score_of(cand[i]) >> 32));
+    const unsigned long long reached = wave_kth(best, lane, (k + kMergeWaves - 1) / kMergeWaves);
+    if (lane == 0) wave_bound[wave] = (uint32_t)(reached >> 32);
+    __syncthreads();
+    uint32_t bound = wave_bound[0];
+#pragma unroll
+    for (int w = 1; w < kMergeWaves; w++) bound = min(bound, wave_bound[w]);
+    const auto enter = [&](unsigned long long score, unsigned long long c) {
+        if ((uint32_t)(score >> 32) < bound) return;
+        const int at = atomicAdd(&pool_n, 1);  // (their order does not matter: sorted below)
+        if (at >= kPool) return;
+        pool[at] = make_ulonglong2(score, c);
+        pool_rank[at] = 0;
+    };
+    if (first < total) enter(s0, c0);
+    for (int i = first + 64 * kMergeWaves; i < total; i += 64 * kMergeWaves) enter(score_of(cand[i]), cand[i]);
     __syncthreads();
     const int found = pool_n;
-    if (found > kPoolLds) return;  // (more than k: no place was left over)
-    for (int c = (int)tid; c < found; c += 64 * kMergeWaves) {
-        const unsigned long long key = sh.pool.key[c];
-        const uint32_t from = sh.pool.from[c];
-        int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < found; i++)
-            rank += sh.pool.key[i] > key || (sh.pool.key[i] == key && sh.pool.from[i] < from) ? 1 : 0;
-        if (rank < k) give(rank, key, (int)(from >> 8), (int)(from & 255u));
+    const auto before = [](ulonglong2 x, ulonglong2 y) {
+        return (int)(x.x > y.x) | ((int)(x.x == y.x) & (int)(x.y > y.y));
+    };
+    if (found > kPool) {
+        ulonglong2 last = make_ulonglong2(~0ull, ~0ull);
+        for (int n = 0; n < k; n++) {  // (k are there)
+            ulonglong2 top = make_ulonglong2(0, 0);
+            for (int i = (int)tid; i < total; i += 64 * kMergeWaves) {
+                const ulonglong2 x = make_ulonglong2(score_of(cand[i]), cand[i]);
+                if (before(last, x) && before(x, top)) top = x;
+            }
+            for (int m = 32; m >= 1; m >>= 1) {
+                const ulonglong2 x = make_ulonglong2(__shfl_xor(top.x, m, kWave), __shfl_xor(top.y, m, kWave));
+                if (before(x, top)) top = x;
+            }
+            if (lane == 0) wave_top[wave] = top;
+            __syncthreads();
+            last = wave_top[0];
+            for (int w = 1; w < kMergeWaves; w++)
+                if (before(wave_top[w], last)) last = wave_top[w];
+            if (tid == 0) give(n, last.x, last.y);
+            __syncthreads();
+        }
+        return;
     }
+    // a lane per candidate, the others to compare with shared out over the waves
+    const int part = (found + kMergeWaves - 1) / kMergeWaves, lo = wave * part, hi = min(lo + part, found);
+    for (int c = (int)lane; c < found; c += 64) {
+        const ulonglong2 me = pool[c];
+        int rank = 0;
+#pragma unroll 4
+        for (int i = lo; i < hi; i++) rank += before(pool[i], me);
+        if (rank) atomicAdd(&pool_rank[c], rank);
+    }
+    __syncthreads();
+    for (int c = (int)tid; c < found; c += 64 * kMergeWaves)
+        if (pool_rank[c] < k) give(pool_rank[c], pool[c].x, pool[c].y);
     for (int n = found + (int)tid; n < k; n += 64 * kMergeWaves) {
         const size_t out = (size_t)seq * k + n;
         A.o_scores[out] = -INFINITY;
@@ -392,19 +464,17 @@ void check_select(k2t_ctx *ctx, int n_seq, int beams, int vocab, int k) {
 
 size_t beam_select_ws_bytes(int n_seq, int beams, int vocab, int k) {
     const size_t lists = (size_t)n_seq * beams * slices_of(vocab);
-    return lists * (sizeof(float2) + (size_t)k * sizeof(unsigned long long)) + (size_t)n_seq * beams * k * 12 + 16;
+    return lists * (sizeof(float2) + (size_t)k * sizeof(unsigned long long)) + 16;
 }
 
 void launch_beam_select(hipStream_t st, const float *logits, int vocab, size_t row_stride, const float *scores,
                         const int *done, int n_seq, int beams, int k, int eos, float *out_scores, int *out_tokens,
                         int *out_parents, int *out_done, void *ws) {
-    SelArgs A{logits, row_stride, vocab, slices_of(vocab), beams, k, eos, scores, done, nullptr, nullptr, nullptr, nullptr,
+    SelArgs A{logits, row_stride, vocab, slices_of(vocab), beams, k, eos, scores, done, nullptr, nullptr,
               out_scores, out_tokens, out_parents, out_done};
     const size_t lists = (size_t)n_seq * beams * A.slices;
     A.stat = (float2 *)ws;
     A.keys = (unsigned long long *)(A.stat + lists);
-    A.far = A.keys + lists * k;
-    A.far_token = (int *)(A.far + (size_t)n_seq * beams * k);
     hipLaunchKernelGGL(select_slice_kernel, dim3(A.slices, n_seq * beams), dim3(kSelThreads), 0, st, A);
     hip_check(hipGetLastError(), "beam_select launch");
     hipLaunchKernelGGL(select_merge_kernel, dim3(n_seq), dim3(64 * kMergeWaves), 0, st, A);
