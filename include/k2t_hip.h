@@ -416,7 +416,12 @@ int32_t k2t_attn_decode_noalloc(k2t_ctx *ctx, int32_t bits, const float *d_q, in
  * (row * n_kv_heads + head) * cap + position; kq / vq: int8 [slot][hd] or NF4 nibbles
  * [slot][hd/2], 16-byte aligned; ks / vs: f32 [slot] or BF16 [slot][hd/64], aligned to one
  * slot's scales.  len: no row holds more positions (0 .. cap); d_len: a device int32 per row
- * with what it holds, read when the kernels run and taken as within 0 .. len, or NULL: len. */
+ * with what it holds, read when the kernels run and taken as within 0 .. len, or NULL: len.
+ * cap <= 2^24.
+ *
+ * All of these calls run on the context's stream, allocate nothing, do not synchronise, and may be
+ * captured into a graph, which then reads positions, counts, lengths, parents and scores at every
+ * replay.  head_dim is 64 or 128.  Buffers of one call do not overlap unless a comment says so. */
 typedef struct k2t_kv_rows {
     void *kq, *ks, *vq, *vs;
     const int32_t *d_len;
@@ -427,7 +432,9 @@ typedef struct k2t_kv_rows {
  * of row b is d_k + (b * ntok + t) * row_stride floats, n_kv_heads post-RoPE heads back to back
  * (d_v likewise: both may point into qkv rows), and goes to position d_pos[b] + t.  d_counts
  * (nullable): row b has min(ntok, d_counts[b]) tokens.  Positions outside 0 .. cap - 1 are not
- * written; nothing else in the cache changes.  kv->len and d_len are not used. */
+ * written; nothing else in the cache changes.  kv->len and d_len are not used.  d_k and d_v are
+ * 16-byte aligned, row_stride a multiple of 4; batch <= 65535, n_kv_heads <= 1024, and
+ * batch * ntok * n_kv_heads <= 2^24. */
 int32_t k2t_kv_append(k2t_ctx *ctx, int32_t bits, const float *d_k, const float *d_v, size_t row_stride,
                       int32_t batch, int32_t ntok, int32_t n_kv_heads, int32_t head_dim, const int32_t *d_pos,
                       const int32_t *d_counts, const k2t_kv_rows *kv);
@@ -440,16 +447,18 @@ int32_t k2t_kv_load(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, int32_t b
  * below its source's length from row d_parents[r], all rows at once; positions at or behind that
  * length keep their bytes, and lengths (kv->d_len) are not changed.  The cache holds n_layers
  * blocks of n_seq * beams rows; a parent outside its row's sequence leaves the row as it was.
- * beams <= 64. */
+ * beams <= 64, n_kv_heads <= 1024, n_layers * n_seq * n_kv_heads <= 2^22, len * head_dim <= 2^26. */
 int32_t k2t_kv_reorder(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const int32_t *d_parents,
                        int32_t n_layers, int32_t n_seq, int32_t beams, int32_t n_kv_heads, int32_t head_dim);
 /* Attention of one token of every row: k2t_attn_decode (int8 queries, same scores and softmax)
  * over its sequence's prefix rows followed by its own tail.  d_q: row r's n_heads post-RoPE
  * query heads at d_q + r * q_stride floats; prefix: a cache of n_seq rows, tail: of n_seq * beams
  * rows (either may be NULL); d_out [n_seq * beams][n_heads][hd].  A row with no positions gets
- * zeros.  d_ws: device workspace of at least k2t_attn_shared_workspace bytes, 16-byte aligned,
- * of this call alone while it runs; it needs no initial value.  Allocates nothing, asynchronous,
- * and may be captured (the lengths are read at every replay). */
+ * zeros; infinities and NaN of one row's query or tail stay in that row.  attn_scale is finite and
+ * not negative.  d_ws: device workspace of at least k2t_attn_shared_workspace bytes, of this call
+ * alone while it runs (two graphs that may run at once need one each); it needs no initial value.
+ * d_q, d_out and d_ws are 16-byte aligned, q_stride a multiple of 4; n_heads <= 1024,
+ * n_seq * beams <= 65535, n_seq * beams * n_heads <= 2^22. */
 int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_stride, int32_t n_seq, int32_t beams,
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const k2t_kv_rows *prefix,
                         const k2t_kv_rows *tail, float attn_scale, float *d_out, void *d_ws, size_t ws_bytes);
@@ -465,8 +474,9 @@ int32_t k2t_attn_shared_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, in
  * then the higher logit, then the lower token.  d_out_* [n_seq][k]: score, token, row of the
  * batch (what k2t_kv_reorder takes), and (nullable) done = the row had ended or token == eos
  * (eos -1: none).  Where a sequence has fewer candidates the rest get score -inf, token max(eos,
- * 0), its first row, and done 1.  With k == beams the outputs may be the input scores and done
- * flags.  vocab <= 262144, beams <= 64, k <= 128.  d_ws as in k2t_attn_shared. */
+ * 0), its first row, and done 1.  With k == beams the output scores and done flags may be the
+ * inputs themselves.  vocab <= 262144, beams <= 64, k <= 128, n_seq * beams <= 65535.  d_ws as in
+ * k2t_attn_shared, k2t_beam_select_workspace bytes. */
 int32_t k2t_beam_select(k2t_ctx *ctx, const float *d_logits, int32_t vocab, size_t row_stride, const float *d_scores,
                         const int32_t *d_done, int32_t n_seq, int32_t beams, int32_t k, int32_t eos,
                         float *d_out_scores, int32_t *d_out_tokens, int32_t *d_out_parents, int32_t *d_out_done,

@@ -843,6 +843,7 @@ SharedShape shared_shape(k2t_ctx *ctx, int n_seq, int beams, int nq, int nkv, in
     branch_arg(hd == 64 || hd == 128, "head_dim must be 64 or 128");
     branch_arg(nq > 0 && nkv > 0 && nq % nkv == 0 && nq <= 1024, "n_heads must be a multiple of n_kv_heads, at most 1024");
     branch_arg(n_seq >= 0 && beams >= 1 && (size_t)n_seq * beams <= 65535, "n_seq * beams must be 0 .. 65535, beams >= 1");
+    branch_arg((size_t)n_seq * beams * nq <= (size_t)1 << 22, "more than 2^22 query heads in one call");
     return SharedShape{n_seq, beams, nq, nkv, hd};
 }
 }  // namespace
@@ -866,6 +867,8 @@ int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
     return branch_guard([&] {
         const SharedShape s = shared_shape(ctx, n_seq, beams, n_heads, n_kv_heads, head_dim);
         branch_arg(prefix || tail, "neither a prefix nor a tail");
+        // (the running maximum takes the largest dot product for the largest score)
+        branch_arg(attn_scale >= 0.0f && attn_scale <= FLT_MAX, "attn_scale must be finite and not negative");
         for (const k2t_kv_rows *kv : {prefix, tail})
             if (kv) check_kv_rows(kv, bits, head_dim);
         if (n_seq == 0) return;

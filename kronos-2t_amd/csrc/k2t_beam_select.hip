@@ -508,6 +508,8 @@ int32_t k2t_beam_select(k2t_ctx *ctx, const float *d_logits, int32_t vocab, size
         if (n_seq == 0) return;
         branch_arg(d_logits && d_scores && d_out_scores && d_out_tokens && d_out_parents && d_ws, "NULL argument");
         branch_arg(reinterpret_cast<uintptr_t>(d_ws) % 16 == 0, "d_ws must be 16-byte aligned");
+        branch_arg(k == beams || (d_out_scores != d_scores && (!d_done || d_out_done != d_done)),
+                   "scores and done flags may be replaced in place only where k == beams");
         const size_t need = beam_select_ws_bytes(n_seq, beams, vocab, k);
         if (ws_bytes < need)
             throw Error(K2T_E_ARG, "the workspace holds " + std::to_string(ws_bytes) + " bytes, " +

@@ -35,10 +35,6 @@ int32_t branch_guard(F &&fn) {
 // Checks of a batched cache (k2t_kv_rows) that is read or written with wide accesses.
 void check_kv_rows(const k2t_kv_rows *kv, int bits, int hd);
 
-// d_k / d_v rows (row_stride floats per token) into the positions pos[row] + t of a batched cache,
-// and back.  `layer` blocks of batch rows lie one behind the other in the cache.
-void launch_kv_append(hipStream_t st, int bits, const float *k, const float *v, size_t row_stride, int batch, int ntok,
-                      int nkv, int hd, const int *pos, const int *counts, const k2t_kv_rows &kv, int layer);
 void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const int *parents, int n_layers, int n_seq,
                        int beams, int nkv, int hd);
 

@@ -1438,6 +1438,7 @@ int32_t k2t_model_beam_search(k2t_model *m, int32_t first_token, int32_t n_beams
         arg(eos >= -1 && eos < m->cfg.vocab, "eos must be -1 (none) or a token");
         arg(first_token >= 0 && first_token < m->cfg.vocab, "token out of range");
         arg(n_steps <= m->cfg.max_seq - m->pos, "generation exceeds max_seq");
+        arg((size_t)n_steps * m->cfg.head_dim <= (size_t)1 << 26, "too many steps");  // (launch_kv_reorder's grid)
         arg(!m->exact, "beam search runs in fast mode only");
         arg(m->ring.window == 0, "beam search needs the full KV cache (no sliding window)");
         hip_check(hipSetDevice(m->ctx->device), "hipSetDevice");

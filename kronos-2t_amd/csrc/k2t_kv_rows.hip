@@ -20,7 +20,6 @@ struct RowsArgs {
     int ntok, nkv;
     const int *pos, *counts;
     k2t_kv_rows kv;
-    size_t row0;  // first cache row
     uint32_t units;  // 64-blocks of a row's tokens: ntok * 2 * nkv * (hd / 64)
 };
 
@@ -43,7 +42,7 @@ __device__ __forceinline__ bool block_at(const RowsArgs &A, uint32_t u, BlockAt 
     const uint32_t head = h.is_v ? hv - A.nkv : hv;
     const long long p = (long long)A.pos[row] + t;
     h.in = ((size_t)row * A.ntok + t) * A.row_stride + (size_t)head * (64 * NB) + 64 * h.b;
-    h.slot = ((A.row0 + row) * A.nkv + head) * (size_t)A.kv.cap + (size_t)p;
+    h.slot = ((size_t)row * A.nkv + head) * (size_t)A.kv.cap + (size_t)p;
     return u < A.units && (!A.counts || (int)t < A.counts[row]) && p >= 0 && p < A.kv.cap;
 }
 
@@ -299,8 +298,7 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs A) {
         move_column<uint16_t, NB>((uint16_t *)s + slot0 + pos, slots, par, A.beams, lens, pos);
 }
 
-RowsArgs rows_args(const k2t_kv_rows &kv, size_t row_stride, int batch, int ntok, int nkv, int hd, const int *pos,
-                   const int *counts, int layer) {
+RowsArgs rows_args(const k2t_kv_rows &kv, size_t row_stride, int ntok, int nkv, int hd, const int *pos, const int *counts) {
     RowsArgs A{};
     A.row_stride = row_stride;
     A.ntok = ntok;
@@ -308,7 +306,6 @@ RowsArgs rows_args(const k2t_kv_rows &kv, size_t row_stride, int batch, int ntok
     A.pos = pos;
     A.counts = counts;
     A.kv = kv;
-    A.row0 = (size_t)layer * batch;
     A.units = (uint32_t)((size_t)ntok * 2 * nkv * (hd / 64));
     return A;
 }
@@ -346,7 +343,8 @@ bool heads_aligned(const float *k, const float *v) {
 void check_heads_call(k2t_ctx *ctx, int bits, int batch, int ntok, int nkv, int hd, size_t row_stride,
                       const void *d_pos, const k2t_kv_rows *kv) {
     branch_arg(ctx != nullptr && kv != nullptr, "NULL argument");
-    branch_arg(batch >= 0 && batch <= 65535 && ntok >= 0 && nkv > 0, "batch must be 0 .. 65535, ntok >= 0, n_kv_heads > 0");
+    branch_arg(batch >= 0 && batch <= 65535 && ntok >= 0 && nkv > 0 && nkv <= 1024,
+               "batch must be 0 .. 65535, ntok >= 0, n_kv_heads 1 .. 1024");
     check_kv_rows(kv, bits, hd);
     branch_arg((size_t)batch * ntok * nkv <= (size_t)1 << 24, "more than 2^24 heads in one call");
     branch_arg(row_stride >= (size_t)nkv * hd && row_stride % 4 == 0,
@@ -366,14 +364,6 @@ void check_kv_rows(const k2t_kv_rows *kv, int bits, int hd) {
     branch_arg((at(kv->kq) | at(kv->vq)) % 16 == 0, "kq and vq must be 16-byte aligned");
     const uintptr_t scale = bits == 8 ? 4 : hd / 32;
     branch_arg((at(kv->ks) | at(kv->vs)) % scale == 0, "ks and vs must be aligned to one slot's scales");
-}
-
-void launch_kv_append(hipStream_t st, int bits, const float *k, const float *v, size_t row_stride, int batch, int ntok,
-                      int nkv, int hd, const int *pos, const int *counts, const k2t_kv_rows &kv, int layer) {
-    RowsArgs A = rows_args(kv, row_stride, batch, ntok, nkv, hd, pos, counts, layer);
-    A.k = k;
-    A.v = v;
-    launch_rows_of<false>(st, bits, hd, A, batch);
 }
 
 void launch_beam_post(hipStream_t st, float *qkv, const float *bias, const float *qn, const float *kn, float eps,
@@ -414,8 +404,10 @@ int32_t k2t_kv_append(k2t_ctx *ctx, int32_t bits, const float *d_k, const float 
         branch_arg(d_k && d_v, "NULL argument");
         branch_arg(heads_aligned(d_k, d_v), "d_k and d_v must be 16-byte aligned");
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
-        launch_kv_append(ctx->stream, bits, d_k, d_v, row_stride, batch, ntok, n_kv_heads, head_dim, d_pos, d_counts,
-                         *kv, 0);
+        RowsArgs A = rows_args(*kv, row_stride, ntok, n_kv_heads, head_dim, d_pos, d_counts);
+        A.k = d_k;
+        A.v = d_v;
+        launch_rows_of<false>(ctx->stream, bits, head_dim, A, batch);
     });
 }
 
@@ -428,7 +420,7 @@ int32_t k2t_kv_load(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, int32_t b
         branch_arg(d_k && d_v, "NULL argument");
         branch_arg(heads_aligned(d_k, d_v), "d_k and d_v must be 16-byte aligned");
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
-        RowsArgs A = rows_args(*kv, row_stride, batch, ntok, n_kv_heads, head_dim, d_pos, d_counts, 0);
+        RowsArgs A = rows_args(*kv, row_stride, ntok, n_kv_heads, head_dim, d_pos, d_counts);
         A.ko = d_k;
         A.vo = d_v;
         launch_rows_of<true>(ctx->stream, bits, head_dim, A, batch);
@@ -440,9 +432,11 @@ int32_t k2t_kv_reorder(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const 
     return branch_guard([&] {
         branch_arg(ctx && kv && d_parents, "NULL argument");
         check_kv_rows(kv, bits, head_dim);
-        branch_arg(n_layers >= 0 && n_seq >= 0 && n_kv_heads > 0, "negative n_layers or n_seq, or no KV heads");
+        branch_arg(n_layers >= 0 && n_seq >= 0 && n_kv_heads > 0 && n_kv_heads <= 1024,
+                   "negative n_layers or n_seq, or n_kv_heads not 1 .. 1024");
         branch_arg(beams >= 1 && beams <= kMaxBeams, "beams must be 1 .. 64");
-        branch_arg((size_t)n_layers * n_seq * n_kv_heads <= (size_t)1 << 22, "too many layers, sequences and heads");
+        branch_arg(n_seq <= 65535 && (size_t)n_layers * n_seq * n_kv_heads <= (size_t)1 << 22,
+                   "too many layers, sequences and heads");
         branch_arg((size_t)kv->len * head_dim <= (size_t)1 << 26, "len too large");
         if (n_layers == 0 || n_seq == 0 || beams == 1 || kv->len == 0) return;
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");

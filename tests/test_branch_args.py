@@ -37,7 +37,8 @@ BAD_CACHE = [rows(kq=0), rows(vs=0), rows(kq=P + 8), rows(vq=P + 1), rows(ks=P +
 def test_append_and_load():
     good = [CTX, 8, P, P, 256, 2, 3, 2, 128, P, None, rows()]
     refused("k2t_kv_append", good, [{0: None}, {1: 5}, {1: 16}, {2: None}, {3: None}, {2: P + 4}, {4: 255}, {4: 258}, {5: -1},
-                                    {6: -1}, {7: 0}, {8: 96}, {9: None}, {11: None}, {5: 1 << 20, 6: 1 << 10}] +
+                                    {6: -1}, {7: 0}, {8: 96}, {9: None}, {11: None}, {5: 1 << 20, 6: 1 << 10},
+                                    {6: 1 << 30, 7: 1 << 30, 4: 1 << 40}, {7: 1025, 4: 1 << 20}] +
             [{11: c} for c in BAD_CACHE])
     good = [CTX, 4, rows(), 2, 3, 2, 128, P, None, P, P, 256]
     refused("k2t_kv_load", good, [{0: None}, {1: 3}, {2: None}, {2: rows(ks=P + 2)}, {6: 32}, {7: None}, {9: None},
@@ -50,7 +51,8 @@ def test_append_and_load():
 def test_reorder():
     good = [CTX, 8, rows(), P, 2, 1, 4, 2, 64]
     refused("k2t_kv_reorder", good, [{0: None}, {1: 7}, {2: None}, {3: None}, {4: -1}, {5: -1}, {6: 0}, {6: 65}, {7: 0}, {8: 63},
-                                     {4: 1 << 20, 5: 100}, {2: rows(cap=1 << 24, length=1 << 24)}] +
+                                     {4: 1 << 20, 5: 100}, {4: 1 << 30, 5: 1 << 30, 7: 16}, {7: 1 << 30},
+                                     {2: rows(cap=1 << 24, length=1 << 24)}] +
             [{2: c} for c in BAD_CACHE])
     if k2t.lib().k2t_device_count() == 0:
         assert call("k2t_kv_reorder", *good) == HIP
@@ -63,7 +65,8 @@ def test_attention():
     good = [CTX, 8, P, 512, 1, 4, 8, 2, 64, rows(), rows(), 0.125, P, P, n.value]
     refused("k2t_attn_shared", good, [{0: None}, {1: 0}, {2: None}, {2: P + 4}, {3: 511}, {3: 514}, {4: -1}, {5: 0}, {6: 7},
                                       {6: 2048}, {7: 0}, {8: 80}, {9: None, 10: None}, {12: None}, {12: P + 4}, {13: None},
-                                      {13: P + 8}, {14: n.value - 1}, {4: 70000}] +
+                                      {13: P + 8}, {14: n.value - 1}, {4: 70000}, {11: -0.125}, {11: float("nan")}, {11: float("inf")},
+                                      {4: 16000, 6: 1024}] +
             [{i: c} for c in BAD_CACHE for i in (9, 10)])
     refused("k2t_attn_shared_workspace", [CTX, 1, 4, 8, 2, 64, 8, 8, C.byref(n)],
             [{0: None}, {1: -1}, {2: 0}, {3: 9}, {5: 256}, {6: -1}, {7: -1}, {8: None}])
@@ -74,10 +77,10 @@ def test_attention():
 def test_select():
     n = C.c_size_t()
     assert call("k2t_beam_select_workspace", CTX, 2, 4, 1000, 8, C.byref(n)) == 0 and n.value >= 16
-    good = [CTX, P, 1000, 1000, P, P, 2, 4, 8, 5, P, P, P, P, P, n.value]
+    good = [CTX, P, 1000, 1000, P, P, 2, 4, 8, 5, 2 * P, P, P, 2 * P, P, n.value]
     refused("k2t_beam_select", good, [{0: None}, {1: None}, {2: 0}, {2: 262145, 3: 262145}, {3: 999}, {4: None}, {6: -1}, {7: 0}, {7: 65}, {8: 0},
                                       {8: 129}, {9: -2}, {9: 1000}, {9: -1}, {10: None}, {11: None}, {12: None}, {14: None},
-                                      {14: P + 8}, {15: n.value - 1}, {6: 20000}])
+                                      {14: P + 8}, {15: n.value - 1}, {6: 20000}, {10: P + 64, 4: P + 64}, {13: P + 64, 5: P + 64}])
     refused("k2t_beam_select_workspace", [CTX, 2, 4, 1000, 8, C.byref(n)], [{0: None}, {2: 65}, {3: 0}, {4: 0}, {5: None}])
     if k2t.lib().k2t_device_count() == 0:
         assert call("k2t_beam_select", *good) == HIP

@@ -264,6 +264,37 @@ def test_attention_without_positions_prefix_or_tail(gpu_ctx, bits, hd):
         assert (err <= bound).all(), float((err / bound).max())
 
 
+@pytest.mark.parametrize("bits,hd", [(8, 128), (4, 64)])
+@pytest.mark.parametrize("prefix", [50, 1500])
+def test_attention_of_bad_rows_stays_in_them(gpu_ctx, bits, hd, prefix):
+    """NaN and infinities in one row's query, K scales and V scales: the other rows' bits do not change."""
+    rng = np.random.default_rng(prefix)
+    beams, nq, nkv, tail = 6, 8, 2, 20
+    pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+    q = rng.standard_normal((beams, nq * hd)).astype(np.float32)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+
+    def run():
+        _, p = rows_of(pre, prefix)
+        _, t = rows_of(tl, tail)
+        out = torch.zeros((beams, nq, hd), device="cuda")
+        gpu_ctx.attn_shared(bits, dev(q), nq * hd, 1, beams, nq, nkv, hd, p, t, hd ** -0.5, out, ws)
+        gpu_ctx.sync()
+        return out.cpu().numpy()
+
+    good = run()
+    assert np.isfinite(good).all()
+    q[1, 5], q[2, hd + 3] = np.nan, np.inf
+    tl[1][3, 0, 7] = np.nan if bits == 8 else 0x7FC0
+    tl[3][4, 1, 2] = np.inf if bits == 8 else 0x7F80
+    bad = run()
+    assert np.array_equal(bad[[0, 5]], good[[0, 5]])
+    for r, heads in ((1, [0]), (2, [1]), (3, [0, 1, 2, 3]), (4, [4, 5, 6, 7])):  # nor do the row's other heads
+        rest = [h for h in range(nq) if h not in heads]
+        assert np.array_equal(bad[r, rest], good[r, rest])
+        assert r == 1 or not np.isfinite(bad[r, heads]).all()
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 def test_attention_weights_far_apart_and_scales_of_any_size(gpu_ctx, bits):
     """One position takes all the weight, wherever it lies; V scales from 1e-12 to 1e12."""
@@ -358,8 +389,9 @@ def run_select(ctx, logits, scores, done, n_seq, beams, k, eos, stride=None):
     return [t.cpu().numpy() for t in o]
 
 
-# exp is off by 4 units, a sum of 4096 in lanes, waves and slices by 40 roundings: the logarithm by
-# less than 2^-18; the score is then rounded once
+# exp is off by 4 units and by a rounding of its exponent, of which 18 bits count in a sum of up to 2^18
+# terms (18 ln 2 2^-24 < 2^-20); a sum of 4096 in lanes, waves and slices by 40 roundings: the logarithm
+# by less than 2^-18; the score is then rounded once
 def score_tol(s):
     return np.where(np.isfinite(s), np.abs(s) * R.U, 0) + 2.0 ** -18
 
@@ -447,3 +479,22 @@ def test_select_in_place_and_without_flags(gpu_ctx):
     gpu_ctx.sync()
     _, wt, wp, _, _ = R.select(logits, scores, None, n, beams, beams, -1)
     assert np.array_equal(tok.cpu().numpy(), wt.reshape(-1)) and np.array_equal(par.cpu().numpy(), wp.reshape(-1))
+
+
+@pytest.mark.parametrize("vocab,k,spread", [(100000, 128, True), (5000, 64, False)])
+def test_select_of_64_rows(gpu_ctx, vocab, k, spread):
+    """More candidates than the merge holds: every third slice far above the others, so that a row has
+    hundreds beyond its bound; all logits and rows equal, so that every candidate reaches the last one."""
+    rng = np.random.default_rng(vocab)
+    logits, scores = np.full((64, vocab), 0.75, np.float32), np.full(64, -2.0, np.float32)
+    if spread:
+        high = np.arange(vocab) // 4096 % 3 == 1
+        for r in range(64):  # (the same values in every row: scores 2^-13 apart tell the rows apart)
+            logits[r, high] = 600 + rng.permutation(high.sum()) / 128
+            logits[r, ~high] = rng.permutation((~high).sum()) / 256
+        scores = (-3 - np.arange(64) / 2.0 ** 13).astype(np.float32)
+    ws, wt, wp, wd, gap = R.select(logits, scores, None, 1, 64, k, 11)
+    assert gap > 2.0 ** -15 or not spread
+    s, t, p, d = run_select(gpu_ctx, logits, scores, None, 1, 64, k, 11)
+    assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(d, wd)
+    assert (np.abs(s - ws) <= score_tol(ws)).all()
