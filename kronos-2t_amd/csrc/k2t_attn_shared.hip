@@ -1,5 +1,26 @@
 // Attention of one token of every row of a batch whose rows share their sequence's prefix cache and
 // have a tail cache each (k2t_attn_shared): int8 or NF4 Hadamard caches, plain or grouped heads.
+//
+// For row r and q head h, over the positions t of its sequence's prefix and then of its tail:
+//   s_t = scale_q scale_k[t] (codes_q . codes_k[t]) attn_scale,  w_t = exp(s_t - max s),
+//   out = ifwht64( sum_t w_t scale_v[t] codes_v[t] / sum_t w_t ).
+// The rows of a sequence and the q heads of a KV head are columns of one matrix against the same K and
+// V, so both products are matrix products: scores S^T = K Q^T by the int8 MFMA, whose sums are exact,
+// and outputs O^T = V^T W^T by the f16 MFMA. V's codes are exact in f16; a weight times its V scale is
+// split into two f16 pieces that hold 21 bits of it, so nothing is lost next to an fp32 product.
+// Maxima are raised lazily, sums and outputs are fp32 and joined in a fixed order.
+//
+// Work is cut into (sequence, KV head, part of the positions, 16 or 32 columns), about two workgroups per
+// CU; the parts' outputs are joined by a second kernel. The waves of a workgroup take tiles of 32
+// positions in turn; K and V go from memory to registers in the operands' own layout, so a tile needs
+// no LDS and no barrier.
+//
+// What bounds it: instructions, not bytes. A tile of 32 positions and 32 columns takes some 340 vector
+// instructions (weights and their pieces, V's codes to f16, scales) next to 40 MFMAs, two waves to a
+// SIMD; a part has few tiles, so its queries' transform and its join count too. Measured (passes in a row):
+// 8 rows x 32 heads x 64, 1500 positions 9.7 us (0.9 TB/s of cache bytes); 64 rows x 32 / 4 heads x 128,
+// 12000 + 333 positions 36.6 us (352 TFLOP/s); 3 sequences of 8 rows x 32 / 8 heads x 128, NF4, 4100 positions
+// 19.2 us, a third of whose instructions look codes up; 4 rows x 9 / 3 heads x 64, 52 positions 5.2 us, a launch.
 #include <float.h>
 #include <math.h>
 
@@ -651,6 +672,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_whole_kernel(SharedArgs
     attend<HD, BITS, 1, true>(A, I, sh);
 }
 
+// Joins the parts: out = ifwht64(sum_i e_i part_i / sum_i e_i l_i), e_i = 2^(m_i - max m). A chain of
+// latencies (lengths, statistics, partials, the transform): 3 to 5 us whatever the sizes here.
 // One (head, row) per WAVES waves: its parts' maxima and sums one per lane, then the outputs of every
 // WAVES-th part, eight or sixteen loads in flight, joined in wave order, and ifwht64.  Parts that hold no
 // positions were not written and count nothing.
@@ -765,7 +788,10 @@ Plan plan_of(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_
         n = (len + each - 1) / each;
     };
     cut(prefix_len, (size_t)s.n_seq * s.nkv * P.pgroups, P.np, P.plen);
-    cut(tail_len, (size_t)s.n_seq * s.beams * s.nkv * P.tgroups, P.nt, P.tlen);
+    // The prefix items count among the tails': where they fill the card, a tail's further parts are only more
+    // queries to transform and parts to join (64 rows x 32 / 4 heads x 128, 12000 + 333 positions: one part per
+    // tail 41.3 us, two 45.1; 16 rows x 32 / 8, 4000 + 333: 16.5 and 18.0 with three).
+    cut(tail_len, (size_t)s.n_seq * s.beams * s.nkv * P.tgroups + (size_t)s.n_seq * s.nkv * P.pgroups * P.np, P.nt, P.tlen);
     return P;
 }
 size_t part_slots(const SharedShape &s, const Plan &P) { return (size_t)s.n_seq * s.beams * s.nq * (P.np + P.nt); }
@@ -790,6 +816,8 @@ void launch_shared(hipStream_t st, int bits, const SharedArgs &A, const SharedSh
     }
     if (items && bits == 8) launch_parts<HD, 8>(st, A, P, items);
     if (items && bits == 4) launch_parts<HD, 4>(st, A, P, items);
+    // Four waves share a head's parts where there are many, and so few heads (4 rows x 9 / 3 heads x 64,
+    // 12000 positions, 95 parts: 10.4 us and 12.9 with one wave; 64 rows x 32 / 4 x 128, 9 parts: 39.9 and 37.3).
     if (A.np + A.nt > 16) hipLaunchKernelGGL((shared_merge_kernel<HD, 4>), dim3(pairs), dim3(256), 0, st, A, pairs);
     else hipLaunchKernelGGL((shared_merge_kernel<HD, 1>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs);
     hip_check(hipGetLastError(), "attn_shared merge launch");
