@@ -457,7 +457,7 @@ int32_t k2t_kv_reorder(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const 
  * zeros; infinities and NaN of one row's query or tail stay in that row.  attn_scale is finite and
  * not negative.  d_ws: device workspace of at least k2t_attn_shared_workspace bytes, of this call
  * alone while it runs (two graphs that may run at once need one each); it needs no initial value.
- * d_q, d_out and d_ws are 16-byte aligned, q_stride a multiple of 4; n_heads <= 1024,
+ * d_q, d_out and d_ws are 16-byte aligned, q_stride a multiple of 4 below 2^31; n_heads <= 1024,
  * n_seq * beams <= 65535, n_seq * beams * n_heads <= 2^22. */
 int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_stride, int32_t n_seq, int32_t beams,
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const k2t_kv_rows *prefix,

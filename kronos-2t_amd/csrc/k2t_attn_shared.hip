@@ -46,7 +46,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 struct SharedArgs {
     const float *q;
-    size_t q_stride;
+    uint32_t q_stride;
+    float per_group;  // 1 / group
     k2t_kv_rows pre, tail;
     int beams, nq, nkv, group;    // group: q heads per KV head
     int np, nt, plen, tlen;       // prefix and tail parts, and their positions
@@ -57,6 +58,16 @@ struct SharedArgs {
     float2 *stat;  // [row][head][np + nt]: maximum (in powers of two), sum
     float *out;
 };
+
+// Row and head (counted from an item's) of column c: c / group by a product, exact for c below 2^22: c + 0.5
+// is half a step at least from a multiple of the group, and the product off by 2^-23 of itself.
+struct Column {
+    uint32_t row, head;
+};
+__device__ __forceinline__ Column column(const SharedArgs &A, int c) {
+    const uint32_t row = (uint32_t)(((float)c + 0.5f) * A.per_group);
+    return Column{row, (uint32_t)c - row * (uint32_t)A.group};
+}
 
 __device__ __forceinline__ int row_len(const k2t_kv_rows &kv, int row) {
     return kv.d_len ? max(0, min(kv.d_len[row], kv.len)) : kv.len;
@@ -351,9 +362,8 @@ struct Quant4 {
     float qas;   // scale of the head's scores, in powers of two
 };
 template <int NB>
-__device__ __forceinline__ Quant4 quantize_block(float4 f, uint64_t mask, uint32_t li, float attn_scale) {
+__device__ __forceinline__ Quant4 quantize_block(float4 f, uint32_t sb, uint32_t li, float attn_scale) {
     float v[4] = {f.x, f.y, f.z, f.w};
-    const uint32_t sb = (uint32_t)(mask >> (4u * li)) & 0xFu;
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = flip_sign(v[j], (sb >> j) & 1u) * 0.125f;
     butterflies_slice4(v, li);
@@ -377,20 +387,18 @@ __device__ __forceinline__ void quantize_queries(const SharedArgs &A, const Item
     constexpr int NB = HD / 64, kTurns = (COLS * NB + 4 * kWaves - 1) / (4 * kWaves);
     const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const float *q0 = A.q + (size_t)I.row0 * A.q_stride + (size_t)I.head0 * HD;
     float4 f[kTurns];  // every load in flight at once
 #pragma unroll
     for (int k = 0; k < kTurns; k++) {
         const int u = 4 * (wave + kWaves * k) + (int)lg, c = I.col0 + min(u / NB, I.n - 1);
-        f[k] = *reinterpret_cast<const float4 *>(A.q + (size_t)(I.row0 + c / A.group) * A.q_stride +
-                                                 (size_t)(I.head0 + c % A.group) * HD + 64 * (u % NB) + 4 * li);
+        const Column at = column(A, c);
+        f[k] = *reinterpret_cast<const float4 *>(q0 + ((uint64_t)at.row * A.q_stride + at.head * HD + 64 * (u % NB) + 4 * li));
     }
-    uint64_t mask[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) mask[b] = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
 #pragma unroll
     for (int k = 0; k < kTurns; k++) {
         const int u = 4 * (wave + kWaves * k) + (int)lg, x = u / NB, b = u % NB;
-        const Quant4 r = quantize_block<NB>(f[k], NB > 1 && b ? mask[NB - 1] : mask[0], li, A.attn_scale);
+        const Quant4 r = quantize_block<NB>(f[k], head_signs4<NB>(b, li), li, A.attn_scale);
         if (x >= COLS) continue;
         *reinterpret_cast<uint32_t *>(&Q.q[x][64 * b + 4 * li]) = r.w;
         if (li == 0 && b == 0) Q.qas[x] = r.qas;
@@ -418,7 +426,6 @@ __device__ __forceinline__ void query_operand(const int8_t *r, uint32_t lg, v4i 
 template <int HD>
 struct Join {
     float m[kWaves][16], l[kWaves][16];
-    uint64_t mask[HD / 64];  // Hadamard signs (WHOLE)
     __align__(16) float o[kWaves][16][HD + 4];
 };
 template <int HD, int BITS, int NQ, bool WHOLE>
@@ -426,13 +433,6 @@ __device__ __forceinline__ void join(const SharedArgs &A, const Item &I, const S
     const uint32_t tid = threadIdx.x, lane = tid & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const float back = S.back();
-    if constexpr (WHOLE) {
-#pragma unroll
-        for (int b = 0; b < HD / 64; b++) {
-            const uint64_t mask = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
-            if (tid == 0) J.mask[b] = mask;
-        }
-    }
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
         if (16 * a >= I.n) break;
@@ -459,7 +459,8 @@ __device__ __forceinline__ void join(const SharedArgs &A, const Item &I, const S
                 L = fmaf(J.l[w][x], e[w], L);
             }
             const int c = I.col0 + 16 * a + x;
-            const size_t pair = (size_t)(I.row0 + c / A.group) * A.nq + I.head0 + c % A.group;
+            const Column to = column(A, c);
+            const size_t pair = (size_t)(I.row0 + to.row) * A.nq + I.head0 + to.head;
             const size_t at = WHOLE ? pair : pair * (A.np + A.nt) + I.part;
 #pragma unroll
             for (int d = 0; d < HD; d += 64) {
@@ -477,7 +478,7 @@ __device__ __forceinline__ void join(const SharedArgs &A, const Item &I, const S
                     const float inv = 1.0f / L;
                     float v[4] = {r.x * inv, r.y * inv, r.z * inv, r.w * inv};
                     butterflies_slice4(v, (uint32_t)sl);
-                    const uint32_t sb = (uint32_t)(J.mask[d / 64] >> (4 * sl)) & 0xFu;
+                    const uint32_t sb = head_signs4<HD / 64>(d / 64, (uint32_t)sl);
                     r = make_float4(flip_sign(v[0] * 0.125f, sb & 1u), flip_sign(v[1] * 0.125f, (sb >> 1) & 1u),
                                     flip_sign(v[2] * 0.125f, (sb >> 2) & 1u), flip_sign(v[3] * 0.125f, sb >> 3));
                 }
@@ -740,7 +741,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs A, int pai
         float r = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) r += sum[w][64 * wave + lane];
-        out[64 * wave + lane] = ifwht_lane(r * inv, wave, lane);
+        out[64 * wave + lane] = flip_sign(wave_butterflies64(r * inv, lane) * 0.125f, head_sign<E>(wave, lane));
     } else {
         // (a lane's two neighbouring elements of HD = 128 to one element of each block)
 #pragma unroll
@@ -751,7 +752,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs A, int pai
                 const float r0 = __shfl(o[0], from, kWave), r1 = __shfl(o[E - 1], from, kWave);
                 r = (lane & 1u) ? r1 : r0;
             }
-            out[64 * b + lane] = ifwht_lane(r * inv, b, lane);
+            out[64 * b + lane] = flip_sign(wave_butterflies64(r * inv, lane) * 0.125f, head_sign<E>(b, lane));
         }
     }
 }
@@ -835,7 +836,8 @@ void launch_attn_shared(k2t_ctx *ctx, hipStream_t st, int bits, const float *q, 
     const Plan P = plan_of(ctx, s, prefix.cap ? prefix.len : 0, tail.cap ? tail.len : 0);
     SharedArgs A{};
     A.q = q;
-    A.q_stride = q_stride;
+    A.q_stride = (uint32_t)q_stride;
+    A.per_group = (float)s.nkv / (float)s.nq;
     A.pre = prefix;
     A.tail = tail;
     A.beams = s.beams;
@@ -902,8 +904,9 @@ int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
         if (n_seq == 0) return;
         branch_arg(d_q && d_out && d_ws, "NULL argument");
         const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p); };
-        branch_arg(q_stride >= (size_t)n_heads * head_dim && q_stride % 4 == 0 && at(d_q) % 16 == 0,
-                   "d_q must be 16-byte aligned, q_stride a multiple of 4 and no smaller than a row");
+        branch_arg(q_stride >= (size_t)n_heads * head_dim && q_stride % 4 == 0 && q_stride < (size_t)1 << 31 &&
+                       at(d_q) % 16 == 0,
+                   "d_q must be 16-byte aligned, q_stride a multiple of 4, no smaller than a row, below 2^31");
         branch_arg((at(d_out) | at(d_ws)) % 16 == 0, "d_out and d_ws must be 16-byte aligned");
         const size_t need = attn_shared_ws_bytes(ctx, s, prefix ? prefix->len : 0, tail ? tail->len : 0);
         if (ws_bytes < need)

@@ -113,6 +113,20 @@ __device__ __forceinline__ uint32_t hadamard_sign_bit(uint64_t block, uint32_t i
     return (uint32_t)(z & 1);
 }
 
+// The signs of a block's 64 elements (bit i = element i), worked out by the compiler: two 64-bit products
+// per lane are a large part of a kernel that does little else.
+constexpr uint64_t hadamard_sign_mask(uint64_t block) {
+    uint64_t mask = 0;
+    for (uint64_t i = 0; i < 64; i++) {
+        uint64_t z = 0x9E3779B97F4A7C15ull + block * 0xBF58476D1CE4E5B9ull + (i + 1) * 0x9E3779B97F4A7C15ull;
+        z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+        z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+        z ^= z >> 31;
+        mask |= (z & 1) << i;
+    }
+    return mask;
+}
+
 // DPP lane moves inside one 16-lane row.
 // (bound_ctrl set: every source lane of these patterns exists, and the compiler can then
 // fold the move into the instruction that uses it)

@@ -12,6 +12,18 @@
 
 namespace k2t {
 
+// Signs of a head's block b (NB blocks): element `lane`, or the four elements 4 sl + j as bits j.
+template <int NB>
+__device__ __forceinline__ uint32_t head_sign(int b, uint32_t lane) {
+    constexpr uint64_t s0 = hadamard_sign_mask(0), s1 = hadamard_sign_mask(1);
+    return (uint32_t)((NB > 1 && b ? s1 : s0) >> lane) & 1u;
+}
+template <int NB>
+__device__ __forceinline__ uint32_t head_signs4(int b, uint32_t sl) {
+    constexpr uint64_t s0 = hadamard_sign_mask(0), s1 = hadamard_sign_mask(1);
+    return (uint32_t)((NB > 1 && b ? s1 : s0) >> (4u * sl)) & 0xFu;
+}
+
 // slot_of_pos (real_llm.rs:1116-1122)
 __device__ __forceinline__ int ring_slot(const KvRing &r, int pos) {
     return (r.ring == 0 || pos < r.sinks) ? pos : r.sinks + (pos - r.sinks) % r.ring;

@@ -90,9 +90,6 @@ template <int NB, int BITS, int TURNS>
 __global__ __launch_bounds__(256) void kv_append_kernel(RowsArgs A) {
     __shared__ __align__(16) float term[BITS == 4 ? 4 : 1][BITS == 4 ? 4 * TURNS : 1][68];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, sl = lane & 15u, lg = lane >> 4, wave = tid >> 6;
-    uint64_t mask[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) mask[b] = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
     BlockAt at[TURNS];
     bool live[TURNS];
     float v[TURNS][4];
@@ -108,7 +105,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(RowsArgs A) {
     }
 #pragma unroll
     for (int k = 0; k < TURNS; k++) {
-        const uint32_t sb = (uint32_t)((NB > 1 && at[k].b ? mask[NB - 1] : mask[0]) >> (4u * sl)) & 0xFu;
+        const uint32_t sb = head_signs4<NB>(at[k].b, sl);
 #pragma unroll
         for (int j = 0; j < 4; j++) v[k][j] = flip_sign(v[k][j], (sb >> j) & 1u) * 0.125f;
         butterflies_slice4(v[k], sl);
@@ -186,9 +183,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(RowsArgs A) {
 template <int NB, int BITS, int TURNS>
 __global__ __launch_bounds__(256) void kv_load_kernel(RowsArgs A) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, sl = lane & 15u, lg = lane >> 4, wave = tid >> 6;
-    uint64_t mask[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) mask[b] = __ballot(hadamard_sign_bit((uint64_t)b, lane) != 0u);
     BlockAt at[TURNS];
     bool live[TURNS];
     uint32_t w[TURNS];
@@ -218,7 +212,7 @@ __global__ __launch_bounds__(256) void kv_load_kernel(RowsArgs A) {
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = (float)(int8_t)((w[k] >> (8 * j)) & 0xFFu) * scale[k];
         butterflies_slice4(v, sl);
-        const uint32_t sb = (uint32_t)((NB > 1 && at[k].b ? mask[NB - 1] : mask[0]) >> (4u * sl)) & 0xFu;
+        const uint32_t sb = head_signs4<NB>(at[k].b, sl);
         if (!live[k]) continue;
         *reinterpret_cast<float4 *>((at[k].is_v ? A.vo : A.ko) + at[k].in + 4 * sl) =
             make_float4(flip_sign(v[0] * 0.125f, sb & 1u), flip_sign(v[1] * 0.125f, (sb >> 1) & 1u),

@@ -63,7 +63,7 @@ def test_attention():
     n = C.c_size_t()
     assert call("k2t_attn_shared_workspace", CTX, 1, 4, 8, 2, 64, 8, 8, C.byref(n)) == 0 and n.value >= 16
     good = [CTX, 8, P, 512, 1, 4, 8, 2, 64, rows(), rows(), 0.125, P, P, n.value]
-    refused("k2t_attn_shared", good, [{0: None}, {1: 0}, {2: None}, {2: P + 4}, {3: 511}, {3: 514}, {4: -1}, {5: 0}, {6: 7},
+    refused("k2t_attn_shared", good, [{0: None}, {1: 0}, {2: None}, {2: P + 4}, {3: 511}, {3: 514}, {3: 1 << 31}, {4: -1}, {5: 0}, {6: 7},
                                       {6: 2048}, {7: 0}, {8: 80}, {9: None, 10: None}, {12: None}, {12: P + 4}, {13: None},
                                       {13: P + 8}, {14: n.value - 1}, {4: 70000}, {11: -0.125}, {11: float("nan")}, {11: float("inf")},
                                       {4: 16000, 6: 1024}] +
