@@ -757,13 +757,13 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs A, int pai
     }
 }
 
-// shared_whole_kernel up to this many positions, times its rounds of four workgroups per CU.  Measured
-// on both sides (8 rows x 32 heads x 64: 320 positions 6.7 us and 8.6 in two launches, 620 8.3 and 8.8,
-// 1220 11.9 and 9.8; 64 rows, two rounds, 320 positions 17.7 and 15.8).
-constexpr size_t kWholeMax = 600;
+// shared_whole_kernel up to this many positions, times its rounds of three workgroups per CU.  Measured
+// on both sides (32 heads x 64, 8 rows: 320 positions 6.2 us and 8.4 in two launches, 720 8.4 and 8.6, 920 9.7
+// and 8.6; 32 rows, two rounds, 320 positions 9.4 and 11.0, 520 11.8 and 11.3).
+constexpr size_t kWholeMax = 720, kWholeRound = 3;
 // Prefix items of two tiles of columns from this many (tile of columns, 32 positions) steps on: fewer
 // instructions per step, but half the workgroups (32 / 4 heads x 128, 12000 positions: 32 rows, 24000
-// steps, 28.0 us and 30.9 with one tile; 16 rows, 12000 steps, 23.2 and 21.2).
+// steps, 28.4 us and 32.3 with one tile; 16 rows, 12000 steps, 22.9 and 21.2).
 constexpr size_t kTwoTiles = 18000;
 
 // How the work is cut.  nq: the prefix items' column tiles; parts so that there are about two
@@ -777,7 +777,7 @@ Plan plan_of(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_
     Plan P{};
     P.tgroups = (group + 15) / 16;
     const size_t cus = (size_t)std::max(1, ctx->num_cus), wholes = (size_t)s.n_seq * s.beams * s.nkv * P.tgroups;
-    P.whole = ((size_t)prefix_len + tail_len) * ((wholes + 4 * cus - 1) / (4 * cus)) <= kWholeMax;
+    P.whole = ((size_t)prefix_len + tail_len) * ((wholes + kWholeRound * cus - 1) / (kWholeRound * cus)) <= kWholeMax;
     if (P.whole) return P;
     const size_t steps = (size_t)s.n_seq * s.nkv * ((cols + 15) / 16) * (prefix_len / kTile);
     P.nq = steps >= kTwoTiles ? 2 : 1;

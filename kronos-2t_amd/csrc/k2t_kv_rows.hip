@@ -6,10 +6,10 @@
 // sum c_i^2), codes again with that scale. load: signs ifwht64(code scale). reorder: row r becomes row
 // parent[r] below its length.
 //
-// What bounds them: 6 rows of 777 tokens, 4 heads x 128, int8 (18 MB each way): append 8.5 us, load 8.2 us
-// under the profiler, 15.3 us the two in a row (2.4 TB/s), of which waves that start, load once, transform and
-// end are the larger part; 515 tokens of 32 heads x 64, NF4: append 9.2 us, its instructions (both roundings
-// of every element, three quotients per block), load 5.2 us; 12.6 us in a row. One token of 4 rows: 2.3 us
+// What bounds them: 6 rows of 777 tokens, 4 heads x 128, int8 (18 MB each way): append 7.8 us, load 7.7 us,
+// 14.2 us the two in a row (2.5 TB/s), of which waves that start, load once, transform and
+// end are the larger part; 515 tokens of 32 heads x 64, NF4: append 7.7 us, its instructions (both roundings
+// of every element, three quotients per block), load 4.6 us; 12.5 us in a row. One token of 4 rows: 2.3 us
 // each, a launch. Sixteen lanes per block, four elements a lane, instead of a wave per head with one
 // element a lane: 26.5 -> 15.2 us and, with the NF4 sums from LDS, 39.6 -> 12.7 us.
 #include <float.h>
@@ -320,8 +320,8 @@ RowsArgs rows_args(const k2t_kv_rows &kv, size_t row_stride, int ntok, int nkv, 
 }
 
 // Two blocks per sixteen lanes from this many on, where every SIMD has its waves anyway (8 x 1024
-// tokens, 8 heads x 128, 262144 blocks: int8 append 23.3 us and 25.1 with one, load 19.9 and 22.0; 515
-// tokens, 32 heads x 64, 32960 blocks: 4.9 and 4.4).
+// tokens, 8 heads x 128, 262144 blocks: NF4 append 38.8 us and 42.8 with one, int8 load 18.9 and 20.2; 515
+// tokens, 32 heads x 64, 32960 blocks: int8 append 4.6 and 4.3, NF4 append 7.8 and 7.7).
 constexpr size_t kManyBlocks = 1 << 16;
 
 template <int NB, int BITS, bool LOAD>

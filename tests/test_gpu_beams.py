@@ -181,7 +181,8 @@ def test_mixture_of_experts_model(gpu_ctx):
         gm.set_moe(li, bank, li, moe[li][1], k, True, 0)
     mats.append(up(300, d))
     gm.set_head(mats[-1], norm(d))
-    check_search(gm, [3, 250, 17], 9, 6, 4)
+    for n_beams in (1, 6):
+        check_search(gm, [3, 250, 17], 9, n_beams, 4)
 
 
 # ---------------------------------------------------------------- the operators in a row
