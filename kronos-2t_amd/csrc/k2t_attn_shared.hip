@@ -18,9 +18,9 @@
 // What bounds it: instructions, not bytes. A tile of 32 positions and 32 columns takes some 340 vector
 // instructions (weights and their pieces, V's codes to f16, scales) next to 40 MFMAs, two waves to a
 // SIMD; a part has few tiles, so its queries' transform and its join count too. Measured (passes in a row):
-// 8 rows x 32 heads x 64, 1500 positions 9.7 us (0.9 TB/s of cache bytes); 64 rows x 32 / 4 heads x 128,
-// 12000 + 333 positions 36.6 us (352 TFLOP/s); 3 sequences of 8 rows x 32 / 8 heads x 128, NF4, 4100 positions
-// 19.2 us, a third of whose instructions look codes up; 4 rows x 9 / 3 heads x 64, 52 positions 5.2 us, a launch.
+// 8 rows x 32 heads x 64, 1500 positions 9.4 us (0.9 TB/s of cache bytes); 64 rows x 32 / 4 heads x 128,
+// 12000 + 333 positions 35.4 us (364 TFLOP/s); 3 sequences of 8 rows x 32 / 8 heads x 128, NF4, 4100 positions
+// 18.9 us, a third of whose instructions look codes up; 4 rows x 9 / 3 heads x 64, 52 positions 5.2 us, a launch.
 #include <float.h>
 #include <math.h>
 

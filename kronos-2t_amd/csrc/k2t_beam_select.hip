@@ -12,7 +12,7 @@
 // both kernels take longer than their bytes, the first for its instructions (some 25 per logit on 3
 // waves per SIMD: 6.0 us there, 8.3 us before exp came down to one v_exp_f32 and keys were only made
 // for what reaches the bound), the second for chains of dependent steps on one CU (6.6 us there; 9.2 us
-// for 16 rows of 151936, k 32).  Both: 8.9 us for one sequence of 4 rows of 8192, 13.6 us and 15.6 us.
+// for 16 rows of 151936, k 32).  Both: 8.8 us for one sequence of 4 rows of 8192, 13.1 us and 15.3 us.
 // Slices of 4096 give 48 rows and up a workgroup per CU; the alternative of fewer, larger ones leaves
 // CUs idle in a single sequence.
 #include <float.h>

@@ -7,9 +7,9 @@
 // parent[r] below its length.
 //
 // What bounds them: 6 rows of 777 tokens, 4 heads x 128, int8 (18 MB each way): append 7.8 us, load 7.7 us,
-// 14.2 us the two in a row (2.5 TB/s), of which waves that start, load once, transform and
+// 13.8 us the two in a row (2.6 TB/s), of which waves that start, load once, transform and
 // end are the larger part; 515 tokens of 32 heads x 64, NF4: append 7.7 us, its instructions (both roundings
-// of every element, three quotients per block), load 4.6 us; 12.5 us in a row. One token of 4 rows: 2.3 us
+// of every element, three quotients per block), load 4.6 us; 12.4 us in a row. One token of 4 rows: 2.3 us
 // each, a launch. Sixteen lanes per block, four elements a lane, instead of a wave per head with one
 // element a lane: 26.5 -> 15.2 us and, with the NF4 sums from LDS, 39.6 -> 12.7 us.
 #include <float.h>
@@ -249,8 +249,8 @@ __global__ __launch_bounds__(64) void beam_post_kernel(float *__restrict__ qkv, 
 // Rows of one (layer, sequence, KV head, K or V) rearranged in place.  A thread owns one column (the
 // same T-sized piece of every row): it reads the column of every row that moves from its source row
 // before it writes any, so no other thread or buffer is involved.
-// Bound by bytes: 24 layers, 8 rows of 32 heads x 64, 200 positions, 256 MB read and written in 65 us
-// (3.9 TB/s; the large copy reaches 5.2), 114 us with 4-byte columns. Up to 32 rows go through
+// Bound by bytes: 24 layers, 8 rows of 32 heads x 64, 200 positions, 256 MB read and written in 64 us
+// (4.0 TB/s; the large copy reaches 5.2), 114 us with 4-byte columns. Up to 32 rows go through
 // registers as 16-byte columns, 64 as 8-byte ones.
 template <typename T, int NB>
 __device__ __forceinline__ void move_column(T *col, size_t pitch, const int *par, int beams, const int *lens, int pos) {
