@@ -145,12 +145,14 @@ def test_long_prompt_and_limits(gpu_ctx):
     tokens, _ = gm.beam_search(5, 3, 10)
     assert gm.position() == 900 and tokens.shape == (3, 10)
     for bad in (dict(n_beams=0), dict(n_beams=65), dict(n_steps=0), dict(eos=cfg["vocab"]), dict(eos=-2), dict(first_token=-1),
-                dict(n_steps=2), dict(n_steps=2 ** 31 - 1)):  # (the last two: past max_seq)
+                dict(n_steps=2)):  # (the last: past max_seq)
         a = dict(first_token=1, n_beams=2, n_steps=1, eos=-1)
         a.update(bad)
         with pytest.raises(k2t.K2TError) as e:
             gm.beam_search(**a)
         assert e.value.code == -1
+    few = np.zeros(64, np.int32)  # (refused before anything is written)
+    assert k2t.lib().k2t_model_beam_search(gm.h, 1, 2, 2 ** 31 - 1, -1, few.ctypes.data, few.ctypes.data) == -1
     gm.reset()
     gm.set_exact(True)
     with pytest.raises(k2t.K2TError, match="fast mode"):
