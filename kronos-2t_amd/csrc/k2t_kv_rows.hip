@@ -6,10 +6,10 @@
 // sum c_i^2), codes again with that scale. load: signs ifwht64(code scale). reorder: row r becomes row
 // parent[r] below its length.
 //
-// What bounds them: 6 rows of 777 tokens, 4 heads x 128, int8 (18 MB each way): append 7.8 us, load 7.7 us,
-// 13.8 us the two in a row (2.6 TB/s), of which waves that start, load once, transform and
+// What bounds them: 6 rows of 777 tokens, 4 heads x 128, int8 (18 MB each way): append 7.8 us, load 6.4 us,
+// 12.6 us the two in a row (2.9 TB/s), of which waves that start, load once, transform and
 // end are the larger part; 515 tokens of 32 heads x 64, NF4: append 7.7 us, its instructions (both roundings
-// of every element, three quotients per block), load 4.6 us; 12.4 us in a row. One token of 4 rows: 2.3 us
+// of every element, three quotients per block), load 4.6 us; 11.9 us in a row. One token of 4 rows: 2.3 us
 // each, a launch. Sixteen lanes per block, four elements a lane, instead of a wave per head with one
 // element a lane: 26.5 -> 15.2 us and, with the NF4 sums from LDS, 39.6 -> 12.7 us.
 #include <float.h>
@@ -24,6 +24,7 @@ namespace k2t {
 namespace {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct RowsArgs {
     const float *k, *v;
@@ -179,7 +180,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(RowsArgs A) {
     }
 }
 
-// The same positions read back: code * scale and ifwht64.
+// The same positions read back: code * scale and ifwht64.  (Stored past L2, where heads of any number do not
+// stay: 6 rows of 777 tokens, 4 heads x 128: 6.4 us and 7.6 with ordinary stores.)
 template <int NB, int BITS, int TURNS>
 __global__ __launch_bounds__(256) void kv_load_kernel(RowsArgs A) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, sl = lane & 15u, lg = lane >> 4, wave = tid >> 6;
@@ -214,9 +216,9 @@ __global__ __launch_bounds__(256) void kv_load_kernel(RowsArgs A) {
         butterflies_slice4(v, sl);
         const uint32_t sb = head_signs4<NB>(at[k].b, sl);
         if (!live[k]) continue;
-        *reinterpret_cast<float4 *>((at[k].is_v ? A.vo : A.ko) + at[k].in + 4 * sl) =
-            make_float4(flip_sign(v[0] * 0.125f, sb & 1u), flip_sign(v[1] * 0.125f, (sb >> 1) & 1u),
-                        flip_sign(v[2] * 0.125f, (sb >> 2) & 1u), flip_sign(v[3] * 0.125f, sb >> 3));
+        const f32x4 out = {flip_sign(v[0] * 0.125f, sb & 1u), flip_sign(v[1] * 0.125f, (sb >> 1) & 1u),
+                           flip_sign(v[2] * 0.125f, (sb >> 2) & 1u), flip_sign(v[3] * 0.125f, sb >> 3)};
+        __builtin_nontemporal_store(out, reinterpret_cast<f32x4 *>((at[k].is_v ? A.vo : A.ko) + at[k].in + 4 * sl));
     }
 }
 
@@ -249,8 +251,9 @@ __global__ __launch_bounds__(64) void beam_post_kernel(float *__restrict__ qkv, 
 // Rows of one (layer, sequence, KV head, K or V) rearranged in place.  A thread owns one column (the
 // same T-sized piece of every row): it reads the column of every row that moves from its source row
 // before it writes any, so no other thread or buffer is involved.
-// Bound by bytes: 24 layers, 8 rows of 32 heads x 64, 200 positions, 256 MB read and written in 64 us
-// (4.0 TB/s; the large copy reaches 5.2), 114 us with 4-byte columns. Up to 32 rows go through
+// Bound by bytes: 24 layers, 8 rows of 32 heads x 64, 200 positions, 256 MB read and written in 48 to 56 us
+// (4.6 to 5.3 TB/s, which is the large copy's), 64 to 70 us with stores that go through L2, 114 us with
+// 4-byte columns too. Up to 32 rows go through
 // registers as 16-byte columns, 64 as 8-byte ones.
 template <typename T, int NB>
 __device__ __forceinline__ void move_column(T *col, size_t pitch, const int *par, int beams, const int *lens, int pos) {
@@ -264,7 +267,7 @@ __device__ __forceinline__ void move_column(T *col, size_t pitch, const int *par
     }
 #pragma unroll
     for (int r = 0; r < NB; r++)
-        if (mv[r]) col[(size_t)r * pitch] = v[r];
+        if (mv[r]) __builtin_nontemporal_store(v[r], col + (size_t)r * pitch);
 }
 
 struct ReorderArgs {
