@@ -364,10 +364,10 @@ int32_t k2t_model_generate(k2t_model *m, int32_t first_token, int32_t n_steps, i
  * best first; eos (-1: none) ends a beam, whose score then stays and whose further tokens are eos.  The
  * beams share the model's cache (k2t_attn_shared) and have tails of their own; afterwards the cache and
  * the position are those of the best one, as k2t_model_generate leaves its own: everything fed but the
- * last token (from an eos on nothing).  Fast mode, full cache (int8 or NF4), n_beams <= 64 and <= the
- * model's max_batch, vocabulary <= 262144.  With one beam it decodes greedily.  The buffers (tails of
- * n_steps positions for every layer and beam, logits) stay with the model; k2t_model_logits keeps the
- * logits of first_token's step. */
+ * last token (from an eos on nothing).  A search whose beams have all ended stops within 16 steps.
+ * Fast mode, full cache (int8 or NF4), n_beams <= 64 and <= the model's max_batch, vocabulary <= 262144.
+ * With one beam it decodes greedily.  The buffers (tails of n_steps positions for every layer and beam,
+ * logits) stay with the model; k2t_model_logits keeps the logits of first_token's step. */
 int32_t k2t_model_beam_search(k2t_model *m, int32_t first_token, int32_t n_beams, int32_t n_steps, int32_t eos,
                               int32_t *tokens_out, float *scores_out);
 /* Device pointer of the last logits (valid after a step; read after k2t_model_sync). */

@@ -868,6 +868,8 @@ void ensure_beams(k2t_model *m, int rows, int n_steps, int prefix) {
     m->beam_cap = n_steps;
 }
 
+constexpr int kDoneSteps = 16;
+
 // The search: the model's step for first_token, then a choice per step over the rows.  Returns the
 // choices (token and parent row of every step), the last scores and the rows' done flags.
 void beam_search(k2t_model *m, int first_token, int rows, int n_steps, int eos, std::vector<int> &tokens,
@@ -884,6 +886,8 @@ void beam_search(k2t_model *m, int first_token, int rows, int n_steps, int eos, 
     int *done = eos >= 0 ? m->beam_done : nullptr;
     launch_beam_select(st, m->logits, c.vocab, c.vocab, m->beam_scores, done, 1, 1, rows, eos, m->beam_scores,
                        m->beam_tokens, m->beam_parents, done, m->beam_ws);
+    int taken = n_steps;
+    std::vector<int> ended(rows);
     for (int t = 1; t < n_steps; t++) {
         int *tok = m->beam_tokens + (size_t)t * rows, *par = m->beam_parents + (size_t)t * rows;
         const BeamStep step{tok - rows, prefix, t};
@@ -893,16 +897,29 @@ void beam_search(k2t_model *m, int first_token, int rows, int n_steps, int eos, 
         k2t_kv_rows tail = m->beam_tail;
         tail.len = t;
         if (rows > 1) launch_kv_reorder(st, bits, tail, par, c.n_layers, 1, rows, c.n_kv_heads, c.head_dim);
+        // Every kDoneSteps steps the host looks whether all rows have ended: further steps choose the same
+        // again.  (One wait for the device next to kDoneSteps steps of a millisecond each.)
+        if (!done || t % kDoneSteps != 0 || t + 1 == n_steps) continue;
+        hip_check(hipMemcpyAsync(ended.data(), done, rows * sizeof(int), hipMemcpyDeviceToHost, st), "done download");
+        hip_check(hipStreamSynchronize(st), "sync");
+        if (std::all_of(ended.begin(), ended.end(), [](int e) { return e != 0; })) {
+            taken = t + 1;
+            break;
+        }
     }
-    const size_t n = (size_t)n_steps * rows;
-    tokens.resize(n);
-    parents.resize(n);
+    tokens.assign((size_t)n_steps * rows, std::max(eos, 0));
+    parents.resize((size_t)n_steps * rows);
     scores.resize(rows);
+    const size_t n = (size_t)taken * rows;
     hip_check(hipMemcpyAsync(tokens.data(), m->beam_tokens, n * sizeof(int), hipMemcpyDeviceToHost, st), "tokens download");
     hip_check(hipMemcpyAsync(parents.data(), m->beam_parents, n * sizeof(int), hipMemcpyDeviceToHost, st), "parents download");
     hip_check(hipMemcpyAsync(scores.data(), m->beam_scores, rows * sizeof(float), hipMemcpyDeviceToHost, st),
               "scores download");
     hip_check(hipStreamSynchronize(st), "sync");
+    for (size_t i = n; i < parents.size(); i++) {  // (rows that are not in use have the first one for parent)
+        const int row = (int)(i % rows);
+        parents[i] = scores[row] > -INFINITY ? row : 0;
+    }
 }
 
 // The first `n` tail positions of row 0 (the best one) join the model's cache behind `prefix`.

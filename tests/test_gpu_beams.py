@@ -123,6 +123,32 @@ def test_eos_ends_beams(gpu_ctx):
         assert any(eos in t for t in tokens)
 
 
+def test_a_search_whose_beams_all_end(gpu_ctx):
+    """Two beams over two tokens of one embedding, so that the same one is the more probable behind the
+    prompt and behind the other: as eos it ends both beams in two steps, and a longer search is that and eos."""
+    cfg = dict(TINY, vocab=2, max_seq=80)
+    layers, head, fn = random_model(cfg, seed=10, fmt="nf4")
+    gm, _ = _gpu_model(gpu_ctx, cfg, layers, head, fn, max_batch=2)
+    gm.set_embedding(k2t.EMBED_F32, rows=np.tile(np.random.default_rng(3).standard_normal(256).astype(np.float32), (2, 1)))
+    tried = 0
+    for prompt in ([0], [1], [0, 1], [1, 1], [0, 0, 1], [1, 0, 1], [1, 1, 0], [0, 0, 0]):
+        a = follow(gm, prompt, 1, [0])[0]
+        eos = int(a.argmax())
+        b = follow(gm, prompt, 1, [1 - eos, 0])[1]
+        if min(a[eos] - a[1 - eos], b[eos] - b[1 - eos]) < 8e-2 * max(np.abs(a).max(), np.abs(b).max()):
+            continue  # (not told apart by two paths of the model, or the other token)
+        tried += 1
+        tokens, scores = check_search(gm, prompt, 1, 2, 60, eos)
+        want = np.full((2, 60), eos)
+        want[1, 0] = 1 - eos
+        assert np.array_equal(tokens, want)
+        for n_steps in (2, 3, 17, 18, 19, 60):
+            t, s = search(gm, prompt, 1, 2, n_steps, eos)
+            assert np.array_equal(t, want[:, :n_steps]) and np.array_equal(s, scores)
+            assert gm.position() == len(prompt) + 1
+    assert tried
+
+
 def test_more_beams_than_tokens(gpu_ctx):
     """The first step has fewer candidates than beams: rows that are not in use, and used ones later."""
     cfg = dict(TINY, vocab=24)
