@@ -498,3 +498,49 @@ def test_select_of_64_rows(gpu_ctx, vocab, k, spread):
     s, t, p, d = run_select(gpu_ctx, logits, scores, None, 1, 64, k, 11)
     assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(d, wd)
     assert (np.abs(s - ws) <= score_tol(ws)).all()
+
+
+def test_the_most_rows(gpu_ctx):
+    """65535 rows in one call of each kind, of one position each: the attention is then the V head read
+    back, a rearrangement permutes what is read back, a choice is the sorted sums."""
+    beams, n_seq, nkv, hd = 15, 4369, 2, 64
+    rows = n_seq * beams
+    assert rows == 65535
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, 6 * hd, generator=g, device="cuda")  # 2 query, 2 K, 2 V heads
+    codes = [torch.zeros(rows, nkv, 1, hd, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(rows, nkv, 1, device="cuda") for _ in range(2)]
+    kv = k2t.KVRows(codes[0], scales[0], codes[1], scales[1], cap=1)
+    zero = torch.zeros(rows, dtype=torch.int32, device="cuda")
+
+    def load():
+        k, v = torch.zeros(rows, nkv, hd, device="cuda"), torch.zeros(rows, nkv, hd, device="cuda")
+        gpu_ctx.kv_load(8, kv, rows, 1, nkv, hd, zero, k, v, nkv * hd)
+        gpu_ctx.sync()
+        return k, v
+
+    at = x.data_ptr()
+    gpu_ctx.kv_append(8, at + 8 * hd, at + 16 * hd, 6 * hd, rows, 1, nkv, hd, zero, kv)
+    k, v = load()
+    # a code is off by half a step of max |r| / 127, and max |r| <= sqrt(64) max |x|; the rotation sums 64
+    assert (v - x[:, 4 * hd:].view(rows, nkv, hd)).abs().max() <= 8 * 8 * x.abs().max() / 254
+    out = torch.full((rows, nkv, hd), float("nan"), device="cuda")
+    ws = workspace(gpu_ctx.attn_shared_workspace(n_seq, beams, nkv, nkv, hd, 0, 1))
+    gpu_ctx.attn_shared(8, x, 6 * hd, n_seq, beams, nkv, nkv, hd, None, kv, 0.125, out, ws)
+    gpu_ctx.sync()
+    assert (out - v).abs().max() <= 2.0 ** -18 * v.abs().max()
+    parents = torch.arange(rows, dtype=torch.int32, device="cuda").view(n_seq, beams).flip(1).contiguous()
+    gpu_ctx.kv_reorder(8, kv, parents, 1, n_seq, beams, nkv, hd)
+    k2, v2 = load()
+    assert torch.equal(k2, k[parents.view(-1).long()]) and torch.equal(v2, v[parents.view(-1).long()])
+    logits, scores = torch.randn(rows, 3, generator=g, device="cuda"), torch.randn(rows, generator=g, device="cuda")
+    o = [torch.zeros(n_seq, 7, dtype=d, device="cuda") for d in (torch.float32, torch.int32, torch.int32)]
+    ws = workspace(gpu_ctx.beam_select_workspace(n_seq, beams, 3, 7))
+    gpu_ctx.beam_select(logits, 3, 3, scores, None, n_seq, beams, 7, -1, *o, None, ws)
+    gpu_ctx.sync()
+    cand = scores.double()[:, None] + torch.log_softmax(logits.double(), 1)
+    want = cand.view(n_seq, -1).sort(1, descending=True).values[:, :7]
+    assert (o[0] - want).abs().max() <= 2.0 ** -18 + 2.0 ** -24 * want.abs().max()
+    chosen = cand[o[2].long(), o[1].long()]  # and the token and row named have that score
+    assert (chosen - want).abs().max() <= 2.0 ** -18
+    assert (o[2] // beams == torch.arange(n_seq, device="cuda")[:, None]).all()
