@@ -63,8 +63,8 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
     v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast:31
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-// Up to this many a bound is found maximum by maximum, beyond by bits: 10.2 us against 10.9 us for 4 rows
-// of 8192 (k 4: 1 and 2 maxima), 15.1 us against 15.5 us for 8 sequences (k 16: 1 of them here).
+// Up to this many a bound is found maximum by maximum, beyond by bits (which took 9.4, 13.9 and 16.0 us where
+// it is 8.8, 13.4 and 15.4 now, in the three cases above; up to 8: no difference from 3).
 constexpr int kFewMaxima = 3;
 
 // A bound that at least r of a wave's keys reach (`ord` the logit's order, 0 for none, `token` unique)
