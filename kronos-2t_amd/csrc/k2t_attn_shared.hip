@@ -711,8 +711,10 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs A, int pai
         load(w0);
         const bool live = mine < n && (mine < A.np ? mine < np : mine - A.np < nt);
         const float mn = fmaxf(m, wave_max_f(live ? st.x : -INFINITY));
-        if (mn == -INFINITY) continue;
-        const float e = live ? __builtin_amdgcn_exp2f(st.x - mn) : 0.0f, corr = __builtin_amdgcn_exp2f(m - mn);
+        if (!__any(live)) continue;
+        // (parts whose scores are all NaN have no maximum either, and a sum of NaN that has to count)
+        const float from = mn == -INFINITY ? 0.0f : mn;
+        const float e = live ? __builtin_amdgcn_exp2f(st.x - from) : 0.0f, corr = __builtin_amdgcn_exp2f(m - from);
         l = fmaf(l, corr, wave_sum_f(live ? st.y * e : 0.0f));
 #pragma unroll
         for (int k = 0; k < E; k++) o[k] *= corr;

@@ -295,6 +295,27 @@ def test_attention_of_bad_rows_stays_in_them(gpu_ctx, bits, hd, prefix):
         assert r == 1 or not np.isfinite(bad[r, heads]).all()
 
 
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 128)])
+@pytest.mark.parametrize("first,last", [(0, 8192), (0, 12000), (8192, 12000), (5000, 5001)])
+def test_attention_of_nan_over_many_parts(gpu_ctx, bits, hd, first, last):
+    """NaN scores on end, for as many positions as the joining of the parts takes at a time: they reach the
+    output, whatever the other positions hold."""
+    rng = np.random.default_rng(first + last)
+    beams, nq, nkv, prefix, tail = 2, 9, 3, 12000, 4
+    pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+    pre[1][:, 1, first:last] = np.nan if bits == 8 else 0x7FC0  # (the middle KV head's: q heads 3 to 5)
+    q = rng.standard_normal((beams, nq * hd)).astype(np.float32)
+    out = torch.zeros((beams, nq, hd), device="cuda")
+    _, p = rows_of(pre, prefix)
+    _, t = rows_of(tl, tail)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(bits, dev(q), nq * hd, 1, beams, nq, nkv, hd, p, t, hd ** -0.5, out, ws)
+    gpu_ctx.sync()
+    out = out.cpu().numpy()
+    assert np.isnan(out[:, 3:6]).all()
+    assert np.isfinite(out[:, :3]).all() and np.isfinite(out[:, 6:]).all()
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 def test_attention_weights_far_apart_and_scales_of_any_size(gpu_ctx, bits):
     """One position takes all the weight, wherever it lies; V scales from 1e-12 to 1e12."""
