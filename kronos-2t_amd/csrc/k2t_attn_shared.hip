@@ -7,8 +7,10 @@
 // The rows of a sequence and the q heads of a KV head are columns of one matrix against the same K and
 // V, so both products are matrix products: scores S^T = K Q^T by the int8 MFMA, whose sums are exact,
 // and outputs O^T = V^T W^T by the f16 MFMA. V's codes are exact in f16; a weight times its V scale is
-// split into two f16 pieces that hold 21 bits of it, so nothing is lost next to an fp32 product.
-// Maxima are raised lazily, sums and outputs are fp32 and joined in a fixed order.
+// split into two f16 pieces that hold 21 bits of it (24 in an fp32 product, at several times the MFMAs).
+// f16's range decides what the running softmax refers to: not a column's largest score, but its largest
+// product of weight and V scale, so that a large scale of small weight takes no bits from the others.
+// References are raised lazily, sums and outputs are fp32 and joined in a fixed order.
 //
 // Work is cut into (sequence, KV head, part of the positions, 16 or 32 columns), about two workgroups per
 // CU; the parts' outputs are joined by a second kernel. The waves of a workgroup take tiles of 32
@@ -39,9 +41,16 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = 4, kTile = 32;  // waves of a workgroup; positions of a wave's tile
-// A running maximum is raised once a score passes it by more than this (in powers of two): raising it
-// rescales the outputs, and some column of a tile would nearly always ask for it.
-constexpr float kSlack = 6.0f;
+// A column's reference m is a power of two such that its products 2^(s - m) * V scale * kLift have reached 2^8
+// and stay below 2^15: pieces below f16's smallest step, 2^-24, are then 2^-32 of the largest product. It is
+// raised (a rescaling of the outputs, which some column of a tile would nearly always ask for) only where a
+// product would pass 2^15, and then to bring that one to 2^8 .. 2^9.  kLift makes s - m, which fp32 rounds by
+// 2^-24 of itself, a small number for scales of the usual size (2^-8 .. 1).
+constexpr float kTop = 9.0f, kLimit = 15.0f, kLift = 256.0f, kLog2Lift = 8.0f;
+// Scales below 2^-100 count as that much in the reference, so that a weight is at most 2^107 and a sum of
+// 2^16 of them finite; an NF4 head's second block has a reference of its own (its scales may be of another
+// size), but a weight refers to the first, which therefore counts as 2^-60 of the second at least.
+constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct SharedArgs {
@@ -55,7 +64,7 @@ struct SharedArgs {
     int pre_items;
     float attn_scale;
     float *part;   // [row][head][np + nt][HD]
-    float2 *stat;  // [row][head][np + nt]: maximum (in powers of two), sum
+    float2 *stat;  // [row][head][np + nt]: reference (in powers of two), sum
     float *out;
 };
 
@@ -215,26 +224,34 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_
     lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
 }
 
-// What a wave carries from tile to tile for NQ tiles of 16 columns: lane li is a column.
-// The factor c = 2^(135 - cexp) brings the largest V scale to 2^8 .. 2^9, so that the weights' f16
-// pieces neither overflow (a weight is at most 2^kSlack) nor lose bits.
-template <int HD, int NQ>
+// What a wave carries from tile to tile for NQ tiles of 16 columns: lane li is a column.  SN: V scales of a
+// slot (NF4 heads of two blocks have one each).
+template <int HD, int NQ, int SN>
 struct State {
-    v4f o[NQ][HD / 16];  // output tile b of column li, times c
-    float m[NQ], l[NQ];  // running maximum (powers of two); this lane's share of the sum
-    uint32_t cexp;       // exponent (biased) of the largest V scale seen, which sets the factor c; 0: none yet
+    v4f o[NQ][HD / 16];  // output tile b of column li: sums of 2^(s - m) V, times kLift (block 1: and 2^(m - m1))
+    float m[NQ], l[NQ];  // reference (a whole number; -FLT_MAX: no score yet); this lane's share of the sum of 2^(s - m)
+    float m1[SN > 1 ? NQ : 1], up1[SN > 1 ? NQ : 1];  // block 1's own reference, and 2^(m - m1) kLift
 
     __device__ __forceinline__ void clear() {
-        cexp = 0;
 #pragma unroll
         for (int a = 0; a < NQ; a++) {
-            m[a] = -INFINITY;
+            m[a] = -FLT_MAX;
             l[a] = 0.0f;
+            if constexpr (SN > 1) {
+                m1[a] = -FLT_MAX;
+                up1[a] = kLift;
+            }
 #pragma unroll
             for (int b = 0; b < HD / 16; b++) o[a][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
-    __device__ __forceinline__ float back() const { return cexp ? __uint_as_float((cexp - 8u) << 23) : 0.0f; }  // 1 / c
+    // What takes output tile b of column tile a back to sums of 2^(s - m) V.
+    __device__ __forceinline__ float back(int a, int b) const {
+        if constexpr (SN > 1) {
+            if (b >= 4) return __builtin_amdgcn_exp2f(m1[a] - m[a]) * (1.0f / kLift);
+        }
+        return 1.0f / kLift;
+    }
 };
 
 // Scores of 16 positions x 16 columns, 64-block b of NB: int8 sums the blocks' dots, which are exact,
@@ -253,54 +270,79 @@ __device__ __forceinline__ void scores(const v4i (&kf)[NB], const v4i (&qb)[NB],
     }
 }
 
+// log2 of a positive float by its bits, plus `add`: they are its exponent and then its mantissa, at most 0.09
+// below the logarithm, and a product so much past the limit is still below f16's largest.
+__device__ __forceinline__ float log2_bits(uint32_t bits, float add) { return fmaf((float)bits, 0x1p-23f, add - 127.0f); }
+__device__ __forceinline__ float column_max(float v) {  // over a column's four lanes
+    v = fmaxf(v, xor_lane(v, 16));
+    return fmaxf(v, xor_lane(v, 32));
+}
+
 // Weights of a tile from its scores: t = dots * K scales of positions 16 j + 4 lg + i of the columns
-// li, n of the tile's 32 exist; vs = V scales.  Leaves pairs of weights times V scale times c as hi and
-// lo pieces.  Maxima and c change in one place, off the usual path.
+// li, n of the tile's 32 exist; vs = V scales.  Leaves pairs of weights times V scale times kLift as hi and
+// lo pieces.  References change in one place, off the usual path: where the largest score of a lane's eight
+// positions with the largest of their scales would pass the limit.
 template <int HD, int NQ, int SN>
-__device__ __forceinline__ void weights(State<HD, NQ> &S, float (&t)[NQ][2][4], const float (&qas)[NQ], float (&vs)[2][4][SN],
+__device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][4], const float (&qas)[NQ], float (&vs)[2][4][SN],
                                         int n, uint32_t lg, uint32_t (&ph)[NQ][SN][4], uint32_t (&pl)[NQ][SN][4]) {
-    float vmax = 0.0f, top[NQ];
+    float lv[SN];
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int k = 0; k < SN; k++) {
+        uint32_t vmax = 0;  // (a negative scale, which is none of the cache's, counts as a large one here)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int k = 0; k < SN; k++) vmax = fmaxf(vmax, fabsf(vs[j][i][k]));
-    const uint32_t e_lane = __float_as_uint(vmax) >> 23;
-    bool news = e_lane > S.cexp;
+            for (int i = 0; i < 4; i++) vmax = max(vmax, __float_as_uint(vs[j][i][k]));
+        lv[k] = log2_bits(max(vmax, __float_as_uint(kLeastScale)), kLog2Lift - kLimit);
+    }
+    if constexpr (SN > 1) lv[0] = fmaxf(lv[0], lv[1] - kApart);
+    float top[NQ];
+    bool news = false;
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
         top[a] = fmaxf(fmaxf(fmaxf(t[a][0][0], t[a][0][1]), fmaxf(t[a][0][2], t[a][0][3])),
                        fmaxf(fmaxf(t[a][1][0], t[a][1][1]), fmaxf(t[a][1][2], t[a][1][3])));
-        top[a] *= qas[a];  // (qas >= 0: the largest t is the largest score)
-        news |= top[a] > S.m[a] + kSlack;
+        // (qas >= 0: the largest t is the largest score)
+        news |= fmaf(top[a], qas[a], lv[0]) > S.m[a];
+        if constexpr (SN > 1) news |= fmaf(top[a], qas[a], lv[1]) > S.m1[a];
     }
     if (__any(news)) {
-        uint32_t e = max(e_lane, (uint32_t)xor_lane((int)e_lane, 16));
-        e = max(e, (uint32_t)xor_lane((int)e, 32));
-        e = max(max(e, S.cexp), 27u);  // (scales below 2^-100 share its factor)
-        const float down = S.cexp ? ldexpf(1.0f, (int)S.cexp - (int)e) : 1.0f;
-        S.cexp = e;
 #pragma unroll
         for (int a = 0; a < NQ; a++) {
-            float mn = fmaxf(top[a], xor_lane(top[a], 16));
-            mn = fmaxf(mn, xor_lane(mn, 32));
-            mn = mn > S.m[a] + kSlack ? mn : S.m[a];
-            const float corr = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
-            S.m[a] = mn;
-            S.l[a] *= corr;
+            float u[SN];
 #pragma unroll
-            for (int b = 0; b < HD / 16; b++) S.o[a][b] = S.o[a][b] * (corr * down);
+            for (int k = 0; k < SN; k++) {
+                u[k] = fmaf(top[a], qas[a], kLog2Lift - 100.0f);  // (kLeastScale)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        u[k] = fmaxf(u[k], fmaf(t[a][j][i], qas[a], log2_bits(__float_as_uint(vs[j][i][k]) & 0x7FFFFFFFu, kLog2Lift)));
+            }
+            if constexpr (SN > 1) u[0] = fmaxf(u[0], u[1] - kApart);
+            const float most = column_max(u[0]), mn = most > S.m[a] + kLimit ? ceilf(most) - kTop : S.m[a];
+            const float down = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
+            float down1 = down;
+            S.m[a] = mn;
+            S.l[a] *= down;
+            if constexpr (SN > 1) {
+                // (no lower than 2^-120 of the first block's: 2^(m - m1) stays finite)
+                const float most1 = column_max(u[SN - 1]);
+                const float m1 = fmaxf(most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - 120.0f);
+                down1 = m1 == S.m1[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m1[a] - m1);
+                S.m1[a] = m1;
+                S.up1[a] = __builtin_amdgcn_exp2f(mn - m1) * kLift;
+            }
+#pragma unroll
+            for (int b = 0; b < HD / 16; b++) S.o[a][b] = S.o[a][b] * (SN > 1 && b >= 4 ? down1 : down);
         }
     }
-    const float c = __uint_as_float((262u - S.cexp) << 23);
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
-        const float m = S.m[a] == -INFINITY ? 0.0f : S.m[a];
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) t[a][j][i] = __builtin_amdgcn_exp2f(fmaf(t[a][j][i], qas[a], -m));
+            for (int i = 0; i < 4; i++) t[a][j][i] = __builtin_amdgcn_exp2f(fmaf(t[a][j][i], qas[a], -S.m[a]));
     }
     if (n < kTile) {  // positions behind the last one repeat it: they weigh nothing
 #pragma unroll
@@ -319,9 +361,15 @@ __device__ __forceinline__ void weights(State<HD, NQ> &S, float (&t)[NQ][2][4], 
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i += 2)
-                    split2(t[a][j][i] * (vs[j][i][k] * c), t[a][j][i + 1] * (vs[j][i + 1][k] * c), ph[a][k][2 * j + i / 2],
-                           pl[a][k][2 * j + i / 2]);
+                for (int i = 0; i < 4; i += 2) {
+                    float x[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        if (SN > 1 && k) x[e] = (t[a][j][i + e] * vs[j][i + e][k]) * S.up1[SN > 1 ? a : 0];
+                        else x[e] = t[a][j][i + e] * (vs[j][i + e][k] * kLift);
+                    }
+                    split2(x[0], x[1], ph[a][k][2 * j + i / 2], pl[a][k][2 * j + i / 2]);
+                }
     }
 }
 
@@ -428,11 +476,10 @@ struct Join {
     float m[kWaves][16], l[kWaves][16];
     __align__(16) float o[kWaves][16][HD + 4];
 };
-template <int HD, int BITS, int NQ, bool WHOLE>
-__device__ __forceinline__ void join(const SharedArgs &A, const Item &I, const State<HD, NQ> &S, Join<HD> &J) {
+template <int HD, int BITS, int NQ, bool WHOLE, int SN>
+__device__ __forceinline__ void join(const SharedArgs &A, const Item &I, const State<HD, NQ, SN> &S, Join<HD> &J) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
-    const float back = S.back();
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
         if (16 * a >= I.n) break;
@@ -446,16 +493,16 @@ __device__ __forceinline__ void join(const SharedArgs &A, const Item &I, const S
 #pragma unroll
         for (int b = 0; b < HD / 16; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) J.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * back;
+            for (int i = 0; i < 4; i++) J.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * S.back(a, b);
         __syncthreads();
         const int x = (int)(tid >> 4), sl = (int)(tid & 15u);  // column, sixteenth of its dimensions
         if (16 * a + x < I.n) {
-            float M = -INFINITY, L = 0.0f, e[kWaves];
+            float M = -FLT_MAX, L = 0.0f, e[kWaves];
 #pragma unroll
             for (int w = 0; w < kWaves; w++) M = fmaxf(M, J.m[w][x]);
 #pragma unroll
             for (int w = 0; w < kWaves; w++) {
-                e[w] = J.m[w][x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(J.m[w][x] - M);
+                e[w] = __builtin_amdgcn_exp2f(J.m[w][x] - M);
                 L = fmaf(J.l[w][x], e[w], L);
             }
             const int c = I.col0 + 16 * a + x;
@@ -539,7 +586,7 @@ __device__ __forceinline__ void attend(const SharedArgs &A, const Item &I, Share
         qas[a] = sh.q.qas[16 * a + li];
         query_operand<HD, BITS>(sh.q.q[16 * a + li], lg, qb[a]);
     }
-    State<HD, NQ> S;
+    State<HD, NQ, SN> S;
     S.clear();
     for (int i = wave; i < tiles; i += kWaves) {
         const int left = i < first ? I.len[0] - kTile * i : I.len[1] - kTile * (i - first);
@@ -593,7 +640,7 @@ __device__ __forceinline__ void attend(const SharedArgs &A, const Item &I, Share
                 for (int a = 0; a < NQ; a++) S.o[a][4 * g + u] = add_tile(va[u], ph[a][g & kBlocks], S.o[a][4 * g + u]);
         }
     }
-    join<HD, BITS, NQ, WHOLE>(A, I, S, sh.j);
+    join<HD, BITS, NQ, WHOLE, SN>(A, I, S, sh.j);
 }
 
 template <int HD, int BITS, int NQ>
@@ -711,10 +758,8 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs A, int pai
         load(w0);
         const bool live = mine < n && (mine < A.np ? mine < np : mine - A.np < nt);
         const float mn = fmaxf(m, wave_max_f(live ? st.x : -INFINITY));
-        if (!__any(live)) continue;
-        // (parts whose scores are all NaN have no maximum either, and a sum of NaN that has to count)
-        const float from = mn == -INFINITY ? 0.0f : mn;
-        const float e = live ? __builtin_amdgcn_exp2f(st.x - from) : 0.0f, corr = __builtin_amdgcn_exp2f(m - from);
+        if (mn == -INFINITY) continue;  // (no live one: -FLT_MAX in a part whose scores are NaN)
+        const float e = live ? __builtin_amdgcn_exp2f(st.x - mn) : 0.0f, corr = __builtin_amdgcn_exp2f(m - mn);
         l = fmaf(l, corr, wave_sum_f(live ? st.y * e : 0.0f));
 #pragma unroll
         for (int k = 0; k < E; k++) o[k] *= corr;

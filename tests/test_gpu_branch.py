@@ -346,6 +346,66 @@ def test_attention_weights_far_apart_and_scales_of_any_size(gpu_ctx, bits):
         assert (err <= bound).all(), (spot, float((err / bound).max()))
 
 
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("beams,nq,nkv,prefix,tail", [(3, 4, 2, 50, 20), (3, 4, 2, 1500, 200), (61, 32, 8, 4600, 3)])
+@pytest.mark.parametrize("kind", ["outlier", "spread", "sink", "blocks", "none"])
+def test_attention_of_v_scales_far_apart(gpu_ctx, bits, hd, beams, nq, nkv, prefix, tail, kind):
+    """V scales that differ from position to position (NF4: from block to block too). outlier: every tile
+    of 32 holds a position of negligible weight whose scale is 2^30 times the others'; spread: any scales
+    within 2^-30 .. 2^30; sink: the position that takes nearly all the weight holds a scale 2^-40 of the others',
+    and every seventh V head is zero; blocks: the scales of NF4's second blocks are 2^-44 of the first's (2^44 in
+    the tails); none: no V scale but zero in the first tiles.  Weights refer to products with V scales here, so an
+    exponent is off by a rounding of up to 2 |z| / ln 2 + 44 + 17, which is 2 (|z| + 43) u in weight and total: within
+    the bound's 2 (8 |z| + 4) u and the 2 x 43 u of its 2 x 288 that sums of at most 128 terms on end leave."""
+    rng = np.random.default_rng(hd + bits + prefix)
+    pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+    for c in (pre, tl):
+        n, rows = c[1].shape[2], c[1].shape[0]
+        # all positions' K heads agree with the queries in element 0, those of `apart` oppose them
+        apart = np.arange(n) % 32 == (9 if n > 32 else 1) if kind == "outlier" else np.arange(n) != 0
+        if kind in ("outlier", "sink"):
+            first = np.where(apart, -100, 100) if kind == "outlier" or c is pre else np.full(n, -100)
+            if bits == 8:
+                c[0][..., 0] = first
+                c[1][:] = 0.02
+            else:
+                c[0][..., 0] = (c[0][..., 0] & 0xF0) | np.where(first > 0, 14, 1)  # (codes 96, -96)
+                c[1][:] = np.float32(0.02).view(np.uint32) >> 16
+        shape = c[3].shape
+        size = np.ones(shape, np.float32)
+        up = (slice(None), slice(None))
+        if kind == "outlier":
+            size[up + (apart,)] = 2.0 ** 30
+        elif kind == "spread":
+            size = (2.0 ** rng.uniform(-30, 30, shape)).astype(np.float32)
+        elif kind == "sink":
+            size[up + (slice(3, None, 7),)] = 0
+            if c is pre:
+                size[up + (0,)] = 2.0 ** -40
+        elif kind == "blocks":
+            size[..., -1] = 2.0 ** -44 if c is pre else 2.0 ** 44  # (int8: the last position's)
+        else:
+            size[up + (slice(0, 300 if n > 300 else 32),)] = 0
+        v = (c[3] if bits == 8 else R.bf16(c[3])) * size
+        c[3][:] = v if bits == 8 else (v.view(np.uint32) >> 16).astype(np.uint16)
+    q = rng.standard_normal((beams, nq, hd))
+    if kind in ("outlier", "sink"):  # some 30 between the scores of the two kinds of positions
+        q[..., 0] = 60 * (hd / 64) ** 0.5
+        q = R.unrotate(q)
+    q = q.astype(np.float32)
+    out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+    _, p = rows_of(pre, prefix)
+    _, t = rows_of(tl, tail)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(bits, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, t, hd ** -0.5, out, ws)
+    gpu_ctx.sync()
+    rows = list(range(beams)) if beams < 4 else [0, 31, 60]  # (the reference of a few rows)
+    want, bound = R.attention(bits, q[rows], pre, [a[rows] for a in tl], [prefix], [tail] * len(rows), len(rows), nq, nkv, hd,
+                              hd ** -0.5)
+    err = np.abs(out.cpu().numpy()[rows] - want)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
 def test_attention_agrees_with_attn_decode(gpu_ctx):
     """A row's output is the one-sequence operator's over its prefix and tail laid end to end."""
     rng = np.random.default_rng(11)
