@@ -463,7 +463,8 @@ int32_t k2t_kv_reorder(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const 
 int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_stride, int32_t n_seq, int32_t beams,
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const k2t_kv_rows *prefix,
                         const k2t_kv_rows *tail, float attn_scale, float *d_out, void *d_ws, size_t ws_bytes);
-/* Its workspace for caches of up to prefix_len and tail_len positions (their `len`). */
+/* Its workspace for caches of up to prefix_len and tail_len positions (their `len`): what serves these
+ * lengths serves every shorter one, and a missing cache. */
 int32_t k2t_attn_shared_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, int32_t n_heads, int32_t n_kv_heads,
                                   int32_t head_dim, int32_t prefix_len, int32_t tail_len, size_t *bytes);
 /* Beam search's choice: the k best continuations of every sequence over its `beams` rows and

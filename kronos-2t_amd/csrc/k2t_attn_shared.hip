@@ -842,7 +842,30 @@ Plan plan_of(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_
     cut(tail_len, (size_t)s.n_seq * s.beams * s.nkv * P.tgroups + (size_t)s.n_seq * s.nkv * P.pgroups * P.np, P.nt, P.tlen);
     return P;
 }
-size_t part_slots(const SharedShape &s, const Plan &P) { return (size_t)s.n_seq * s.beams * s.nq * (P.np + P.nt); }
+size_t part_slots(const SharedShape &s, int parts) { return (size_t)s.n_seq * s.beams * s.nq * parts; }
+size_t ws_bytes_of(const SharedShape &s, int parts) {
+    return std::max<size_t>(16, part_slots(s, parts) * (s.hd * sizeof(float) + sizeof(float2)));
+}
+// At least the parts (np + nt) of every plan of up to these lengths.  One plan's are not monotone: parts are
+// whole tiles for every wave, so that a longer cache may be cut into fewer.  For every width of prefix items (two
+// tiles of columns only where the longest has them) and np: as many tail parts as such a plan may want.
+int most_parts(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_len) {
+    const Plan P = plan_of(ctx, s, prefix_len, tail_len);
+    if (P.whole) return 0;  // (and so is every shorter one)
+    const int least = kTile * kWaves, cols = s.beams * (s.nq / s.nkv);
+    const size_t cus = (size_t)std::max(1, ctx->num_cus), heads = (size_t)s.n_seq * s.nkv;
+    const auto cut = [&](int len, size_t items) {
+        const size_t want = std::max<size_t>(1, 2 * cus / std::max<size_t>(1, items));
+        return (int)std::min<size_t>(((size_t)len + least - 1) / least, want);
+    };
+    int most = 0;
+    for (int nq = 1; nq <= P.nq; nq++) {
+        const size_t pre = heads * ((cols + 16 * nq - 1) / (16 * nq));
+        for (int np = 0; np <= cut(prefix_len, pre); np++)
+            most = std::max(most, np + cut(tail_len, heads * s.beams * P.tgroups + pre * np));
+    }
+    return most;
+}
 
 template <int HD, int BITS>
 void launch_parts(hipStream_t st, const SharedArgs &A, const Plan &P, size_t items) {
@@ -874,8 +897,7 @@ void launch_shared(hipStream_t st, int bits, const SharedArgs &A, const SharedSh
 }  // namespace
 
 size_t attn_shared_ws_bytes(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_len) {
-    const Plan P = plan_of(ctx, s, prefix_len, tail_len);
-    return std::max<size_t>(16, part_slots(s, P) * (s.hd * sizeof(float) + sizeof(float2)));
+    return ws_bytes_of(s, most_parts(ctx, s, prefix_len, tail_len));
 }
 
 void launch_attn_shared(k2t_ctx *ctx, hipStream_t st, int bits, const float *q, size_t q_stride, const SharedShape &s,
@@ -899,7 +921,7 @@ void launch_attn_shared(k2t_ctx *ctx, hipStream_t st, int bits, const float *q, 
     A.tgroups = P.tgroups;
     A.attn_scale = attn_scale;
     A.part = (float *)ws;
-    A.stat = (float2 *)(A.part + part_slots(s, P) * s.hd);
+    A.stat = (float2 *)(A.part + part_slots(s, P.np + P.nt) * s.hd);
     A.out = out;
     const size_t units = (size_t)s.n_seq * s.nkv * P.np;
     const size_t pre = (units + 7) / 8 * 8 * P.pgroups, tails = (size_t)s.n_seq * s.beams * s.nkv * P.nt * P.tgroups;
@@ -955,7 +977,8 @@ int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
                        at(d_q) % 16 == 0,
                    "d_q must be 16-byte aligned, q_stride a multiple of 4, no smaller than a row, below 2^31");
         branch_arg((at(d_out) | at(d_ws)) % 16 == 0, "d_out and d_ws must be 16-byte aligned");
-        const size_t need = attn_shared_ws_bytes(ctx, s, prefix ? prefix->len : 0, tail ? tail->len : 0);
+        const Plan P = plan_of(ctx, s, prefix ? prefix->len : 0, tail ? tail->len : 0);
+        const size_t need = ws_bytes_of(s, P.np + P.nt);
         if (ws_bytes < need)
             throw Error(K2T_E_ARG, "the workspace holds " + std::to_string(ws_bytes) + " bytes, " +
                                        std::to_string(need) + " are needed");

@@ -41,6 +41,7 @@ void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const in
 struct SharedShape {
     int n_seq, beams, nq, nkv, hd;
 };
+// Workspace for caches of up to these lengths.
 size_t attn_shared_ws_bytes(const k2t_ctx *ctx, const SharedShape &s, int prefix_len, int tail_len);
 // prefix / tail: their row caches' descriptions (cap 0: none); the layer's block is the caller's
 // pointer arithmetic (kv_rows_at).

@@ -833,8 +833,8 @@ void free_beams(k2t_model *m) {
 void ensure_beams(k2t_model *m, int rows, int n_steps, int prefix) {
     const k2t_model_config &c = m->cfg;
     const SharedShape shape{1, rows, c.n_heads, c.n_kv_heads, c.head_dim};
-    size_t ws = std::max(beam_select_ws_bytes(1, rows, c.vocab, rows), beam_select_ws_bytes(1, 1, c.vocab, rows));
-    for (int t = 1; t < n_steps; t++) ws = std::max(ws, attn_shared_ws_bytes(m->ctx, shape, prefix, t));
+    const size_t ws = std::max({beam_select_ws_bytes(1, rows, c.vocab, rows), beam_select_ws_bytes(1, 1, c.vocab, rows),
+                                attn_shared_ws_bytes(m->ctx, shape, prefix, n_steps - 1)});
     if (rows == m->beam_rows && n_steps <= m->beam_cap && ws <= m->beam_ws_bytes) return;
     hip_check(hipStreamSynchronize(m->stream), "beam workspace sync");
     free_beams(m);

@@ -3,6 +3,8 @@ argument is K2T_E_ARG before anything touches a device (where there is none, a c
 checks ends in K2T_E_HIP)."""
 import ctypes as C
 
+import pytest
+
 import branch_ref as R
 import k2t
 
@@ -72,6 +74,38 @@ def test_attention():
             [{0: None}, {1: -1}, {2: 0}, {3: 9}, {5: 256}, {6: -1}, {7: -1}, {8: None}])
     if k2t.lib().k2t_device_count() == 0:
         assert call("k2t_attn_shared", *good) == HIP
+
+
+@pytest.mark.parametrize("shape", [(1, 8, 32, 32, 64), (3, 8, 32, 8, 128), (1, 8, 32, 8, 128), (1, 8, 32, 4, 128),
+                                   (1, 64, 32, 4, 128), (1, 1, 1, 1, 64), (1, 4, 9, 3, 64), (4, 64, 32, 8, 128), (2, 3, 40, 2, 64)])
+def test_attention_workspace_serves_shorter_caches(shape):
+    """k2t_attn_shared_workspace of the longest caches is enough for a call with any shorter ones (a longer
+    cache may be cut into fewer parts than a shorter one), and no less than that of the shorter ones."""
+    ctx = (C.c_int32 * 1024)(*[256] * 1024)  # a context of 256 CUs, on a device that no machine has
+
+    def workspace(p, t):
+        n = C.c_size_t()
+        assert call("k2t_attn_shared_workspace", ctx, *shape, p, t, C.byref(n)) == 0
+        return n.value
+
+    def accepted(p, t, ws):
+        n_seq, beams, nq, nkv, hd = shape
+        pre, tail = (rows(cap=1 << 24, length=n) if n else None for n in (p, t))
+        if not (p or t):
+            pre = rows(length=0)
+        rc = call("k2t_attn_shared", ctx, 8, P, nq * hd, *shape, pre, tail, 0.125, P, P, ws)
+        assert rc in (ARG, HIP)
+        return rc == HIP  # (past the checks: the device is the one that does not exist)
+
+    lengths = [0, 1, 31, 45, 90, 127, 128, 129, 384, 385, 511, 700, 768, 769, 1000, 1153, 1280, 1400, 2048, 2100, 3840, 4100, 9000,
+               65537, 1 << 20]
+    for p, t in [(2100, 64), (2048, 64), (1400, 90), (45, 769), (1000, 385), (4100, 90), (0, 4100), (9000, 0), (1 << 20, 1 << 20),
+                 (65537, 700)]:
+        ws = workspace(p, t)
+        for a in [n for n in lengths if n <= p]:
+            for b in [n for n in lengths if n <= t]:
+                assert accepted(a, b, ws), (p, t, a, b)
+                assert workspace(a, b) <= ws, (p, t, a, b)
 
 
 def test_select():
