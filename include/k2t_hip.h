@@ -470,10 +470,12 @@ int32_t k2t_attn_shared_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, in
 /* Beam search's choice: the k best continuations of every sequence over its `beams` rows and
  * the vocabulary.  Row r's logits are d_logits + r * row_stride, its score so far is d_scores[r]
  * (-inf: the row is not in use); the candidate (r, token) scores d_scores[r] + log softmax(logits
- * of r)[token], summed in 64 bits.  A logit of NaN counts as -inf, +inf as the largest float;
- * scores of -inf or NaN are no candidates.  d_done[r] != 0 (nullable; needs eos >= 0): the row has
- * ended, its one candidate is (r, eos) at its score.  Best first; equal scores: the lower row,
- * then the higher logit, then the lower token.  d_out_* [n_seq][k]: score, token, row of the
+ * of r)[token], in 64 bits but for the sums of exponentials of 4096 logits each, which are fp32: a
+ * row's log softmax is off by less than 2^-18, by the same for all its tokens, so that candidates of
+ * two rows within 2^-17 may come in either order.  A logit of NaN counts as -inf, +inf as the
+ * largest float; scores of -inf or NaN are no candidates.  d_done[r] != 0 (nullable; needs eos >= 0):
+ * the row has ended, its one candidate is (r, eos) at its score.  Best first; equal scores: the lower
+ * row, then the higher logit, then the lower token.  d_out_* [n_seq][k]: score, token, row of the
  * batch (what k2t_kv_reorder takes), and (nullable) done = the row had ended or token == eos
  * (eos -1: none).  Where a sequence has fewer candidates the rest get score -inf, token max(eos,
  * 0), its first row, and done 1.  With k == beams the output scores and done flags may be the

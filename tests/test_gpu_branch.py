@@ -522,6 +522,26 @@ def test_select_ties_masks_and_odd_values(gpu_ctx):
         assert np.array_equal(s[~fin], w32[~fin]) and (np.abs(s - ws)[fin] <= score_tol(ws)[fin]).all(), scores
 
 
+def test_select_joins_slices_in_64_bits(gpu_ctx):
+    """One logit in every 4096, so that no fp32 sum has two terms: rows whose scores are 2^-45 apart come in
+    order. (A row's score so far is the fp32 next to its log-sum, so that all the best ones are next to zero.)"""
+    rng = np.random.default_rng(12)
+    beams, slices = 48, 9
+    logits = np.full((beams, 4096 * slices), -np.inf, np.float32)
+    lse = np.empty(beams)
+    for r in range(beams):
+        x = rng.uniform(-3, 0, slices).astype(np.float32)
+        x[rng.integers(slices)] = 0
+        logits[r, np.arange(slices) * 4096 + rng.integers(0, 4096, slices)] = x
+        lse[r] = np.log(np.exp(x.astype(np.float64)).sum())
+    scores = lse.astype(np.float32)
+    ws, wt, wp, wd, gap = R.select(logits, scores, None, 1, beams, beams, -1)
+    assert gap > 2.0 ** -45 and len(set(wp[0])) == beams  # (one candidate of every row; 64 bits' own roundings: 2^-50)
+    s, t, p, d = run_select(gpu_ctx, logits, scores, None, 1, beams, beams, -1)
+    assert np.array_equal(t, wt) and np.array_equal(p, wp) and np.array_equal(d, wd)
+    assert (np.abs(s - ws) <= np.abs(ws) * R.U + 2.0 ** -50).all()
+
+
 @pytest.mark.parametrize("order", ["rising", "falling", "blocks", "equal"])
 def test_select_of_ordered_logits(gpu_ctx, order):
     """The k best all in one place, or all equal: the same choice however the slices are cut."""
