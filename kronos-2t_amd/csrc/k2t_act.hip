@@ -18,11 +18,12 @@ namespace k2t {
 
 // One wave's chunk c of a row: sign flip with the chunk's mask, butterflies and int8.
 __device__ __forceinline__ void quant_chunk(float v, int c, size_t gc, uint32_t lane, const uint64_t *signs,
-                                            int8_t *q, float *scales, int32_t *sums) {
+                                            int8_t *q, float *scales, int32_t *sums, ActTiles tiles = ActTiles{},
+                                            int tok = 0, int nc = 0) {
     // (the context's table holds the masks of the first kSignBlocks chunks)
     const uint32_t neg = c < kSignBlocks ? (uint32_t)(signs[c] >> lane) & 1u : hadamard_sign_bit((uint64_t)c, lane);
     v = wave_butterflies64(flip_sign(v, neg) * 0.125f, lane);
-    quant_chunk_store(v, lane, q + gc * 64, scales + gc, sums + gc);
+    quant_chunk_store(v, lane, q + gc * 64, scales + gc, sums + gc, tiles.xt, tiles.st, tiles.ut, tok, c, nc);
 }
 
 __global__ __launch_bounds__(256) void act_quant_kernel(const float *__restrict__ x,
@@ -30,7 +31,7 @@ __global__ __launch_bounds__(256) void act_quant_kernel(const float *__restrict_
                                                         const float *__restrict__ inv_rms, int K,
                                                         int total_chunks, const uint64_t *__restrict__ signs,
                                                         int8_t *__restrict__ q, float *__restrict__ scales,
-                                                        int32_t *__restrict__ sums) {
+                                                        int32_t *__restrict__ sums, ActTiles tiles) {
     const uint32_t lane = threadIdx.x & 63;
     const int gc = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (gc >= total_chunks) return;
@@ -38,7 +39,7 @@ __global__ __launch_bounds__(256) void act_quant_kernel(const float *__restrict_
     const int tok = gc / nc, c = gc - tok * nc;
     float v = x[(size_t)gc * 64 + lane];
     if (w) v = (v * inv_rms[tok]) * w[(size_t)c * 64 + lane];
-    quant_chunk(v, c, (size_t)gc, lane, signs, q, scales, sums);
+    quant_chunk(v, c, (size_t)gc, lane, signs, q, scales, sums, tiles, tok, nc);
 }
 
 // RMSNorm + FWHT + int8 in one launch: inv_rms = 1 / sqrt(sum(x^2)/K + eps) (real_llm.rs:6929)
@@ -141,11 +142,11 @@ void launch_expf_map(hipStream_t st, const float *x, float *y, size_t n) {
 }
 
 void launch_act_quant(k2t_ctx *ctx, const float *x, const float *w, const float *inv_rms, int K,
-                      int ntok, int8_t *q, float *scales, int32_t *sums) {
+                      int ntok, int8_t *q, float *scales, int32_t *sums, ActTiles tiles) {
     const int total = (K / 64) * ntok;
     if (total <= 0) return;
     hipLaunchKernelGGL(act_quant_kernel, dim3((total + 3) / 4), dim3(256), 0, ctx->stream, x, w,
-                       inv_rms, K, total, ctx->signs, q, scales, sums);
+                       inv_rms, K, total, ctx->signs, q, scales, sums, tiles);
     hip_check(hipGetLastError(), "act_quant launch");
 }
 

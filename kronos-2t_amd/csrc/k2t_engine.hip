@@ -442,7 +442,9 @@ struct BeamStep {
 // One forward pass over `ntok` tokens already in m->tokens, positions pos..pos+ntok-1.
 // Logits (of the last token) go to m->logits; the device position advances by ntok.
 // With `beam` the tokens are rows that continue the model's cache, each with a tail cache; every row's
-// logits go to m->beam_logits, and the model's cache and position stay as they are.
+// logits go to m->beam_logits, and the model's cache and position stay as they are.  (Every activation that a
+// batched GEMV reads in tiles is written in tiles by its producer: that GEMV's own copy would go to the context's
+// scratch, which a call on the context's stream may be using.)
 // ctx_bound: the position after the batch's last token when the host knows it (prefill;
 // never a captured step, whose position moves between replays), else 0.
 void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0, const BeamStep *beam = nullptr) {
@@ -484,6 +486,8 @@ void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0, const 
         // One token: qkv_post's work runs inside the attention kernel.  A batch stores every
         // token's K / V first (a later token of the batch attends to them).
         AttnPost post{};
+        // (none for one token: the grouped kernel writes none)
+        const ActTiles to = act_tiles_for(m, L.o, ntok);
         if (beam) {
             const size_t slots = (size_t)l * ntok * nkv * m->beam_cap;
             k2t_kv_rows tail = kv_rows_at(m->beam_tail, m->ring.bits, hd, slots), prefix{};
@@ -499,15 +503,13 @@ void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0, const 
             prefix.len = beam->prefix;
             launch_attn_shared(ctx, st, m->ring.bits, m->qkv, (size_t)(nq + 2 * nkv) * hd, SharedShape{1, ntok, nq, nkv, hd},
                                prefix, tail, attn_scale, m->attn_f, m->beam_ws);
-            launch_act_quant(ctx, m->attn_f, nullptr, nullptr, nq * hd, ntok, m->xq, m->xs, m->xsum);
+            launch_act_quant(ctx, m->attn_f, nullptr, nullptr, nq * hd, ntok, m->xq, m->xs, m->xsum, to);
         } else if (ntok == 1) {
             post = AttnPost{1, L.bias, L.q_norm, L.k_norm, m->rope, c.rms_eps};
         } else if (!qkv_posted) {
             launch_qkv_post(st, m->qkv, L.bias, L.q_norm, L.k_norm, c.rms_eps, m->rope, m->pos_dev, nq, nkv, hd, ntok,
                             l, m->ring, m->kq, m->vq, m->ks, m->vs, false);
         }
-        // (none for one token: the grouped kernel writes none)
-        const ActTiles to = beam ? ActTiles{} : act_tiles_for(m, L.o, ntok);
         if (!beam)
             launch_attention(st, m->qkv, (nq + 2 * nkv) * hd, m->kq, m->vq, m->ks, m->vs, post, m->pos_dev, l, nq, nkv,
                              hd, m->ring, attn_scale, nsplit, ntok, m->attn_part, nullptr, m->xq, m->xs, m->xsum,
@@ -547,8 +549,9 @@ void forward(k2t_model *m, int ntok, bool with_logits, int ctx_bound = 0, const 
         }
     }
     if (beam) {
-        launch_rmsnorm_act(st, ctx->signs, m->hidden, m->final_norm, c.rms_eps, d, ntok, m->xq, m->xs, m->xsum);
-        launch_gemv_ex(ctx, m->head, m->xq, m->xs, m->xsum, ntok, m->beam_logits, c.vocab, false);
+        const ActTiles th = act_tiles_for(m, m->head, ntok);
+        launch_rmsnorm_act(st, ctx->signs, m->hidden, m->final_norm, c.rms_eps, d, ntok, m->xq, m->xs, m->xsum, th);
+        launch_gemv_ex(ctx, m->head, m->xq, m->xs, m->xsum, ntok, m->beam_logits, c.vocab, false, 0, th);
         launch_advance_pos(st, m->beam_pos, 1);
         return;
     }

@@ -258,7 +258,7 @@ void check_span_timeout(k2t_ctx *ctx);
 void model_adopt(k2t_model *m, k2t_mat *mat);
 
 void launch_act_quant(k2t_ctx *ctx, const float *x, const float *w, const float *inv_rms, int K,
-                      int ntok, int8_t *q, float *scales, int32_t *sums);
+                      int ntok, int8_t *q, float *scales, int32_t *sums, ActTiles tiles = ActTiles{});
 // RMSNorm (inv_rms computed in the launch) + FWHT + int8.
 void launch_rmsnorm_quant(k2t_ctx *ctx, const float *x, const float *w, float eps, int K, int ntok, int8_t *q,
                           float *scales, int32_t *sums);

@@ -213,6 +213,48 @@ def test_mixture_of_experts_model(gpu_ctx):
         check_search(gm, [3, 250, 17], 9, n_beams, 4)
 
 
+@pytest.mark.parametrize("fmt,planes", [("nf4", None), ("n4", P55454)])
+def test_search_beside_batched_gemvs_of_the_context(gpu_ctx, fmt, planes):
+    """From 16 beams on a search's batched GEMVs read their activations in tiles. The context's scratch, into
+    which a GEMV would copy them, belongs to calls on the context's stream: products queued there come out as
+    they do alone, and so does a search that runs beside them."""
+    cfg = dict(n_layers=1, hidden=1024, n_heads=16, n_kv_heads=4, head_dim=64, intermediate=1536, vocab=4096, max_seq=40,
+               rms_eps=1e-5, rope_theta=10000.0)
+    layers, head, fn = random_model(cfg, seed=3, fmt=fmt, planes=planes)
+    gm, mats = _gpu_model(gpu_ctx, cfg, layers, head, fn, max_batch=48)
+    mat, ntok = mats[-1], 512  # (the lm_head once more, for more tokens than the search has)
+    gpu_ctx.set_stream(torch.cuda.Stream())
+    try:
+        g = torch.Generator(device="cuda").manual_seed(7)
+        xq = torch.randint(-127, 128, (ntok, 1024), generator=g, device="cuda").to(torch.int8)
+        xs = torch.rand(ntok, 16, generator=g, device="cuda") / 127
+        xsum = xq.view(ntok, 16, 64).sum(-1, dtype=torch.int32)
+        outs = [torch.empty(ntok, 4096, device="cuda") for _ in range(60)]
+        torch.cuda.synchronize()
+        gpu_ctx.gemv(mat, xq, xs, xsum, outs[0], ntok=ntok, out_stride=4096)
+        gpu_ctx.sync()
+        want = outs[0].clone()
+        for n_beams in (16, 48):
+            alone = search(gm, [3, 9, 250], 77, n_beams, 5)
+            gpu_ctx.set_mfma(2)  # (the GEMVs' own copies)
+            copied = search(gm, [3, 9, 250], 77, n_beams, 5)
+            gpu_ctx.set_mfma(1)
+            assert np.array_equal(copied[0], alone[0]) and np.array_equal(copied[1], alone[1])
+            for o in outs:
+                o.zero_()
+            torch.cuda.synchronize()
+            for o in outs:
+                gpu_ctx.gemv(mat, xq, xs, xsum, o, ntok=ntok, out_stride=4096)
+            beside = search(gm, [3, 9, 250], 77, n_beams, 5)
+            gpu_ctx.sync()
+            assert np.array_equal(beside[0], alone[0]) and np.array_equal(beside[1], alone[1])
+            assert all(torch.equal(o, want) for o in outs)
+    finally:
+        gpu_ctx.sync()
+        gpu_ctx.set_mfma(1)
+        gpu_ctx.set_stream(torch.cuda.current_stream())
+
+
 # ---------------------------------------------------------------- the operators in a row
 class Program:
     """A step of beam search over one layer's worth of heads: append the rows' K / V, attend, choose,
