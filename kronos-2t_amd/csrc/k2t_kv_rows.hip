@@ -115,7 +115,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(RowsArgs A) {
 #pragma unroll
         for (int k = 0; k < TURNS; k++) {
             float mx = group_max(fmaxf(fmaxf(fabsf(v[k][0]), fabsf(v[k][1])), fmaxf(fabsf(v[k][2]), fabsf(v[k][3]))));
-            if (NB > 1) mx = fmaxf(mx, xor_lane(mx, 16));
+            // (kv_store_head's maximum of a one-block head starts from zero: nothing but NaN is a head of zeros)
+            mx = fmaxf(mx, NB > 1 ? xor_lane(mx, 16) : 0.0f);
             const bool tiny = mx <= FLT_EPSILON;
             const float inv = 127.0f / mx;
             uint32_t w = 0;

@@ -94,6 +94,31 @@ def test_append_equals_kv_store(gpu_ctx, bits):
 
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("hd", [64, 128])
+def test_append_of_odd_values_equals_kv_store(gpu_ctx, bits, hd):
+    """Heads that hold NaN, infinities, the largest and smallest floats, one value, or nothing but -0."""
+    rng = np.random.default_rng(hd)
+    kinds = [np.nan, -np.nan, np.inf, -np.inf, 3e38, -3e38, 1e-38, 1e-45, -0.0, 1e-31, 1.2e-7, 1.0]
+    x = []
+    for v in kinds:
+        a, b, c = rng.standard_normal(hd), np.full(hd, v), np.zeros(hd)
+        a[rng.integers(hd)] = v
+        c[hd - 1] = v
+        x += [a, b, c, np.where(np.arange(hd) < 32, v, -v)]
+    x = np.array(x, np.float32)
+    n = len(x)
+    dx = dev(x)
+    a, kv = rows_of(R.new_cache(bits, 1, 1, n, hd), n)
+    gpu_ctx.kv_append(bits, dx, dx, hd, 1, n, 1, hd, ints([0]), kv)
+    b, _ = rows_of(R.new_cache(bits, 1, 1, n, hd), n)
+    gpu_ctx.kv_store(bits, dx, n, hd, b[0], b[1])
+    gpu_ctx.sync()
+    for i in range(2):
+        assert np.array_equal(a[i].cpu().numpy().view(np.uint8), b[i].cpu().numpy().view(np.uint8))
+        assert np.array_equal(a[i + 2].cpu().numpy().view(np.uint8), b[i].cpu().numpy().view(np.uint8))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 128])
 def test_append_and_load_of_many_tokens(gpu_ctx, bits, hd):
     """Enough blocks for two per group of lanes, ragged rows: append against k2t_kv_store's bytes, load
     against append's."""
