@@ -228,14 +228,17 @@ def _k2t():
 
 
 @functools.lru_cache(None)
-def _context():
-    return _k2t().Ctx(0)
+def _context(stream):
+    """A context whose calls run on `stream` (a stream's handle): a state's calls stay on the stream that
+    was current when it was prepared, whatever is prepared after it."""
+    ctx = _k2t().Ctx(0)
+    ctx.set_stream(stream)
+    return ctx
 
 
 def _plan(st):
     """What a program keeps beside its data: the context, the caches' descriptions and a workspace."""
-    k2t, case, ctx = _k2t(), st["case"], _context()
-    ctx.set_stream(torch.cuda.current_stream())
+    k2t, case, ctx = _k2t(), st["case"], _context(torch.cuda.current_stream().cuda_stream)
     st["ctx"], ws = ctx, 0
     if case["kind"] == "kv":
         st["cache"] = k2t.KVRows(st["kq"], st["ks"], st["vq"], st["vs"], cap=st["kq"].shape[2])
