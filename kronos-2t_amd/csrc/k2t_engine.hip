@@ -874,7 +874,7 @@ void ensure_beams(k2t_model *m, int rows, int n_steps, int prefix) {
 constexpr int kDoneSteps = 16;
 
 // The search: the model's step for first_token, then a choice per step over the rows.  Returns the
-// choices (token and parent row of every step), the last scores and the rows' done flags.
+// choices (token and parent row of every step) and the last scores.
 void beam_search(k2t_model *m, int first_token, int rows, int n_steps, int eos, std::vector<int> &tokens,
                  std::vector<int> &parents, std::vector<float> &scores) {
     const k2t_model_config &c = m->cfg;
