@@ -51,6 +51,10 @@ constexpr float kTop = 9.0f, kLimit = 15.0f, kLift = 256.0f, kLog2Lift = 8.0f;
 // 2^16 of them finite; an NF4 head's second block has a reference of its own (its scales may be of another
 // size), but a weight refers to the first, which therefore counts as 2^-60 of the second at least.
 constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f;
+// Scores so far from zero that fp32 does not tell whole numbers apart.  An exact product less the reference would
+// be up to half a step of the score off then, which may be any power of two: in a column that has met one, scores
+// are rounded before the reference, a rounded one itself, is taken off.
+constexpr float kFar = 0x1p24f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct SharedArgs {
@@ -231,8 +235,10 @@ struct State {
     v4f o[NQ][HD / 16];  // output tile b of column li: sums of 2^(s - m) V, times kLift (block 1: and 2^(m - m1))
     float m[NQ], l[NQ];  // reference (a whole number; -FLT_MAX: no score yet); this lane's share of the sum of 2^(s - m)
     float m1[SN > 1 ? NQ : 1], up1[SN > 1 ? NQ : 1];  // block 1's own reference, and 2^(m - m1) kLift
+    bool far;            // some column of the wave has a reference beyond kFar
 
     __device__ __forceinline__ void clear() {
+        far = false;
 #pragma unroll
         for (int a = 0; a < NQ; a++) {
             m[a] = -FLT_MAX;
@@ -320,7 +326,9 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                         u[k] = fmaxf(u[k], fmaf(t[a][j][i], qas[a], log2_bits(__float_as_uint(vs[j][i][k]) & 0x7FFFFFFFu, kLog2Lift)));
             }
             if constexpr (SN > 1) u[0] = fmaxf(u[0], u[1] - kApart);
-            const float most = column_max(u[0]), mn = most > S.m[a] + kLimit ? ceilf(most) - kTop : S.m[a];
+            const float most = column_max(u[0]);
+            const float mn = most > S.m[a] + kLimit ? (fabsf(most) >= kFar ? most : ceilf(most) - kTop) : S.m[a];
+            S.far |= __any(fabsf(mn) >= kFar && mn > -FLT_MAX) != 0;
             const float down = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
             float down1 = down;
             S.m[a] = mn;
@@ -328,7 +336,8 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
             if constexpr (SN > 1) {
                 // (no lower than 2^-120 of the first block's: 2^(m - m1) stays finite)
                 const float most1 = column_max(u[SN - 1]);
-                const float m1 = fmaxf(most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - 120.0f);
+                float m1 = fmaxf(most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - 120.0f);
+                if (fabsf(mn) >= kFar) m1 = mn;
                 down1 = m1 == S.m1[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m1[a] - m1);
                 S.m1[a] = m1;
                 S.up1[a] = __builtin_amdgcn_exp2f(mn - m1) * kLift;
@@ -337,12 +346,31 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
             for (int b = 0; b < HD / 16; b++) S.o[a][b] = S.o[a][b] * (SN > 1 && b >= 4 ? down1 : down);
         }
     }
+    float by[NQ], from[NQ];
+#pragma unroll
+    for (int a = 0; a < NQ; a++) {
+        by[a] = qas[a];
+        from[a] = S.m[a];
+    }
+    if (S.far) {
+#pragma unroll
+        for (int a = 0; a < NQ; a++) {
+            const bool far = fabsf(S.m[a]) >= kFar;  // (the other columns: t * 1 - 0)
+            const float by0 = far ? qas[a] : 1.0f, from0 = far ? S.m[a] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) t[a][j][i] = t[a][j][i] * by0 - from0;
+            by[a] = far ? 1.0f : qas[a];
+            from[a] = far ? 0.0f : S.m[a];
+        }
+    }
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) t[a][j][i] = __builtin_amdgcn_exp2f(fmaf(t[a][j][i], qas[a], -S.m[a]));
+            for (int i = 0; i < 4; i++) t[a][j][i] = __builtin_amdgcn_exp2f(fmaf(t[a][j][i], by[a], -from[a]));
     }
     if (n < kTile) {  // positions behind the last one repeat it: they weigh nothing
 #pragma unroll

@@ -431,6 +431,77 @@ def test_attention_of_v_scales_far_apart(gpu_ctx, bits, hd, beams, nq, nkv, pref
     assert (err <= bound).all(), float((err / bound).max())
 
 
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("beams,nq,nkv,prefix,tail", [(3, 4, 2, 50, 20), (3, 4, 2, 1500, 200)])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e7, 1e9, 1e13, 1e20])
+def test_attention_of_scores_of_any_size(gpu_ctx, bits, hd, beams, nq, nkv, prefix, tail, size):
+    """Scores from thousands to 1e20, where fp32 does not tell whole numbers apart: the best position of a head
+    takes all the weight, and the output is its V."""
+    rng = np.random.default_rng(hd + bits + prefix)
+    pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+    q = rng.standard_normal((beams, nq, hd)).astype(np.float32)
+    scale = np.float32(size)
+    out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+    _, p = rows_of(pre, prefix)
+    _, t = rows_of(tl, tail)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(bits, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, t, float(scale), out, ws)
+    gpu_ctx.sync()
+    got = out.cpu().numpy()
+    import oracle as O
+    pk, pv, tk, tv = (R.values(bits, *c) for c in (pre[:2], pre[2:], tl[:2], tl[2:]))
+    told = 0
+    for r in range(beams):
+        for h in range(nq):
+            g = h // (nq // nkv)
+            code, qs = O.kv_quant_head(q[r, h])
+            z = np.concatenate((pk[0, g], tk[r, g])) @ (code.astype(np.float64) * np.float64(qs)) * float(scale)
+            first, second = np.sort(z)[[-1, -2]]
+            # a score is off by 5 roundings: told apart beyond that, and by enough for the second to weigh nothing
+            if first - second < 24 + 10 * R.U * max(first, -z.min()):
+                continue
+            told += 1
+            v = np.concatenate((pv[0, g], tv[r, g]))[z.argmax()]
+            # pieces of 2^-21, sums of one term, the rotation's 8 roundings
+            bound = (2.0 ** -21 + 8 * R.U) * R.block_sums(np.abs(v)) / 8 + 2.0 ** -30
+            assert (np.abs(got[r, h] - R.unrotate(v)) <= bound).all(), (r, h)
+    assert told >= beams * nq // 2 and np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("prefix", [50, 1500])
+def test_attention_of_far_scores_stays_in_its_rows(gpu_ctx, bits, hd, prefix):
+    """Infinite and enormous scores, and V scales far above or below, of one row's query or tail: the other
+    rows' bits do not change."""
+    rng = np.random.default_rng(prefix + 1)
+    beams, nq, nkv, tail = 6, 8, 2, 20
+    pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+    q = rng.standard_normal((beams, nq * hd)).astype(np.float32)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+
+    def run():
+        _, p = rows_of(pre, prefix)
+        _, t = rows_of(tl, tail)
+        out = torch.zeros((beams, nq, hd), device="cuda")
+        gpu_ctx.attn_shared(bits, dev(q), nq * hd, 1, beams, nq, nkv, hd, p, t, hd ** -0.5, out, ws)
+        gpu_ctx.sync()
+        return out.cpu().numpy()
+
+    def bf(v):
+        return v if bits == 8 else np.float32(v).view(np.uint32) >> 16
+
+    good = run()
+    assert np.isfinite(good).all()
+    q[1] *= 1e12
+    q[2, 3 * hd:4 * hd] *= 1e30
+    tl[1][3, 0, 7] = bf(np.inf)
+    tl[3][4, 1, 2], tl[3][4, 0, 5] = bf(1e30), bf(1e-30)
+    bad = run()
+    assert np.array_equal(bad[[0, 5]], good[[0, 5]])
+    assert np.array_equal(np.delete(bad[2], 3, 0), np.delete(good[2], 3, 0)) and np.isfinite(bad[1]).all()
+    assert np.array_equal(bad[3, 4:], good[3, 4:])
+
+
 def test_attention_agrees_with_attn_decode(gpu_ctx):
     """A row's output is the one-sequence operator's over its prefix and tail laid end to end."""
     rng = np.random.default_rng(11)
