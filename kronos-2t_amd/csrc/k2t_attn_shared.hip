@@ -17,12 +17,14 @@
 // positions in turn; K and V go from memory to registers in the operands' own layout, so a tile needs
 // no LDS and no barrier.
 //
-// What bounds it: instructions, not bytes. A tile of 32 positions and 32 columns takes some 340 vector
+// What bounds it: instructions, not bytes. A tile of 32 positions and 32 columns takes some 280 vector
 // instructions (weights and their pieces, V's codes to f16, scales) next to 40 MFMAs, two waves to a
 // SIMD; a part has few tiles, so its queries' transform and its join count too. Measured (passes in a row):
-// 8 rows x 32 heads x 64, 1500 positions 9.4 us (0.9 TB/s of cache bytes); 64 rows x 32 / 4 heads x 128,
-// 12000 + 333 positions 35.4 us (364 TFLOP/s); 3 sequences of 8 rows x 32 / 8 heads x 128, NF4, 4100 positions
-// 18.9 us, a third of whose instructions look codes up; 4 rows x 9 / 3 heads x 64, 52 positions 5.2 us, a launch.
+// 8 rows x 32 heads x 64, 1500 positions 9.5 us (0.9 TB/s of cache bytes); 64 rows x 32 / 4 heads x 128,
+// 12000 + 333 positions 35.3 us (365 TFLOP/s); 3 sequences of 8 rows x 32 / 8 heads x 128, NF4, 4100 positions
+// 19.0 us, a third of whose instructions look codes up; 4 rows x 9 / 3 heads x 64, 52 positions 5.2 us, a launch.
+// References by products instead of scores cost NF4 heads of two blocks 2 to 3 % (a reference each: 19.9 and
+// 20.3 us, full tails, and 47.2 and 48.4 us with 64 rows), the others nothing.
 #include <float.h>
 #include <math.h>
 

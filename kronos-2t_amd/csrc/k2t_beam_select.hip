@@ -11,8 +11,8 @@
 // What bounds it: the logits have to be read once (12.6 MB at 8 sequences of 8 rows of 49152: 2.4 us), but
 // both kernels take longer than their bytes, the first for its instructions (some 30 vector ones per logit of a lane on 3
 // waves per SIMD: 6.0 us there, 8.3 us before exp came down to one v_exp_f32 and keys were only made
-// for what reaches the bound), the second for chains of dependent steps on one CU (6.6 us there; 9.2 us
-// for 16 rows of 151936, k 32).  Both: 8.8 us for one sequence of 4 rows of 8192, 13.1 us and 15.3 us.
+// for what reaches the bound), the second for chains of dependent steps on one CU (6.6 us there; 9.0 us
+// for 16 rows of 151936, k 32).  Both: 8.9 us for one sequence of 4 rows of 8192, 13.3 us and 15.4 us.
 // With slices of 4096, 22 rows of 49152 give every CU a workgroup; larger ones would leave more CUs idle under
 // fewer rows, and smaller ones repeat a slice's fixed part (bound, sums, sort: about half of it).
 #include <float.h>

@@ -6,11 +6,11 @@
 // sum c_i^2), codes again with that scale. load: signs ifwht64(code scale). reorder: row r becomes row
 // parent[r] below its length.
 //
-// What bounds them: 6 rows of 777 tokens, 4 heads x 128, int8 (18 MB each way): append 7.8 us, load 6.4 us,
-// 12.6 us the two in a row (2.9 TB/s), of which waves that start, load once, transform and
-// end are the larger part; 515 tokens of 32 heads x 64, NF4: append 7.7 us, its instructions (both roundings
-// of every element, three quotients per block), load 4.6 us; 11.9 us in a row. One token of 4 rows: 2.3 us
-// each, a launch. Sixteen lanes per block, four elements a lane, instead of a wave per head with one
+// What bounds them: 6 rows of 777 tokens, 4 heads x 128, int8 (24 MB each): append 7.8 us, load 6.4 us (3.1 and
+// 3.7 TB/s); rows of 389 to 777 tokens, the two in a row, 36 MB in all: 12.8 us. Waves that start, load once,
+// transform and end are the larger part; 515 tokens of 32 heads x 64, NF4: append 7.7 us (9.1 by the profiler's
+// clock), its instructions (both roundings of every element, three quotients per block), load 4.1 us (4.5); 11.9 us
+// in a row. One token of 4 rows: 2.2 us each, a launch. Sixteen lanes per block, four elements a lane, instead of a wave per head with one
 // element a lane: 26.5 -> 15.2 us and, with the NF4 sums from LDS, 39.6 -> 12.7 us.
 #include <float.h>
 #include <math.h>
@@ -252,8 +252,8 @@ __global__ __launch_bounds__(64) void beam_post_kernel(float *__restrict__ qkv, 
 // Rows of one (layer, sequence, KV head, K or V) rearranged in place.  A thread owns one column (the
 // same T-sized piece of every row): it reads the column of every row that moves from its source row
 // before it writes any, so no other thread or buffer is involved.
-// Bound by bytes: 24 layers, 8 rows of 32 heads x 64, 200 positions, 256 MB read and written in 48 to 56 us
-// (4.6 to 5.3 TB/s, which is the large copy's), 64 to 70 us with stores that go through L2, 114 us with
+// Bound by bytes: 24 layers, 8 rows of 32 heads x 64, 200 positions, 256 MB read and written in 47 to 57 us
+// (4.5 to 5.4 TB/s, which is the large copy's), 64 to 70 us with stores that go through L2, 114 us with
 // 4-byte columns too. Up to 32 rows go through
 // registers as 16-byte columns, 64 as 8-byte ones.
 template <typename T, int NB>
