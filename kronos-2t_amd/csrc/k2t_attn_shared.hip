@@ -50,7 +50,7 @@ constexpr int kWaves = 4, kTile = 32;  // waves of a workgroup; positions of a w
 // 2^-24 of itself, a small number for scales of the usual size (2^-8 .. 1).
 constexpr float kTop = 9.0f, kLimit = 15.0f, kLift = 256.0f, kLog2Lift = 8.0f;
 // Scales below 2^-100 count as that much in the reference, so that a weight is at most 2^107 and a sum of
-// 2^16 of them finite; an NF4 head's second block has a reference of its own (its scales may be of another
+// 2^16 of them finite (from 2^120 on, half of the largest scale that a head has, kLift overflows); an NF4 head's second block has a reference of its own (its scales may be of another
 // size), but a weight refers to the first, which therefore counts as 2^-60 of the second at least.
 constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f;
 // Scores so far from zero that fp32 does not tell whole numbers apart.  An exact product less the reference would
