@@ -488,6 +488,113 @@ int32_t k2t_beam_select(k2t_ctx *ctx, const float *d_logits, int32_t vocab, size
 int32_t k2t_beam_select_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, int32_t vocab, int32_t k,
                                   size_t *bytes);
 
+/* ---- blocks of tokens: prompts of a batch, drafted continuations ------------- */
+
+/* No counterparts in the reference.  Token t < ntok of row b is row b * ntok + t of the call's buffers and,
+ * as in k2t_kv_append, goes to position d_pos[b] + t of the row's cache (k2t_kv_rows); d_counts (nullable): row b
+ * has min(ntok, d_counts[b]) tokens, and nothing is written for the others.  A block is a part of a prompt, or a tree
+ * of drafted tokens that lie side by side in the cache until k2t_kv_keep leaves one path of it.
+ *
+ * All of these calls run on the context's stream, allocate nothing, do not synchronise, and may be captured into a
+ * graph, which then reads positions, counts, depths, masks, histories and lists at every replay. */
+
+/* Rotary positions.  A plan holds, for every pair i < rot_dim / 2, its turns per position (its angular
+ * frequency over 2 pi), and the factor of rotated elements.  k2t_rope_plan_make fills one: frequency
+ * f_i = theta^(-2 i / rot_dim), stretched for contexts past `original` positions by `scaling`:
+ *   K2T_ROPE_PLAIN   f_i
+ *   K2T_ROPE_LINEAR  f_i / factor
+ *   K2T_ROPE_BASE    theta * factor^(rot_dim / (rot_dim - 2)) in theta's place (k2t.py's load_llama_config does this)
+ *   K2T_ROPE_RAMP    pairs that make `high` turns or more over `original` positions keep f_i, those of `low` or fewer
+ *                    have f_i / factor, a linear ramp over i between (its ends rounded outwards to whole pairs);
+ *                    rotated elements times 0.1 ln(factor) + 1
+ *   K2T_ROPE_WAVE    the same ends, but linear in the turns between, no factor
+ * low = high = 0 stand for 1 and 32 (RAMP), 1 and 4 (WAVE); 0 < low < high.  theta is at least 1 (RAMP: above), factor
+ * positive.  A program may fill in turns of its own. */
+#define K2T_ROPE_HALF 0        /* pairs (i, i + rot_dim / 2) of a head */
+#define K2T_ROPE_INTERLEAVED 1 /* pairs (2 i, 2 i + 1) */
+#define K2T_ROPE_PLAIN 0
+#define K2T_ROPE_LINEAR 1
+#define K2T_ROPE_BASE 2
+#define K2T_ROPE_RAMP 3
+#define K2T_ROPE_WAVE 4
+typedef struct k2t_rope_config {
+    int32_t layout, rot_dim; /* rot_dim: even, 2 .. 128; elements of a head behind it stay */
+    int32_t scaling, original;
+    double theta, factor, low, high;
+} k2t_rope_config;
+typedef struct k2t_rope_plan {
+    int32_t layout, rot_dim;
+    double scale, turns[64];
+} k2t_rope_plan;
+int32_t k2t_rope_plan_make(const k2t_rope_config *cfg, k2t_rope_plan *out); /* host only */
+/* Rotates n_heads heads of every token, back to back at d_x + (b * ntok + t) * x_stride floats (the q heads of
+ * a qkv row and its k heads are one run), into d_out likewise; d_out may be d_x itself with the same stride.
+ * The token's position is d_pos[b] + t, or with d_depth (nullable, [batch * ntok]) d_pos[b] + d_depth[b * ntok + t]: a
+ * drafted token stands at its depth in the tree, not at its cache position.  Angles, cosines and sines are
+ * 64-bit (an angle off by less than 2^-20 turns at any position) and rounded once to fp32.  plan->turns within +-1, its
+ * scale finite.  head_dim 64 or 128, rot_dim <= head_dim; d_x and d_out 16-byte aligned, strides multiples of 4;
+ * batch <= 65535, n_heads <= 2048, batch * ntok * n_heads <= 2^24. */
+int32_t k2t_rope(k2t_ctx *ctx, const float *d_x, size_t x_stride, int32_t batch, int32_t ntok, int32_t n_heads,
+                 int32_t head_dim, const int32_t *d_pos, const int32_t *d_depth, const int32_t *d_counts,
+                 const k2t_rope_plan *plan, float *d_out, size_t out_stride);
+
+/* Attention of a block of tokens of every row over the row's cache, which holds the block's own K and V already:
+ * k2t_attn_decode (int8 queries, same scores and softmax) for each token.  Token t of row b attends to the positions
+ * below d_pos[b] and, within the block, d_sees = NULL: to tokens 0 .. t (causal); else (ntok <= 64) to the tokens j whose
+ * bit j of d_sees[b * ntok + t] is set; in both cases only to tokens that the row has and to positions 0 .. kv->len - 1
+ * (d_len is not used).  A token that sees nothing gets zeros.  What the cache holds at positions that a token does not
+ * see (infinities and NaN among scales) does not reach its output, nor do other tokens' queries.  d_q: token's n_heads post-RoPE
+ * query heads at d_q + (b * ntok + t) * q_stride floats; d_out [batch * ntok][n_heads][hd].  attn_scale is finite and
+ * not negative.  d_ws: device workspace of k2t_attn_tokens_workspace bytes, of this call alone while it runs (two
+ * graphs that may run at once need one each); it needs no initial value.  d_q, d_out and d_ws are 16-byte aligned,
+ * q_stride a multiple of 4 below 2^31; head_dim 64 or 128, n_heads <= 1024, batch <= 65535, batch * ntok * n_heads <= 2^22. */
+int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_stride, int32_t batch, int32_t ntok,
+                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const int32_t *d_pos,
+                        const int32_t *d_counts, const uint64_t *d_sees, const k2t_kv_rows *kv, float attn_scale,
+                        float *d_out, void *d_ws, size_t ws_bytes);
+/* Its workspace for blocks of up to ntok tokens over caches of up to len positions (their `len`): what serves these
+ * serves every smaller block and shorter cache. */
+int32_t k2t_attn_tokens_workspace(k2t_ctx *ctx, int32_t batch, int32_t ntok, int32_t n_heads, int32_t n_kv_heads,
+                                  int32_t head_dim, int32_t len, size_t *bytes);
+
+/* What k2t_logits_adjust does to rows of logits; every list is per row, NULL where it is not wanted.
+ *   d_history [rows][history_stride]: the row's tokens so far, the first min(history_len, d_history_len[r]) of them;
+ *     those that stand before d_prompt_len[r] (nullable: 0) count for d_repeat only.
+ *   d_repeat, d_presence, d_frequency [rows]: penalties of tokens in the history (NULL: 1, 0, 0).
+ *   d_bias_tokens, d_bias [rows][bias_stride]: values added to tokens' logits, the first min(bias_len, d_bias_len[r]);
+ *     a token that is listed twice gets both.
+ *   d_mask [mask_rows][mask_stride] words: bit t % 32 of word t / 32 allows token t; row r is ruled by mask row
+ *     d_mask_row[r] (d_mask_row NULL: r), and by none if that is outside 0 .. mask_rows - 1.
+ * Tokens outside the vocabulary are passed over.  history_len <= 2^20, bias_len <= 4096. */
+typedef struct k2t_logits_rules {
+    const int32_t *d_history, *d_history_len, *d_prompt_len;
+    const float *d_repeat, *d_presence, *d_frequency;
+    const int32_t *d_bias_tokens;
+    const float *d_bias;
+    const int32_t *d_bias_len;
+    const uint32_t *d_mask;
+    const int32_t *d_mask_row;
+    size_t history_stride, bias_stride, mask_stride;
+    int32_t history_len, bias_len, mask_rows;
+} k2t_logits_rules;
+/* For every row and token with logit x:  a token of the history: x > 0 ? x / repeat : x * repeat; one that stands c > 0
+ * times behind the prompt: less presence + frequency * c; then plus its biases; -inf where the mask does not allow
+ * it.  In 64 bits, rounded once; a logit that nothing applies to keeps its bits (NaN too).  Rows at d_logits +
+ * r * row_stride, results at d_out + r * out_stride; d_out may be d_logits itself with the same stride (then only
+ * changed logits are written).  What k2t_beam_select takes.  vocab <= 2^24, rows <= 65535. */
+int32_t k2t_logits_adjust(k2t_ctx *ctx, const float *d_logits, int32_t vocab, size_t row_stride, int32_t rows,
+                          const k2t_logits_rules *rules, float *d_out, size_t out_stride);
+
+/* Moves the positions that a row keeps together, in place, in all layers at once: position d_pos[r] + j of row r takes
+ * the K and V of position d_pos[r] + d_keep[r * keep_stride + j], for j < min(n_keep, d_counts[r]) (d_counts nullable), as if all
+ * were read before any is written.  Entries with d_keep < j, and those of positions outside 0 .. cap - 1, leave
+ * position d_pos[r] + j as it was; nothing else in the cache changes.  (The accepted path of a drafted tree; what an
+ * eviction leaves of a context.)  The cache holds n_layers blocks of `rows` rows; kv->len and d_len are not used.
+ * rows <= 65535, n_kv_heads <= 1024, n_layers * rows * n_kv_heads <= 2^22, n_keep <= 2^24. */
+int32_t k2t_kv_keep(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const int32_t *d_pos, const int32_t *d_keep,
+                    size_t keep_stride, const int32_t *d_counts, int32_t n_keep, int32_t n_layers, int32_t rows,
+                    int32_t n_kv_heads, int32_t head_dim);
+
 /* ---- sparse-MoE experts (.k2tm shards) ------------------------------------- */
 
 /* K2tmShardHeader (moe_800b.rs:792-854): page 0 of a .k2tm shard ("K2TM800B_V1\0", then

@@ -311,6 +311,68 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs A) {
         move_column<uint16_t, NB>((uint16_t *)s + slot0 + pos, slots, par, A.beams, lens, pos);
 }
 
+// Positions of one (layer, row, KV head, K or V) moved together: position p0 + j from p0 + keep[j], keep[j] >= j.
+// Entries are taken in order, a chunk of them at a time: a chunk's sources are all read before its
+// positions are written, and those that earlier chunks have written lie before every later source.
+constexpr int kKeepPieces = 4;  // pieces of a thread in flight
+
+struct KeepArgs {
+    k2t_kv_rows kv;
+    const int *pos, *keep, *counts;
+    size_t keep_stride;
+    int n_keep, rows, nkv;
+    int code_bytes, scale_bytes;  // per slot
+};
+
+// Entries a .. b - 1 of the list, at most kKeepPieces * 256 / PER of them, each a slot of PER pieces of type T.
+template <typename T, int PER>
+__device__ __forceinline__ void keep_chunk(T *base, const int *keep, long long p0, int cap, int a, int b) {
+    T v[kKeepPieces];
+    long long to[kKeepPieces];
+#pragma unroll
+    for (int k = 0; k < kKeepPieces; k++) {
+        const int g = (int)threadIdx.x + 256 * k, j = a + g / PER;
+        to[k] = -1;
+        if (j >= b) continue;
+        const int from = keep[j];
+        const long long t = p0 + j, f = p0 + from;
+        if (from <= j || t < 0 || f >= cap) continue;  // (from == j: it is there already)
+        to[k] = t * PER + g % PER;
+        v[k] = base[f * PER + g % PER];
+    }
+    // (the loads themselves, not only their issue, come before any wave's stores)
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#endif
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kKeepPieces; k++)
+        if (to[k] >= 0) base[to[k]] = v[k];
+    __syncthreads();
+}
+
+template <int CODE>  // bytes of a slot's codes
+__global__ __launch_bounds__(256) void kv_keep_kernel(const KeepArgs A) {
+    constexpr int PER = CODE / 16, kCodes = kKeepPieces * 256 / PER, kScales = kKeepPieces * 256;
+    // grid x: ((layer * rows + row) * nkv + head) * 2 + (K, V)
+    const size_t g = blockIdx.x / 2;
+    const int is_v = blockIdx.x & 1, row = (int)(g / A.nkv % A.rows);
+    const int n = A.counts ? max(0, min(A.counts[row], A.n_keep)) : A.n_keep;
+    const int *keep = A.keep + (size_t)row * A.keep_stride;
+    const long long p0 = A.pos[row];
+    const size_t slot = g * (size_t)A.kv.cap;
+    if (blockIdx.y == 0) {
+        u32x4 *q = (u32x4 *)(is_v ? A.kv.vq : A.kv.kq) + slot * PER;
+        for (int a = 0; a < n; a += kCodes) keep_chunk<u32x4, PER>(q, keep, p0, A.kv.cap, a, min(a + kCodes, n));
+        return;
+    }
+    void *s = is_v ? A.kv.vs : A.kv.ks;
+    for (int a = 0; a < n; a += kScales) {
+        if (A.scale_bytes == 4) keep_chunk<uint32_t, 1>((uint32_t *)s + slot, keep, p0, A.kv.cap, a, min(a + kScales, n));
+        else keep_chunk<uint16_t, 1>((uint16_t *)s + slot, keep, p0, A.kv.cap, a, min(a + kScales, n));
+    }
+}
+
 RowsArgs rows_args(const k2t_kv_rows &kv, size_t row_stride, int ntok, int nkv, int hd, const int *pos, const int *counts) {
     RowsArgs A{};
     A.row_stride = row_stride;
@@ -402,6 +464,16 @@ void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const in
     hip_check(hipGetLastError(), "kv_reorder launch");
 }
 
+void launch_kv_keep(hipStream_t st, int bits, const k2t_kv_rows &kv, const int *pos, const int *keep, size_t keep_stride,
+                    const int *counts, int n_keep, int n_layers, int rows, int nkv, int hd) {
+    const KeepArgs A{kv, pos, keep, counts, keep_stride, n_keep, rows, nkv, bits == 8 ? hd : hd / 2, bits == 8 ? 4 : hd / 32};
+    const dim3 grid((unsigned)(2 * (size_t)n_layers * rows * nkv), 2);
+    if (A.code_bytes == 128) hipLaunchKernelGGL((kv_keep_kernel<128>), grid, dim3(256), 0, st, A);
+    else if (A.code_bytes == 64) hipLaunchKernelGGL((kv_keep_kernel<64>), grid, dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((kv_keep_kernel<32>), grid, dim3(256), 0, st, A);
+    hip_check(hipGetLastError(), "kv_keep launch");
+}
+
 }  // namespace k2t
 
 using namespace k2t;
@@ -454,6 +526,26 @@ int32_t k2t_kv_reorder(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const 
         if (n_layers == 0 || n_seq == 0 || beams == 1 || kv->len == 0) return;
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
         launch_kv_reorder(ctx->stream, bits, *kv, d_parents, n_layers, n_seq, beams, n_kv_heads, head_dim);
+    });
+}
+
+int32_t k2t_kv_keep(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const int32_t *d_pos, const int32_t *d_keep,
+                    size_t keep_stride, const int32_t *d_counts, int32_t n_keep, int32_t n_layers, int32_t rows,
+                    int32_t n_kv_heads, int32_t head_dim) {
+    return branch_guard([&] {
+        branch_arg(ctx && kv, "NULL argument");
+        check_kv_rows(kv, bits, head_dim);
+        branch_arg(n_layers >= 0 && rows >= 0 && rows <= 65535 && n_kv_heads > 0 && n_kv_heads <= 1024,
+                   "negative n_layers, rows not 0 .. 65535, or n_kv_heads not 1 .. 1024");
+        branch_arg((size_t)n_layers * rows <= (size_t)1 << 22 && (size_t)n_layers * rows * n_kv_heads <= (size_t)1 << 22,
+                   "too many layers, rows and heads");
+        branch_arg(n_keep >= 0 && n_keep <= 1 << 24 && keep_stride >= (size_t)n_keep && keep_stride < (size_t)1 << 40,
+                   "n_keep must be 0 .. 2^24, keep_stride no smaller");
+        if (n_layers == 0 || rows == 0 || n_keep == 0) return;
+        branch_arg(d_pos && d_keep, "NULL argument");
+        hip_check(hipSetDevice(ctx->device), "hipSetDevice");
+        launch_kv_keep(ctx->stream, bits, *kv, d_pos, d_keep, keep_stride, d_counts, n_keep, n_layers, rows, n_kv_heads,
+                       head_dim);
     });
 }
 

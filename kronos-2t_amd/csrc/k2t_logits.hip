@@ -1,0 +1,204 @@
+// What a choice of the next token is made from: penalties for repeated tokens, biases and grammar masks on rows
+// of logits (k2t_logits_adjust).
+//
+// For a row and a token with logit x, s: the token stands in the history, c: how often behind the prompt,
+//   y = s ? (x > 0 ? x / repeat : x repeat) : x,  y -= c > 0 ? presence + frequency c : 0,  y += its biases,
+//   y = -inf where the mask does not allow it,
+// in 64 bits for the few tokens that the lists name; the others are copied bit for bit.
+//
+// A workgroup takes a slice of a row's vocabulary: it counts the history's tokens that fall into the slice in LDS
+// (integer atomics: any order gives the same counts), notes for every token the first entry of the bias list that names
+// it, and then passes over its logits once. A token's biases are added in the list's order by the thread that
+// owns the token, so that the sum does not depend on scheduling.
+#include <math.h>
+
+#include <algorithm>
+
+#include "k2t_branch.h"
+#include "k2t_device.h"
+
+namespace k2t {
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kLogitSlice = 4096, kGroups = kLogitSlice / 4 / kThreads;  // groups of four logits per thread
+constexpr int kMaxHistory = 1 << 20, kMaxBias = 4096;
+constexpr uint32_t kSeen = 1u << 31;    // over the count of a token behind the prompt
+constexpr uint32_t kNone = 0xFFFFu, kAgain = 1u << 15;  // no bias; more entries than the first name the token
+
+struct LogitsArgs {
+    const float *x;
+    float *out;
+    size_t x_stride, out_stride;
+    int vocab;
+    k2t_logits_rules R;
+};
+
+// LISTS: the row may have a history or biases.  VEC: rows start at multiples of 16 bytes.
+template <bool LISTS, bool VEC>
+__global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
+    __shared__ __align__(16) uint32_t count[LISTS ? kLogitSlice : 4], first[LISTS ? kLogitSlice : 4];
+    const int row = (int)blockIdx.y, v0 = (int)blockIdx.x * kLogitSlice, tid = (int)threadIdx.x;
+    const int n = min(kLogitSlice, A.vocab - v0);
+    const float *x = A.x + (size_t)row * A.x_stride + v0;
+    float *out = A.out + (size_t)row * A.out_stride + v0;
+    const bool moved = A.out != A.x;
+    const auto load = [&](int i) {
+        f32x4 f;
+        if (VEC && i + 4 <= n) return *reinterpret_cast<const f32x4 *>(x + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) f[j] = x[min(i + j, n - 1)];
+        return f;
+    };
+    f32x4 f[kGroups];
+    if (moved) {  // (in place most groups are never read)
+#pragma unroll
+        for (int g = 0; g < kGroups; g++) f[g] = load(4 * min(tid + kThreads * g, (n - 1) / 4));
+    }
+    const k2t_logits_rules &R = A.R;
+    const uint32_t *mask = nullptr;
+    if (R.d_mask) {
+        const int m = R.d_mask_row ? R.d_mask_row[row] : row;
+        if (m >= 0 && m < R.mask_rows) mask = R.d_mask + (size_t)m * R.mask_stride + v0 / 32;
+    }
+    int biases = 0;
+    if constexpr (LISTS) {
+        for (int i = 4 * tid; i < kLogitSlice; i += 4 * kThreads) {
+            *reinterpret_cast<uint4 *>(count + i) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(first + i) = make_uint4(kNone, kNone, kNone, kNone);
+        }
+        __syncthreads();
+        if (R.d_history) {
+            const int len = R.d_history_len ? max(0, min(R.d_history_len[row], R.history_len)) : R.history_len;
+            const int prompt = R.d_prompt_len ? R.d_prompt_len[row] : 0;
+            const int *h = R.d_history + (size_t)row * R.history_stride;
+            for (int i = tid; i < len; i += kThreads) {
+                const uint32_t t = (uint32_t)h[i] - (uint32_t)v0;
+                if (t >= (uint32_t)n) continue;
+                atomicOr(&count[t], kSeen);
+                if (i >= prompt) atomicAdd(&count[t], 1u);
+            }
+        }
+        const int *names = R.d_bias_tokens + (size_t)row * R.bias_stride;
+        if (R.d_bias_tokens) {
+            biases = R.d_bias_len ? max(0, min(R.d_bias_len[row], R.bias_len)) : R.bias_len;
+            for (int i = tid; i < biases; i += kThreads) {
+                const uint32_t t = (uint32_t)names[i] - (uint32_t)v0;
+                if (t < (uint32_t)n) atomicMin(&first[t], (uint32_t)i);
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < biases; i += kThreads) {
+            const uint32_t t = (uint32_t)names[i] - (uint32_t)v0;
+            if (t < (uint32_t)n && (first[t] & (kAgain - 1)) != (uint32_t)i) atomicOr(&first[t], kAgain);
+        }
+        __syncthreads();
+    }
+    const double repeat = LISTS && R.d_repeat ? (double)R.d_repeat[row] : 1.0;
+    const double presence = LISTS && R.d_presence ? (double)R.d_presence[row] : 0.0;
+    const double frequency = LISTS && R.d_frequency ? (double)R.d_frequency[row] : 0.0;
+    const auto adjust = [&](float v, int i, uint32_t c, uint32_t b) {
+        double y = (double)v;
+        if (c & kSeen) y = y > 0.0 ? y / repeat : y * repeat;
+        const uint32_t fresh = c & ~kSeen;
+        if (fresh) y -= presence + frequency * (double)fresh;
+        if (b != kNone) {
+            const float *value = R.d_bias + (size_t)row * R.bias_stride;
+            const int *names = R.d_bias_tokens + (size_t)row * R.bias_stride;
+            const int at = (int)(b & (kAgain - 1));
+            y += (double)value[at];
+            if (b & kAgain)
+                for (int k = at + 1; k < biases; k++)
+                    if (names[k] == v0 + i) y += (double)value[k];
+        }
+        return (float)y;
+    };
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+        const int i = 4 * (tid + kThreads * g);
+        if (i >= n) break;
+        uint32_t allowed = 0xFu, c[4] = {}, b[4] = {kNone, kNone, kNone, kNone};
+        if (mask) allowed = mask[i / 32] >> (i % 32) & 0xFu;
+        bool listed = false;
+        if constexpr (LISTS) {
+            const uint4 cc = *reinterpret_cast<const uint4 *>(count + i), bb = *reinterpret_cast<const uint4 *>(first + i);
+            c[0] = cc.x, c[1] = cc.y, c[2] = cc.z, c[3] = cc.w;
+            b[0] = bb.x, b[1] = bb.y, b[2] = bb.z, b[3] = bb.w;
+            listed = (cc.x | cc.y | cc.z | cc.w) != 0 || (bb.x & bb.y & bb.z & bb.w) != kNone;
+        }
+        if (!moved) {
+            if (!listed && allowed == 0xFu) continue;
+            f[g] = load(i);
+        }
+        if (listed) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if ((c[j] != 0 || b[j] != kNone) && i + j < n) f[g][j] = adjust(f[g][j], i + j, c[j], b[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) f[g][j] = allowed >> j & 1u ? f[g][j] : -INFINITY;
+        if (VEC && i + 4 <= n) {
+            *reinterpret_cast<f32x4 *>(out + i) = f[g];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < n) out[i + j] = f[g][j];
+        }
+    }
+}
+
+}  // namespace
+
+}  // namespace k2t
+
+using namespace k2t;
+
+extern "C" {
+
+int32_t k2t_logits_adjust(k2t_ctx *ctx, const float *d_logits, int32_t vocab, size_t row_stride, int32_t rows,
+                          const k2t_logits_rules *rules, float *d_out, size_t out_stride) {
+    return branch_guard([&] {
+        branch_arg(ctx && rules, "NULL argument");
+        const k2t_logits_rules &R = *rules;
+        branch_arg(vocab >= 1 && vocab <= 1 << 24, "vocab must be 1 .. 2^24");
+        branch_arg(rows >= 0 && rows <= 65535, "rows must be 0 .. 65535");
+        branch_arg(row_stride >= (size_t)vocab && out_stride >= (size_t)vocab, "a stride is smaller than the vocabulary");
+        branch_arg(row_stride < (size_t)1 << 40 && out_stride < (size_t)1 << 40, "a stride is out of range");
+        if (R.d_history)
+            branch_arg(R.history_len >= 0 && R.history_len <= kMaxHistory && R.history_stride >= (size_t)R.history_len &&
+                           R.history_stride < (size_t)1 << 40,
+                       "history_len must be 0 .. 2^20, history_stride no smaller");
+        else
+            branch_arg(!R.d_repeat && !R.d_presence && !R.d_frequency, "penalties without a history");
+        branch_arg((R.d_bias_tokens != nullptr) == (R.d_bias != nullptr), "biases need both their tokens and their values");
+        if (R.d_bias)
+            branch_arg(R.bias_len >= 0 && R.bias_len <= kMaxBias && R.bias_stride >= (size_t)R.bias_len &&
+                           R.bias_stride < (size_t)1 << 40,
+                       "bias_len must be 0 .. 4096, bias_stride no smaller");
+        if (R.d_mask)
+            branch_arg(R.mask_rows >= (R.d_mask_row ? 0 : rows) && R.mask_stride >= ((size_t)vocab + 31) / 32 &&
+                           R.mask_stride < (size_t)1 << 40,
+                       "mask_rows or mask_stride too small");
+        else
+            branch_arg(!R.d_mask_row, "mask rows without masks");
+        if (rows == 0) return;
+        branch_arg(d_logits && d_out, "NULL argument");
+        const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p); };
+        branch_arg((at(d_logits) | at(d_out)) % 4 == 0, "d_logits and d_out must be aligned to floats");
+        branch_arg(d_logits != d_out || row_stride == out_stride, "in place the strides must be the same");
+        hip_check(hipSetDevice(ctx->device), "hipSetDevice");
+        LogitsArgs A{d_logits, d_out, row_stride, out_stride, vocab, R};
+        const bool vec = (at(d_logits) | at(d_out)) % 16 == 0 && row_stride % 4 == 0 && out_stride % 4 == 0;
+        const bool lists = (R.d_history && R.history_len) || (R.d_bias && R.bias_len);
+        const dim3 grid((unsigned)((vocab + kLogitSlice - 1) / kLogitSlice), (unsigned)rows), block(kThreads);
+        if (lists && vec) hipLaunchKernelGGL((logits_kernel<true, true>), grid, block, 0, ctx->stream, A);
+        else if (lists) hipLaunchKernelGGL((logits_kernel<true, false>), grid, block, 0, ctx->stream, A);
+        else if (vec) hipLaunchKernelGGL((logits_kernel<false, true>), grid, block, 0, ctx->stream, A);
+        else hipLaunchKernelGGL((logits_kernel<false, false>), grid, block, 0, ctx->stream, A);
+        hip_check(hipGetLastError(), "logits_adjust launch");
+    });
+}
+
+}  // extern "C"

@@ -122,11 +122,20 @@ SIGNATURES = {
     "k2t_attn_shared_workspace": (I32, [VP, I32, I32, I32, I32, I32, I32, I32, C.POINTER(SZ)]),
     "k2t_beam_select": (I32, [VP, VP, I32, SZ, VP, VP, I32, I32, I32, I32, VP, VP, VP, VP, VP, SZ]),
     "k2t_beam_select_workspace": (I32, [VP, I32, I32, I32, I32, C.POINTER(SZ)]),
+    "k2t_rope_plan_make": (I32, [VP, VP]),
+    "k2t_rope": (I32, [VP, VP, SZ, I32, I32, I32, I32, VP, VP, VP, VP, VP, SZ]),
+    "k2t_attn_tokens": (I32, [VP, I32, VP, SZ, I32, I32, I32, I32, I32, VP, VP, VP, VP, C.c_float, VP, VP, SZ]),
+    "k2t_attn_tokens_workspace": (I32, [VP, I32, I32, I32, I32, I32, I32, C.POINTER(SZ)]),
+    "k2t_logits_adjust": (I32, [VP, VP, I32, SZ, I32, VP, VP, SZ]),
+    "k2t_kv_keep": (I32, [VP, I32, VP, VP, VP, SZ, VP, I32, I32, I32, I32, I32]),
     "k2t_attn_decode_noalloc": (I32, [VP, I32, VP, I32, I32, I32, VP, VP, VP, VP, I32, I32, I32, I32, C.c_float,
                                       VP]),
 }
 
 MOE_SOFTMAX, MOE_TOPK_SOFTMAX, MOE_SIGMOID = 0, 1, 2
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP, ROPE_WAVE = 0, 1, 2, 3, 4
 
 EMBED_TIED, EMBED_F32, EMBED_BF16, EMBED_NF4 = 0, 1, 2, 3
 
@@ -158,6 +167,49 @@ class KVRows(C.Structure):
     def __init__(self, kq, ks, vq, vs, cap, len=None, d_len=None):
         super().__init__(_p(kq), _p(ks), _p(vq), _p(vs), _p(d_len), cap, cap if len is None else len)
         self._keep = (kq, ks, vq, vs, d_len)
+
+
+class RopeConfig(C.Structure):
+    """k2t_rope_config."""
+    _fields_ = [("layout", I32), ("rot_dim", I32), ("scaling", I32), ("original", I32), ("theta", C.c_double),
+                ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+class RopePlan(C.Structure):
+    """k2t_rope_plan: the frequencies that Ctx.rope turns heads by (k2t_rope_plan_make); `turns` and
+    `scale` may be set to a program's own."""
+    _fields_ = [("layout", I32), ("rot_dim", I32), ("scale", C.c_double), ("turns", C.c_double * 64)]
+
+    def __init__(self, layout, rot_dim, theta, scaling=ROPE_PLAIN, factor=1.0, original=0, low=0.0, high=0.0):
+        super().__init__()
+        cfg = RopeConfig(layout, rot_dim, scaling, original, theta, factor, low, high)
+        check(lib().k2t_rope_plan_make(C.addressof(cfg), C.addressof(self)))
+
+
+class LogitsRules(C.Structure):
+    """k2t_logits_rules: int32 / float32 tensors, one row of each per row of logits (mask: rows of int32
+    words); None: not applied."""
+    _fields_ = [(n, VP) for n in ("history", "history_len", "prompt_len", "repeat", "presence", "frequency",
+                                  "bias_tokens", "bias", "bias_len", "mask", "mask_row")] + \
+        [("history_stride", SZ), ("bias_stride", SZ), ("mask_stride", SZ), ("history_max", I32), ("bias_max", I32),
+         ("mask_rows", I32)]
+
+    def __init__(self, history=None, history_len=None, prompt_len=None, repeat=None, presence=None, frequency=None,
+                 bias_tokens=None, bias=None, bias_len=None, mask=None, mask_row=None):
+        def shape(t):
+            if t is None:
+                return 0, 0, 0
+            if t.shape[1] > 1 and t.stride(1) != 1:
+                raise ValueError("lists and masks are rows of consecutive words")
+            return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        _, hn, hs = shape(history)
+        _, bn, bs = shape(bias_tokens)
+        if bias_tokens is not None and (bias is None or bias.shape != bias_tokens.shape or shape(bias)[2] != bs):
+            raise ValueError("bias and bias_tokens differ in shape or stride")
+        rows, _, ms = shape(mask)
+        lists = (history, history_len, prompt_len, repeat, presence, frequency, bias_tokens, bias, bias_len, mask, mask_row)
+        super().__init__(*(_p(t) for t in lists), hs, bs, ms, hn, bn, rows)
+        self._keep = lists
 
 
 def k2tm_read_header(page):
@@ -375,6 +427,34 @@ class Ctx:
         n = SZ()
         check(lib().k2t_beam_select_workspace(self.h, n_seq, beams, vocab, k, C.byref(n)))
         return n.value
+
+    # -- blocks of tokens: prompts of a batch, drafted continuations
+    def rope(self, x, x_stride, batch, ntok, n_heads, head_dim, pos, plan, out, out_stride, depth=None, counts=None):
+        """k2t_rope: rotary positions pos[row] + t (or + depth[row][t]) of n_heads heads of every token, by a RopePlan;
+        out may be x."""
+        check(lib().k2t_rope(self.h, _p(x), x_stride, batch, ntok, n_heads, head_dim, _p(pos), _p(depth), _p(counts),
+                             _ref(plan), _p(out), out_stride))
+
+    def attn_tokens(self, bits, q, q_stride, batch, ntok, n_heads, n_kv_heads, head_dim, pos, kv, attn_scale, out, ws,
+                    counts=None, sees=None):
+        """k2t_attn_tokens: ntok tokens of every row, at positions pos[row] + t of its KVRows cache, causal or (sees:
+        int64 tensor, a bit per token of the block) as a drafted tree; ws: uint8 tensor of attn_tokens_workspace bytes."""
+        check(lib().k2t_attn_tokens(self.h, bits, _p(q), q_stride, batch, ntok, n_heads, n_kv_heads, head_dim, _p(pos),
+                                    _p(counts), _p(sees), _ref(kv), attn_scale, _p(out), _p(ws), _nbytes(ws)))
+
+    def attn_tokens_workspace(self, batch, ntok, n_heads, n_kv_heads, head_dim, length):
+        n = SZ()
+        check(lib().k2t_attn_tokens_workspace(self.h, batch, ntok, n_heads, n_kv_heads, head_dim, length, C.byref(n)))
+        return n.value
+
+    def logits_adjust(self, logits, vocab, row_stride, rows, rules, out, out_stride):
+        """k2t_logits_adjust: penalties, biases and masks of a LogitsRules on rows of logits; out may be logits."""
+        check(lib().k2t_logits_adjust(self.h, _p(logits), vocab, row_stride, rows, _ref(rules), _p(out), out_stride))
+
+    def kv_keep(self, bits, kv, pos, keep, keep_stride, counts, n_keep, n_layers, rows, n_kv_heads, head_dim):
+        """k2t_kv_keep: position pos[row] + j takes position pos[row] + keep[row][j], in place, all layers."""
+        check(lib().k2t_kv_keep(self.h, bits, _ref(kv), _p(pos), _p(keep), keep_stride, _p(counts), n_keep, n_layers,
+                                rows, n_kv_heads, head_dim))
 
     def gemv_chunk_dots(self, m, xq, xsum, dots):
         check(lib().k2t_gemv_chunk_dots(self.h, m.h, _p(xq), _p(xsum), _p(dots)))
