@@ -1,12 +1,24 @@
-// Attention of a block of tokens of every row of a batch over the row's Hadamard cache (k2t_attn_tokens).
+// Attention of a block of tokens of every row of a batch over the row's Hadamard cache (k2t_attn_tokens): prompts
+// (causal) and trees of drafted tokens (a mask), int8 or NF4, plain or grouped heads.
+//
+// For token t and q head h, over the positions p that t sees:
+//   s_p = scale_q scale_k[p] (codes_q . codes_k[p]) attn_scale,  w_p = exp(s_p - max s),
+//   out = ifwht64( sum_p w_p scale_v[p] codes_v[p] / sum_p w_p ).
+// A row's tokens and the q heads of a KV head are the columns of matrix products against the same K and V
+// (k2t_attn_tile.h); column c is head c % group of token c / group.
+//
+// Few columns (short drafts, single tokens): the waves of a workgroup share 16 or 32 columns and take tiles of 32
+// positions in turn, K and V from memory to registers (tokens_few_kernel).  Many: the waves have 16 or 32 columns each, and
+// a tile of positions is brought to LDS once for all of them, V as the f16 operand itself, so that its conversion is shared
+// too (tokens_block_kernel).  Where that gives fewer than two workgroups per CU, positions are cut into parts, which a
+// second kernel joins.
 #include <float.h>
 #include <math.h>
 
 #include <algorithm>
 
+#include "k2t_attn_tile.h"
 #include "k2t_branch.h"
-#include "k2t_device.h"
-#include "k2t_kv_dev.h"
 
 namespace k2t {
 
@@ -14,105 +26,468 @@ namespace {
 
 constexpr int kMaxTree = 64;
 
-struct TokensArgs {
-    const float *q;
-    size_t q_stride;
-    int ntok, nq, nkv;
+struct TokensArgs : ColumnArgs {
+    int ntok, nkv;
     const int *pos, *counts;
     const uint64_t *sees;
     k2t_kv_rows kv;
-    float attn_scale;
-    float *out;
+    int plen;        // positions of a part
+    int cgs, units;  // column groups of a row; (row, KV head, part)
 };
 
-// One workgroup per (token, head, row): a position per thread, 256 at a time.
-template <int HD, int BITS>
-__global__ __launch_bounds__(256) void tokens_simple_kernel(const TokensArgs A) {
-    constexpr int NB = HD / 64;
-    __shared__ int8_t q[HD];
-    __shared__ float w[256], red[4], qs, o[256];
-    const int tid = (int)threadIdx.x, head = (int)blockIdx.y, t = (int)blockIdx.x, row = (int)blockIdx.z;
-    const uint32_t lane = tid & 63u, wave = tid >> 6;
-    const int count = A.counts ? min(A.counts[row], A.ntok) : A.ntok;
-    if (t >= count) return;
-    const size_t token = (size_t)row * A.ntok + t;
-    const float *qh = A.q + token * A.q_stride + (size_t)head * HD;
-    if (wave == 0) {
-        const float r0 = fwht_lane(qh[lane], 0, lane), r1 = NB > 1 ? fwht_lane(qh[64 + lane], 1, lane) : 0.0f;
-        const float mx = wave_max_f(fmaxf(fabsf(r0), fabsf(r1)));
-        const bool tiny = mx <= FLT_EPSILON;
-        q[lane] = tiny ? 0 : (int8_t)(int)rintf(r0 * (127.0f / mx));
-        if (NB > 1) q[64 + lane] = tiny ? 0 : (int8_t)(int)rintf(r1 * (127.0f / mx));
-        if (lane == 0) qs = tiny ? 0.0f : (mx / 127.0f) * A.attn_scale;
+// A row of the call: how many tokens it has, the position of its first, and how many positions its last one sees.
+struct Row {
+    int count, start, end;
+};
+__device__ __forceinline__ int clamp_pos(const TokensArgs &A, long long p) {
+    return (int)max(0ll, min(p, (long long)A.kv.len));
+}
+__device__ __forceinline__ Row row_of(const TokensArgs &A, int row) {
+    Row R;
+    R.count = A.counts ? max(0, min(A.counts[row], A.ntok)) : A.ntok;
+    R.start = A.pos[row];
+    R.end = R.count ? clamp_pos(A, (long long)R.start + R.count) : 0;
+    return R;
+}
+// What token t sees: positions below `limit` and, of the block's tokens j (at positions start + j), those of `bits`.
+struct Sees {
+    int limit;
+    uint64_t bits;
+};
+__device__ __forceinline__ Sees sees_of(const TokensArgs &A, const Row &R, int row, int t) {
+    if (!A.sees) return Sees{clamp_pos(A, (long long)R.start + t + 1), 0};
+    // tokens that the row has, at positions of the cache
+    const long long lo = max(0ll, -(long long)R.start), hi = min((long long)R.count, (long long)A.kv.len - R.start);
+    uint64_t m = hi <= lo ? 0 : (hi >= 64 ? ~0ull : (1ull << hi) - 1) & ~(lo >= 64 ? ~0ull : (1ull << lo) - 1);
+    return Sees{clamp_pos(A, R.start), A.sees[(size_t)row * A.ntok + t] & m};
+}
+// How many positions the tokens up to t (of a tree: any) see at most.
+__device__ __forceinline__ int reach(const TokensArgs &A, const Row &R, int t) {
+    return A.sees ? R.end : clamp_pos(A, (long long)R.start + t + 1);
+}
+
+// What NQ columns of a lane see of the 32 positions from p0 on.
+template <int NQ>
+struct Seen {
+    static constexpr bool kHidden = true;
+    int limit[NQ], least;  // least: of all of the wave's columns
+    uint64_t bits[NQ];
+    int start;
+    int p0, lg;
+    __device__ __forceinline__ bool whole() const { return p0 + kTile <= least; }
+    __device__ __forceinline__ bool operator()(int a, int j, int i) const {
+        const int p = p0 + 16 * j + 4 * lg + i;
+        const uint32_t t = (uint32_t)(p - start);
+        return p < limit[a] || (t < 64u && (bits[a] >> t & 1u) != 0);
     }
-    __syncthreads();
-    const long long start = A.pos[row], end = min((long long)A.kv.len, start + count);
-    const size_t slot = ((size_t)row * A.nkv + head / (A.nq / A.nkv)) * A.kv.cap;
-    const auto code = [&](const void *base, size_t s, int e) {
-        if (BITS == 8) return (int)((const int8_t *)base)[s * HD + e];
-        const uint8_t b = ((const uint8_t *)base)[s * (HD / 2) + e / 32 * 16 + e % 16];
-        return nf4_cb_value(e & 16 ? b >> 4 : b & 15);
-    };
-    const auto scale = [&](const void *base, size_t s, int b) {
-        if (BITS == 8) return ((const float *)base)[s];
-        return __uint_as_float((uint32_t)((const uint16_t *)base)[s * NB + b] << 16);
-    };
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    const int d = tid % HD, part = tid / HD;
-    for (long long p0 = 0; p0 < end; p0 += 256) {
-        const long long p = p0 + tid, j = p - start;
-        const bool live = p < end && (j < 0 || (A.sees ? (A.sees[token] >> j & 1) != 0 : j <= t));
-        float s = -INFINITY;
-        if (live) {
-            s = 0.0f;
-            for (int b = 0; b < NB; b++) {
-                int dot = 0;
-                for (int e = 64 * b; e < 64 * b + 64; e++) dot += q[e] * code(A.kv.kq, slot + p, e);
-                s += (float)dot * scale(A.kv.ks, slot + p, b);
-            }
-            s *= qs;
+    // Columns c0 + 16 a + li of an item whose last column is c1 (those behind it repeat it).
+    __device__ __forceinline__ void set(const TokensArgs &A, const Row &R, int row, int c0, int c1, uint32_t li) {
+        start = R.start;
+        least = 1 << 30;
+#pragma unroll
+        for (int a = 0; a < NQ; a++) {
+            const Sees s = sees_of(A, R, row, (int)column(A, min(c0 + 16 * a + (int)li, c1)).row);
+            limit[a] = s.limit;
+            bits[a] = s.bits;
+            least = min(least, s.limit);
         }
-        float mx = wave_max_f(s);
-        if (lane == 0) red[wave] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float mn = fmaxf(m, mx);
-        const float corr = mn == -INFINITY || m == mn ? 1.0f : expf(m - mn);
-        w[tid] = live ? expf(s - mn) : 0.0f;
-        m = mn;
-        __syncthreads();
-        l *= corr;
-        acc *= corr;
-        const int n = (int)min(256ll, end - p0);
-        for (int i = 0; i < n; i++) l += w[i];
-        for (int i = part; i < n; i += 256 / HD)
-            if (w[i] != 0.0f) acc += w[i] * ((float)code(A.kv.vq, slot + p0 + i, d) * scale(A.kv.vs, slot + p0 + i, d / 64));
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) least = min(least, xor_lane(least, m));
+        least = __builtin_amdgcn_readfirstlane(least);
+    }
+};
+
+// Few columns: an item is (row, KV head, part, 16 NQ columns).
+template <int HD, int BITS, int NQ, bool WHOLE>
+__global__ __launch_bounds__(64 * kWaves, 2) void tokens_few_kernel(const TokensArgs A) {
+    __shared__ Shared<HD, NQ> sh;
+    const uint32_t lane = threadIdx.x & 63u;
+    const int unit = (int)blockIdx.x % A.units, cg = A.cgs - 1 - (int)blockIdx.x / A.units;
+    const int rh = unit / A.parts, head = rh % A.nkv, row = rh / A.nkv;
+    const Row R = row_of(A, row);
+    Item I;
+    I.part = unit % A.parts;
+    I.col0 = 16 * NQ * cg;
+    I.n = min(16 * NQ, R.count * A.group - I.col0);
+    if (I.n <= 0) return;
+    const int t0 = I.part * A.plen, last = I.col0 + I.n - 1;
+    I.kv[0] = I.kv[1] = A.kv;
+    I.slot[0] = I.slot[1] = ((size_t)row * A.nkv + head) * (size_t)A.kv.cap + t0;
+    I.len[0] = min(reach(A, R, (int)column(A, last).row) - t0, A.plen);
+    I.len[1] = 0;
+    I.row0 = row * A.ntok;
+    I.head0 = head * A.group;
+    if (I.len[0] <= 0) {
+        if constexpr (WHOLE) {  // nothing to see
+            for (int i = (int)threadIdx.x; i < I.n * HD; i += 64 * kWaves) {
+                const Column c = column(A, I.col0 + i / HD);
+                A.out[((size_t)(I.row0 + c.row) * A.nq + I.head0 + c.head) * HD + i % HD] = 0.0f;
+            }
+        }
+        return;
+    }
+    Seen<NQ> seen;
+    seen.set(A, R, row, I.col0, last, lane & 15u);
+    seen.lg = (int)(lane >> 4);
+    const auto live_at = [&](int i, int) {
+        seen.p0 = t0 + kTile * i;
+        return seen;
+    };
+    const auto any = [&](int c) {
+        const Sees s = sees_of(A, R, row, (int)column(A, c).row);
+        return s.limit > 0 || s.bits != 0;
+    };
+    attend<HD, BITS, NQ, WHOLE>(A, I, live_at, any, sh);
+}
+
+// ---- many columns
+template <int HD, int BITS>
+struct BlockTile {
+    static constexpr int P = 8192 / HD, S = P / kTile, DB = HD / 16, SN = TileK<HD, BITS>::SN;  // positions; subtiles of 32
+    __align__(16) uint8_t k[P * HD];      // int8 rows of HD / 16 pieces, pieces permuted (k_at)
+    uint4 v[S][DB][64];                   // the f16 operand of (32 positions, 16 dimensions), as lanes read it
+    __align__(16) float ks[P][SN], vs[P][SN];
+
+    // Piece c of row r: eight lanes that read the same piece of eight rows find them in different banks.
+    static __device__ __forceinline__ int k_at(int r, int c) {
+        return 16 * (r * (HD / 16) + (c ^ (HD == 128 ? r & 7 : r >> 1 & 3)));
+    }
+};
+
+// A tile on its way from memory: what thread tid loads of it.  K: pieces tid and tid + 256 (NF4: half as many bytes); V: the
+// words of four output tiles g of subtile s, for positions 16 j + 4 lg + i; scales: one position's K or V scales.
+template <int HD, int BITS>
+struct BlockLoad {
+    using T = BlockTile<HD, BITS>;
+    static constexpr int RB = BITS == 8 ? HD : HD / 2, PC = HD / 16;
+    uint32_t k[2][BITS == 8 ? 4 : 2], v[2][4], scale;
+
+    // Positions p0 .. of which the ones behind the last, n - 1, repeat it; base: their row's and head's slot 0.
+    __device__ __forceinline__ void load(const k2t_kv_rows &kv, size_t base, int p0, int n) {
+        const int tid = (int)threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int left = n - 1 - p0;
+        const uint8_t *kq = (const uint8_t *)kv.kq + (base + p0) * RB, *vq = (const uint8_t *)kv.vq + (base + p0) * RB;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int c = tid + 256 * x, r = min(c / PC, left);
+            if constexpr (BITS == 8) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(kq + (uint32_t)(r * RB + 16 * (c % PC)));
+                k[x][0] = w.x, k[x][1] = w.y, k[x][2] = w.z, k[x][3] = w.w;
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2 *>(kq + (uint32_t)(r * RB + 8 * (c % PC)));
+                k[x][0] = w.x, k[x][1] = w.y;
+            }
+        }
+        const int s = HD == 128 ? wave >> 1 : wave, g = HD == 128 ? wave & 1 : 0;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = min(32 * s + 16 * j + 4 * lg + i, left);
+                if constexpr (BITS == 8)
+                    v[j][i] = *reinterpret_cast<const uint32_t *>(vq + (uint32_t)(r * RB + HD / 16 * li + 4 * g));
+                else
+                    v[j][i] = *reinterpret_cast<const uint16_t *>(vq + (uint32_t)(r * RB + 32 * g + 2 * li));
+            }
+        if (tid < 2 * T::P) {
+            const void *p = tid < T::P ? kv.ks : kv.vs;
+            const size_t at = base + p0 + min(tid % T::P, left);
+            if constexpr (BITS == 8 || HD == 128) scale = ((const uint32_t *)p)[at];
+            else scale = ((const uint16_t *)p)[at];
+        }
+    }
+    __device__ __forceinline__ void store(T &tile, const Nf4 &cb) const {
+        const int tid = (int)threadIdx.x, lane = tid & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int c = tid + 256 * x;
+            *reinterpret_cast<v4i *>(tile.k + T::k_at(c / PC, c % PC)) = k_operand<BITS>(k[x], cb);
+        }
+        const int s = HD == 128 ? wave >> 1 : wave, g = HD == 128 ? wave & 1 : 0;
+        uint32_t h[2][4][2];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            v_halves(v_word<BITS>(v[j][0], cb), v_word<BITS>(v[j][1], cb), v_word<BITS>(v[j][2], cb), v_word<BITS>(v[j][3], cb), h[j]);
+#pragma unroll
+        for (int u = 0; u < 4; u++) tile.v[s][4 * g + u][lane] = make_uint4(h[0][u][0], h[0][u][1], h[1][u][0], h[1][u][1]);
+        if (tid < 2 * T::P) {
+            float *p = tid < T::P ? tile.ks[tid] : tile.vs[tid - T::P];
+#pragma unroll
+            for (int n = 0; n < T::SN; n++) p[n] = TileK<HD, BITS>::scale(scale, n);
+        }
+    }
+};
+
+template <int HD, int BITS, int NQ>
+struct BlockShared {
+    union {
+        BlockTile<HD, BITS> tile[2];
+        Queries<HD, 16 * NQ> q[kWaves];
+        float o[kWaves][16][HD + 4];
+    };
+    __device__ BlockShared() {}
+};
+
+// An item is (row, KV head, part, 16 NQ columns for each of four waves).
+template <int HD, int BITS, int NQ>
+__global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const TokensArgs A) {
+    using T = BlockTile<HD, BITS>;
+    constexpr int NB = HD / 64, DB = HD / 16, SN = T::SN, W = 16 * NQ;
+    __shared__ BlockShared<HD, BITS, NQ> sh;
+    const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    // (the last columns first: theirs are the longest items of a prompt)
+    const int unit = (int)blockIdx.x % A.units, cg = A.cgs - 1 - (int)blockIdx.x / A.units;
+    const int rh = unit / A.parts, head = rh % A.nkv, row = rh / A.nkv, part = unit % A.parts;
+    const Row R = row_of(A, row);
+    const int col0 = W * kWaves * cg, cols = R.count * A.group, n_all = min(W * kWaves, cols - col0);
+    if (n_all <= 0) return;
+    const int t0 = part * A.plen;
+    const int end = min(reach(A, R, (int)column(A, col0 + n_all - 1).row), t0 + A.plen);  // of the item's positions
+    const bool none = end <= t0;
+    if (none && A.parts > 1) return;
+    // this wave's columns; a wave without any repeats the last one and writes nothing
+    const int c0 = min(col0 + W * wave, cols - 1), n = max(0, min(W, cols - col0 - W * wave)), c1 = min(c0 + W, cols) - 1;
+    const size_t base = ((size_t)row * A.nkv + head) * (size_t)A.kv.cap;
+    const float *q0 = A.q + (size_t)row * A.ntok * A.q_stride + (size_t)head * A.group * HD;
+    Nf4 cb{};
+    if constexpr (BITS == 4) nf4_xor_tables(kNf4Cb0, kNf4Cb1, kNf4Cb2, kNf4Cb3, cb.t0, cb.t1, cb.u0, cb.u1);
+    BlockLoad<HD, BITS> next;
+    if (!none) next.load(A.kv, base, t0, end);
+    // queries: four 64-blocks of columns at a time
+    constexpr int kTurns = W * NB / 4, kBatch = kTurns < 8 ? kTurns : 8;
+    for (int k0 = 0; k0 < kTurns; k0 += kBatch) {
+        float4 f[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            const int u = 4 * (k0 + k) + (int)lg;
+            const Column at = column(A, min(c0 + u / NB, c1));
+            f[k] = *reinterpret_cast<const float4 *>(q0 + ((uint64_t)at.row * A.q_stride + at.head * HD + 64 * (u % NB) + 4 * li));
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            const int u = 4 * (k0 + k) + (int)lg, x = u / NB, b = u % NB;
+            const Quant4 r = quantize_block<NB>(f[k], head_signs4<NB>(b, li), li, A.attn_scale);
+            *reinterpret_cast<uint32_t *>(&sh.q[wave].q[x][64 * b + 4 * li]) = r.w;
+            if (li == 0 && b == 0) sh.q[wave].qas[x] = r.qas;
+        }
+    }
+    Seen<NQ> seen;
+    seen.set(A, R, row, c0, c1, li);
+    seen.lg = (int)lg;
+    const int far = min(end, reach(A, R, (int)column(A, c1).row));  // the wave's own last position
+    __syncthreads();
+    v4i qb[NQ][NB];
+    float qas[NQ];
+#pragma unroll
+    for (int a = 0; a < NQ; a++) {
+        qas[a] = sh.q[wave].qas[16 * a + li];
+        query_operand<HD, BITS>(sh.q[wave].q[16 * a + li], lg, qb[a]);
+    }
+    State<HD, NQ, SN> S;
+    S.clear();
+    __syncthreads();
+    const int tiles = none ? 0 : (end - t0 + T::P - 1) / T::P;
+    if (!none) {
+        next.store(sh.tile[0], cb);
+        next.load(A.kv, base, min(t0 + T::P, end - 1), end);
+    }
+    __syncthreads();
+    for (int i = 0; i < tiles; i++) {
+        const T &tile = sh.tile[i & 1];
+        // the next tile into the other half, which all waves have left, and the one behind it on its way
+        if (i + 1 < tiles) next.store(sh.tile[(i + 1) & 1], cb);
+        next.load(A.kv, base, min(t0 + T::P * (i + 2), end - 1), end);
+#pragma unroll 1
+        for (int s = 0; s < T::S; s++) {
+            seen.p0 = t0 + T::P * i + kTile * s;
+            if (seen.p0 >= far || n == 0) break;
+            float t[NQ][2][4], vs[2][4][SN];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int r = kTile * s + 16 * j;
+                v4i kf[NB];
+                float ks[4][SN];
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    kf[b] = *reinterpret_cast<const v4i *>(tile.k + T::k_at(r + (int)li, 4 * b + (int)lg));
+#pragma unroll
+                for (int x = 0; x < SN; x++) {
+                    const float4 a = *reinterpret_cast<const float4 *>(&tile.ks[r + 4 * lg][0] + 4 * x);
+                    const float4 b = *reinterpret_cast<const float4 *>(&tile.vs[r + 4 * lg][0] + 4 * x);
+                    const float fa[4] = {a.x, a.y, a.z, a.w}, fb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        ks[(4 * x + e) / SN][(4 * x + e) % SN] = fa[e];
+                        vs[j][(4 * x + e) / SN][(4 * x + e) % SN] = fb[e];
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < NQ; a++) scores<BITS>(kf, qb[a], [&](int e, int b) { return ks[e][SN > 1 ? b : 0]; }, t[a][j]);
+            }
+            uint32_t ph[NQ][SN][4], pl[NQ][SN][4];
+            weights(S, t, qas, vs, seen, ph, pl);
+#pragma unroll
+            for (int g = 0; g < DB / 4; g++) {
+                constexpr int kBlocks = SN - 1;  // (NF4 blocks have weights of their own)
+                v8h va[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) va[u] = __builtin_bit_cast(v8h, tile.v[s][4 * g + u][lane]);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int a = 0; a < NQ; a++) S.o[a][4 * g + u] = add_tile(va[u], pl[a][g & kBlocks], S.o[a][4 * g + u]);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int a = 0; a < NQ; a++) S.o[a][4 * g + u] = add_tile(va[u], ph[a][g & kBlocks], S.o[a][4 * g + u]);
+            }
+        }
         __syncthreads();
     }
-    o[tid] = acc;
-    __syncthreads();
-    if ((int)wave < NB) {
-        float v = 0.0f;
-        for (int k = 0; k < 256 / HD; k++) v += o[k * HD + tid];
-        v = m == -INFINITY && l == 0.0f ? 0.0f : v / l;
-        A.out[(token * A.nq + head) * HD + tid] = ifwht_lane(v, wave, lane);
+    // outputs: 16 columns of every wave at a time, four of them by sixteen lanes each
+#pragma unroll
+    for (int a = 0; a < NQ; a++) {
+        float l = S.l[a];
+        l += xor_lane(l, 16);
+        l += xor_lane(l, 32);
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sh.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * S.back(a, b);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int x = 4 * k + (int)lg;
+            const float L = __shfl(l, x, kWave), M = __shfl(S.m[a], x, kWave);
+            const int c = min(c0 + 16 * a + x, c1);
+            const Column to = column(A, c);
+            const size_t pair = (size_t)(row * A.ntok + (int)to.row) * A.nq + head * A.group + to.head;
+            const bool mine = 16 * a + x < n;
+            float inv = 1.0f;
+            if (A.parts == 1) {
+                const Sees s = sees_of(A, R, row, (int)to.row);
+                inv = s.limit > 0 || s.bits != 0 ? 1.0f / L : 0.0f;
+            } else if (mine && li == 0) {
+                A.stat[pair * A.parts + part] = make_float2(M, L);
+            }
+            float *out = A.parts == 1 ? A.out + pair * HD : A.part + (pair * A.parts + part) * HD;
+#pragma unroll
+            for (int d = 0; d < HD; d += 64) {
+                const float4 f = *reinterpret_cast<const float4 *>(&sh.o[wave][x][d + 4 * li]);
+                float v[4] = {f.x, f.y, f.z, f.w};
+                if (A.parts == 1) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] *= inv;
+                    butterflies_slice4(v, li);
+                    const uint32_t sb = head_signs4<NB>(d / 64, li);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = flip_sign(v[e] * 0.125f, sb >> e & 1u);
+                }
+                if (mine) *reinterpret_cast<float4 *>(out + d + 4 * li) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        }
+        __syncthreads();
     }
 }
 
-template <int HD>
-void launch_tokens(hipStream_t st, int bits, const TokensArgs &A, int batch) {
-    const dim3 grid((unsigned)A.ntok, (unsigned)A.nq, (unsigned)batch);
-    if (bits == 8) hipLaunchKernelGGL((tokens_simple_kernel<HD, 8>), grid, dim3(256), 0, st, A);
-    else hipLaunchKernelGGL((tokens_simple_kernel<HD, 4>), grid, dim3(256), 0, st, A);
+// Joins the parts of every token that its row has (merge_parts).  item: columns of a workgroup that wrote them.
+template <int HD, int WAVES>
+__global__ __launch_bounds__(256) void tokens_merge_kernel(const TokensArgs A, int pairs, int item) {
+    __shared__ float sum[WAVES > 1 ? WAVES : 1][HD];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int pair = WAVES == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x;
+    if (pair >= pairs) return;
+    const int token = pair / A.nq, row = token / A.ntok, t = token - row * A.ntok;
+    const Row R = row_of(A, row);
+    if (t >= R.count) return;
+    const Sees s = sees_of(A, R, row, t);
+    // an item wrote the parts that its last column reaches
+    const int c = t * A.group + pair % A.nq % A.group, last = min(c / item * item + item, R.count * A.group) - 1;
+    const int live = (reach(A, R, last / A.group) + A.plen - 1) / A.plen;
+    merge_parts<HD, WAVES>(A, pair, [=](int i) { return i < live; }, s.limit > 0 || s.bits != 0, sum);
+}
+
+struct TokensShape {
+    int batch, ntok, nq, nkv, hd;
+};
+
+// How the work is cut.  block: tokens_block_kernel, nq column tiles per wave; else tokens_few_kernel, nq per workgroup.
+struct Plan {
+    bool block;
+    int nq, cgs, parts, plen;
+    int item() const { return (block ? kWaves : 1) * 16 * nq; }
+};
+constexpr int kFewColumns = 32, kLeastPart = 256;
+
+// Parts of the positions so that `items` items per part come to about two workgroups for every CU.
+int parts_wanted(const k2t_ctx *ctx, size_t items) {
+    return (int)std::max<size_t>(1, 2 * (size_t)std::max(1, ctx->num_cus) / std::max<size_t>(1, items));
+}
+Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int len) {
+    const int cols = s.ntok * (s.nq / s.nkv);
+    Plan P{};
+    P.block = cols > kFewColumns;
+    P.nq = cols > (P.block ? 64 : 16) ? 2 : 1;
+    P.cgs = (cols + P.item() - 1) / P.item();
+    const int want = parts_wanted(ctx, (size_t)s.batch * s.nkv * P.cgs);
+    P.plen = std::max(kLeastPart, ((len + want - 1) / want + 127) / 128 * 128);
+    P.parts = std::max(1, (len + P.plen - 1) / P.plen);
+    return P;
+}
+size_t part_slots(const TokensShape &s, int parts) { return (size_t)s.batch * s.ntok * s.nq * parts; }
+size_t slot_bytes(int hd) { return hd * sizeof(float) + sizeof(float2); }
+size_t ws_bytes_of(const TokensShape &s, int parts) { return parts == 1 ? 16 : part_slots(s, parts) * slot_bytes(s.hd); }
+// At least that of every plan of up to so many tokens and positions: for every number of column groups of
+// each kind of item, as many columns as it has and as many parts as it may want (fewer where there are more groups).
+size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
+    const int cols = s.ntok * (s.nq / s.nkv);
+    const size_t heads = (size_t)s.batch * s.nkv;
+    size_t most = 0;
+    for (int item : {16, 32, 64, 128}) {
+        const int least = item == 16 ? 1 : item == 128 ? 65 : item / 2 + 1;  // columns of the smallest call with such items
+        if (cols < least) break;
+        for (int cgs = 1; (cgs - 1) * item < cols; cgs++) {
+            const int parts = std::min(parts_wanted(ctx, heads * cgs), (len + kLeastPart - 1) / kLeastPart);
+            if (parts <= 1) break;
+            most = std::max(most, heads * std::min(cols, cgs * item) * parts * slot_bytes(s.hd));
+        }
+    }
+    return std::max<size_t>(16, most);
+}
+
+template <int HD, int BITS>
+void launch_parts(hipStream_t st, const TokensArgs &A, const Plan &P) {
+    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * kWaves);
+    if (P.block && P.nq == 2) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 2>), grid, block, 0, st, A);
+    else if (P.block) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 1>), grid, block, 0, st, A);
+    else if (P.nq == 2 && P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, true>), grid, block, 0, st, A);
+    else if (P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, false>), grid, block, 0, st, A);
+    else if (P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, true>), grid, block, 0, st, A);
+    else hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, false>), grid, block, 0, st, A);
     hip_check(hipGetLastError(), "attn_tokens launch");
 }
 
-void check_tokens_shape(k2t_ctx *ctx, int batch, int ntok, int nq, int nkv, int hd) {
+template <int HD>
+void launch_tokens(hipStream_t st, int bits, const TokensArgs &A, const TokensShape &s, const Plan &P) {
+    if (bits == 8) launch_parts<HD, 8>(st, A, P);
+    else launch_parts<HD, 4>(st, A, P);
+    if (P.parts == 1) return;
+    const int pairs = s.batch * s.ntok * s.nq;
+    if (P.parts > 16) hipLaunchKernelGGL((tokens_merge_kernel<HD, 4>), dim3(pairs), dim3(256), 0, st, A, pairs, P.item());
+    else hipLaunchKernelGGL((tokens_merge_kernel<HD, 1>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
+    hip_check(hipGetLastError(), "attn_tokens merge launch");
+}
+
+TokensShape tokens_shape(k2t_ctx *ctx, int batch, int ntok, int nq, int nkv, int hd) {
     branch_arg(ctx != nullptr, "ctx is NULL");
     branch_arg(hd == 64 || hd == 128, "head_dim must be 64 or 128");
     branch_arg(nq > 0 && nkv > 0 && nq % nkv == 0 && nq <= 1024, "n_heads must be a multiple of n_kv_heads, at most 1024");
     branch_arg(batch >= 0 && batch <= 65535 && ntok >= 0, "batch must be 0 .. 65535, ntok >= 0");
     branch_arg((size_t)batch * ntok * nq <= (size_t)1 << 22, "more than 2^22 query heads in one call");
+    return TokensShape{batch, ntok, nq, nkv, hd};
 }
 
 }  // namespace
@@ -127,9 +502,9 @@ int32_t k2t_attn_tokens_workspace(k2t_ctx *ctx, int32_t batch, int32_t ntok, int
                                   int32_t head_dim, int32_t len, size_t *bytes) {
     return branch_guard([&] {
         branch_arg(bytes != nullptr, "NULL argument");
-        check_tokens_shape(ctx, batch, ntok, n_heads, n_kv_heads, head_dim);
+        const TokensShape s = tokens_shape(ctx, batch, ntok, n_heads, n_kv_heads, head_dim);
         branch_arg(len >= 0 && len <= 1 << 24, "len out of range");
-        *bytes = 16;
+        *bytes = most_ws_bytes(ctx, s, len);
     });
 }
 
@@ -138,10 +513,11 @@ int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
                         const int32_t *d_counts, const uint64_t *d_sees, const k2t_kv_rows *kv, float attn_scale,
                         float *d_out, void *d_ws, size_t ws_bytes) {
     return branch_guard([&] {
-        check_tokens_shape(ctx, batch, ntok, n_heads, n_kv_heads, head_dim);
+        const TokensShape s = tokens_shape(ctx, batch, ntok, n_heads, n_kv_heads, head_dim);
         branch_arg(kv != nullptr, "NULL argument");
         check_kv_rows(kv, bits, head_dim);
         branch_arg(!d_sees || ntok <= kMaxTree, "a tree has at most 64 tokens");
+        // (the running maximum takes the largest dot product for the largest score)
         branch_arg(attn_scale >= 0.0f && attn_scale <= FLT_MAX, "attn_scale must be finite and not negative");
         if (batch == 0 || ntok == 0) return;
         branch_arg(d_q && d_out && d_ws && d_pos, "NULL argument");
@@ -151,14 +527,36 @@ int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
                    "d_q must be 16-byte aligned, q_stride a multiple of 4, no smaller than a token's heads, below 2^31");
         branch_arg((at(d_out) | at(d_ws)) % 16 == 0, "d_out and d_ws must be 16-byte aligned");
         branch_arg(at(d_sees) % 8 == 0, "d_sees must be 8-byte aligned");
-        const size_t need = 16;
+        const Plan P = plan_of(ctx, s, kv->len);
+        const size_t need = ws_bytes_of(s, P.parts);
         if (ws_bytes < need)
             throw Error(K2T_E_ARG, "the workspace holds " + std::to_string(ws_bytes) + " bytes, " +
                                        std::to_string(need) + " are needed");
+        const size_t units = (size_t)batch * n_kv_heads * P.parts;
+        branch_arg(units * P.cgs <= (size_t)1 << 24, "too many rows, heads and positions in one call");
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
-        TokensArgs A{d_q, q_stride, ntok, n_heads, n_kv_heads, d_pos, d_counts, d_sees, *kv, attn_scale, d_out};
-        if (head_dim == 128) launch_tokens<128>(ctx->stream, bits, A, batch);
-        else launch_tokens<64>(ctx->stream, bits, A, batch);
+        TokensArgs A{};
+        A.q = d_q;
+        A.q_stride = (uint32_t)q_stride;
+        A.per_group = (float)n_kv_heads / (float)n_heads;
+        A.nq = n_heads;
+        A.group = n_heads / n_kv_heads;
+        A.attn_scale = attn_scale;
+        A.parts = P.parts;
+        A.part = (float *)d_ws;
+        A.stat = (float2 *)(A.part + part_slots(s, P.parts) * s.hd);
+        A.out = d_out;
+        A.ntok = ntok;
+        A.nkv = n_kv_heads;
+        A.pos = d_pos;
+        A.counts = d_counts;
+        A.sees = d_sees;
+        A.kv = *kv;
+        A.plen = P.plen;
+        A.cgs = P.cgs;
+        A.units = (int)units;
+        if (head_dim == 128) launch_tokens<128>(ctx->stream, bits, A, s, P);
+        else launch_tokens<64>(ctx->stream, bits, A, s, P);
     });
 }
 
