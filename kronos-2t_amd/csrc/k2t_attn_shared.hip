@@ -48,8 +48,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_part_kernel(SharedArgs 
         Shared<HD, 1> tail;
         __device__ U() {}
     } sh;
-    const int lg = (int)(threadIdx.x & 63u) >> 4;
-    const auto live_at = [lg](int, int left) { return Repeated{left, lg}; };
     const auto all = [](int) { return true; };
     const int id = (int)blockIdx.x;
     Item I;
@@ -69,7 +67,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_part_kernel(SharedArgs 
         I.head0 = head * A.group;
         I.col0 = 16 * NQ * cg;
         I.n = min(16 * NQ, A.beams * A.group - I.col0);
-        attend<HD, BITS, NQ, false>(A, I, live_at, all, sh.prefix);
+        attend<HD, BITS, NQ, false>(A, I, NoMask{}, all, sh.prefix);
         return;
     }
     int t = id - A.pre_items;
@@ -89,7 +87,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_part_kernel(SharedArgs 
     I.head0 = head * A.group;
     I.col0 = 16 * cg;
     I.n = min(16, A.group - I.col0);
-    attend<HD, BITS, 1, false>(A, I, live_at, all, sh.tail);
+    attend<HD, BITS, 1, false>(A, I, NoMask{}, all, sh.tail);
 }
 
 // Few positions: one workgroup per (row, KV head, 16 q heads) takes the prefix and the tail and writes
@@ -97,8 +95,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_part_kernel(SharedArgs 
 template <int HD, int BITS>
 __global__ __launch_bounds__(64 * kWaves, 2) void shared_whole_kernel(SharedArgs A) {
     __shared__ Shared<HD, 1> sh;
-    const int lg = (int)(threadIdx.x & 63u) >> 4;
-    const auto live_at = [lg](int, int left) { return Repeated{left, lg}; };
     int t = (int)blockIdx.x;
     const int cg = t % A.tgroups;
     t /= A.tgroups;
@@ -120,7 +116,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_whole_kernel(SharedArgs
         for (int i = (int)threadIdx.x; i < I.n * HD; i += 64 * kWaves) out[i] = 0.0f;
         return;
     }
-    attend<HD, BITS, 1, true>(A, I, live_at, [](int) { return true; }, sh);
+    attend<HD, BITS, 1, true>(A, I, NoMask{}, [](int) { return true; }, sh);
 }
 
 // Joins the parts (merge_parts).

@@ -11,6 +11,8 @@
 #include <float.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "k2t_device.h"
 #include "k2t_kv_dev.h"
 
@@ -263,33 +265,13 @@ __device__ __forceinline__ float column_max(float v) {  // over a column's four 
     return fmaxf(v, xor_lane(v, 32));
 }
 
-// Which positions of a tile count: all of them (whole), or those that live(a, j, i) names for the lane's column
-// of tile a.  The positions of a tile that the cache does not hold repeat the last one: they weigh nothing.
-struct Repeated {
-    static constexpr bool kHidden = false;  // others hold nothing foreign: their scores may be looked at
-    int n, lg;                              // n of the tile's 32 exist
-    __device__ __forceinline__ bool whole() const { return n >= kTile; }
-    __device__ __forceinline__ bool operator()(int, int j, int i) const { return 16 * j + 4 * lg + i < n; }
-};
-
 // Weights of a tile from its scores: t = dots * K scales of positions 16 j + 4 lg + i of the columns
-// li; vs = V scales.  Leaves pairs of weights times V scale times kLift as hi and
+// li, n of the tile's 32 exist; vs = V scales.  Leaves pairs of weights times V scale times kLift as hi and
 // lo pieces.  References change in one place, off the usual path: where the largest score of a lane's eight
-// positions with the largest of their scales would pass the limit.  Live::kHidden: what does not count may hold any
-// value. Its score is -inf before it is looked at, and its product zero behind the scale (which may be NaN).
-template <int HD, int NQ, int SN, typename Live>
+// positions with the largest of their scales would pass the limit.
+template <int HD, int NQ, int SN>
 __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][4], const float (&qas)[NQ], float (&vs)[2][4][SN],
-                                        const Live &live, uint32_t (&ph)[NQ][SN][4], uint32_t (&pl)[NQ][SN][4]) {
-    if constexpr (Live::kHidden) {
-        if (!live.whole()) {
-#pragma unroll
-            for (int a = 0; a < NQ; a++)
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) t[a][j][i] = live(a, j, i) ? t[a][j][i] : -INFINITY;
-        }
-    }
+                                        int n, uint32_t lg, uint32_t (&ph)[NQ][SN][4], uint32_t (&pl)[NQ][SN][4]) {
     float lv[SN];
 #pragma unroll
     for (int k = 0; k < SN; k++) {
@@ -371,14 +353,14 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
 #pragma unroll
             for (int i = 0; i < 4; i++) t[a][j][i] = __builtin_amdgcn_exp2f(fmaf(t[a][j][i], by[a], -from[a]));
     }
-    if (!live.whole()) {
+    if (n < kTile) {  // positions behind the last one repeat it: they weigh nothing
 #pragma unroll
         for (int a = 0; a < NQ; a++)
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (!live(a, j, i)) t[a][j][i] = 0.0f;
+                    if (16 * j + 4 * (int)lg + i >= n) t[a][j][i] = 0.0f;
     }
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
@@ -395,14 +377,38 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                         if (SN > 1 && k) x[e] = (t[a][j][i + e] * vs[j][i + e][k]) * S.up1[SN > 1 ? a : 0];
                         else x[e] = t[a][j][i + e] * (vs[j][i + e][k] * kLift);
                     }
-                    if constexpr (Live::kHidden) {
-                        if (!live.whole()) {
-                            x[0] = live(a, j, i) ? x[0] : 0.0f;
-                            x[1] = live(a, j, i + 1) ? x[1] : 0.0f;
-                        }
-                    }
                     split2(x[0], x[1], ph[a][k][2 * j + i / 2], pl[a][k][2 * j + i / 2]);
                 }
+    }
+}
+
+// Takes out of a tile what its columns do not see: bit 4 j + i of counts(a), the lane's column of tile a, is set for what it
+// sees.  A score of -inf weighs nothing (the columns' qas are positive).  What is not seen may have any V scale, and a
+// weight of zero times NaN is NaN: a scale that is not finite counts as zero, and the columns that do see its position get
+// a NaN score, so that their outputs are NaN.
+template <int NQ, int SN, typename Counts>
+__device__ __forceinline__ void hide_tile(float (&t)[NQ][2][4], float (&vs)[2][4][SN], const Counts &counts) {
+    bool bad[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            bad[j][i] = false;
+#pragma unroll
+            for (int k = 0; k < SN; k++) {
+                const bool b = !(fabsf(vs[j][i][k]) <= FLT_MAX);
+                vs[j][i][k] = b ? 0.0f : vs[j][i][k];
+                bad[j][i] |= b;
+            }
+        }
+#pragma unroll
+    for (int a = 0; a < NQ; a++) {
+        const uint32_t m = counts(a);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                t[a][j][i] = m >> (4 * j + i) & 1u ? (bad[j][i] ? NAN : t[a][j][i]) : -INFINITY;
     }
 }
 
@@ -502,6 +508,15 @@ __device__ __forceinline__ void query_operand(const int8_t *r, uint32_t lg, v4i 
         }
     }
 }
+// Scores that are all zero, by a scale above zero: what hide_tile needs.
+template <int NB>
+__device__ __forceinline__ void above_zero(float &qas, v4i (&qb)[NB]) {
+    if (qas != 0.0f) return;
+    qas = FLT_MIN;
+#pragma unroll
+    for (int b = 0; b < NB; b++) qb[b] = v4i{0, 0, 0, 0};
+}
+
 // The waves' results, added in wave order, 16 columns at a time: a part for the merge, or (WHOLE) the
 // output itself.
 template <int HD>
@@ -556,8 +571,9 @@ __device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const S
                 }
                 if constexpr (WHOLE) {
                     // ifwht64 with four elements on each of sixteen lanes (those of a column take part together)
-                    const float inv = any(c) ? 1.0f / L : 0.0f;
+                    const float inv = 1.0f / L;
                     float v[4] = {r.x * inv, r.y * inv, r.z * inv, r.w * inv};
+                    if (!any(c)) v[0] = v[1] = v[2] = v[3] = 0.0f;
                     butterflies_slice4(v, (uint32_t)sl);
                     const uint32_t sb = head_signs4<HD / 64>(d / 64, (uint32_t)sl);
                     r = make_float4(flip_sign(v[0] * 0.125f, sb & 1u), flip_sign(v[1] * 0.125f, (sb >> 1) & 1u),
@@ -578,9 +594,10 @@ struct Shared {
     Queries<HD, 16 * NQ> q;
     Join<HD> j;
 };
-// live_at(i, left): what counts of tile i, of whose positions `left` are left.
-template <int HD, int BITS, int NQ, bool WHOLE, typename LiveAt, typename Any>
-__device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const LiveAt &live_at, const Any &any, Shared<HD, NQ> &sh) {
+// hide(i, t, vs): takes out of tile i what a column does not see (Hidden); NoMask: columns see all positions of the item.
+struct NoMask {};
+template <int HD, int BITS, int NQ, bool WHOLE, typename Hide, typename Any>
+__device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const Hide &hide, const Any &any, Shared<HD, NQ> &sh) {
     constexpr int NB = HD / 64, DB = HD / 16, SN = TileK<HD, BITS>::SN;
     const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -620,6 +637,7 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
     for (int a = 0; a < NQ; a++) {
         qas[a] = sh.q.qas[16 * a + li];
         query_operand<HD, BITS>(sh.q.q[16 * a + li], lg, qb[a]);
+        if constexpr (!std::is_same<Hide, NoMask>::value) above_zero(qas[a], qb[a]);
     }
     State<HD, NQ, SN> S;
     S.clear();
@@ -646,7 +664,12 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
         __builtin_amdgcn_sched_barrier(0);
         next_k(i + kWaves);
         uint32_t ph[NQ][SN][4], pl[NQ][SN][4];
-        weights(S, s, qas, vs, live_at(i, left), ph, pl);
+        if constexpr (std::is_same<Hide, NoMask>::value) {
+            weights<HD, NQ, SN>(S, s, qas, vs, left, lg, ph, pl);
+        } else {  // (which takes out the positions behind the last one as well)
+            hide(i, s, vs);
+            weights<HD, NQ, SN>(S, s, qas, vs, kTile, lg, ph, pl);
+        }
         // four output tiles (one 4-byte word of V per position) at a time
 #pragma unroll
         for (int g = 0; g < DB / 4; g++) {

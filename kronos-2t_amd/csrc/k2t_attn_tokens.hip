@@ -69,16 +69,18 @@ __device__ __forceinline__ int reach(const TokensArgs &A, const Row &R, int t) {
 // What NQ columns of a lane see of the 32 positions from p0 on.
 template <int NQ>
 struct Seen {
-    static constexpr bool kHidden = true;
     int limit[NQ], least;  // least: of all of the wave's columns
     uint64_t bits[NQ];
     int start;
     int p0, lg;
     __device__ __forceinline__ bool whole() const { return p0 + kTile <= least; }
-    __device__ __forceinline__ bool operator()(int a, int j, int i) const {
-        const int p = p0 + 16 * j + 4 * lg + i;
-        const uint32_t t = (uint32_t)(p - start);
-        return p < limit[a] || (t < 64u && (bits[a] >> t & 1u) != 0);
+    __device__ __forceinline__ uint32_t counts(int a) const {
+        // bits p - p0 of 32 positions: those below the limit, and the block's tokens from position start on
+        const int under = limit[a] - p0, at = start - p0;
+        uint32_t m = under <= 0 ? 0u : under >= 32 ? ~0u : (1u << under) - 1u;
+        m |= at >= 32 || at <= -64 ? 0u : at >= 0 ? (uint32_t)bits[a] << at : (uint32_t)(bits[a] >> -at);
+        m >>= 4 * lg;
+        return (m & 0xFu) | (m >> 12 & 0xF0u);
     }
     // Columns c0 + 16 a + li of an item whose last column is c1 (those behind it repeat it).
     __device__ __forceinline__ void set(const TokensArgs &A, const Row &R, int row, int c0, int c1, uint32_t li) {
@@ -129,15 +131,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_few_kernel(const Tokens
     Seen<NQ> seen;
     seen.set(A, R, row, I.col0, last, lane & 15u);
     seen.lg = (int)(lane >> 4);
-    const auto live_at = [&](int i, int) {
+    const auto hide = [&](int i, auto &t, auto &vs) {
         seen.p0 = t0 + kTile * i;
-        return seen;
+        if (!seen.whole()) hide_tile(t, vs, [&](int a) { return seen.counts(a); });
     };
     const auto any = [&](int c) {
         const Sees s = sees_of(A, R, row, (int)column(A, c).row);
         return s.limit > 0 || s.bits != 0;
     };
-    attend<HD, BITS, NQ, WHOLE>(A, I, live_at, any, sh);
+    attend<HD, BITS, NQ, WHOLE>(A, I, hide, any, sh);
 }
 
 // ---- many columns
@@ -285,6 +287,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const Toke
     for (int a = 0; a < NQ; a++) {
         qas[a] = sh.q[wave].qas[16 * a + li];
         query_operand<HD, BITS>(sh.q[wave].q[16 * a + li], lg, qb[a]);
+        above_zero(qas[a], qb[a]);
     }
     State<HD, NQ, SN> S;
     S.clear();
@@ -328,7 +331,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const Toke
                 for (int a = 0; a < NQ; a++) scores<BITS>(kf, qb[a], [&](int e, int b) { return ks[e][SN > 1 ? b : 0]; }, t[a][j]);
             }
             uint32_t ph[NQ][SN][4], pl[NQ][SN][4];
-            weights(S, t, qas, vs, seen, ph, pl);
+            if (!seen.whole()) hide_tile(t, vs, [&](int a) { return seen.counts(a); });
+            weights<HD, NQ, SN>(S, t, qas, vs, kTile, lg, ph, pl);
 #pragma unroll
             for (int g = 0; g < DB / 4; g++) {
                 constexpr int kBlocks = SN - 1;  // (NF4 blocks have weights of their own)
@@ -366,13 +370,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const Toke
             const Column to = column(A, c);
             const size_t pair = (size_t)(row * A.ntok + (int)to.row) * A.nq + head * A.group + to.head;
             const bool mine = 16 * a + x < n;
-            float inv = 1.0f;
+            bool any = true;
             if (A.parts == 1) {
                 const Sees s = sees_of(A, R, row, (int)to.row);
-                inv = s.limit > 0 || s.bits != 0 ? 1.0f / L : 0.0f;
+                any = s.limit > 0 || s.bits != 0;
             } else if (mine && li == 0) {
                 A.stat[pair * A.parts + part] = make_float2(M, L);
             }
+            const float inv = 1.0f / L;
             float *out = A.parts == 1 ? A.out + pair * HD : A.part + (pair * A.parts + part) * HD;
 #pragma unroll
             for (int d = 0; d < HD; d += 64) {
@@ -380,7 +385,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const Toke
                 float v[4] = {f.x, f.y, f.z, f.w};
                 if (A.parts == 1) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] *= inv;
+                    for (int e = 0; e < 4; e++) v[e] = any ? v[e] * inv : 0.0f;
                     butterflies_slice4(v, li);
                     const uint32_t sb = head_signs4<NB>(d / 64, li);
 #pragma unroll
@@ -406,8 +411,9 @@ __global__ __launch_bounds__(256) void tokens_merge_kernel(const TokensArgs A, i
     const Sees s = sees_of(A, R, row, t);
     // an item wrote the parts that its last column reaches
     const int c = t * A.group + pair % A.nq % A.group, last = min(c / item * item + item, R.count * A.group) - 1;
-    const int live = (reach(A, R, last / A.group) + A.plen - 1) / A.plen;
-    merge_parts<HD, WAVES>(A, pair, [=](int i) { return i < live; }, s.limit > 0 || s.bits != 0, sum);
+    const bool any = s.limit > 0 || s.bits != 0;  // (else parts may hold the NaN of a query without positions)
+    const int live = any ? (reach(A, R, last / A.group) + A.plen - 1) / A.plen : 0;
+    merge_parts<HD, WAVES>(A, pair, [=](int i) { return i < live; }, any, sum);
 }
 
 struct TokensShape {
