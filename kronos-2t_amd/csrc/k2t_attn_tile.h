@@ -265,13 +265,28 @@ __device__ __forceinline__ float column_max(float v) {  // over a column's four 
     return fmaxf(v, xor_lane(v, 32));
 }
 
+// The largest of three: fmaxf's result, without the instructions that quiet each operand first.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+#else
+    return fmaxf(fmaxf(a, b), c);
+#endif
+}
+__device__ __forceinline__ float max8(const float (&t)[2][4]) {
+    return max3(max3(t[0][0], t[0][1], t[0][2]), max3(t[0][3], t[1][0], t[1][1]), fmaxf(t[1][2], t[1][3]));
+}
+
 // Weights of a tile from its scores: t = dots * K scales of positions 16 j + 4 lg + i of the columns
 // li, n of the tile's 32 exist; vs = V scales.  Leaves pairs of weights times V scale times kLift as hi and
 // lo pieces.  References change in one place, off the usual path: where the largest score of a lane's eight
-// positions with the largest of their scales would pass the limit.
-template <int HD, int NQ, int SN>
+// positions with the largest of their scales would pass the limit.  LIFTED: vs are V scales times kLift already.
+template <int HD, int NQ, int SN, bool LIFTED = false>
 __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][4], const float (&qas)[NQ], float (&vs)[2][4][SN],
                                         int n, uint32_t lg, uint32_t (&ph)[NQ][SN][4], uint32_t (&pl)[NQ][SN][4]) {
+    constexpr float kLifted = LIFTED ? kLift : 1.0f, kToLift = LIFTED ? 0.0f : kLog2Lift;
     float lv[SN];
 #pragma unroll
     for (int k = 0; k < SN; k++) {
@@ -280,15 +295,14 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) vmax = max(vmax, __float_as_uint(vs[j][i][k]));
-        lv[k] = log2_bits(max(vmax, __float_as_uint(kLeastScale)), kLog2Lift - kLimit);
+        lv[k] = log2_bits(max(vmax, __float_as_uint(kLeastScale * kLifted)), kToLift - kLimit);
     }
     if constexpr (SN > 1) lv[0] = fmaxf(lv[0], lv[1] - kApart);
     float top[NQ];
     bool news = false;
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
-        top[a] = fmaxf(fmaxf(fmaxf(t[a][0][0], t[a][0][1]), fmaxf(t[a][0][2], t[a][0][3])),
-                       fmaxf(fmaxf(t[a][1][0], t[a][1][1]), fmaxf(t[a][1][2], t[a][1][3])));
+        top[a] = max8(t[a]);
         // (qas >= 0: the largest t is the largest score)
         news |= fmaf(top[a], qas[a], lv[0]) > S.m[a];
         if constexpr (SN > 1) news |= fmaf(top[a], qas[a], lv[1]) > S.m1[a];
@@ -304,7 +318,7 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                 for (int j = 0; j < 2; j++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        u[k] = fmaxf(u[k], fmaf(t[a][j][i], qas[a], log2_bits(__float_as_uint(vs[j][i][k]) & 0x7FFFFFFFu, kLog2Lift)));
+                        u[k] = fmaxf(u[k], fmaf(t[a][j][i], qas[a], log2_bits(__float_as_uint(vs[j][i][k]) & 0x7FFFFFFFu, kToLift)));
             }
             if constexpr (SN > 1) u[0] = fmaxf(u[0], u[1] - kApart);
             const float most = column_max(u[0]);
@@ -374,8 +388,8 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                     float x[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        if (SN > 1 && k) x[e] = (t[a][j][i + e] * vs[j][i + e][k]) * S.up1[SN > 1 ? a : 0];
-                        else x[e] = t[a][j][i + e] * (vs[j][i + e][k] * kLift);
+                        if (SN > 1 && k) x[e] = (t[a][j][i + e] * vs[j][i + e][k]) * (S.up1[SN > 1 ? a : 0] * (1.0f / kLifted));
+                        else x[e] = t[a][j][i + e] * (LIFTED ? vs[j][i + e][k] : vs[j][i + e][k] * kLift);
                     }
                     split2(x[0], x[1], ph[a][k][2 * j + i / 2], pl[a][k][2 * j + i / 2]);
                 }

@@ -148,7 +148,7 @@ struct BlockTile {
     static constexpr int P = 8192 / HD, S = P / kTile, DB = HD / 16, SN = TileK<HD, BITS>::SN;  // positions; subtiles of 32
     __align__(16) uint8_t k[P * HD];      // int8 rows of HD / 16 pieces, pieces permuted (k_at)
     uint4 v[S][DB][64];                   // the f16 operand of (32 positions, 16 dimensions), as lanes read it
-    __align__(16) float ks[P][SN], vs[P][SN];
+    __align__(16) float ks[P][SN], vs[P][SN];  // vs: V scales times kLift
 
     // Piece c of row r: eight lanes that read the same piece of eight rows find them in different banks.
     static __device__ __forceinline__ int k_at(int r, int c) {
@@ -156,95 +156,121 @@ struct BlockTile {
     }
 };
 
-// A tile on its way from memory: what thread tid loads of it.  K: pieces tid and tid + 256 (NF4: half as many bytes); V: the
-// words of four output tiles g of subtile s, for positions 16 j + 4 lg + i; scales: one position's K or V scales.
-template <int HD, int BITS>
+// A tile on its way from memory, in eight portions which the waves share: of K, pieces 64 w .. 64 w + 63; of V, of subtile s
+// and its half j the words of four output tiles g, for positions 4 lg + i.  Scales: one position's K or V scales.
+template <int HD, int BITS, int WV>
 struct BlockLoad {
     using T = BlockTile<HD, BITS>;
-    static constexpr int RB = BITS == 8 ? HD : HD / 2, PC = HD / 16;
-    uint32_t k[2][BITS == 8 ? 4 : 2], v[2][4], scale;
+    static constexpr int RB = BITS == 8 ? HD : HD / 2, PC = HD / 16, KP = RB / PC, N = 8 / WV;
+    uint32_t k[N][KP / 4], v[N][4], scale;
 
-    // Positions p0 .. of which the ones behind the last, n - 1, repeat it; base: their row's and head's slot 0.
-    __device__ __forceinline__ void load(const k2t_kv_rows &kv, size_t base, int p0, int n) {
-        const int tid = (int)threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
-        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        const int left = n - 1 - p0;
+    // Portion of V: subtile, tile group, half.
+    static __device__ __forceinline__ void portion(int wave, int n, int &s, int &g, int &j) {
+        const int x = N * wave + n;
+        s = HD == 128 ? x >> 2 : x >> 1;
+        g = HD == 128 ? x >> 1 & 1 : 0;
+        j = x & 1;
+    }
+    // Positions p0 .. of a row's and head's slots from `base` on.  Past the cache's end the last of them, cap - 1, is repeated;
+    // up to there, what lies behind the row's positions is loaded and hidden with all that a column does not see.
+    __device__ __forceinline__ void load(const k2t_kv_rows &kv, size_t base, int p0) {
+        const uint32_t tid = threadIdx.x, li = tid & 15u, lg = tid >> 4 & 3u;
+        const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
+        p0 = min(p0, kv.cap - 1);
         const uint8_t *kq = (const uint8_t *)kv.kq + (base + p0) * RB, *vq = (const uint8_t *)kv.vq + (base + p0) * RB;
+        // (a wave takes K scales or V scales, or none)
+        const bool is_v = wave >= T::P / 64;
+        constexpr int SB = BITS == 8 || HD == 128 ? 4 : 2;
+        const uint8_t *sc = (const uint8_t *)(is_v ? kv.vs : kv.ks) + (base + p0) * SB;
+        const uint32_t at = tid % T::P;
+        const bool inside = p0 + T::P <= kv.cap;  // (one offset per lane and immediate ones from it)
+        const uint32_t left = kv.cap - 1 - p0;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const int c = tid + 256 * x, r = min(c / PC, left);
+        for (int n = 0; n < N; n++) {
+            const uint32_t c = tid + 256 * n;
+            const uint32_t off = inside ? tid * KP : min(c / PC, left) * RB + KP * (c % PC);
+            const uint8_t *from = inside ? kq + 256 * KP * n : kq;
             if constexpr (BITS == 8) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(kq + (uint32_t)(r * RB + 16 * (c % PC)));
-                k[x][0] = w.x, k[x][1] = w.y, k[x][2] = w.z, k[x][3] = w.w;
+                const uint4 w = *reinterpret_cast<const uint4 *>(from + off);
+                k[n][0] = w.x, k[n][1] = w.y, k[n][2] = w.z, k[n][3] = w.w;
             } else {
-                const uint2 w = *reinterpret_cast<const uint2 *>(kq + (uint32_t)(r * RB + 8 * (c % PC)));
-                k[x][0] = w.x, k[x][1] = w.y;
+                const uint2 w = *reinterpret_cast<const uint2 *>(from + off);
+                k[n][0] = w.x, k[n][1] = w.y;
             }
         }
-        const int s = HD == 128 ? wave >> 1 : wave, g = HD == 128 ? wave & 1 : 0;
+        const auto word = [&](const uint8_t *from, uint32_t off) -> uint32_t {
+            if constexpr (BITS == 8) return *reinterpret_cast<const uint32_t *>(from + off);
+            else return *reinterpret_cast<const uint16_t *>(from + off);
+        };
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int n = 0; n < N; n++) {
+            int s, g, j;
+            portion(wave, n, s, g, j);
+            const uint32_t col = BITS == 8 ? HD / 16 * li + 4 * g : 32 * g + 2 * li;
+            if (inside) {
+                const uint8_t *from = vq + (size_t)(32 * s + 16 * j) * RB;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = min(32 * s + 16 * j + 4 * lg + i, left);
-                if constexpr (BITS == 8)
-                    v[j][i] = *reinterpret_cast<const uint32_t *>(vq + (uint32_t)(r * RB + HD / 16 * li + 4 * g));
-                else
-                    v[j][i] = *reinterpret_cast<const uint16_t *>(vq + (uint32_t)(r * RB + 32 * g + 2 * li));
+                for (int i = 0; i < 4; i++) v[n][i] = word(from + i * RB, 4 * lg * RB + col);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[n][i] = word(vq, min(32 * s + 16 * j + 4 * lg + i, left) * RB + col);
             }
-        if (tid < 2 * T::P) {
-            const void *p = tid < T::P ? kv.ks : kv.vs;
-            const size_t at = base + p0 + min(tid % T::P, left);
-            if constexpr (BITS == 8 || HD == 128) scale = ((const uint32_t *)p)[at];
-            else scale = ((const uint16_t *)p)[at];
+        }
+        if (wave < 2 * T::P / 64) {
+            const uint32_t off = (inside ? at : min(at, left)) * SB;
+            if constexpr (SB == 4) scale = *reinterpret_cast<const uint32_t *>(sc + off);
+            else scale = *reinterpret_cast<const uint16_t *>(sc + off);
         }
     }
     __device__ __forceinline__ void store(T &tile, const Nf4 &cb) const {
         const int tid = (int)threadIdx.x, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        uint32_t h[N][4][2];
+        int s, g, j;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const int c = tid + 256 * x;
-            *reinterpret_cast<v4i *>(tile.k + T::k_at(c / PC, c % PC)) = k_operand<BITS>(k[x], cb);
+        for (int n = 0; n < N; n++) {
+            const int c = tid + 256 * n;
+            *reinterpret_cast<v4i *>(tile.k + T::k_at(c / PC, c % PC)) = k_operand<BITS>(k[n], cb);
+            portion(wave, n, s, g, j);
+            v_halves(v_word<BITS>(v[n][0], cb), v_word<BITS>(v[n][1], cb), v_word<BITS>(v[n][2], cb), v_word<BITS>(v[n][3], cb), h[n]);
         }
-        const int s = HD == 128 ? wave >> 1 : wave, g = HD == 128 ? wave & 1 : 0;
-        uint32_t h[2][4][2];
 #pragma unroll
-        for (int j = 0; j < 2; j++)
-            v_halves(v_word<BITS>(v[j][0], cb), v_word<BITS>(v[j][1], cb), v_word<BITS>(v[j][2], cb), v_word<BITS>(v[j][3], cb), h[j]);
-#pragma unroll
-        for (int u = 0; u < 4; u++) tile.v[s][4 * g + u][lane] = make_uint4(h[0][u][0], h[0][u][1], h[1][u][0], h[1][u][1]);
+        for (int u = 0; u < 4; u++) {
+            uint4 *to = &tile.v[s][4 * g + u][lane];  // (two portions: the two halves of one)
+            if constexpr (N == 2) *to = make_uint4(h[0][u][0], h[0][u][1], h[N - 1][u][0], h[N - 1][u][1]);
+            else reinterpret_cast<uint2 *>(to)[j] = make_uint2(h[0][u][0], h[0][u][1]);
+        }
         if (tid < 2 * T::P) {
             float *p = tid < T::P ? tile.ks[tid] : tile.vs[tid - T::P];
 #pragma unroll
-            for (int n = 0; n < T::SN; n++) p[n] = TileK<HD, BITS>::scale(scale, n);
+            for (int n = 0; n < T::SN; n++) p[n] = TileK<HD, BITS>::scale(scale, n) * (tid < T::P ? 1.0f : kLift);
         }
     }
 };
 
-template <int HD, int BITS, int NQ>
+template <int HD, int BITS, int WV>
 struct BlockShared {
     union {
         BlockTile<HD, BITS> tile[2];
-        Queries<HD, 16 * NQ> q[kWaves];
-        float o[kWaves][16][HD + 4];
+        Queries<HD, 16> q[WV];
+        float o[WV][16][HD + 4];
     };
     __device__ BlockShared() {}
 };
 
-// An item is (row, KV head, part, 16 NQ columns for each of four waves).
-template <int HD, int BITS, int NQ>
-__global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const TokensArgs A) {
+// An item is (row, KV head, part, 16 columns for each of WV waves).
+template <int HD, int BITS, int WV>
+__global__ __launch_bounds__(64 * WV, HD == 128 && WV == 4 ? 3 : 4) void tokens_block_kernel(const TokensArgs A) {
     using T = BlockTile<HD, BITS>;
-    constexpr int NB = HD / 64, DB = HD / 16, SN = T::SN, W = 16 * NQ;
-    __shared__ BlockShared<HD, BITS, NQ> sh;
+    constexpr int NB = HD / 64, DB = HD / 16, SN = T::SN, NQ = 1, W = 16;
+    __shared__ BlockShared<HD, BITS, WV> sh;
     const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // (the last columns first: theirs are the longest items of a prompt)
     const int unit = (int)blockIdx.x % A.units, cg = A.cgs - 1 - (int)blockIdx.x / A.units;
     const int rh = unit / A.parts, head = rh % A.nkv, row = rh / A.nkv, part = unit % A.parts;
     const Row R = row_of(A, row);
-    const int col0 = W * kWaves * cg, cols = R.count * A.group, n_all = min(W * kWaves, cols - col0);
+    const int col0 = W * WV * cg, cols = R.count * A.group, n_all = min(W * WV, cols - col0);
     if (n_all <= 0) return;
     const int t0 = part * A.plen;
     const int end = min(reach(A, R, (int)column(A, col0 + n_all - 1).row), t0 + A.plen);  // of the item's positions
@@ -256,8 +282,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const Toke
     const float *q0 = A.q + (size_t)row * A.ntok * A.q_stride + (size_t)head * A.group * HD;
     Nf4 cb{};
     if constexpr (BITS == 4) nf4_xor_tables(kNf4Cb0, kNf4Cb1, kNf4Cb2, kNf4Cb3, cb.t0, cb.t1, cb.u0, cb.u1);
-    BlockLoad<HD, BITS> next;
-    if (!none) next.load(A.kv, base, t0, end);
+    BlockLoad<HD, BITS, WV> next;
+    if (!none) next.load(A.kv, base, t0);
     // queries: four 64-blocks of columns at a time
     constexpr int kTurns = W * NB / 4, kBatch = kTurns < 8 ? kTurns : 8;
     for (int k0 = 0; k0 < kTurns; k0 += kBatch) {
@@ -295,14 +321,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const Toke
     const int tiles = none ? 0 : (end - t0 + T::P - 1) / T::P;
     if (!none) {
         next.store(sh.tile[0], cb);
-        next.load(A.kv, base, min(t0 + T::P, end - 1), end);
+        next.load(A.kv, base, t0 + T::P);
     }
     __syncthreads();
     for (int i = 0; i < tiles; i++) {
         const T &tile = sh.tile[i & 1];
         // the next tile into the other half, which all waves have left, and the one behind it on its way
         if (i + 1 < tiles) next.store(sh.tile[(i + 1) & 1], cb);
-        next.load(A.kv, base, min(t0 + T::P * (i + 2), end - 1), end);
+        next.load(A.kv, base, t0 + T::P * (i + 2));
 #pragma unroll 1
         for (int s = 0; s < T::S; s++) {
             seen.p0 = t0 + T::P * i + kTile * s;
@@ -332,7 +358,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_block_kernel(const Toke
             }
             uint32_t ph[NQ][SN][4], pl[NQ][SN][4];
             if (!seen.whole()) hide_tile(t, vs, [&](int a) { return seen.counts(a); });
-            weights<HD, NQ, SN>(S, t, qas, vs, kTile, lg, ph, pl);
+            weights<HD, NQ, SN, true>(S, t, qas, vs, kTile, lg, ph, pl);
 #pragma unroll
             for (int g = 0; g < DB / 4; g++) {
                 constexpr int kBlocks = SN - 1;  // (NF4 blocks have weights of their own)
@@ -420,11 +446,10 @@ struct TokensShape {
     int batch, ntok, nq, nkv, hd;
 };
 
-// How the work is cut.  block: tokens_block_kernel, nq column tiles per wave; else tokens_few_kernel, nq per workgroup.
+// How the work is cut.  waves: of tokens_block_kernel's workgroups; 0: tokens_few_kernel, nq column tiles per workgroup.
 struct Plan {
-    bool block;
-    int nq, cgs, parts, plen;
-    int item() const { return (block ? kWaves : 1) * 16 * nq; }
+    int waves, nq, cgs, parts, plen;
+    int item() const { return 16 * (waves ? waves : nq); }
 };
 constexpr int kFewColumns = 32, kLeastPart = 256;
 
@@ -435,8 +460,8 @@ int parts_wanted(const k2t_ctx *ctx, size_t items) {
 Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int len) {
     const int cols = s.ntok * (s.nq / s.nkv);
     Plan P{};
-    P.block = cols > kFewColumns;
-    P.nq = cols > (P.block ? 64 : 16) ? 2 : 1;
+    P.waves = cols <= kFewColumns ? 0 : cols <= 64 ? 4 : 8;
+    P.nq = cols > 16 ? 2 : 1;
     P.cgs = (cols + P.item() - 1) / P.item();
     const int want = parts_wanted(ctx, (size_t)s.batch * s.nkv * P.cgs);
     P.plen = std::max(kLeastPart, ((len + want - 1) / want + 127) / 128 * 128);
@@ -453,7 +478,7 @@ size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
     const size_t heads = (size_t)s.batch * s.nkv;
     size_t most = 0;
     for (int item : {16, 32, 64, 128}) {
-        const int least = item == 16 ? 1 : item == 128 ? 65 : item / 2 + 1;  // columns of the smallest call with such items
+        const int least = item == 16 ? 1 : item / 2 + 1;  // columns of the smallest call with such items
         if (cols < least) break;
         for (int cgs = 1; (cgs - 1) * item < cols; cgs++) {
             const int parts = std::min(parts_wanted(ctx, heads * cgs), (len + kLeastPart - 1) / kLeastPart);
@@ -466,9 +491,9 @@ size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
 
 template <int HD, int BITS>
 void launch_parts(hipStream_t st, const TokensArgs &A, const Plan &P) {
-    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * kWaves);
-    if (P.block && P.nq == 2) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 2>), grid, block, 0, st, A);
-    else if (P.block) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 1>), grid, block, 0, st, A);
+    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * (P.waves ? P.waves : kWaves));
+    if (P.waves == 8) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 8>), grid, block, 0, st, A);
+    else if (P.waves == 4) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 4>), grid, block, 0, st, A);
     else if (P.nq == 2 && P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, true>), grid, block, 0, st, A);
     else if (P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, false>), grid, block, 0, st, A);
     else if (P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, true>), grid, block, 0, st, A);
