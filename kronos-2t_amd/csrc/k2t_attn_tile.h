@@ -36,7 +36,9 @@ constexpr float kTop = 9.0f, kLimit = 15.0f, kLift = 256.0f, kLog2Lift = 8.0f;
 constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f;
 // Scores so far from zero that fp32 does not tell whole numbers apart.  An exact product less the reference would
 // be up to half a step of the score off then, which may be any power of two: in a column that has met one, scores
-// are rounded before the reference, a rounded one itself, is taken off.
+// are rounded before the reference, a rounded one itself, is taken off.  The largest score's weight is then a power of two that
+// its scale asks for where a step of the score leaves it, else one: a reference that took in the scale before it was
+// rounded could lie a whole step above every score.
 constexpr float kFar = 0x1p24f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -307,6 +309,10 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
         news |= fmaf(top[a], qas[a], lv[0]) > S.m[a];
         if constexpr (SN > 1) news |= fmaf(top[a], qas[a], lv[1]) > S.m1[a];
     }
+    if (S.far) {  // (a step of the score may be more than the limit)
+#pragma unroll
+        for (int a = 0; a < NQ; a++) news |= fabsf(S.m[a]) >= kFar && top[a] * qas[a] > S.m[a];
+    }
     if (__any(news)) {
 #pragma unroll
         for (int a = 0; a < NQ; a++) {
@@ -322,7 +328,15 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
             }
             if constexpr (SN > 1) u[0] = fmaxf(u[0], u[1] - kApart);
             const float most = column_max(u[0]);
-            const float mn = most > S.m[a] + kLimit ? (fabsf(most) >= kFar ? most : ceilf(most) - kTop) : S.m[a];
+            float mn = most > S.m[a] + kLimit ? ceilf(most) - kTop : S.m[a];
+            if (fabsf(most) >= kFar) {
+                const float rounded = column_max(top[a] * qas[a]);
+                float scale = lv[0];
+                if constexpr (SN > 1) scale = fmaxf(scale, lv[1]);
+                scale = fminf(column_max(scale) + kLimit, 100.0f);  // log2 of the largest V scale times kLift
+                const float with = rounded + scale;
+                mn = fmaxf(fabsf((with - rounded) - scale) <= 4.0f ? with : rounded, S.m[a]);
+            }
             S.far |= __any(fabsf(mn) >= kFar && mn > -FLT_MAX) != 0;
             const float down = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
             float down1 = down;

@@ -468,6 +468,40 @@ def test_attention_of_scores_of_any_size(gpu_ctx, bits, hd, beams, nq, nkv, pref
     assert told >= beams * nq // 2 and np.isfinite(got).all()
 
 
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("prefix", [50, 1500])
+@pytest.mark.parametrize("size", [3e8, 1e10, 1e14])
+def test_attention_of_many_heads_with_scores_past_whole_numbers(gpu_ctx, bits, hd, prefix, size):
+    """2048 heads whose scores' steps are 32 and more: whatever a step does to the largest score and to what it is
+    referred to, its weight is not lost, and the head's output is its V."""
+    beams, nq, nkv = 64, 32, 4
+    rng = np.random.default_rng(hd + bits)
+    pre = R.new_cache(bits, 1, nkv, prefix, hd, rng)
+    q = rng.standard_normal((beams, nq, hd)).astype(np.float32)
+    out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+    _, p = rows_of(pre, prefix)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, 0))
+    gpu_ctx.attn_shared(bits, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, None, size, out, ws)
+    gpu_ctx.sync()
+    got = out.cpu().numpy()
+    assert np.isfinite(got).all()
+    import oracle as O
+    code = np.stack([[c.astype(np.float64) * np.float64(s) for c, s in (O.kv_quant_head(h) for h in row)] for row in q])
+    told = 0
+    for g in range(nkv):
+        k, v = (R.values(bits, pre[i][0, g], pre[i + 1][0, g]) for i in (0, 2))
+        heads = slice(g * nq // nkv, (g + 1) * nq // nkv)
+        z = (code[:, heads] @ k.T) * float(np.float32(size))
+        first, second = np.moveaxis(np.sort(z, -1)[..., [-1, -2]], -1, 0)
+        apart = first - second >= 24 + 10 * R.U * np.maximum(first, -z.min(-1))  # (as above)
+        best = v[z.argmax(-1)]
+        bound = (2.0 ** -21 + 8 * R.U) * R.block_sums(np.abs(best)) / 8 + 2.0 ** -30
+        off = np.abs(got[:, heads] - R.unrotate(best))
+        assert (off <= bound)[apart].all()
+        told += int(apart.sum())
+    assert told >= beams * nq * 3 // 4
+
+
 @pytest.mark.parametrize("bits,hd", [(8, 128), (4, 64), (4, 128)])
 @pytest.mark.parametrize("prefix", [50, 1500])
 def test_attention_of_far_scores_stays_in_its_rows(gpu_ctx, bits, hd, prefix):
