@@ -143,6 +143,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_few_kernel(const Tokens
 }
 
 // ---- many columns
+constexpr int kBlockWaves = 8;
+
 template <int HD, int BITS>
 struct BlockTile {
     static constexpr int P = 8192 / HD, S = P / kTile, DB = HD / 16, SN = TileK<HD, BITS>::SN;  // positions; subtiles of 32
@@ -156,20 +158,19 @@ struct BlockTile {
     }
 };
 
-// A tile on its way from memory, in eight portions which the waves share: of K, pieces 64 w .. 64 w + 63; of V, of subtile s
-// and its half j the words of four output tiles g, for positions 4 lg + i.  Scales: one position's K or V scales.
-template <int HD, int BITS, int WV>
+// A tile on its way from memory, in a portion for each of eight waves: 64 pieces of K; of V, of subtile s and its half j the
+// words of four output tiles g, for positions 4 lg + i; one position's K or V scales.
+template <int HD, int BITS>
 struct BlockLoad {
     using T = BlockTile<HD, BITS>;
-    static constexpr int RB = BITS == 8 ? HD : HD / 2, PC = HD / 16, KP = RB / PC, N = 8 / WV;
-    uint32_t k[N][KP / 4], v[N][4], scale;
+    static constexpr int RB = BITS == 8 ? HD : HD / 2, PC = HD / 16, KP = RB / PC;
+    uint32_t k[KP / 4], v[4], scale;
 
     // Portion of V: subtile, tile group, half.
-    static __device__ __forceinline__ void portion(int wave, int n, int &s, int &g, int &j) {
-        const int x = N * wave + n;
-        s = HD == 128 ? x >> 2 : x >> 1;
-        g = HD == 128 ? x >> 1 & 1 : 0;
-        j = x & 1;
+    static __device__ __forceinline__ void portion(int wave, int &s, int &g, int &j) {
+        s = HD == 128 ? wave >> 2 : wave >> 1;
+        g = HD == 128 ? wave >> 1 & 1 : 0;
+        j = wave & 1;
     }
     // Positions p0 .. of a row's and head's slots from `base` on.  Past the cache's end the last of them, cap - 1, is repeated;
     // up to there, what lies behind the row's positions is loaded and hidden with all that a column does not see.
@@ -185,61 +186,45 @@ struct BlockLoad {
         const uint32_t at = tid % T::P;
         const bool inside = p0 + T::P <= kv.cap;  // (one offset per lane and immediate ones from it)
         const uint32_t left = kv.cap - 1 - p0;
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            const uint32_t c = tid + 256 * n;
-            const uint32_t off = inside ? tid * KP : min(c / PC, left) * RB + KP * (c % PC);
-            const uint8_t *from = inside ? kq + 256 * KP * n : kq;
-            if constexpr (BITS == 8) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(from + off);
-                k[n][0] = w.x, k[n][1] = w.y, k[n][2] = w.z, k[n][3] = w.w;
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2 *>(from + off);
-                k[n][0] = w.x, k[n][1] = w.y;
-            }
+        const uint32_t off = inside ? tid * KP : min(tid / PC, left) * RB + KP * (tid % PC);
+        if constexpr (BITS == 8) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(kq + off);
+            k[0] = w.x, k[1] = w.y, k[2] = w.z, k[3] = w.w;
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2 *>(kq + off);
+            k[0] = w.x, k[1] = w.y;
         }
         const auto word = [&](const uint8_t *from, uint32_t off) -> uint32_t {
             if constexpr (BITS == 8) return *reinterpret_cast<const uint32_t *>(from + off);
             else return *reinterpret_cast<const uint16_t *>(from + off);
         };
+        int s, g, j;
+        portion(wave, s, g, j);
+        const uint32_t col = BITS == 8 ? HD / 16 * li + 4 * g : 32 * g + 2 * li;
+        if (inside) {
+            const uint8_t *from = vq + (size_t)(32 * s + 16 * j) * RB;
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            int s, g, j;
-            portion(wave, n, s, g, j);
-            const uint32_t col = BITS == 8 ? HD / 16 * li + 4 * g : 32 * g + 2 * li;
-            if (inside) {
-                const uint8_t *from = vq + (size_t)(32 * s + 16 * j) * RB;
+            for (int i = 0; i < 4; i++) v[i] = word(from + i * RB, 4 * lg * RB + col);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[n][i] = word(from + i * RB, 4 * lg * RB + col);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[n][i] = word(vq, min(32 * s + 16 * j + 4 * lg + i, left) * RB + col);
-            }
+            for (int i = 0; i < 4; i++) v[i] = word(vq, min(32 * s + 16 * j + 4 * lg + i, left) * RB + col);
         }
         if (wave < 2 * T::P / 64) {
-            const uint32_t off = (inside ? at : min(at, left)) * SB;
-            if constexpr (SB == 4) scale = *reinterpret_cast<const uint32_t *>(sc + off);
-            else scale = *reinterpret_cast<const uint16_t *>(sc + off);
+            const uint32_t to = (inside ? at : min(at, left)) * SB;
+            if constexpr (SB == 4) scale = *reinterpret_cast<const uint32_t *>(sc + to);
+            else scale = *reinterpret_cast<const uint16_t *>(sc + to);
         }
     }
     __device__ __forceinline__ void store(T &tile, const Nf4 &cb) const {
         const int tid = (int)threadIdx.x, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        uint32_t h[N][4][2];
+        *reinterpret_cast<v4i *>(tile.k + T::k_at(tid / PC, tid % PC)) = k_operand<BITS>(k, cb);
+        uint32_t h[4][2];
         int s, g, j;
+        portion(wave, s, g, j);
+        v_halves(v_word<BITS>(v[0], cb), v_word<BITS>(v[1], cb), v_word<BITS>(v[2], cb), v_word<BITS>(v[3], cb), h);
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int c = tid + 256 * n;
-            *reinterpret_cast<v4i *>(tile.k + T::k_at(c / PC, c % PC)) = k_operand<BITS>(k[n], cb);
-            portion(wave, n, s, g, j);
-            v_halves(v_word<BITS>(v[n][0], cb), v_word<BITS>(v[n][1], cb), v_word<BITS>(v[n][2], cb), v_word<BITS>(v[n][3], cb), h[n]);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            uint4 *to = &tile.v[s][4 * g + u][lane];  // (two portions: the two halves of one)
-            if constexpr (N == 2) *to = make_uint4(h[0][u][0], h[0][u][1], h[N - 1][u][0], h[N - 1][u][1]);
-            else reinterpret_cast<uint2 *>(to)[j] = make_uint2(h[0][u][0], h[0][u][1]);
-        }
+        for (int u = 0; u < 4; u++) reinterpret_cast<uint2 *>(&tile.v[s][4 * g + u][lane])[j] = make_uint2(h[u][0], h[u][1]);
         if (tid < 2 * T::P) {
             float *p = tid < T::P ? tile.ks[tid] : tile.vs[tid - T::P];
 #pragma unroll
@@ -248,29 +233,29 @@ struct BlockLoad {
     }
 };
 
-template <int HD, int BITS, int WV>
+template <int HD, int BITS>
 struct BlockShared {
     union {
         BlockTile<HD, BITS> tile[2];
-        Queries<HD, 16> q[WV];
-        float o[WV][16][HD + 4];
+        Queries<HD, 16> q[kBlockWaves];
+        float o[kBlockWaves][16][HD + 4];
     };
     __device__ BlockShared() {}
 };
 
-// An item is (row, KV head, part, 16 columns for each of WV waves).
-template <int HD, int BITS, int WV>
-__global__ __launch_bounds__(64 * WV, HD == 128 && WV == 4 ? 3 : 4) void tokens_block_kernel(const TokensArgs A) {
+// An item is (row, KV head, part, 16 columns for each of eight waves).
+template <int HD, int BITS>
+__global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const TokensArgs A) {
     using T = BlockTile<HD, BITS>;
     constexpr int NB = HD / 64, DB = HD / 16, SN = T::SN, NQ = 1, W = 16;
-    __shared__ BlockShared<HD, BITS, WV> sh;
+    __shared__ BlockShared<HD, BITS> sh;
     const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // (the last columns first: theirs are the longest items of a prompt)
     const int unit = (int)blockIdx.x % A.units, cg = A.cgs - 1 - (int)blockIdx.x / A.units;
     const int rh = unit / A.parts, head = rh % A.nkv, row = rh / A.nkv, part = unit % A.parts;
     const Row R = row_of(A, row);
-    const int col0 = W * WV * cg, cols = R.count * A.group, n_all = min(W * WV, cols - col0);
+    const int col0 = W * kBlockWaves * cg, cols = R.count * A.group, n_all = min(W * kBlockWaves, cols - col0);
     if (n_all <= 0) return;
     const int t0 = part * A.plen;
     const int end = min(reach(A, R, (int)column(A, col0 + n_all - 1).row), t0 + A.plen);  // of the item's positions
@@ -282,7 +267,7 @@ __global__ __launch_bounds__(64 * WV, HD == 128 && WV == 4 ? 3 : 4) void tokens_
     const float *q0 = A.q + (size_t)row * A.ntok * A.q_stride + (size_t)head * A.group * HD;
     Nf4 cb{};
     if constexpr (BITS == 4) nf4_xor_tables(kNf4Cb0, kNf4Cb1, kNf4Cb2, kNf4Cb3, cb.t0, cb.t1, cb.u0, cb.u1);
-    BlockLoad<HD, BITS, WV> next;
+    BlockLoad<HD, BITS> next;
     if (!none) next.load(A.kv, base, t0);
     // queries: four 64-blocks of columns at a time
     constexpr int kTurns = W * NB / 4, kBatch = kTurns < 8 ? kTurns : 8;
@@ -446,54 +431,83 @@ struct TokensShape {
     int batch, ntok, nq, nkv, hd;
 };
 
-// How the work is cut.  waves: of tokens_block_kernel's workgroups; 0: tokens_few_kernel, nq column tiles per workgroup.
+// How the work is cut.  block: tokens_block_kernel; else tokens_few_kernel, nq column tiles per workgroup.
 struct Plan {
-    int waves, nq, cgs, parts, plen;
-    int item() const { return 16 * (waves ? waves : nq); }
+    bool block;
+    int nq, cgs, parts, plen;
+    int item() const { return 16 * (block ? kBlockWaves : nq); }
 };
-constexpr int kFewColumns = 32, kLeastPart = 256;
+// Items of one tile of columns (16) up to so much work: more workgroups, and a shorter way through each.  Measured on both
+// sides (us, one tile and two): 300 tokens, 32 heads x 64: 2.8 rounds, 7.0 and 8.5; 8 x 13 tokens behind 2100, 32 / 8 x 128: 16.5
+// rounds, 20.0 and 25.2; 777 tokens, 32 heads x 64: 18 rounds, 17.9 and 15.8; 64 tokens behind 12000, 32 / 4 x 128: 47 rounds, 51.5 and
+// 42.4.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.5 and 42.7 with it;
+// 2048, two: 83.6 and 78.5; 8192, eight: 923 and 770), and for NF4 heads of two blocks, whose lookups it shares, wherever there is
+// work for it (515 tokens behind 4100, 32 / 8 x 128: 148 and 127).
+constexpr double kLittleWork = 17.0;
+constexpr int kLeastPart = 256;
 
-// Parts of the positions so that `items` items per part come to about two workgroups for every CU.
-int parts_wanted(const k2t_ctx *ctx, size_t items) {
-    return (int)std::max<size_t>(1, 2 * (size_t)std::max(1, ctx->num_cus) / std::max<size_t>(1, items));
+// The most parts that a call of so many items per part is cut into: two workgroups for every CU.
+int most_parts(const k2t_ctx *ctx, size_t items, int len) {
+    const size_t want = 2 * (size_t)std::max(1, ctx->num_cus) / std::max<size_t>(1, items);
+    return (int)std::max<size_t>(1, std::min<size_t>(want, (len + kLeastPart - 1) / kLeastPart));
 }
-Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int len) {
+// What a call cut into n parts of `each` positions costs, in microseconds: rounds of items on the card, the transforms at
+// an item's ends, and the joining (3 us and its bytes).
+double plan_cost(const TokensShape &s, const Plan &P, int bits, size_t cus, size_t items, int n, int each) {
+    const double position = (P.block ? 0.025 : 0.008) * (s.hd / 128.0) * (bits == 4 ? 1.4 : 1.0), ends = 5.0;
+    const double rounds = (double)((items + cus - 1) / cus);
+    const double join = n == 1 ? 0.0 : 3.0 + (double)s.batch * s.ntok * s.nq * n * s.hd * 1.5e-6;
+    return rounds * each * position + (items > 2 * cus ? rounds / 2 : 1) * ends + join;
+}
+Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int len) {
     const int cols = s.ntok * (s.nq / s.nkv);
+    const size_t cus = (size_t)std::max(1, ctx->num_cus), heads = (size_t)s.batch * s.nkv;
     Plan P{};
-    P.waves = cols <= kFewColumns ? 0 : cols <= 64 ? 4 : 8;
-    P.nq = cols > 16 ? 2 : 1;
+    const auto items = [&](int item) { return std::max<size_t>(1, heads * ((cols + item - 1) / item)); };
+    // rounds of 128 positions that items of one tile of columns make on a CU
+    const double work = (double)items(16) * (tree ? len : std::max(len - s.ntok / 2, 1)) / 128 / cus;
+    P.block = bits == 4 && s.hd == 128 ? cols >= 128 && work > kLittleWork : 2 * items(16 * kBlockWaves) >= 3 * cus;
+    P.nq = work <= kLittleWork ? 1 : 2;
     P.cgs = (cols + P.item() - 1) / P.item();
-    const int want = parts_wanted(ctx, (size_t)s.batch * s.nkv * P.cgs);
-    P.plen = std::max(kLeastPart, ((len + want - 1) / want + 127) / 128 * 128);
-    P.parts = std::max(1, (len + P.plen - 1) / P.plen);
+    const size_t each_part = items(P.item());
+    const int most = most_parts(ctx, each_part, len);
+    P.parts = 1;
+    P.plen = std::max(len, 1);
+    double least = plan_cost(s, P, bits, cus, each_part, 1, len);
+    for (int n = 2; n <= most; n++) {
+        const int each = ((len + n - 1) / n + 127) / 128 * 128;
+        if ((len + each - 1) / each < n) continue;  // (as many parts as a smaller n's)
+        const double cost = plan_cost(s, P, bits, cus, each_part * n, n, each);
+        if (cost >= least) continue;
+        least = cost;
+        P.parts = n;
+        P.plen = each;
+    }
     return P;
 }
 size_t part_slots(const TokensShape &s, int parts) { return (size_t)s.batch * s.ntok * s.nq * parts; }
 size_t slot_bytes(int hd) { return hd * sizeof(float) + sizeof(float2); }
 size_t ws_bytes_of(const TokensShape &s, int parts) { return parts == 1 ? 16 : part_slots(s, parts) * slot_bytes(s.hd); }
-// At least that of every plan of up to so many tokens and positions: for every number of column groups of
-// each kind of item, as many columns as it has and as many parts as it may want (fewer where there are more groups).
+// At least that of every plan of up to so many tokens and positions: for every kind of item and number of column groups, as
+// many columns as it has and as many parts as it may be cut into (fewer where there are more groups).
 size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
     const int cols = s.ntok * (s.nq / s.nkv);
     const size_t heads = (size_t)s.batch * s.nkv;
-    size_t most = 0;
-    for (int item : {16, 32, 64, 128}) {
-        const int least = item == 16 ? 1 : item / 2 + 1;  // columns of the smallest call with such items
-        if (cols < least) break;
+    size_t most = 16;
+    for (int item : {16, 32, 16 * kBlockWaves}) {
         for (int cgs = 1; (cgs - 1) * item < cols; cgs++) {
-            const int parts = std::min(parts_wanted(ctx, heads * cgs), (len + kLeastPart - 1) / kLeastPart);
+            const int parts = most_parts(ctx, heads * cgs, len);
             if (parts <= 1) break;
             most = std::max(most, heads * std::min(cols, cgs * item) * parts * slot_bytes(s.hd));
         }
     }
-    return std::max<size_t>(16, most);
+    return most;
 }
 
 template <int HD, int BITS>
 void launch_parts(hipStream_t st, const TokensArgs &A, const Plan &P) {
-    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * (P.waves ? P.waves : kWaves));
-    if (P.waves == 8) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 8>), grid, block, 0, st, A);
-    else if (P.waves == 4) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, 4>), grid, block, 0, st, A);
+    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * (P.block ? kBlockWaves : kWaves));
+    if (P.block) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS>), grid, block, 0, st, A);
     else if (P.nq == 2 && P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, true>), grid, block, 0, st, A);
     else if (P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, false>), grid, block, 0, st, A);
     else if (P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, true>), grid, block, 0, st, A);
@@ -558,7 +572,7 @@ int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
                    "d_q must be 16-byte aligned, q_stride a multiple of 4, no smaller than a token's heads, below 2^31");
         branch_arg((at(d_out) | at(d_ws)) % 16 == 0, "d_out and d_ws must be 16-byte aligned");
         branch_arg(at(d_sees) % 8 == 0, "d_sees must be 8-byte aligned");
-        const Plan P = plan_of(ctx, s, kv->len);
+        const Plan P = plan_of(ctx, s, bits, d_sees != nullptr, kv->len);
         const size_t need = ws_bytes_of(s, P.parts);
         if (ws_bytes < need)
             throw Error(K2T_E_ARG, "the workspace holds " + std::to_string(ws_bytes) + " bytes, " +

@@ -23,8 +23,8 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256, kLogitSlice = 4096, kGroups = kLogitSlice / 4 / kThreads;  // groups of four logits per thread
-constexpr int kMaxHistory = 1 << 20, kMaxBias = 4096;
+constexpr int kThreads = 256, kLogitSlice = 2048, kGroups = kLogitSlice / 4 / kThreads;  // groups of four logits per thread
+constexpr int kMaxHistory = 1 << 20, kMaxBias = 4096, kAhead = 8;
 constexpr uint32_t kSeen = 1u << 31;    // over the count of a token behind the prompt
 constexpr uint32_t kNone = 0xFFFFu, kAgain = 1u << 15;  // no bias; more entries than the first name the token
 
@@ -74,11 +74,19 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
             const int len = R.d_history_len ? max(0, min(R.d_history_len[row], R.history_len)) : R.history_len;
             const int prompt = R.d_prompt_len ? R.d_prompt_len[row] : 0;
             const int *h = R.d_history + (size_t)row * R.history_stride;
-            for (int i = tid; i < len; i += kThreads) {
-                const uint32_t t = (uint32_t)h[i] - (uint32_t)v0;
-                if (t >= (uint32_t)n) continue;
-                atomicOr(&count[t], kSeen);
-                if (i >= prompt) atomicAdd(&count[t], 1u);
+            // (several loads in flight: the list is the longest chain of a short row)
+            for (int i0 = tid; i0 < len; i0 += kAhead * kThreads) {
+                int token[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; k++) token[k] = h[min(i0 + k * kThreads, len - 1)];
+#pragma unroll
+                for (int k = 0; k < kAhead; k++) {
+                    const int i = i0 + k * kThreads;
+                    const uint32_t t = (uint32_t)token[k] - (uint32_t)v0;
+                    if (i >= len || t >= (uint32_t)n) continue;
+                    atomicOr(&count[t], kSeen);
+                    if (i >= prompt) atomicAdd(&count[t], 1u);
+                }
             }
         }
         const int *names = R.d_bias_tokens + (size_t)row * R.bias_stride;
@@ -140,7 +148,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
 #pragma unroll
         for (int j = 0; j < 4; j++) f[g][j] = allowed >> j & 1u ? f[g][j] : -INFINITY;
         if (VEC && i + 4 <= n) {
-            *reinterpret_cast<f32x4 *>(out + i) = f[g];
+            __builtin_nontemporal_store(f[g], reinterpret_cast<f32x4 *>(out + i));
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)

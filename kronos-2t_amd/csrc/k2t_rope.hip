@@ -57,7 +57,7 @@ __device__ __forceinline__ void unit_at(const k2t_rope_plan &P, int u, int &a, i
     }
 }
 
-constexpr int kMaxPer = 8, kFlight = 4;  // tokens of a workgroup; units in flight per thread
+constexpr int kMaxPer = 3, kFlight = 4;  // tokens of a workgroup; units in flight per thread
 
 // VEC 8: rot_dim is a multiple of 8, so that a unit is two 16-byte pieces; else VEC 2, a pair at a time.
 template <int VEC>
@@ -71,8 +71,13 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs A) {
         f32x4 a, b;
     };
     const auto live = [&](int token) {
-        return !A.counts || token % A.ntok < A.counts[token / A.ntok];
+        const int row = token / A.ntok;
+        return !A.counts || token - row * A.ntok < A.counts[row];
     };
+    // (a workgroup whose tokens its rows do not have; one of them is loaded even so where others are there)
+    bool some = false;
+    for (int t = 0; t < n; t++) some |= live(first + t);
+    if (!some) return;
     const auto load = [&](int g, Piece &p) {
         const int t = g / A.units, u = g - t * A.units, head = u >> A.hd_shift, e = u & ((1 << A.hd_shift) - 1);
         int a, b;
@@ -115,8 +120,8 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs A) {
             }
         }
         if constexpr (VEC == 8) {
-            *reinterpret_cast<f32x4 *>(o + a) = f32x4{y[0], y[1], y[2], y[3]};
-            *reinterpret_cast<f32x4 *>(o + b) = f32x4{y[4], y[5], y[6], y[7]};
+            __builtin_nontemporal_store((f32x4{y[0], y[1], y[2], y[3]}), reinterpret_cast<f32x4 *>(o + a));
+            __builtin_nontemporal_store((f32x4{y[4], y[5], y[6], y[7]}), reinterpret_cast<f32x4 *>(o + b));
         } else {
             o[a] = y[0];
             o[b] = y[1];

@@ -114,7 +114,7 @@ def check(got, want, bound):
     assert ok.all(), (np.argwhere(~ok)[:4], got[~ok][:4], want[~ok][:4], bound[~ok][:4], (off / bound)[~gone].max())
 
 
-def case(rng, bits, batch, ntok, nq, nkv, hd, start, with_counts, with_tree, spare=3):
+def case(rng, bits, batch, ntok, nq, nkv, hd, start, with_counts, with_tree, spare=3, first=None):
     cap = start + ntok + spare
     cache = B.new_cache(bits, batch, nkv, cap, hd, rng)
     q = rng.standard_normal((batch, ntok, nq, hd)).astype(np.float32)
@@ -124,6 +124,8 @@ def case(rng, bits, batch, ntok, nq, nkv, hd, start, with_counts, with_tree, spa
     if with_counts:
         counts = rng.integers(0, ntok + 2, batch).astype(np.int32)
         counts[-1] = (ntok + 1) // 2
+    if first is not None:  # row 0: all of its tokens, from this position on
+        pos[0], counts[0] = first, ntok
     sees = np.stack([tree(rng, ntok) for _ in range(batch)]) if with_tree else None
     # what lies behind a row's block is never read: NaN scales
     for r in range(batch):
@@ -247,6 +249,95 @@ def test_attention_masked_scores_above_all_others(gpu_ctx):
         cache[1][0, :, big] = 900.0 if bits == 8 else 0x4461
         want, bound = R.attention(bits, q, cache, pos, np.full(1, ntok), sees, nq, nkv, hd, 0.3, cap)
         check(attend(gpu_ctx, bits, q, cache, pos, counts, sees, nq, nkv, hd, 0.3, cap), want, bound)
+
+
+def attention_on_gpu(bits, q, cache, pos, counts, sees, nq, nkv, hd, scale, length):
+    """block_ref.attention's outputs and bounds for many tokens: a row's KV head at a time in 64 bits on the GPU."""
+    import oracle as O
+    batch, ntok = q.shape[:2]
+    g = nq // nkv
+    flat = q.reshape(-1, hd)
+    codes = [O.kv_quant_head(x) for x in flat]
+    qv = np.stack([c.astype(np.float64) * np.float64(s) for c, s in codes]).reshape(batch, ntok, nkv, g, hd) * float(np.float32(scale))
+    out, bound = np.full((batch, ntok, nq, hd), np.nan), np.full((batch, ntok, nq, hd), np.nan)
+    for r in range(batch):
+        n = int(max(0, min(ntok, counts[r])))
+        end = int(max(0, min(length, pos[r] + n)))
+        if n == 0:
+            continue
+        see = torch.from_numpy(R.visible(ntok, int(pos[r]), n, end, None if sees is None else [int(x) for x in sees[r]])[:n]).cuda()
+        for h in range(nkv):
+            k, v = (dev(B.values(bits, cache[i][r, h, :end], cache[i + 1][r, h, :end])) for i in (0, 2))
+            x = dev(qv[r, :n, h]).reshape(n * g, hd)
+            parts = (x.view(-1, hd // 64, 64).transpose(0, 1).contiguous() @ k.view(-1, hd // 64, 64).permute(1, 2, 0).contiguous()) if bits == 4 \
+                else (x @ k.T.contiguous())[None]
+            m = see[:, None].expand(n, g, end).reshape(n * g, end)
+            z, size = parts.sum(0).masked_fill(~m, -np.inf), parts.abs().sum(0).masked_fill(~m, 0)
+            none = ~m.any(1)
+            w = torch.softmax(z, 1).masked_fill(none[:, None], 0)
+            o, a = (w @ v).cpu().numpy(), (w @ v.abs()).cpu().numpy()
+            rel = (2 * (9 * size.amax(1) + 4) + 2 * (m.sum(1) / 32 + 128)).cpu().numpy()[:, None] * R.U + 2.0 ** -21
+            out[r, :n, h * g:(h + 1) * g] = B.unrotate(o).reshape(n, g, hd)
+            b = (rel * B.block_sums(a) + 7 * R.U * B.block_sums(np.abs(o))) / 8 + 1e-37
+            b[none.cpu().numpy()] = 0
+            bound[r, :n, h * g:(h + 1) * g] = b.reshape(n, g, hd)
+    return out, bound
+
+
+# many workgroups of columns (nkv * batch * columns / 128), or a cache of many positions (`room`), of which the rows
+# hold few: what is chosen goes by the room
+LARGE = [(8, 64, 64, 64, 3, 200, 40, 0, False), (8, 64, 128, 64, 4, 90, 0, 0, True), (8, 128, 96, 48, 5, 130, 70, 0, False),
+         (8, 128, 32, 4, 16, 64, 100, 0, True), (4, 64, 66, 33, 6, 150, 30, 0, False), (4, 128, 32, 4, 2, 64, 300, 9000, True),
+         (4, 128, 16, 2, 3, 300, 0, 12000, False), (8, 128, 32, 4, 2, 64, 700, 20000, True), (8, 64, 32, 32, 1, 60, 500, 30000, True),
+         (8, 128, 8, 2, 2, 40, 900, 6000, False), (4, 64, 9, 3, 3, 50, 40, 50000, True), (8, 64, 12, 4, 1, 1100, 0, 0, False)]
+
+
+@pytest.mark.parametrize("bits,hd,nq,nkv,batch,ntok,start,room,with_tree", LARGE)
+def test_attention_of_many_columns_and_parts(gpu_ctx, bits, hd, nq, nkv, batch, ntok, start, room, with_tree):
+    with_tree = with_tree and ntok <= 64
+    print(f"attn_tokens bits={bits} hd={hd} heads={nq}/{nkv} batch={batch} ntok={ntok} start={start} room={room} tree={with_tree}", flush=True)
+    rng = np.random.default_rng(hd * ntok + nq)
+    q, cache, pos, counts, sees, cap = case(rng, bits, batch, ntok, nq, nkv, hd, start, True, with_tree, spare=3 + room,
+                                            first=0 if with_tree else start)
+    if with_tree:
+        sees[0, ::5] = 0  # (row 0 has nothing in front: these see nothing)
+    want, bound = attention_on_gpu(bits, q, cache, pos, counts, sees, nq, nkv, hd, 0.17, cap)
+    check(attend(gpu_ctx, bits, q, cache, pos, counts, sees, nq, nkv, hd, 0.17, cap, extra=ntok), want, bound)
+    # a NaN and an infinite V scale of one token reach only those that see it
+    t = ntok // 3
+    r = int(np.argmax(np.minimum(counts, ntok) > t))
+    c = [a.copy() for a in cache]
+    c[3][r, :, pos[r] + t] = np.nan if bits == 8 else 0x7F80
+    got = attend(gpu_ctx, bits, q, c, pos, counts, sees, nq, nkv, hd, 0.17, cap)
+    see = R.visible(ntok, int(pos[r]), int(min(counts[r], ntok)), cap, None if sees is None else [int(x) for x in sees[r]])[:, pos[r] + t]
+    others = ~np.isnan(bound)
+    others[r, see] = False
+    assert (np.abs(got - want)[others] <= bound[others]).all()
+    assert not np.isfinite(got[r][see & (np.arange(ntok) < counts[r])]).any(-1).all(-1).any()
+
+
+@pytest.mark.parametrize("bits,hd,nq,nkv,batch,ntok,start,room,with_tree", [LARGE[i] for i in (0, 3, 5, 6, 7, 9)])
+@pytest.mark.parametrize("kind", ["large", "vscales", "zero", "far"])
+def test_attention_of_many_columns_and_values_of_any_size(gpu_ctx, bits, hd, nq, nkv, batch, ntok, start, room, with_tree, kind):
+    rng = np.random.default_rng(hd + ntok)
+    q, cache, pos, counts, sees, cap = case(rng, bits, batch, ntok, nq, nkv, hd, start, False, with_tree, spare=3 + room)
+    end = start + ntok
+    shape = cache[1][:, :, :end].shape
+
+    def scales(lo, hi):
+        f = np.exp2(rng.uniform(lo, hi, shape)).astype(np.float32)
+        return f if bits == 8 else (f.view(np.uint32) >> 16).astype(np.uint16)
+    if kind in ("large", "far"):
+        cache[1][:, :, :end] = scales(4, 6) if kind == "large" else scales(20, 24)
+    elif kind == "vscales":
+        cache[3][:, :, :end] = scales(-60, 20)
+    else:
+        q[:, ::2] = 0.0
+    for r in range(batch):
+        for a in (cache[1], cache[3]):
+            a[r, :, pos[r] + ntok:] = np.nan if bits == 8 else 0x7FC0
+    want, bound = attention_on_gpu(bits, q, cache, pos, np.full(batch, ntok), sees, nq, nkv, hd, 0.1, cap)
+    check(attend(gpu_ctx, bits, q, cache, pos, counts, sees, nq, nkv, hd, 0.1, cap), want, np.minimum(bound, 1e300))
 
 
 @pytest.mark.parametrize("bits", [8, 4])
