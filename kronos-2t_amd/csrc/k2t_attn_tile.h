@@ -761,23 +761,29 @@ __device__ __forceinline__ void merge_parts(const ColumnArgs &A, int pair, const
         };
         const float2 st = A.stat[at + min(mine, n - 1)];
         load(w0);
+        __builtin_amdgcn_sched_barrier(0);  // (all of them in flight before the reductions)
         const bool live = mine < n && live_part(mine);
         const float mn = fmaxf(m, wave_max_f(live ? st.x : -INFINITY));
-        if (mn == -INFINITY) continue;  // (no live one: -FLT_MAX in a part whose scores are NaN)
-        const float e = live ? __builtin_amdgcn_exp2f(st.x - mn) : 0.0f, corr = __builtin_amdgcn_exp2f(m - mn);
+        // (-inf: no live one yet; -FLT_MAX in a part whose scores are NaN)
+        const float e = live ? __builtin_amdgcn_exp2f(st.x - mn) : 0.0f;
+        const float corr = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
         l = fmaf(l, corr, wave_sum_f(live ? st.y * e : 0.0f));
 #pragma unroll
         for (int k = 0; k < E; k++) o[k] *= corr;
         m = mn;
-        for (int j0 = w0; j0 < cnt; j0 += kAhead * WAVES) {
-            if (j0 > w0) load(j0);
+        // (e is zero behind the last part; the first batch outside the loop, and no branch before it: its loads would sink there)
+        const auto add = [&](int j0) {
 #pragma unroll
             for (int u = 0; u < kAhead; u++) {
-                const int j = j0 + u * WAVES;
-                const float w = j < cnt ? lane_val(e, j) : 0.0f;
+                const float w = lane_val(e, j0 + u * WAVES);
 #pragma unroll
                 for (int k = 0; k < E; k++) o[k] = w != 0.0f ? fmaf(v[u][k], w, o[k]) : o[k];
             }
+        };
+        add(w0);
+        for (int j0 = w0 + kAhead * WAVES; j0 < cnt; j0 += kAhead * WAVES) {
+            load(j0);
+            add(j0);
         }
     }
     if constexpr (WAVES > 1) {
