@@ -440,9 +440,10 @@ struct Plan {
 // Items of one tile of columns (16) up to so much work: more workgroups, and a shorter way through each.  Measured on both
 // sides (us, one tile and two): 300 tokens, 32 heads x 64: 2.8 rounds, 7.0 and 8.5; 8 x 13 tokens behind 2100, 32 / 8 x 128: 16.5
 // rounds, 20.0 and 25.2; 777 tokens, 32 heads x 64: 18 rounds, 17.9 and 15.8; 64 tokens behind 12000, 32 / 4 x 128: 47 rounds, 51.5 and
-// 42.4.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.5 and 42.7 with it;
-// 2048, two: 83.6 and 78.5; 8192, eight: 923 and 770), and for NF4 heads of two blocks, whose lookups it shares, wherever there is
-// work for it (515 tokens behind 4100, 32 / 8 x 128: 148 and 127).
+// 37.0.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.5 and 42.7 with it;
+// 2048, two: 83.6 and 78.5; 8192, eight: 923 and 770), and for NF4 heads of two blocks, whose lookups it shares, from more than one
+// for four CUs on (4 x 64 tokens behind 2100, 32 / 8 x 128, one for four: 40.5 and 46.1; 300 tokens, five for sixteen: 59.2 and 56.2;
+// 515 behind 4100, one for two: 133 and 126).
 constexpr double kLittleWork = 17.0;
 constexpr int kLeastPart = 256;
 
@@ -455,7 +456,9 @@ int most_parts(const k2t_ctx *ctx, size_t items, int len) {
 // an item's ends, and the joining (3 us and its bytes).
 double plan_cost(const TokensShape &s, const Plan &P, int bits, size_t cus, size_t items, int n, int each) {
     const double position = (P.block ? 0.025 : 0.008) * (s.hd / 128.0) * (bits == 4 ? 1.4 : 1.0), ends = 5.0;
-    const double rounds = (double)((items + cus - 1) / cus);
+    // (two items of two tiles on a CU hide some of each other's waits: 64 tokens behind 20000, 32 heads x 64, one on a CU and
+    // two: 50.4 and 39.4 us; 2 x 40 behind 6100, 32 / 8 x 128: 31.6 and 29.4)
+    const double rounds = (double)((items + cus - 1) / cus) * (!P.block && P.nq == 2 && items > cus ? 0.8 : 1.0);
     const double join = n == 1 ? 0.0 : 3.0 + (double)s.batch * s.ntok * s.nq * n * s.hd * 1.5e-6;
     return rounds * each * position + (items > 2 * cus ? rounds / 2 : 1) * ends + join;
 }
@@ -466,7 +469,8 @@ Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int 
     const auto items = [&](int item) { return std::max<size_t>(1, heads * ((cols + item - 1) / item)); };
     // rounds of 128 positions that items of one tile of columns make on a CU
     const double work = (double)items(16) * (tree ? len : std::max(len - s.ntok / 2, 1)) / 128 / cus;
-    P.block = bits == 4 && s.hd == 128 ? cols >= 128 && work > kLittleWork : 2 * items(16 * kBlockWaves) >= 3 * cus;
+    const size_t blocks = items(16 * kBlockWaves);
+    P.block = bits == 4 && s.hd == 128 ? 4 * blocks > cus : 2 * blocks >= 3 * cus;
     P.nq = work <= kLittleWork ? 1 : 2;
     P.cgs = (cols + P.item() - 1) / P.item();
     const size_t each_part = items(P.item());
