@@ -496,7 +496,8 @@ int32_t k2t_beam_select_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, in
  * of drafted tokens that lie side by side in the cache until k2t_kv_keep leaves one path of it.
  *
  * All of these calls run on the context's stream, allocate nothing, do not synchronise, and may be captured into a
- * graph, which then reads positions, counts, depths, masks, histories and lists at every replay. */
+ * graph, which then reads positions, counts, depths, masks, histories and lists at every replay.  What a call writes
+ * overlaps none of its other buffers, unless it says so. */
 
 /* Rotary positions.  A plan holds, for every pair i < rot_dim / 2, its turns per position (its angular
  * frequency over 2 pi), and the factor of rotated elements.  k2t_rope_plan_make fills one: frequency

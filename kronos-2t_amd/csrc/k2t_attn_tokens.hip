@@ -581,8 +581,8 @@ int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
         if (ws_bytes < need)
             throw Error(K2T_E_ARG, "the workspace holds " + std::to_string(ws_bytes) + " bytes, " +
                                        std::to_string(need) + " are needed");
+        // (with cgs at most as many as there are columns, or two workgroups for every CU: grids are within 2^23)
         const size_t units = (size_t)batch * n_kv_heads * P.parts;
-        branch_arg(units * P.cgs <= (size_t)1 << 24, "too many rows, heads and positions in one call");
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
         TokensArgs A{};
         A.q = d_q;

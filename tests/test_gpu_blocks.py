@@ -726,3 +726,106 @@ def test_calls_in_a_graph_follow_what_is_on_the_device():
                 assert torch.equal(a, b), i
         eager.close()
     ctx.close()
+
+
+# ---------------------------------------------------------------- the largest calls, and calls beside each other
+def test_the_most_rows_of_blocks(gpu_ctx):
+    """65535 rows of one token in one call of each kind: what a call of few rows does to each of them."""
+    rows, few, hd, cap = 65535, 7, 64, 3
+    g = torch.Generator(device="cuda").manual_seed(3)
+    many = torch.arange(rows, device="cuda") % few
+    x = torch.randn(few, hd, generator=g, device="cuda")
+    cache = [torch.randint(-127, 128, (few, 1, cap, hd), generator=g, device="cuda", dtype=torch.int8),
+             torch.rand(few, 1, cap, generator=g, device="cuda")]
+    cache += [a.flip(0).contiguous() for a in cache]
+    pos, lists = ints([2, 0, 1, 2, 2, 1, 0]), ints([[i % 3, 2] for i in range(few)])
+    rules = dict(history=ints([[i, i, 4 - i % 5] for i in range(few)]), frequency=torch.rand(few, generator=g, device="cuda"))
+    logits = torch.randn(few, 5, generator=g, device="cuda")
+    plan = k2t.RopePlan(k2t.ROPE_INTERLEAVED, 30, 1e4)
+
+    def calls(n, x, cache, pos, lists, rules, logits):
+        out, rot, adj = torch.zeros(n, hd, device="cuda"), torch.zeros(n, hd, device="cuda"), torch.zeros(n, 5, device="cuda")
+        kv = k2t.KVRows(*cache, cap=cap)
+        ws = workspace(gpu_ctx.attn_tokens_workspace(n, 1, 1, 1, hd, cap))
+        gpu_ctx.attn_tokens(8, x, hd, n, 1, 1, 1, hd, pos, kv, 0.1, out, ws)
+        gpu_ctx.rope(x, hd, n, 1, 1, hd, pos, plan, rot, hd)
+        gpu_ctx.logits_adjust(logits, 5, 5, n, k2t.LogitsRules(**rules), adj, 5)
+        gpu_ctx.kv_keep(8, kv, torch.zeros_like(pos), lists, 2, None, 2, 1, n, 1, hd)
+        gpu_ctx.sync()
+        return [out, rot, adj, *cache]
+
+    take = lambda t: t[many].contiguous()  # noqa: E731
+    got = calls(rows, take(x), [take(a) for a in cache], take(pos), take(lists), {n: take(a) for n, a in rules.items()}, take(logits))
+    want = calls(few, x, cache, pos, lists, rules, logits)
+    assert want[0].abs().min(1).values.min() > 0 and not torch.equal(want[1], x) and not torch.equal(want[2], logits)
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), take(b).view(torch.uint8))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("nq,nkv,ntok", [(1024, 1, 2), (1024, 1024, 3), (1024, 32, 5)])
+def test_attention_of_the_most_heads(gpu_ctx, bits, nq, nkv, ntok):
+    print(f"attn_tokens bits={bits} heads={nq}/{nkv} ntok={ntok}", flush=True)
+    rng = np.random.default_rng(nkv)
+    q, cache, pos, counts, sees, cap = case(rng, bits, 2, ntok, nq, nkv, 64, 37, True, True)
+    got = attend(gpu_ctx, bits, q, cache, pos, counts, sees, nq, nkv, 64, 0.17, cap)
+    check(got, *R.attention(bits, q, cache, pos, counts, sees, nq, nkv, 64, 0.17, cap))
+
+
+def test_strides_past_32_bits(gpu_ctx):
+    """Rows 2^31 floats apart, and more than 2^32 bytes."""
+    stride, hd, vocab = (1 << 31) + 64, 64, 6
+    buf = torch.empty(2 * stride, device="cuda")
+    x = torch.randn(3, hd, device="cuda")
+    at = [buf[i * stride:i * stride + hd] for i in range(2)] + [buf[-hd:]]
+    plan = k2t.RopePlan(k2t.ROPE_HALF, hd, 1e4)
+    want, out = torch.zeros(2, hd, device="cuda"), torch.zeros(2, hd, device="cuda")
+    for i in range(2):
+        at[i].copy_(x[i])
+    gpu_ctx.rope(x, hd, 1, 2, 1, hd, ints([9]), plan, want, hd)
+    gpu_ctx.rope(buf, stride, 1, 2, 1, hd, ints([9]), plan, out, hd)
+    gpu_ctx.rope(buf, stride, 1, 2, 1, hd, ints([9]), plan, buf, stride)
+    gpu_ctx.sync()
+    assert torch.equal(out, want) and torch.equal(torch.stack(at[:2]), want)
+    rules = k2t.LogitsRules(history=ints([[0, 2], [5, 9]]), repeat=torch.tensor([2.0, 4.0], device="cuda"))
+    gpu_ctx.logits_adjust(buf, vocab, stride, 2, rules, buf, stride)
+    gpu_ctx.sync()
+    for i, tokens in enumerate(([0, 2], [5])):
+        r = 2.0 * (i + 1)
+        for t in tokens:
+            want[i, t] = want[i, t] / r if want[i, t] > 0 else want[i, t] * r
+    assert torch.equal(torch.stack(at[:2]), want)
+
+
+@pytest.mark.parametrize("bits,hd,nq,nkv,ntok,start", [(8, 64, 9, 3, 10, 300), (8, 128, 32, 4, 300, 2000), (4, 128, 16, 4, 600, 900)])
+def test_contexts_on_two_streams_do_not_meet(bits, hd, nq, nkv, ntok, start):
+    """Two contexts' calls under way at once, each with a workspace and buffers of its own: the results of each alone."""
+    rng = np.random.default_rng(ntok)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [k2t.Ctx(0, s) for s in streams]
+    cap = start + ntok
+    runs = []
+    for c in ctxs:
+        t, kv = rows_of(B.new_cache(bits, 1, nkv, cap, hd, rng), cap)
+        q = torch.from_numpy(rng.standard_normal((ntok, nq * hd)).astype(np.float32)).cuda()
+        runs.append((c, t, kv, q, ints([start]), workspace(c.attn_tokens_workspace(1, ntok, nq, nkv, hd, cap)),
+                     [torch.zeros(ntok, nq * hd, device="cuda") for _ in range(6)]))
+    torch.cuda.synchronize()
+
+    def go(run, i):
+        c, t, kv, q, pos, ws, out = run
+        c.attn_tokens(bits, q, nq * hd, 1, ntok, nq, nkv, hd, pos, kv, 0.125, out[i], ws)
+
+    for run in runs:
+        go(run, 0)
+        run[0].sync()
+    for i in range(1, 6):
+        for run in runs:
+            go(run, i)
+    for run, c in zip(runs, ctxs):
+        c.sync()
+        assert run[6][0].abs().sum() > 0
+        for o in run[6][1:]:
+            assert torch.equal(o, run[6][0])
+    for c in ctxs:
+        c.close()
