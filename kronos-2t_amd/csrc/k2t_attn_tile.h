@@ -23,7 +23,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-constexpr int kWaves = 4, kTile = 32;  // waves of a workgroup; positions of a wave's tile
+constexpr int kWaves = 4, kTile = 32;  // waves of a workgroup (where none is given); positions of a wave's tile
 // A column's reference m is a power of two such that its products 2^(s - m) * V scale * kLift have reached 2^8
 // and stay below 2^15: pieces below f16's smallest step, 2^-24, are then 2^-32 of the largest product. It is
 // raised (a rescaling of the outputs, which some column of a tile would nearly always ask for) only where a
@@ -497,22 +497,22 @@ __device__ __forceinline__ Quant4 quantize_block(float4 f, uint32_t sb, uint32_t
 }
 
 // The item's queries (columns behind the last repeat it) into LDS.
-template <int HD, int COLS>
+template <int WAVES, int HD, int COLS>
 __device__ __forceinline__ void quantize_queries(const ColumnArgs &A, const Item &I, Queries<HD, COLS> &Q) {
-    constexpr int NB = HD / 64, kTurns = (COLS * NB + 4 * kWaves - 1) / (4 * kWaves);
+    constexpr int NB = HD / 64, kTurns = (COLS * NB + 4 * WAVES - 1) / (4 * WAVES);
     const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const float *q0 = A.q + (size_t)I.row0 * A.q_stride + (size_t)I.head0 * HD;
     float4 f[kTurns];  // every load in flight at once
 #pragma unroll
     for (int k = 0; k < kTurns; k++) {
-        const int u = 4 * (wave + kWaves * k) + (int)lg, c = I.col0 + min(u / NB, I.n - 1);
+        const int u = 4 * (wave + WAVES * k) + (int)lg, c = I.col0 + min(u / NB, I.n - 1);
         const Column at = column(A, c);
         f[k] = *reinterpret_cast<const float4 *>(q0 + ((uint64_t)at.row * A.q_stride + at.head * HD + 64 * (u % NB) + 4 * li));
     }
 #pragma unroll
     for (int k = 0; k < kTurns; k++) {
-        const int u = 4 * (wave + kWaves * k) + (int)lg, x = u / NB, b = u % NB;
+        const int u = 4 * (wave + WAVES * k) + (int)lg, x = u / NB, b = u % NB;
         const Quant4 r = quantize_block<NB>(f[k], head_signs4<NB>(b, li), li, A.attn_scale);
         if (x >= COLS) continue;
         *reinterpret_cast<uint32_t *>(&Q.q[x][64 * b + 4 * li]) = r.w;
@@ -547,14 +547,14 @@ __device__ __forceinline__ void above_zero(float &qas, v4i (&qb)[NB]) {
 
 // The waves' results, added in wave order, 16 columns at a time: a part for the merge, or (WHOLE) the
 // output itself.
-template <int HD>
+template <int HD, int WAVES>
 struct Join {
-    float m[kWaves][16], l[kWaves][16];
-    __align__(16) float o[kWaves][16][HD + 4];
+    float m[WAVES][16], l[WAVES][16];
+    __align__(16) float o[WAVES][16][HD + 4];
 };
 // any(c): column c has a position at all (else its output is zeros).
-template <int HD, int BITS, int NQ, bool WHOLE, int SN, typename Any>
-__device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const State<HD, NQ, SN> &S, const Any &any, Join<HD> &J) {
+template <int HD, int BITS, int NQ, bool WHOLE, int SN, int WAVES, typename Any>
+__device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const State<HD, NQ, SN> &S, const Any &any, Join<HD, WAVES> &J) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
 #pragma unroll
@@ -572,13 +572,14 @@ __device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const S
 #pragma unroll
             for (int i = 0; i < 4; i++) J.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * S.back(a, b);
         __syncthreads();
-        const int x = (int)(tid >> 4), sl = (int)(tid & 15u);  // column, sixteenth of its dimensions
-        if (16 * a + x < I.n) {
-            float M = -FLT_MAX, L = 0.0f, e[kWaves];
+        // column, sixteenth of a 64-block's dimensions, and the first such block (four waves take one at a time)
+        const int x = (int)(tid >> 4 & 15u), sl = (int)(tid & 15u), d0 = 64 * (wave >> 2);
+        if (16 * a + x < I.n && d0 < HD) {
+            float M = -FLT_MAX, L = 0.0f, e[WAVES];
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) M = fmaxf(M, J.m[w][x]);
+            for (int w = 0; w < WAVES; w++) M = fmaxf(M, J.m[w][x]);
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) {
+            for (int w = 0; w < WAVES; w++) {
                 e[w] = __builtin_amdgcn_exp2f(J.m[w][x] - M);
                 L = fmaf(J.l[w][x], e[w], L);
             }
@@ -587,10 +588,10 @@ __device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const S
             const size_t pair = (size_t)(I.row0 + to.row) * A.nq + I.head0 + to.head;
             const size_t at = WHOLE ? pair : pair * A.parts + I.part;
 #pragma unroll
-            for (int d = 0; d < HD; d += 64) {
+            for (int d = d0; d < HD; d += 16 * WAVES) {
                 float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int w = 0; w < kWaves; w++) {
+                for (int w = 0; w < WAVES; w++) {
                     const float4 v = *reinterpret_cast<const float4 *>(&J.o[w][x][d + 4 * sl]);
                     r.x = fmaf(v.x, e[w], r.x);
                     r.y = fmaf(v.y, e[w], r.y);
@@ -609,23 +610,23 @@ __device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const S
                 }
                 *reinterpret_cast<float4 *>((WHOLE ? A.out : A.part) + at * HD + d + 4 * sl) = r;
             }
-            if (!WHOLE && sl == 0) A.stat[at] = make_float2(M, L);
+            if (!WHOLE && sl == 0 && d0 == 0) A.stat[at] = make_float2(M, L);
         }
         __syncthreads();
     }
 }
 
-// An item's columns (16 NQ at most): each wave takes every fourth tile of 32 positions.  The next tile's K is
+// An item's columns (16 NQ at most): each wave takes every WAVES-th tile of 32 positions.  The next tile's K is
 // loaded as soon as this one's scores are taken, the next V once this one's products are under way.
-template <int HD, int NQ>
+template <int HD, int NQ, int WAVES = kWaves>
 struct Shared {
     Queries<HD, 16 * NQ> q;
-    Join<HD> j;
+    Join<HD, WAVES> j;
 };
 // hide(i, t, vs): takes out of tile i what a column does not see (Hidden); NoMask: columns see all positions of the item.
 struct NoMask {};
-template <int HD, int BITS, int NQ, bool WHOLE, typename Hide, typename Any>
-__device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const Hide &hide, const Any &any, Shared<HD, NQ> &sh) {
+template <int HD, int BITS, int NQ, bool WHOLE, int WAVES, typename Hide, typename Any>
+__device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const Hide &hide, const Any &any, Shared<HD, NQ, WAVES> &sh) {
     constexpr int NB = HD / 64, DB = HD / 16, SN = TileK<HD, BITS>::SN;
     const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -658,7 +659,7 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
     };
     next_k(wave);
     next_v(wave);
-    quantize_queries(A, I, sh.q);
+    quantize_queries<WAVES>(A, I, sh.q);
     v4i qb[NQ][NB];
     float qas[NQ];
 #pragma unroll
@@ -669,7 +670,7 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
     }
     State<HD, NQ, SN> S;
     S.clear();
-    for (int i = wave; i < tiles; i += kWaves) {
+    for (int i = wave; i < tiles; i += WAVES) {
         const int left = i < first ? I.len[0] - kTile * i : I.len[1] - kTile * (i - first);
         float s[NQ][2][4], vs[2][4][SN];
         v4i kf[2][NB];
@@ -690,7 +691,7 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
                 for (int n = 0; n < SN; n++) vs[j][i][n] = K.scale(K.vs[j][i], n);
         // (behind the last use, so that the same registers take the load: a copy of them would wait for it)
         __builtin_amdgcn_sched_barrier(0);
-        next_k(i + kWaves);
+        next_k(i + WAVES);
         uint32_t ph[NQ][SN][4], pl[NQ][SN][4];
         if constexpr (std::is_same<Hide, NoMask>::value) {
             weights<HD, NQ, SN>(S, s, qas, vs, left, lg, ph, pl);
@@ -708,7 +709,7 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
                          v_word<BITS>(V.v[j][3][g], cb), h[j]);
             if (g + 1 == DB / 4) {
                 __builtin_amdgcn_sched_barrier(0);
-                next_v(i + kWaves);
+                next_v(i + WAVES);
             }
             // the small pieces of all four tiles, then the large ones: no product waits for the one before
             constexpr int kBlocks = SN - 1;  // (NF4 blocks have weights of their own)

@@ -8,10 +8,10 @@
 // (k2t_attn_tile.h); column c is head c % group of token c / group.
 //
 // Few columns (short drafts, single tokens): the waves of a workgroup share 16 or 32 columns and take tiles of 32
-// positions in turn, K and V from memory to registers (tokens_few_kernel).  Many: the waves have 16 or 32 columns each, and
+// positions in turn, K and V from memory to registers (tokens_few_kernel).  Many: eight waves have 16 columns each, and
 // a tile of positions is brought to LDS once for all of them, V as the f16 operand itself, so that its conversion is shared
-// too (tokens_block_kernel).  Where that gives fewer than two workgroups per CU, positions are cut into parts, which a
-// second kernel joins.
+// too (tokens_block_kernel).  Where that leaves CUs without a workgroup (tokens_block_kernel: without a second one),
+// positions are cut into parts, which a second kernel joins.
 #include <float.h>
 #include <math.h>
 
@@ -100,9 +100,9 @@ struct Seen {
 };
 
 // Few columns: an item is (row, KV head, part, 16 NQ columns).
-template <int HD, int BITS, int NQ, bool WHOLE>
-__global__ __launch_bounds__(64 * kWaves, 2) void tokens_few_kernel(const TokensArgs A) {
-    __shared__ Shared<HD, NQ> sh;
+template <int HD, int BITS, int NQ, bool WHOLE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void tokens_few_kernel(const TokensArgs A) {
+    __shared__ Shared<HD, NQ, WAVES> sh;
     const uint32_t lane = threadIdx.x & 63u;
     const int unit = (int)blockIdx.x % A.units, cg = A.cgs - 1 - (int)blockIdx.x / A.units;
     const int rh = unit / A.parts, head = rh % A.nkv, row = rh / A.nkv;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tokens_few_kernel(const Tokens
     I.head0 = head * A.group;
     if (I.len[0] <= 0) {
         if constexpr (WHOLE) {  // nothing to see
-            for (int i = (int)threadIdx.x; i < I.n * HD; i += 64 * kWaves) {
+            for (int i = (int)threadIdx.x; i < I.n * HD; i += 64 * WAVES) {
                 const Column c = column(A, I.col0 + i / HD);
                 A.out[((size_t)(I.row0 + c.row) * A.nq + I.head0 + c.head) * HD + i % HD] = 0.0f;
             }
@@ -431,34 +431,32 @@ struct TokensShape {
     int batch, ntok, nq, nkv, hd;
 };
 
-// How the work is cut.  block: tokens_block_kernel; else tokens_few_kernel, nq column tiles per workgroup.
+// How the work is cut.  block: tokens_block_kernel; else tokens_few_kernel, nq column tiles per workgroup of `waves`.
 struct Plan {
     bool block;
-    int nq, cgs, parts, plen;
+    int nq, waves, cgs, parts, plen;
     int item() const { return 16 * (block ? kBlockWaves : nq); }
 };
 // Items of one tile of columns (16) up to so much work: more workgroups, and a shorter way through each.  Measured on both
 // sides (us, one tile and two): 300 tokens, 32 heads x 64: 2.8 rounds, 7.0 and 8.5; 8 x 13 tokens behind 2100, 32 / 8 x 128: 16.5
-// rounds, 20.0 and 25.2; 777 tokens, 32 heads x 64: 18 rounds, 17.9 and 15.8; 64 tokens behind 12000, 32 / 4 x 128: 47 rounds, 51.5 and
-// 37.0.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.5 and 42.7 with it;
+// rounds, 20.1 and 23.0; 777 tokens, 32 heads x 64: 18 rounds, 17.9 and 15.8; 64 tokens behind 12000, 32 / 4 x 128: 47 rounds, 51.7 and
+// 37.3.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.5 and 42.7 with it;
 // 2048, two: 83.6 and 78.5; 8192, eight: 923 and 770), and for NF4 heads of two blocks, whose lookups it shares, from more than one
 // for four CUs on (4 x 64 tokens behind 2100, 32 / 8 x 128, one for four: 40.5 and 46.1; 300 tokens, five for sixteen: 59.2 and 56.2;
 // 515 behind 4100, one for two: 133 and 126).
 constexpr double kLittleWork = 17.0;
 constexpr int kLeastPart = 256;
 
-// The most parts that a call of so many items per part is cut into: two workgroups for every CU.
-int most_parts(const k2t_ctx *ctx, size_t items, int len) {
-    const size_t want = 2 * (size_t)std::max(1, ctx->num_cus) / std::max<size_t>(1, items);
+// The most parts that a call of so many items per part is cut into: a workgroup for every CU, two of tokens_block_kernel.
+int most_parts(const k2t_ctx *ctx, bool block, size_t items, int len) {
+    const size_t want = (block ? 2 : 1) * (size_t)std::max(1, ctx->num_cus) / std::max<size_t>(1, items);
     return (int)std::max<size_t>(1, std::min<size_t>(want, (len + kLeastPart - 1) / kLeastPart));
 }
 // What a call cut into n parts of `each` positions costs, in microseconds: rounds of items on the card, the transforms at
 // an item's ends, and the joining (3 us and its bytes).
 double plan_cost(const TokensShape &s, const Plan &P, int bits, size_t cus, size_t items, int n, int each) {
-    const double position = (P.block ? 0.025 : 0.008) * (s.hd / 128.0) * (bits == 4 ? 1.4 : 1.0), ends = 5.0;
-    // (two items of two tiles on a CU hide some of each other's waits: 64 tokens behind 20000, 32 heads x 64, one on a CU and
-    // two: 50.4 and 39.4 us; 2 x 40 behind 6100, 32 / 8 x 128: 31.6 and 29.4)
-    const double rounds = (double)((items + cus - 1) / cus) * (!P.block && P.nq == 2 && items > cus ? 0.8 : 1.0);
+    const double position = (P.block ? 0.025 : P.nq == 2 ? 0.0095 : 0.007) * (s.hd / 128.0) * (bits == 4 ? 1.4 : 1.0), ends = 5.0;
+    const double rounds = (double)((items + cus - 1) / cus);
     const double join = n == 1 ? 0.0 : 3.0 + (double)s.batch * s.ntok * s.nq * n * s.hd * 1.5e-6;
     return rounds * each * position + (items > 2 * cus ? rounds / 2 : 1) * ends + join;
 }
@@ -474,7 +472,11 @@ Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int 
     P.nq = work <= kLittleWork ? 1 : 2;
     P.cgs = (cols + P.item() - 1) / P.item();
     const size_t each_part = items(P.item());
-    const int most = most_parts(ctx, each_part, len);
+    const int most = most_parts(ctx, P.block, each_part, len);
+    // tokens_few_kernel: eight waves where a CU has one workgroup at most, and there is more than a tile for each of four
+    // (8 x 13 tokens behind 2100, 32 / 8 x 128 NF4, one workgroup on a CU: 26.0 us and 31.4 with four waves; 64 tokens behind
+    // 2000, 32 heads x 64, one on two: 13.1 and 17.8, 14.2 in parts; 300 tokens, 32 heads x 64, two on a CU: 13.2 and 7.1).
+    P.waves = P.block ? kBlockWaves : each_part <= cus && len > 4 * kTile ? 8 : 4;
     P.parts = 1;
     P.plen = std::max(len, 1);
     double least = plan_cost(s, P, bits, cus, each_part, 1, len);
@@ -500,7 +502,7 @@ size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
     size_t most = 16;
     for (int item : {16, 32, 16 * kBlockWaves}) {
         for (int cgs = 1; (cgs - 1) * item < cols; cgs++) {
-            const int parts = most_parts(ctx, heads * cgs, len);
+            const int parts = most_parts(ctx, item == 16 * kBlockWaves, heads * cgs, len);
             if (parts <= 1) break;
             most = std::max(most, heads * std::min(cols, cgs * item) * parts * slot_bytes(s.hd));
         }
@@ -510,12 +512,14 @@ size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
 
 template <int HD, int BITS>
 void launch_parts(hipStream_t st, const TokensArgs &A, const Plan &P) {
-    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * (P.block ? kBlockWaves : kWaves));
+    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * P.waves);
     if (P.block) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS>), grid, block, 0, st, A);
-    else if (P.nq == 2 && P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, true>), grid, block, 0, st, A);
-    else if (P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, false>), grid, block, 0, st, A);
-    else if (P.parts == 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, true>), grid, block, 0, st, A);
-    else hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, false>), grid, block, 0, st, A);
+    else if (P.parts > 1 && P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, false, 8>), grid, block, 0, st, A);
+    else if (P.parts > 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, false, 8>), grid, block, 0, st, A);
+    else if (P.waves == 8 && P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, true, 8>), grid, block, 0, st, A);
+    else if (P.waves == 8) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, true, 8>), grid, block, 0, st, A);
+    else if (P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, true, 4>), grid, block, 0, st, A);
+    else hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, true, 4>), grid, block, 0, st, A);
     hip_check(hipGetLastError(), "attn_tokens launch");
 }
 
