@@ -735,10 +735,10 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
 // One (head, row) per WAVES waves: its parts' maxima and sums one per lane, then the outputs of every
 // WAVES-th part, eight or sixteen loads in flight, joined in wave order, and ifwht64.  Parts that hold no
 // positions (not live_part) were not written and count nothing; any: there is one that does.
-template <int HD, int WAVES, typename LivePart>
+template <int HD, int WAVES, int AHEAD = (WAVES > 1 ? 8 : 16), typename LivePart>
 __device__ __forceinline__ void merge_parts(const ColumnArgs &A, int pair, const LivePart &live_part, bool any,
                                             float (*sum)[HD]) {
-    constexpr int E = HD / 64, kAhead = WAVES > 1 ? 8 : 16;  // values per lane; loads in flight
+    constexpr int E = HD / 64, kAhead = AHEAD;  // values per lane; loads in flight
     const uint32_t lane = threadIdx.x & 63u;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int w0 = WAVES == 1 ? 0 : wave, n = A.parts;

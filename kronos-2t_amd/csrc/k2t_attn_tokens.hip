@@ -410,7 +410,7 @@ __global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const
 }
 
 // Joins the parts of every token that its row has (merge_parts).  item: columns of a workgroup that wrote them.
-template <int HD, int WAVES>
+template <int HD, int WAVES, int AHEAD>
 __global__ __launch_bounds__(256) void tokens_merge_kernel(const TokensArgs A, int pairs, int item) {
     __shared__ float sum[WAVES > 1 ? WAVES : 1][HD];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void tokens_merge_kernel(const TokensArgs A, i
     const int c = t * A.group + pair % A.nq % A.group, last = min(c / item * item + item, R.count * A.group) - 1;
     const bool any = s.limit > 0 || s.bits != 0;  // (else parts may hold the NaN of a query without positions)
     const int live = any ? (reach(A, R, last / A.group) + A.plen - 1) / A.plen : 0;
-    merge_parts<HD, WAVES>(A, pair, [=](int i) { return i < live; }, any, sum);
+    merge_parts<HD, WAVES, AHEAD>(A, pair, [=](int i) { return i < live; }, any, sum);
 }
 
 struct TokensShape {
@@ -529,8 +529,9 @@ void launch_tokens(hipStream_t st, int bits, const TokensArgs &A, const TokensSh
     else launch_parts<HD, 4>(st, A, P);
     if (P.parts == 1) return;
     const int pairs = s.batch * s.ntok * s.nq;
-    if (P.parts > 16) hipLaunchKernelGGL((tokens_merge_kernel<HD, 4>), dim3(pairs), dim3(256), 0, st, A, pairs, P.item());
-    else hipLaunchKernelGGL((tokens_merge_kernel<HD, 1>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
+    if (P.parts > 16) hipLaunchKernelGGL((tokens_merge_kernel<HD, 4, 8>), dim3(pairs), dim3(256), 0, st, A, pairs, P.item());
+    else if (P.parts > 4) hipLaunchKernelGGL((tokens_merge_kernel<HD, 1, 16>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
+    else hipLaunchKernelGGL((tokens_merge_kernel<HD, 1, 4>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
     hip_check(hipGetLastError(), "attn_tokens merge launch");
 }
 
