@@ -31,8 +31,9 @@ struct TokensArgs : ColumnArgs {
     const int *pos, *counts;
     const uint64_t *sees;
     k2t_kv_rows kv;
-    int plen;        // positions of a part
-    int cgs, units;  // column groups of a row; (row, KV head, part)
+    int plen;          // positions of a part; of a tile of tokens_block_kernel's
+    int cgs, units;    // column groups of a row; (row, KV head, part), of tokens_block_kernel (row, KV head)
+    int tiles, chunk;  // tokens_block_kernel: tiles of an item's positions, and of a workgroup's (0: uncut)
 };
 
 // A row of the call: how many tokens it has, the position of its first, and how many positions its last one sees.
@@ -165,6 +166,7 @@ struct BlockLoad {
     using T = BlockTile<HD, BITS>;
     static constexpr int RB = BITS == 8 ? HD : HD / 2, PC = HD / 16, KP = RB / PC;
     uint32_t k[KP / 4], v[4], scale;
+    uint32_t tid;
 
     // Portion of V: subtile, tile group, half.
     static __device__ __forceinline__ void portion(int wave, int &s, int &g, int &j) {
@@ -175,7 +177,7 @@ struct BlockLoad {
     // Positions p0 .. of a row's and head's slots from `base` on.  Past the cache's end the last of them, cap - 1, is repeated;
     // up to there, what lies behind the row's positions is loaded and hidden with all that a column does not see.
     __device__ __forceinline__ void load(const k2t_kv_rows &kv, size_t base, int p0) {
-        const uint32_t tid = threadIdx.x, li = tid & 15u, lg = tid >> 4 & 3u;
+        const uint32_t li = tid & 15u, lg = tid >> 4 & 3u;
         const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
         p0 = min(p0, kv.cap - 1);
         const uint8_t *kq = (const uint8_t *)kv.kq + (base + p0) * RB, *vq = (const uint8_t *)kv.vq + (base + p0) * RB;
@@ -216,7 +218,7 @@ struct BlockLoad {
         }
     }
     __device__ __forceinline__ void store(T &tile, const Nf4 &cb) const {
-        const int tid = (int)threadIdx.x, lane = tid & 63;
+        const int tid = (int)this->tid, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         *reinterpret_cast<v4i *>(tile.k + T::k_at(tid / PC, tid % PC)) = k_operand<BITS>(k, cb);
         uint32_t h[4][2];
@@ -243,22 +245,23 @@ struct BlockShared {
     __device__ BlockShared() {}
 };
 
-// An item is (row, KV head, part, 16 columns for each of eight waves).
+// The workgroup that has an item's first tile, where items are cut.
+__device__ __forceinline__ int first_chunk(const TokensArgs &A, int item) { return item * A.tiles / A.chunk; }
+
+// Positions t0 .. t1 - 1 of an item: (row, KV head, 16 columns for each of eight waves).
 template <int HD, int BITS>
-__global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const TokensArgs A) {
+__device__ __forceinline__ void block_item(const TokensArgs &A, int item, int part, int t0, int t1, uint32_t tid, BlockShared<HD, BITS> &sh) {
     using T = BlockTile<HD, BITS>;
     constexpr int NB = HD / 64, DB = HD / 16, SN = T::SN, NQ = 1, W = 16;
-    __shared__ BlockShared<HD, BITS> sh;
-    const uint32_t lane = threadIdx.x & 63u, li = lane & 15u, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t lane = tid & 63u, li = lane & 15u, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(tid >> 6));
     // (the last columns first: theirs are the longest items of a prompt)
-    const int unit = (int)blockIdx.x % A.units, cg = A.cgs - 1 - (int)blockIdx.x / A.units;
-    const int rh = unit / A.parts, head = rh % A.nkv, row = rh / A.nkv, part = unit % A.parts;
+    const int rh = item % A.units, cg = A.cgs - 1 - item / A.units;
+    const int head = rh % A.nkv, row = rh / A.nkv;
     const Row R = row_of(A, row);
     const int col0 = W * kBlockWaves * cg, cols = R.count * A.group, n_all = min(W * kBlockWaves, cols - col0);
     if (n_all <= 0) return;
-    const int t0 = part * A.plen;
-    const int end = min(reach(A, R, (int)column(A, col0 + n_all - 1).row), t0 + A.plen);  // of the item's positions
+    const int end = min(reach(A, R, (int)column(A, col0 + n_all - 1).row), t1);
     const bool none = end <= t0;
     if (none && A.parts > 1) return;
     // this wave's columns; a wave without any repeats the last one and writes nothing
@@ -268,6 +271,7 @@ __global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const
     Nf4 cb{};
     if constexpr (BITS == 4) nf4_xor_tables(kNf4Cb0, kNf4Cb1, kNf4Cb2, kNf4Cb3, cb.t0, cb.t1, cb.u0, cb.u1);
     BlockLoad<HD, BITS> next;
+    next.tid = tid;
     if (!none) next.load(A.kv, base, t0);
     // queries: four 64-blocks of columns at a time
     constexpr int kTurns = W * NB / 4, kBatch = kTurns < 8 ? kTurns : 8;
@@ -409,6 +413,33 @@ __global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const
     }
 }
 
+// CUT: workgroups take `chunk` tiles each of all items' positions one after another, from wherever an item has got to, so
+// that a few long items fill the card evenly (515 tokens behind 4100, 32 / 8 heads x 128 NF4, 136 items for 512 workgroups:
+// 119.5 us, 130 in three equal parts of every item); an item has a part for every workgroup that comes to it.  Else a
+// workgroup has an item.
+template <int HD, int BITS, bool CUT>
+__global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const TokensArgs A) {
+    constexpr int P = BlockTile<HD, BITS>::P;
+    __shared__ BlockShared<HD, BITS> sh;
+    if constexpr (!CUT) {
+        block_item<HD, BITS>(A, (int)blockIdx.x, 0, 0, A.kv.len, threadIdx.x, sh);
+        return;
+    }
+    int item = (int)blockIdx.x * A.chunk / A.tiles, first = (int)blockIdx.x * A.chunk - item * A.tiles;
+    int left = min(A.chunk, A.units * A.cgs * A.tiles - (int)blockIdx.x * A.chunk);
+#pragma unroll 1
+    do {
+        const int n = min(A.tiles - first, left);
+        // (as if not known before: lanes' offsets kept from item to item would not fit the registers)
+        uint32_t tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        block_item<HD, BITS>(A, item, (int)blockIdx.x - first_chunk(A, item), P * first, P * (first + n), tid, sh);
+        item++;
+        first = 0;
+        left -= n;
+    } while (left > 0);
+}
+
 // Joins the parts of every token that its row has (merge_parts).  item: columns of a workgroup that wrote them.
 template <int HD, int WAVES, int AHEAD>
 __global__ __launch_bounds__(256) void tokens_merge_kernel(const TokensArgs A, int pairs, int item) {
@@ -423,7 +454,12 @@ __global__ __launch_bounds__(256) void tokens_merge_kernel(const TokensArgs A, i
     // an item wrote the parts that its last column reaches
     const int c = t * A.group + pair % A.nq % A.group, last = min(c / item * item + item, R.count * A.group) - 1;
     const bool any = s.limit > 0 || s.bits != 0;  // (else parts may hold the NaN of a query without positions)
-    const int live = any ? (reach(A, R, last / A.group) + A.plen - 1) / A.plen : 0;
+    const int end = any ? reach(A, R, last / A.group) : 0;
+    int live = (end + A.plen - 1) / A.plen;
+    if (A.chunk && end > 0) {
+        const int at = (A.cgs - 1 - c / item) * A.units + row * A.nkv + pair % A.nq / A.group;
+        live = (at * A.tiles + (end - 1) / A.plen) / A.chunk - first_chunk(A, at) + 1;
+    }
     merge_parts<HD, WAVES, AHEAD>(A, pair, [=](int i) { return i < live; }, any, sum);
 }
 
@@ -434,31 +470,36 @@ struct TokensShape {
 // How the work is cut.  block: tokens_block_kernel; else tokens_few_kernel, nq column tiles per workgroup of `waves`.
 struct Plan {
     bool block;
-    int nq, waves, cgs, parts, plen;
+    int nq, waves, cgs, parts, plen;  // plen: see TokensArgs
+    int tiles, chunk;                 // (tokens_block_kernel)
     int item() const { return 16 * (block ? kBlockWaves : nq); }
 };
 // Items of one tile of columns (16) up to so much work: more workgroups, and a shorter way through each.  Measured on both
 // sides (us, one tile and two): 300 tokens, 32 heads x 64: 2.8 rounds, 7.0 and 8.5; 8 x 13 tokens behind 2100, 32 / 8 x 128: 16.5
 // rounds, 20.1 and 23.0; 777 tokens, 32 heads x 64: 18 rounds, 17.9 and 15.8; 64 tokens behind 12000, 32 / 4 x 128: 47 rounds, 51.7 and
-// 37.3.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.5 and 42.7 with it;
-// 2048, two: 83.6 and 78.5; 8192, eight: 923 and 770), and for NF4 heads of two blocks, whose lookups it shares, from more than one
-// for four CUs on (4 x 64 tokens behind 2100, 32 / 8 x 128, one for four: 40.5 and 46.1; 300 tokens, five for sixteen: 59.2 and 56.2;
-// 515 behind 4100, one for two: 133 and 126).
+// 37.3.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.0 and 42.2 with it;
+// 2048, two: 83.9 and 80.0; 8192, eight: 923 and 770).  For NF4, whose lookups it shares, also behind long contexts (512 tokens,
+// 32 / 8 x 128, behind 0, 2100, 4100 and 16000 positions: 22, 68, 107 and 357, and 33, 80, 108 and 287 with it; int8 behind 4100
+// and 16000: 72 and 234, 90 and 233; 515 tokens, NF4, behind 4100: 152 and 120), if there is one for eight CUs (64 tokens behind
+// 12000, 32 / 4 x 128, one for 16: 47 and 60).
 constexpr double kLittleWork = 17.0;
-constexpr int kLeastPart = 256;
+constexpr int kLeastPart = 256, kLongContext = 4000;
 
-// The most parts that a call of so many items per part is cut into: a workgroup for every CU, two of tokens_block_kernel.
+// The most parts that an item is cut into where a call has so many: a workgroup for every CU; two of tokens_block_kernel,
+// and a part more where an item begins and ends within other items' workgroups.
 int most_parts(const k2t_ctx *ctx, bool block, size_t items, int len) {
-    const size_t want = (block ? 2 : 1) * (size_t)std::max(1, ctx->num_cus) / std::max<size_t>(1, items);
-    return (int)std::max<size_t>(1, std::min<size_t>(want, (len + kLeastPart - 1) / kLeastPart));
+    const size_t slots = (block ? 2 : 1) * (size_t)std::max(1, ctx->num_cus), longest = ((size_t)len + kLeastPart - 1) / kLeastPart;
+    if (!block) return (int)std::max<size_t>(1, std::min(slots / std::max<size_t>(1, items), longest));
+    return items >= slots || longest <= 1 ? 1 : (int)std::min((slots + items - 1) / items, longest) + 1;
 }
 // What a call cut into n parts of `each` positions costs, in microseconds: rounds of items on the card, the transforms at
 // an item's ends, and the joining (3 us and its bytes).
 double plan_cost(const TokensShape &s, const Plan &P, int bits, size_t cus, size_t items, int n, int each) {
     const double position = (P.block ? 0.025 : P.nq == 2 ? 0.0095 : 0.007) * (s.hd / 128.0) * (bits == 4 ? 1.4 : 1.0), ends = 5.0;
-    const double rounds = (double)((items + cus - 1) / cus);
+    // (a workgroup of tokens_block_kernel by itself waits at its barriers)
+    const double rounds = (double)((items + cus - 1) / cus) * (P.block && items <= cus ? 1.15 : 1.0);
     const double join = n == 1 ? 0.0 : 3.0 + (double)s.batch * s.ntok * s.nq * n * s.hd * 1.5e-6;
-    return rounds * each * position + (items > 2 * cus ? rounds / 2 : 1) * ends + join;
+    return rounds * each * position + (items > 2 * cus || (P.block && n > 1) ? std::max(rounds / 2, 2.0) : 1) * ends + join;
 }
 Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int len) {
     const int cols = s.ntok * (s.nq / s.nkv);
@@ -466,9 +507,10 @@ Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int 
     Plan P{};
     const auto items = [&](int item) { return std::max<size_t>(1, heads * ((cols + item - 1) / item)); };
     // rounds of 128 positions that items of one tile of columns make on a CU
-    const double work = (double)items(16) * (tree ? len : std::max(len - s.ntok / 2, 1)) / 128 / cus;
+    const int mean = tree ? len : std::max(len - s.ntok / 2, 1);
+    const double work = (double)items(16) * mean / 128 / cus;
     const size_t blocks = items(16 * kBlockWaves);
-    P.block = bits == 4 && s.hd == 128 ? 4 * blocks > cus : 2 * blocks >= 3 * cus;
+    P.block = 2 * blocks >= 3 * cus || (bits == 4 && mean >= kLongContext && 8 * blocks >= cus);
     P.nq = work <= kLittleWork ? 1 : 2;
     P.cgs = (cols + P.item() - 1) / P.item();
     const size_t each_part = items(P.item());
@@ -479,6 +521,19 @@ Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int 
     P.waves = P.block ? kBlockWaves : each_part <= cus && len > 4 * kTile ? 8 : 4;
     P.parts = 1;
     P.plen = std::max(len, 1);
+    if (P.block) {
+        P.plen = 8192 / s.hd;
+        P.tiles = std::max(1, (len + P.plen - 1) / P.plen);
+        if (most == 1) return P;
+        const size_t slots = 2 * cus, total = each_part * P.tiles;
+        const int chunk = (int)std::max((total + slots - 1) / slots, (size_t)kLeastPart / P.plen);
+        const int parts = (P.tiles + chunk - 2) / chunk + 1;
+        if (parts > 1 && plan_cost(s, P, bits, cus, (total + chunk - 1) / chunk, parts, chunk * P.plen) < plan_cost(s, P, bits, cus, each_part, 1, len)) {
+            P.parts = parts;
+            P.chunk = chunk;
+        }
+        return P;
+    }
     double least = plan_cost(s, P, bits, cus, each_part, 1, len);
     for (int n = 2; n <= most; n++) {
         const int each = ((len + n - 1) / n + 127) / 128 * 128;
@@ -512,8 +567,10 @@ size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
 
 template <int HD, int BITS>
 void launch_parts(hipStream_t st, const TokensArgs &A, const Plan &P) {
-    const dim3 grid((unsigned)((size_t)A.units * A.cgs)), block(64 * P.waves);
-    if (P.block) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS>), grid, block, 0, st, A);
+    const size_t items = (size_t)A.units * A.cgs;
+    const dim3 grid((unsigned)(A.chunk ? (items * A.tiles + A.chunk - 1) / A.chunk : items)), block(64 * P.waves);
+    if (P.block && P.parts > 1) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, true>), grid, block, 0, st, A);
+    else if (P.block) hipLaunchKernelGGL((tokens_block_kernel<HD, BITS, false>), grid, block, 0, st, A);
     else if (P.parts > 1 && P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, false, 8>), grid, block, 0, st, A);
     else if (P.parts > 1) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 1, false, 8>), grid, block, 0, st, A);
     else if (P.waves == 8 && P.nq == 2) hipLaunchKernelGGL((tokens_few_kernel<HD, BITS, 2, true, 8>), grid, block, 0, st, A);
@@ -587,7 +644,7 @@ int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
             throw Error(K2T_E_ARG, "the workspace holds " + std::to_string(ws_bytes) + " bytes, " +
                                        std::to_string(need) + " are needed");
         // (with cgs at most as many as there are columns, or two workgroups for every CU: grids are within 2^23)
-        const size_t units = (size_t)batch * n_kv_heads * P.parts;
+        const size_t units = (size_t)batch * n_kv_heads * (P.block ? 1 : P.parts);
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
         TokensArgs A{};
         A.q = d_q;
@@ -609,6 +666,8 @@ int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
         A.plen = P.plen;
         A.cgs = P.cgs;
         A.units = (int)units;
+        A.tiles = P.tiles;
+        A.chunk = P.chunk;
         if (head_dim == 128) launch_tokens<128>(ctx->stream, bits, A, s, P);
         else launch_tokens<64>(ctx->stream, bits, A, s, P);
     });

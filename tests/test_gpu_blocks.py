@@ -316,6 +316,21 @@ def test_attention_of_many_columns_and_parts(gpu_ctx, bits, hd, nq, nkv, batch, 
     assert not np.isfinite(got[r][see & (np.arange(ntok) < counts[r])]).any(-1).all(-1).any()
 
 
+# items of many columns whose positions workgroups share, each from where the one before stops (few items for two on every CU)
+CUT = [(8, 64, 16, 16, 8, 380, 3100, 0, False), (8, 128, 8, 8, 7, 1000, 0, 9000, False), (4, 64, 8, 4, 3, 256, 4100, 0, False),
+       (4, 128, 8, 8, 4, 130, 4500, 300, False), (4, 128, 16, 4, 8, 40, 4500, 50, True), (4, 64, 20, 2, 3, 64, 900, 8000, True)]
+
+
+@pytest.mark.parametrize("bits,hd,nq,nkv,batch,ntok,start,room,with_tree", CUT)
+def test_attention_of_items_cut_between_workgroups(gpu_ctx, bits, hd, nq, nkv, batch, ntok, start, room, with_tree):
+    print(f"attn_tokens bits={bits} hd={hd} heads={nq}/{nkv} batch={batch} ntok={ntok} start={start} room={room} tree={with_tree}", flush=True)
+    rng = np.random.default_rng(hd * ntok + nq)
+    q, cache, pos, counts, sees, cap = case(rng, bits, batch, ntok, nq, nkv, hd, start, True, with_tree, spare=3 + room, first=max(0, start - 9))
+    counts[1:3] = [0, 1]
+    want, bound = attention_on_gpu(bits, q, cache, pos, counts, sees, nq, nkv, hd, 0.17, cap)
+    check(attend(gpu_ctx, bits, q, cache, pos, counts, sees, nq, nkv, hd, 0.17, cap), want, bound)
+
+
 @pytest.mark.parametrize("bits,hd,nq,nkv,batch,ntok,start,room,with_tree", [LARGE[i] for i in (0, 3, 5, 6, 7, 9)])
 @pytest.mark.parametrize("kind", ["large", "vscales", "zero", "far"])
 def test_attention_of_many_columns_and_values_of_any_size(gpu_ctx, bits, hd, nq, nkv, batch, ntok, start, room, with_tree, kind):
