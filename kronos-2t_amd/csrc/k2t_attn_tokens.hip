@@ -586,9 +586,11 @@ void launch_tokens(hipStream_t st, int bits, const TokensArgs &A, const TokensSh
     else launch_parts<HD, 4>(st, A, P);
     if (P.parts == 1) return;
     const int pairs = s.batch * s.ntok * s.nq;
+    // Loads ahead: as many as there are parts, or nearly (515 tokens, 32 heads x 128, three parts: 13.7 us with sixteen, 11.5 with
+    // four).  Four waves for a head's parts where there are many, and so few heads.
     if (P.parts > 16) hipLaunchKernelGGL((tokens_merge_kernel<HD, 4, 8>), dim3(pairs), dim3(256), 0, st, A, pairs, P.item());
-    else if (P.parts > 4) hipLaunchKernelGGL((tokens_merge_kernel<HD, 1, 16>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
-    else hipLaunchKernelGGL((tokens_merge_kernel<HD, 1, 4>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
+    else if (P.parts > 8) hipLaunchKernelGGL((tokens_merge_kernel<HD, 1, 16>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
+    else hipLaunchKernelGGL((tokens_merge_kernel<HD, 1, 8>), dim3((pairs + 3) / 4), dim3(256), 0, st, A, pairs, P.item());
     hip_check(hipGetLastError(), "attn_tokens merge launch");
 }
 
