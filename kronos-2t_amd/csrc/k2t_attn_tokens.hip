@@ -13,7 +13,7 @@
 // too (tokens_block_kernel).  Where that leaves CUs without a workgroup (tokens_block_kernel: without a second one),
 // positions are cut into parts, which a second kernel joins.
 //
-// What bounds it.  8192 tokens from the start, 32 / 4 heads x 128, int8: 780 to 820 us, 0.55 PFLOP that count at 0.7 PFLOP/s.  The
+// What bounds it.  8192 tokens from the start, 32 / 4 heads x 128, int8: 780 to 865 us by the card, 0.55 PFLOP that count at 0.7 PFLOP/s.  The
 // matrix cores and the power they draw (the core's clock is down at 2.0 GHz): outputs are done twice, for a weight's two
 // pieces, and all products would take 555 us at the rate of a large one (1.24 PFLOP/s f16, int8 twice that).  68 us are the
 // ends of items, queries and outputs (268 MB).  6 prompts of 389 to 777 tokens, 32 heads x 64: 39 us, the ends half of them.
