@@ -11,7 +11,10 @@ from test_branch_args import BAD_CACHE, CTX, HIP, P, call, refused, rows
 
 KINDS = {"plain": k2t.ROPE_PLAIN, "linear": k2t.ROPE_LINEAR, "base": k2t.ROPE_BASE, "ramp": k2t.ROPE_RAMP,
          "wave": k2t.ROPE_WAVE}
-NO_GPU = k2t.lib().k2t_device_count() == 0
+
+
+def no_gpu():
+    return k2t.lib().k2t_device_count() == 0
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
@@ -68,7 +71,7 @@ def test_rope():
                                {12: 128}, {12: 260}, {12: 258}, {3: 60000, 4: 60000}, {2: 1 << 40, 12: 1 << 40},
                                {10: at(plan(128))}, {10: at(plan(layout=2))}, {10: at(plan(rot_dim=0))}, {10: at(plan(rot_dim=7))},
                                {10: at(plan(scale=float("nan")))}, {10: at(plan(turns=1.5))}, {10: at(plan(turns=float("nan")))}])
-    if NO_GPU:
+    if no_gpu():
         assert call("k2t_rope", *good) == HIP
         for nothing in ({3: 0}, {4: 0}):
             args = list(good)
@@ -89,7 +92,7 @@ def test_attention():
                                       {11: P + 4}, {11: P, 5: 65}, {4: 60000, 5: 60000}] + [{12: c} for c in BAD_CACHE])
     refused("k2t_attn_tokens_workspace", [CTX, *shape, 8, C.byref(n)],
             [{0: None}, {1: -1}, {2: -1}, {3: 9}, {4: 0}, {5: 256}, {6: -1}, {6: (1 << 24) + 1}, {7: None}])
-    if NO_GPU:
+    if no_gpu():
         assert call("k2t_attn_tokens", *good) == HIP
         assert call("k2t_attn_tokens", CTX, 8, None, 512, 0, *shape[1:], None, None, None, rows(), 0.125, None, None, 0) == 0
 
@@ -144,7 +147,7 @@ def test_logits():
                                            dict(bias=None), dict(bias_tokens=None), dict(bias_stride=19), dict(bias_max=-1),
                                            dict(bias_max=4097, bias_stride=5000), dict(mask_stride=31), dict(mask_rows=-1),
                                            dict(mask_row=None, mask_rows=2), dict(mask=None))])
-    if NO_GPU:
+    if no_gpu():
         assert call("k2t_logits_adjust", *good) == HIP
         assert call("k2t_logits_adjust", CTX, None, 1000, 1000, 0, at(rules()), None, 1000) == 0
         assert call("k2t_logits_adjust", CTX, P, 1000, 1000, 3, at(rules(mask=None, mask_row=None)), P, 1000) == HIP
@@ -155,7 +158,7 @@ def test_keep():
     refused("k2t_kv_keep", good, [{0: None}, {1: 6}, {2: None}, {3: None}, {4: None}, {5: 4}, {5: 1 << 40}, {7: -1}, {7: (1 << 24) + 1, 5: 1 << 25},
                                   {8: -1}, {9: -1}, {9: 65536}, {10: 0}, {10: 1025}, {11: 32}, {8: 1 << 20, 9: 100},
                                   {8: 1 << 30, 9: 65535, 10: 1024}] + [{2: c} for c in BAD_CACHE])
-    if NO_GPU:
+    if no_gpu():
         assert call("k2t_kv_keep", *good) == HIP
         for nothing in (7, 8, 9):
             args = list(good)
