@@ -259,8 +259,8 @@ struct BlockShared {
 // The workgroup that has an item's first tile, where items are cut.
 __device__ __forceinline__ int first_chunk(const TokensArgs &A, int item) { return item * A.tiles / A.chunk; }
 
-// Positions t0 .. t1 - 1 of an item: (row, KV head, 16 columns for each of eight waves).
-template <int HD, int BITS>
+// Positions t0 .. t1 - 1 of an item: (row, KV head, 16 columns for each of eight waves).  CUT: a part of it, for the merge.
+template <int HD, int BITS, bool CUT>
 __device__ __forceinline__ void block_item(const TokensArgs &A, int item, int part, int t0, int t1, uint32_t tid, BlockShared<HD, BITS> &sh) {
     using T = BlockTile<HD, BITS>;
     constexpr int NB = HD / 64, DB = HD / 16, SN = T::SN, NQ = 1, W = 16;
@@ -274,7 +274,7 @@ __device__ __forceinline__ void block_item(const TokensArgs &A, int item, int pa
     if (n_all <= 0) return;
     const int end = min(reach(A, R, (int)column(A, col0 + n_all - 1).row), t1);
     const bool none = end <= t0;
-    if (none && A.parts > 1) return;
+    if (none && CUT) return;
     // this wave's columns; a wave without any repeats the last one and writes nothing
     const int c0 = min(col0 + W * wave, cols - 1), n = max(0, min(W, cols - col0 - W * wave)), c1 = min(c0 + W, cols) - 1;
     const size_t base = ((size_t)row * A.nkv + head) * (size_t)A.kv.cap;
@@ -397,19 +397,19 @@ __device__ __forceinline__ void block_item(const TokensArgs &A, int item, int pa
             const size_t pair = (size_t)(row * A.ntok + (int)to.row) * A.nq + head * A.group + to.head;
             const bool mine = 16 * a + x < n;
             bool any = true;
-            if (A.parts == 1) {
+            if constexpr (!CUT) {
                 const Sees s = sees_of(A, R, row, (int)to.row);
                 any = s.limit > 0 || s.bits != 0;
             } else if (mine && li == 0) {
                 A.stat[pair * A.parts + part] = make_float2(M, L);
             }
             const float inv = 1.0f / L;
-            float *out = A.parts == 1 ? A.out + pair * HD : A.part + (pair * A.parts + part) * HD;
+            float *out = CUT ? A.part + (pair * A.parts + part) * HD : A.out + pair * HD;
 #pragma unroll
             for (int d = 0; d < HD; d += 64) {
                 const float4 f = *reinterpret_cast<const float4 *>(&sh.o[wave][x][d + 4 * li]);
                 float v[4] = {f.x, f.y, f.z, f.w};
-                if (A.parts == 1) {
+                if constexpr (!CUT) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) v[e] = any ? v[e] * inv : 0.0f;
                     butterflies_slice4(v, li);
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const
     constexpr int P = BlockTile<HD, BITS>::P;
     __shared__ BlockShared<HD, BITS> sh;
     if constexpr (!CUT) {
-        block_item<HD, BITS>(A, (int)blockIdx.x, 0, 0, A.kv.len, threadIdx.x, sh);
+        block_item<HD, BITS, CUT>(A, (int)blockIdx.x, 0, 0, A.kv.len, threadIdx.x, sh);
         return;
     }
     int item = (int)blockIdx.x * A.chunk / A.tiles, first = (int)blockIdx.x * A.chunk - item * A.tiles;
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const
         // (as if not known before: lanes' offsets kept from item to item would not fit the registers)
         uint32_t tid = threadIdx.x;
         asm volatile("" : "+v"(tid));
-        block_item<HD, BITS>(A, item, (int)blockIdx.x - first_chunk(A, item), P * first, P * (first + n), tid, sh);
+        block_item<HD, BITS, CUT>(A, item, (int)blockIdx.x - first_chunk(A, item), P * first, P * (first + n), tid, sh);
         item++;
         first = 0;
         left -= n;
