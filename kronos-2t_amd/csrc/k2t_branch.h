@@ -38,7 +38,7 @@ void check_kv_rows(const k2t_kv_rows *kv, int bits, int hd);
 void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const int *parents, int n_layers, int n_seq,
                        int beams, int nkv, int hd);
 
-void launch_kv_keep(hipStream_t st, int bits, const k2t_kv_rows &kv, const int *pos, const int *keep, size_t keep_stride,
+void launch_kv_keep(int cus, hipStream_t st, int bits, const k2t_kv_rows &kv, const int *pos, const int *keep, size_t keep_stride,
                     const int *counts, int n_keep, int n_layers, int rows, int nkv, int hd);
 
 struct SharedShape {

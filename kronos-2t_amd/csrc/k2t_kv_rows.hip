@@ -315,10 +315,11 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs A) {
 // Positions of one (layer, row, KV head, K or V) moved together: position p0 + j from p0 + keep[j], keep[j] >= j.
 // Entries are taken in order, a chunk of them at a time: a chunk's sources are all read before its
 // positions are written, and those that earlier chunks have written lie before every later source.
-// What bounds it: bytes, as far as one chunk after another lets them. 24 layers, 32 heads x 64, 3000 of 4000 positions (627 MB
-// read and written): 117 to 138 us by where the buffers lie, 4.5 to 5.4 TB/s, which a large copy reaches too. 30 layers, 4 rows,
-// 4 of 10 positions: 3.6 us, a launch. Four pieces a thread: registers for one chunk's sources.
-constexpr int kKeepPieces = 4;  // pieces of a thread in flight
+// What bounds it: bytes. 24 layers, 32 heads x 64, 3000 of 4000 positions (627 MB read and written): 105 to 124 us by where
+// the buffers lie, 5 to 6 TB/s, partly from the Infinity Cache (143 with a chunk's stores before the next one's loads). Few
+// heads: the chain of chunks (17 layers, 3 rows, 2 heads x 128, 6027 positions, 325 MB: 54 us; 124 in chunks of 128 one
+// after another). 30 layers, 4 rows, 4 of 10 positions: 3.6 us, a launch.
+constexpr int kKeepPieces = 4;  // of a thread and chunk
 
 struct KeepArgs {
     k2t_kv_rows kv;
@@ -328,36 +329,54 @@ struct KeepArgs {
     int code_bytes, scale_bytes;  // per slot
 };
 
-// Entries a .. b - 1 of the list, at most kKeepPieces * 256 / PER of them, each a slot of PER pieces of type T.
-template <typename T, int PER>
-__device__ __forceinline__ void keep_chunk(T *base, const int *keep, long long p0, int cap, int a, int b) {
+// What a chunk moves: entries a .. of the list, kKeepPieces * THREADS / PER of them, each a slot of PER pieces of type T.
+template <typename T, int PER, int THREADS>
+struct KeepChunk {
+    static constexpr int kEntries = kKeepPieces * THREADS / PER;
     T v[kKeepPieces];
     long long to[kKeepPieces];
+
+    __device__ __forceinline__ void load(const T *base, const int *keep, long long p0, int cap, int a, int n) {
 #pragma unroll
-    for (int k = 0; k < kKeepPieces; k++) {
-        const int g = (int)threadIdx.x + 256 * k, j = a + g / PER;
-        to[k] = -1;
-        if (j >= b) continue;
-        const int from = keep[j];
-        const long long t = p0 + j, f = p0 + from;
-        if (from <= j || t < 0 || f >= cap) continue;  // (from == j: it is there already)
-        to[k] = t * PER + g % PER;
-        v[k] = base[f * PER + g % PER];
+        for (int k = 0; k < kKeepPieces; k++) {
+            const int g = (int)threadIdx.x + THREADS * k, j = a + g / PER;
+            to[k] = -1;
+            if (j >= n) continue;
+            const int from = keep[j];
+            const long long t = p0 + j, f = p0 + from;
+            if (from <= j || t < 0 || f >= cap) continue;  // (from == j: it is there already)
+            to[k] = t * PER + g % PER;
+            v[k] = base[f * PER + g % PER];
+        }
     }
-    // (the loads themselves, not only their issue, come before any wave's stores)
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#endif
-    __syncthreads();
+    __device__ __forceinline__ void store(T *base) const {
 #pragma unroll
-    for (int k = 0; k < kKeepPieces; k++)
-        if (to[k] >= 0) base[to[k]] = v[k];
-    __syncthreads();
+        for (int k = 0; k < kKeepPieces; k++)
+            if (to[k] >= 0) base[to[k]] = v[k];
+    }
+};
+
+// A chunk is written once every wave has read it, and while the next one is read: that one's sources lie behind all
+// that this one writes, and what it writes in turn is no source of this one any more.
+template <typename T, int PER, int THREADS>
+__device__ __forceinline__ void keep_slots(T *base, const int *keep, long long p0, int cap, int n) {
+    using Chunk = KeepChunk<T, PER, THREADS>;
+    Chunk now, next;
+    now.load(base, keep, p0, cap, 0, n);
+    for (int a = 0; a < n; a += Chunk::kEntries) {
+        // (the loads themselves, not only their issue, come before any wave's stores)
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#endif
+        __syncthreads();
+        next.load(base, keep, p0, cap, a + Chunk::kEntries, n);
+        now.store(base);
+        now = next;
+    }
 }
 
-template <int CODE>  // bytes of a slot's codes
-__global__ __launch_bounds__(256) void kv_keep_kernel(const KeepArgs A) {
-    constexpr int PER = CODE / 16, kCodes = kKeepPieces * 256 / PER, kScales = kKeepPieces * 256;
+template <int CODE, int THREADS>  // bytes of a slot's codes
+__global__ __launch_bounds__(THREADS) void kv_keep_kernel(const KeepArgs A) {
     // grid x: ((layer * rows + row) * nkv + head) * 2 + (K, V)
     const size_t g = blockIdx.x / 2;
     const int is_v = blockIdx.x & 1, row = (int)(g / A.nkv % A.rows);
@@ -366,15 +385,12 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(const KeepArgs A) {
     const long long p0 = A.pos[row];
     const size_t slot = g * (size_t)A.kv.cap;
     if (blockIdx.y == 0) {
-        u32x4 *q = (u32x4 *)(is_v ? A.kv.vq : A.kv.kq) + slot * PER;
-        for (int a = 0; a < n; a += kCodes) keep_chunk<u32x4, PER>(q, keep, p0, A.kv.cap, a, min(a + kCodes, n));
+        keep_slots<u32x4, CODE / 16, THREADS>((u32x4 *)(is_v ? A.kv.vq : A.kv.kq) + slot * (CODE / 16), keep, p0, A.kv.cap, n);
         return;
     }
     void *s = is_v ? A.kv.vs : A.kv.ks;
-    for (int a = 0; a < n; a += kScales) {
-        if (A.scale_bytes == 4) keep_chunk<uint32_t, 1>((uint32_t *)s + slot, keep, p0, A.kv.cap, a, min(a + kScales, n));
-        else keep_chunk<uint16_t, 1>((uint16_t *)s + slot, keep, p0, A.kv.cap, a, min(a + kScales, n));
-    }
+    if (A.scale_bytes == 4) keep_slots<uint32_t, 1, THREADS>((uint32_t *)s + slot, keep, p0, A.kv.cap, n);
+    else keep_slots<uint16_t, 1, THREADS>((uint16_t *)s + slot, keep, p0, A.kv.cap, n);
 }
 
 RowsArgs rows_args(const k2t_kv_rows &kv, size_t row_stride, int ntok, int nkv, int hd, const int *pos, const int *counts) {
@@ -468,13 +484,22 @@ void launch_kv_reorder(hipStream_t st, int bits, const k2t_kv_rows &kv, const in
     hip_check(hipGetLastError(), "kv_reorder launch");
 }
 
-void launch_kv_keep(hipStream_t st, int bits, const k2t_kv_rows &kv, const int *pos, const int *keep, size_t keep_stride,
+template <int THREADS>
+static void launch_keep(dim3 grid, hipStream_t st, const KeepArgs &A) {
+    if (A.code_bytes == 128) hipLaunchKernelGGL((kv_keep_kernel<128, THREADS>), grid, dim3(THREADS), 0, st, A);
+    else if (A.code_bytes == 64) hipLaunchKernelGGL((kv_keep_kernel<64, THREADS>), grid, dim3(THREADS), 0, st, A);
+    else hipLaunchKernelGGL((kv_keep_kernel<32, THREADS>), grid, dim3(THREADS), 0, st, A);
+}
+
+void launch_kv_keep(int cus, hipStream_t st, int bits, const k2t_kv_rows &kv, const int *pos, const int *keep, size_t keep_stride,
                     const int *counts, int n_keep, int n_layers, int rows, int nkv, int hd) {
     const KeepArgs A{kv, pos, keep, counts, keep_stride, n_keep, rows, nkv, bits == 8 ? hd : hd / 2, bits == 8 ? 4 : hd / 32};
     const dim3 grid((unsigned)(2 * (size_t)n_layers * rows * nkv), 2);
-    if (A.code_bytes == 128) hipLaunchKernelGGL((kv_keep_kernel<128>), grid, dim3(256), 0, st, A);
-    else if (A.code_bytes == 64) hipLaunchKernelGGL((kv_keep_kernel<64>), grid, dim3(256), 0, st, A);
-    else hipLaunchKernelGGL((kv_keep_kernel<32>), grid, dim3(256), 0, st, A);
+    // Sixteen waves, and chunks four times as long, where there are few workgroups or long lists (us, four waves and sixteen: 204
+    // workgroups of heads x 128, 6027 entries 98 and 54; 384 of 3000 59 and 40; 768 of 3000 121 and 110; 1536 of heads x
+    // 64 124 both; 256 of 150 to 400 the same; but 960 of 293 9.8 and 13.1, some 3000 of 400 46 and 52).
+    if (grid.x <= 2 * (unsigned)cus || n_keep >= 1024) launch_keep<1024>(grid, st, A);
+    else launch_keep<256>(grid, st, A);
     hip_check(hipGetLastError(), "kv_keep launch");
 }
 
@@ -548,7 +573,7 @@ int32_t k2t_kv_keep(k2t_ctx *ctx, int32_t bits, const k2t_kv_rows *kv, const int
         if (n_layers == 0 || rows == 0 || n_keep == 0) return;
         branch_arg(d_pos && d_keep, "NULL argument");
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
-        launch_kv_keep(ctx->stream, bits, *kv, d_pos, d_keep, keep_stride, d_counts, n_keep, n_layers, rows, n_kv_heads,
+        launch_kv_keep(ctx->num_cus, ctx->stream, bits, *kv, d_pos, d_keep, keep_stride, d_counts, n_keep, n_layers, rows, n_kv_heads,
                        head_dim);
     });
 }

@@ -499,7 +499,7 @@ def test_logits_of_the_longest_lists(gpu_ctx):
 # ---------------------------------------------------------------- keep
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("layers,rows,nkv,cap,n_keep", [(1, 1, 1, 1, 1), (2, 3, 2, 40, 9), (1, 2, 3, 700, 300), (3, 1, 1, 5000, 4000), (1, 4, 1, 130, 129)])
+@pytest.mark.parametrize("layers,rows,nkv,cap,n_keep", [(1, 1, 1, 1, 1), (2, 3, 2, 40, 9), (1, 2, 3, 700, 300), (3, 1, 1, 5000, 4000), (1, 4, 1, 130, 129), (9, 30, 1, 700, 300)])
 def test_keep(gpu_ctx, bits, hd, layers, rows, nkv, cap, n_keep):
     print(f"kv_keep bits={bits} hd={hd} layers={layers} rows={rows} nkv={nkv} cap={cap} n_keep={n_keep}", flush=True)
     rng = np.random.default_rng(cap + n_keep)
