@@ -8,13 +8,14 @@
 //
 // A workgroup takes a slice of a row's vocabulary: it counts the history's tokens that fall into the slice in LDS
 // (integer atomics: any order gives the same counts), notes for every token the first entry of the bias list that names
-// it, and then passes over its logits once. A token's biases are added in the list's order by the thread that
-// owns the token, so that the sum does not depend on scheduling.
+// it, and the entries of the list that fall into the slice, and then passes over its logits once. A token's biases are
+// added in the list's order by the thread that owns the token, so that the sum does not depend on scheduling.
 //
 // What bounds it: bytes, and every slice's pass over the row's lists. 64 rows of 151936, histories of 2000, 40 biases and a
 // mask (78 MB read and written): 18.8 us, 4.2 TB/s; slices of 1024, 4096 and 8192 logits 22.8, 23.7 and 32 us (more passes
 // over the lists; fewer loads in flight), one load of the history at a time and cached stores 26.8. 4 rows of 49152: 4.1 us, a launch
-// and the lists.
+// and the lists. Tokens that are named twice (4 rows of 10536, 213 biases: 8.1 us; 128 rows of 32000, 300: 14.8): 17.0 and
+// 33.4 with a search through the row's whole list. (4000 biases in 5 slices, most named twice: 356 us, 1890.)
 #include <math.h>
 
 #include <algorithm>
@@ -30,8 +31,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256, kLogitSlice = 2048, kGroups = kLogitSlice / 4 / kThreads;  // groups of four logits per thread
 constexpr int kMaxHistory = 1 << 20, kMaxBias = 4096, kAhead = 8;
+constexpr int kFewBiases = 64, kManyBiases = 2048, kTokenBits = 11;  // (see NAMED)
 constexpr uint32_t kSeen = 1u << 31;    // over the count of a token behind the prompt
 constexpr uint32_t kNone = 0xFFFFu, kAgain = 1u << 15;  // no bias; more entries than the first name the token
+
+static_assert(kLogitSlice == 1 << kTokenBits && kMaxBias <= 1 << (32 - kTokenBits), "an entry of `named` holds both");
 
 struct LogitsArgs {
     const float *x;
@@ -41,10 +45,13 @@ struct LogitsArgs {
     k2t_logits_rules R;
 };
 
-// LISTS: the row may have a history or biases.  VEC: rows start at multiples of 16 bytes.
-template <bool LISTS, bool VEC>
+// NAMED: biases that are noted, as index << kTokenBits | token: the row's whole list (kFewBiases; ~0: of another slice), or the
+// slice's; 0: the row has neither history nor biases.  VEC: rows start at multiples of 16 bytes.
+template <int NAMED, bool VEC>
 __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
-    __shared__ __align__(16) uint32_t count[LISTS ? kLogitSlice : 4], first[LISTS ? kLogitSlice : 4];
+    constexpr bool LISTS = NAMED > 0, WHOLE = NAMED == kFewBiases;
+    __shared__ __align__(16) uint32_t count[LISTS ? kLogitSlice : 4], first[LISTS ? kLogitSlice : 4], named[LISTS ? NAMED : 4];
+    __shared__ int before[kThreads / 64];
     const int row = (int)blockIdx.y, v0 = (int)blockIdx.x * kLogitSlice, tid = (int)threadIdx.x;
     const int n = min(kLogitSlice, A.vocab - v0);
     const float *x = A.x + (size_t)row * A.x_stride + v0;
@@ -68,7 +75,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
         const int m = R.d_mask_row ? R.d_mask_row[row] : row;
         if (m >= 0 && m < R.mask_rows) mask = R.d_mask + (size_t)m * R.mask_stride + v0 / 32;
     }
-    int biases = 0;
+    int biases = 0, mine = 0;  // of the row; that name the slice's tokens
     if constexpr (LISTS) {
         for (int i = 4 * tid; i < kLogitSlice; i += 4 * kThreads) {
             *reinterpret_cast<uint4 *>(count + i) = make_uint4(0, 0, 0, 0);
@@ -100,14 +107,44 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
             for (int i = tid; i < biases; i += kThreads) {
                 const uint32_t t = (uint32_t)names[i] - (uint32_t)v0;
                 if (t < (uint32_t)n) atomicMin(&first[t], (uint32_t)i);
+                if (WHOLE) named[i] = t < (uint32_t)n ? (uint32_t)i << kTokenBits | t : ~0u;
             }
         }
         __syncthreads();
-        for (int i = tid; i < biases; i += kThreads) {
-            const uint32_t t = (uint32_t)names[i] - (uint32_t)v0;
-            if (t < (uint32_t)n && (first[t] & (kAgain - 1)) != (uint32_t)i) atomicOr(&first[t], kAgain);
+        if constexpr (WHOLE) {
+            mine = biases;
+            for (int i = tid; i < biases; i += kThreads) {
+                const uint32_t t = named[i] & (kLogitSlice - 1);
+                if (named[i] != ~0u && (first[t] & (kAgain - 1)) != (uint32_t)i) atomicOr(&first[t], kAgain);
+            }
+            __syncthreads();
+        } else if (biases) {  // the slice's entries, in order: a thread takes some that follow each other
+            const int per = (biases + kThreads - 1) / kThreads, a = min(tid * per, biases), b = min(a + per, biases);
+            int own = 0;
+            for (int i = a; i < b; i++) own += (uint32_t)names[i] - (uint32_t)v0 < (uint32_t)n;
+            int upto = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int v = __shfl_up(upto, d, 64);
+                upto += (tid & 63) >= d ? v : 0;
+            }
+            if ((tid & 63) == 63) before[tid >> 6] = upto;
+            __syncthreads();
+            int at = upto - own;
+#pragma unroll
+            for (int w = 0; w < kThreads / 64; w++) {
+                at += w < tid >> 6 ? before[w] : 0;
+                mine += before[w];
+            }
+            for (int i = a; i < b; i++) {
+                const uint32_t t = (uint32_t)names[i] - (uint32_t)v0;
+                if (t >= (uint32_t)n) continue;
+                if ((first[t] & (kAgain - 1)) != (uint32_t)i) atomicOr(&first[t], kAgain);
+                if (at < NAMED) named[at] = (uint32_t)i << kTokenBits | t;
+                at++;
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
     const double repeat = LISTS && R.d_repeat ? (double)R.d_repeat[row] : 1.0;
     const double presence = LISTS && R.d_presence ? (double)R.d_presence[row] : 0.0;
@@ -122,9 +159,15 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
             const int *names = R.d_bias_tokens + (size_t)row * R.bias_stride;
             const int at = (int)(b & (kAgain - 1));
             y += (double)value[at];
-            if (b & kAgain)
+            if (b & kAgain && mine <= NAMED) {
+                for (int k = 0; k < mine; k++) {
+                    const uint32_t e = named[k];
+                    if (e != ~0u && (e & (kLogitSlice - 1)) == (uint32_t)i && (int)(e >> kTokenBits) > at) y += (double)value[e >> kTokenBits];
+                }
+            } else if (b & kAgain) {  // (more biases than tokens)
                 for (int k = at + 1; k < biases; k++)
                     if (names[k] == v0 + i) y += (double)value[k];
+            }
         }
         return (float)y;
     };
@@ -160,6 +203,12 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsArgs A) {
                 if (i + j < n) out[i + j] = f[g][j];
         }
     }
+}
+
+template <int NAMED>
+void launch_logits(bool vec, dim3 grid, hipStream_t st, const LogitsArgs &A) {
+    if (vec) hipLaunchKernelGGL((logits_kernel<NAMED, true>), grid, dim3(kThreads), 0, st, A);
+    else hipLaunchKernelGGL((logits_kernel<NAMED, false>), grid, dim3(kThreads), 0, st, A);
 }
 
 }  // namespace
@@ -205,11 +254,12 @@ int32_t k2t_logits_adjust(k2t_ctx *ctx, const float *d_logits, int32_t vocab, si
         LogitsArgs A{d_logits, d_out, row_stride, out_stride, vocab, R};
         const bool vec = (at(d_logits) | at(d_out)) % 16 == 0 && row_stride % 4 == 0 && out_stride % 4 == 0;
         const bool lists = (R.d_history && R.history_len) || (R.d_bias && R.bias_len);
-        const dim3 grid((unsigned)((vocab + kLogitSlice - 1) / kLogitSlice), (unsigned)rows), block(kThreads);
-        if (lists && vec) hipLaunchKernelGGL((logits_kernel<true, true>), grid, block, 0, ctx->stream, A);
-        else if (lists) hipLaunchKernelGGL((logits_kernel<true, false>), grid, block, 0, ctx->stream, A);
-        else if (vec) hipLaunchKernelGGL((logits_kernel<false, true>), grid, block, 0, ctx->stream, A);
-        else hipLaunchKernelGGL((logits_kernel<false, false>), grid, block, 0, ctx->stream, A);
+        const dim3 grid((unsigned)((vocab + kLogitSlice - 1) / kLogitSlice), (unsigned)rows);
+        // (a short list needs no sorting out by slices, and less LDS: 64 rows of 151936, 40 biases, 19.2 and 22.9 us; but
+        // 4 rows of 10536, 213 biases that name tokens twice, 15.9 and 8.1)
+        if (!lists) launch_logits<0>(vec, grid, ctx->stream, A);
+        else if (!R.d_bias || R.bias_len <= kFewBiases) launch_logits<kFewBiases>(vec, grid, ctx->stream, A);
+        else launch_logits<kManyBiases>(vec, grid, ctx->stream, A);
         hip_check(hipGetLastError(), "logits_adjust launch");
     });
 }
