@@ -9,7 +9,8 @@
 // under way, then rotate eight elements (four pairs) at a time.
 //
 // What bounds it: bytes. 6 rows of 389 to 777 tokens, 36 heads x 128 (129 MB read and written): 21 to 23 us, 5.5 to 6 TB/s (the
-// inputs partly from the Infinity Cache); 34.7 with one piece in flight per thread and cached stores. One token of 4
+// inputs partly from the Infinity Cache); 34.7 with one piece in flight per thread and cached stores. 6 rows of 777, 168 MB: 28.5,
+// interleaved 28.9 (49.9 with a thread's two pieces side by side), rot_dim 98, halves, a pair at a time, 54. One token of 4
 // rows, 12 heads x 64: 3.6 us, a launch and the chain from position to angle to output.
 #include <math.h>
 
@@ -48,22 +49,27 @@ __device__ __forceinline__ float2 turn_cos_sin(double turn, double scale) {
     return make_float2((float)((k == 1 || k == 2 ? -a : a) * scale), (float)((k >= 2 ? -b : b) * scale));
 }
 
-// Two elements' places in a head for unit u's pairs 0 and (VEC 8) 4 elements on: first and second members.
+// Where unit u's two halves lie in a head: of VEC / 2 elements each, and such that neighbouring units' lie next to each other.
+// K2T_ROPE_HALF: first and second members of the same pairs, then halves of what is behind rot_dim.  INTERLEAVED: whole
+// pairs each, of all of the head.
 template <int VEC>
-__device__ __forceinline__ void unit_at(const k2t_rope_plan &P, int u, int &a, int &b) {
+__device__ __forceinline__ void unit_at(const k2t_rope_plan &P, int hd, int u, int &a, int &b) {
     constexpr int H = VEC / 2;
-    if (VEC * u >= P.rot_dim || P.layout == K2T_ROPE_INTERLEAVED) {
-        a = VEC * u;
-        b = a + H;
-    } else {
+    if (P.layout == K2T_ROPE_INTERLEAVED) {
+        a = H * u;
+        b = a + hd / 2;
+    } else if (VEC * u < P.rot_dim) {
         a = H * u;
         b = a + P.rot_dim / 2;
+    } else {
+        a = P.rot_dim + H * (u - P.rot_dim / VEC);
+        b = a + (hd - P.rot_dim) / 2;
     }
 }
 
 constexpr int kMaxPer = 3, kFlight = 4;  // tokens of a workgroup, whose angles wait in LDS; units in flight per thread
 
-// VEC 8: rot_dim is a multiple of 8, so that a unit is two 16-byte pieces; else VEC 2, a pair at a time.
+// VEC 8: units of two 16-byte pieces; VEC 2: K2T_ROPE_HALF whose rot_dim is no multiple of 8, a pair at a time.
 template <int VEC>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs A) {
     constexpr int H = VEC / 2;
@@ -85,7 +91,7 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs A) {
     const auto load = [&](int g, Piece &p) {
         const int t = g / A.units, u = g - t * A.units, head = u >> A.hd_shift, e = u & ((1 << A.hd_shift) - 1);
         int a, b;
-        unit_at<VEC>(A.plan, e, a, b);
+        unit_at<VEC>(A.plan, A.hd, e, a, b);
         const float *x = A.x + (size_t)(first + t) * A.x_stride + (size_t)head * A.hd;
         if constexpr (VEC == 8) {
             p.a = *reinterpret_cast<const f32x4 *>(x + a);
@@ -97,10 +103,10 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs A) {
     };
     const auto rotate = [&](int g, const Piece &p) {
         const int t = g / A.units, u = g - t * A.units, head = u >> A.hd_shift, e = u & ((1 << A.hd_shift) - 1);
-        const bool turns = VEC * e < A.plan.rot_dim;
-        if (!live(first + t) || (!turns && !moved)) return;
         int a, b;
-        unit_at<VEC>(A.plan, e, a, b);
+        unit_at<VEC>(A.plan, A.hd, e, a, b);
+        const bool turns = a < A.plan.rot_dim;
+        if (!live(first + t) || (!turns && !moved)) return;
         float *o = A.out + (size_t)(first + t) * A.out_stride + (size_t)head * A.hd;
         float x[VEC], y[VEC];
 #pragma unroll
@@ -110,17 +116,21 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs A) {
             y[j] = x[j];
             y[H + j] = x[H + j];
         }
-        if (turns) {
+        if (VEC == 8 && A.plan.layout == K2T_ROPE_INTERLEAVED) {
+#pragma unroll
+            for (int j = 0; j < H; j++) {
+                const int pair = (j < H / 2 ? a : b) / 2 + j % (H / 2);
+                if (pair >= pairs) continue;
+                const float c = cs[t][0][pair], s = cs[t][1][pair];
+                y[2 * j] = x[2 * j] * c - x[2 * j + 1] * s;
+                y[2 * j + 1] = x[2 * j + 1] * c + x[2 * j] * s;
+            }
+        } else if (turns) {
 #pragma unroll
             for (int j = 0; j < H; j++) {
                 const float c = cs[t][0][H * e + j], s = cs[t][1][H * e + j];
-                if (VEC == 8 && A.plan.layout == K2T_ROPE_INTERLEAVED) {
-                    y[2 * j] = x[2 * j] * c - x[2 * j + 1] * s;
-                    y[2 * j + 1] = x[2 * j + 1] * c + x[2 * j] * s;
-                } else {
-                    y[j] = x[j] * c - x[H + j] * s;
-                    y[H + j] = x[H + j] * c + x[j] * s;
-                }
+                y[j] = x[j] * c - x[H + j] * s;
+                y[H + j] = x[H + j] * c + x[j] * s;
             }
         }
         if constexpr (VEC == 8) {
@@ -232,7 +242,7 @@ int32_t k2t_rope(k2t_ctx *ctx, const float *d_x, size_t x_stride, int32_t batch,
                    "d_x and d_out must be 16-byte aligned");
         branch_arg(d_x != d_out || x_stride == out_stride, "in place the strides must be the same");
         hip_check(hipSetDevice(ctx->device), "hipSetDevice");
-        const bool wide = plan->rot_dim % 8 == 0;
+        const bool wide = plan->rot_dim % 8 == 0 || plan->layout == K2T_ROPE_INTERLEAVED;
         RopeArgs A{};
         A.x = d_x;
         A.out = d_out;
