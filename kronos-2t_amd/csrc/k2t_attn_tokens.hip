@@ -491,10 +491,12 @@ struct Plan {
 // 37.3.  tokens_block_kernel: from three workgroups for two CUs on (1024 tokens, 32 / 4 x 128, one for a CU: 32.0 and 42.2 with it;
 // 2048, two: 83.9 and 80.0; 8192, eight: 923 and 770).  For NF4, whose lookups it shares, also behind long contexts (512 tokens,
 // 32 / 8 x 128, behind 0, 2100, 4100 and 16000 positions: 22, 68, 107 and 357, and 33, 80, 108 and 287 with it; int8 behind 4100
-// and 16000: 72 and 234, 90 and 233; 515 tokens, NF4, behind 4100: 152 and 120), if there is one for eight CUs (64 tokens behind
-// 12000, 32 / 4 x 128, one for 16: 47 and 60).
+// and 16000: 72 and 234, 90 and 233; 515 tokens, NF4, behind 4100: 152 and 120), if there is one for four CUs (2 x 40 tokens
+// behind 6100, one for eight: 37 and 46; 8 x 40, one for two: 136 and 106).  Never where half of its columns would be idle (64 rows x 4, 8 and 16 tokens behind
+// 2000, 32 / 8 x 128: 48, 54 and 95, and 65, 75 and 86; 16 rows x 30 and 60, 32 x 64: 32 and 54, and 52 and 57).  Columns that fill
+// one tile take one (64 rows x 1 token behind 2000, 32 / 8 x 128, one and two: 45 and 48, NF4 41 and 53).
 constexpr double kLittleWork = 17.0;
-constexpr int kLeastPart = 256, kLongContext = 4000;
+constexpr int kLeastPart = 256, kLongContext = 4000, kBlockColumns = 64;
 
 // The most parts that an item is cut into where a call has so many: a workgroup for every CU; two of tokens_block_kernel,
 // and a part more where an item begins and ends within other items' workgroups.
@@ -521,8 +523,8 @@ Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int 
     const int mean = tree ? len : std::max(len - s.ntok / 2, 1);
     const double work = (double)items(16) * mean / 128 / cus;
     const size_t blocks = items(16 * kBlockWaves);
-    P.block = 2 * blocks >= 3 * cus || (bits == 4 && mean >= kLongContext && 8 * blocks >= cus);
-    P.nq = work <= kLittleWork ? 1 : 2;
+    P.block = cols >= kBlockColumns && (2 * blocks >= 3 * cus || (bits == 4 && mean >= kLongContext && 4 * blocks >= cus));
+    P.nq = cols <= 16 || work <= kLittleWork ? 1 : 2;
     P.cgs = (cols + P.item() - 1) / P.item();
     const size_t each_part = items(P.item());
     const int most = most_parts(ctx, P.block, each_part, len);

@@ -317,7 +317,7 @@ def test_attention_of_many_columns_and_parts(gpu_ctx, bits, hd, nq, nkv, batch, 
 
 
 # items of many columns whose positions workgroups share, each from where the one before stops (few items for two on every CU)
-CUT = [(8, 64, 16, 16, 8, 380, 3100, 0, False), (8, 128, 8, 8, 7, 1000, 0, 9000, False), (4, 64, 8, 4, 3, 256, 4100, 0, False),
+CUT = [(8, 64, 16, 16, 8, 380, 3100, 0, False), (8, 128, 8, 8, 7, 1000, 0, 9000, False), (4, 64, 8, 4, 4, 256, 4100, 0, False),
        (4, 128, 8, 8, 4, 130, 4500, 300, False), (4, 128, 16, 4, 8, 40, 4500, 50, True), (4, 64, 20, 2, 3, 64, 900, 8000, True)]
 
 
