@@ -17,8 +17,8 @@
 // matrix cores and the power they draw (the core's clock is down at 2.0 GHz): outputs are done twice, for a weight's two
 // pieces, and all products would take 555 us at the rate of a large one (1.24 PFLOP/s f16, int8 twice that).  68 us are the
 // ends of items, queries and outputs (268 MB).  6 prompts of 389 to 777 tokens, 32 heads x 64: 39 us, the ends half of them.
-// Chunks of a prompt behind a context: NF4's lookups, the ends, the join (515 tokens behind 4100, 32 / 8 x 128, NF4: 118 us,
-// 15 and 12 of them).  Drafts behind a context: latencies at two waves per SIMD, and what one CU loads at a time (64 tokens
+// Chunks of a prompt behind a context: NF4's lookups, the ends, the join (515 tokens behind 4100, 32 / 8 x 128, NF4: 107 to
+// 118 us, 15 and 12 of them).  Drafts behind a context: latencies at two waves per SIMD, and what one CU loads at a time (64 tokens
 // behind 12000, 32 / 4 x 128: 35 us, 4.6 of them the join; 8 x 13 behind 2100, 32 / 8 x 128, NF4: 24).  Short drafts: a launch,
 // a few tiles and the transforms (10 tokens behind 300, 9 / 3 x 64: 5.9 us).
 #include <float.h>
@@ -492,9 +492,10 @@ struct Plan {
 // 2048, two: 83.9 and 80.0; 8192, eight: 923 and 770).  For NF4, whose lookups it shares, also behind long contexts (512 tokens,
 // 32 / 8 x 128, behind 0, 2100, 4100 and 16000 positions: 22, 68, 107 and 357, and 33, 80, 108 and 287 with it; int8 behind 4100
 // and 16000: 72 and 234, 90 and 233; 515 tokens, NF4, behind 4100: 152 and 120), if there is one for four CUs (2 x 40 tokens
-// behind 6100, one for eight: 37 and 46; 8 x 40, one for two: 136 and 106).  Never where half of its columns would be idle (64 rows x 4, 8 and 16 tokens behind
-// 2000, 32 / 8 x 128: 48, 54 and 95, and 65, 75 and 86; 16 rows x 30 and 60, 32 x 64: 32 and 54, and 52 and 57).  Columns that fill
-// one tile take one (64 rows x 1 token behind 2000, 32 / 8 x 128, one and two: 45 and 48, NF4 41 and 53).
+// behind 6100, one for eight: 37 and 46; 8 x 40, one for two: 136 and 106).  Never where half of its columns would be idle (64
+// rows x 4, 8 and 16 tokens behind 2000, 32 / 8 x 128: 48, 54 and 95, and 65, 75 and 86; 16 rows x 30 and 60, 32 x 64: 32 and
+// 54, and 52 and 57).  Columns that fill one tile take one (64 rows x 1 token behind 2000, 32 / 8 x 128, one and two: 45 and 48,
+// NF4 41 and 53).
 constexpr double kLittleWork = 17.0;
 constexpr int kLeastPart = 256, kLongContext = 4000, kBlockColumns = 64;
 
@@ -541,7 +542,8 @@ Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int 
         const size_t slots = 2 * cus, total = each_part * P.tiles;
         const int chunk = (int)std::max((total + slots - 1) / slots, (size_t)kLeastPart / P.plen);
         const int parts = (P.tiles + chunk - 2) / chunk + 1;
-        if (parts > 1 && plan_cost(s, P, bits, cus, (total + chunk - 1) / chunk, parts, chunk * P.plen) < plan_cost(s, P, bits, cus, each_part, 1, len)) {
+        const double cut = plan_cost(s, P, bits, cus, (total + chunk - 1) / chunk, parts, chunk * P.plen);
+        if (parts > 1 && cut < plan_cost(s, P, bits, cus, each_part, 1, len)) {
             P.parts = parts;
             P.chunk = chunk;
         }
