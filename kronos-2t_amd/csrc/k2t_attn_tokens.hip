@@ -13,10 +13,11 @@
 // too (tokens_block_kernel).  Where that leaves CUs without a workgroup (tokens_block_kernel: without a second one),
 // positions are cut into parts, which a second kernel joins.
 //
-// What bounds it.  8192 tokens from the start, 32 / 4 heads x 128, int8: 780 to 865 us by the card, 0.55 PFLOP that count at 0.7 PFLOP/s.  The
-// matrix cores and the power they draw (the core's clock is down at 2.0 GHz): outputs are done twice, for a weight's two
-// pieces, and all products would take 555 us at the rate of a large one (1.24 PFLOP/s f16, int8 twice that).  68 us are the
-// ends of items, queries and outputs (268 MB).  6 prompts of 389 to 777 tokens, 32 heads x 64: 39 us, the ends half of them.
+// What bounds it.  8192 tokens from the start, 32 / 4 heads x 128, int8: 780 to 865 us by the card, 0.55 PFLOP that count at
+// 0.7 PFLOP/s.  The matrix cores and the power they draw (the core's clock is down at 2.0 GHz): outputs are done twice, for
+// a weight's two pieces, and all products would take 555 us at the rate of a large one (1.24 PFLOP/s f16, int8 twice
+// that).  68 us are the ends of items, queries and outputs (268 MB).  6 prompts of 389 to 777 tokens, 32 heads x 64: 39 us,
+// the ends half of them.
 // Chunks of a prompt behind a context: NF4's lookups, the ends, the join (515 tokens behind 4100, 32 / 8 x 128, NF4: 107 to
 // 118 us, 15 and 12 of them).  Drafts behind a context: latencies at two waves per SIMD, and what one CU loads at a time (64 tokens
 // behind 12000, 32 / 4 x 128: 35 us, 4.6 of them the join; 8 x 13 behind 2100, 32 / 8 x 128, NF4: 24).  Short drafts: a launch,

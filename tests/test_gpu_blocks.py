@@ -289,7 +289,8 @@ def attention_on_gpu(bits, q, cache, pos, counts, sees, nq, nkv, hd, scale, leng
 LARGE = [(8, 64, 64, 64, 3, 200, 40, 0, False), (8, 64, 128, 64, 4, 90, 0, 0, True), (8, 128, 96, 48, 5, 130, 70, 0, False),
          (8, 128, 32, 4, 16, 64, 100, 0, True), (4, 64, 66, 33, 6, 150, 30, 0, False), (4, 128, 32, 4, 2, 64, 300, 9000, True),
          (4, 128, 16, 2, 3, 300, 0, 12000, False), (8, 128, 32, 4, 2, 64, 700, 20000, True), (8, 64, 32, 32, 1, 60, 500, 30000, True),
-         (8, 128, 8, 2, 2, 40, 900, 6000, False), (4, 64, 9, 3, 3, 50, 40, 50000, True), (8, 64, 12, 4, 1, 1100, 0, 0, False)]
+         (8, 128, 8, 2, 2, 40, 900, 6000, False), (4, 64, 9, 3, 3, 50, 40, 50000, True), (8, 64, 12, 4, 1, 1100, 0, 0, False),
+         (4, 128, 16, 16, 6, 500, 0, 0, False)]
 
 
 @pytest.mark.parametrize("bits,hd,nq,nkv,batch,ntok,start,room,with_tree", LARGE)
