@@ -731,7 +731,7 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
 }
 
 // Joins the parts of one column: out = ifwht64(sum_i e_i part_i / sum_i e_i l_i), e_i = 2^(m_i - max m). A chain of
-// latencies (lengths, statistics, partials, the transform): 3 to 5 us whatever the sizes here.
+// latencies (lengths, statistics, partials, the transform): 3 to 5 us where the parts are a few MB (16480 heads of 128, 42 MB: 12).
 // One (head, row) per WAVES waves: its parts' maxima and sums one per lane, then the outputs of every
 // WAVES-th part, eight or sixteen loads in flight, joined in wave order, and ifwht64.  Parts that hold no
 // positions (not live_part) were not written and count nothing; any: there is one that does.
