@@ -744,7 +744,7 @@ void forward_mk(k2t_model *m, int token, int *next) {
             hip_check(hipMalloc(&trace, ntr * 8), "trace");
             trace_cap = ntr;
         }
-        hip_check(hipMemset(trace, 0, ntr * 8), "trace clear");
+        hip_check(hipMemsetAsync(trace, 0, ntr * 8, m->stream), "trace clear");
         P.trace = trace;
     }
 #endif
@@ -770,12 +770,13 @@ void check_mk_error(k2t_model *m) {
     int e = 0;
     hip_check(hipMemcpy(&e, m->err_dev, sizeof(int), hipMemcpyDeviceToHost), "error flag");
     if (e) {
-        (void)hipMemset(m->err_dev, 0, sizeof(int));
+        (void)hipMemsetAsync(m->err_dev, 0, sizeof(int), m->stream);
         // a timed-out wait leaves the span attention's counters and words
         // inconsistent: start its epochs over
-        (void)hipMemset(m->attn_cnt, 0, 2 * sizeof(unsigned int));
-        (void)hipMemset(m->attn_words, 0,
-                        attn_span_words(m->cfg.max_seq, m->cfg.n_heads, m->cfg.head_dim) * sizeof(unsigned long long));
+        (void)hipMemsetAsync(m->attn_cnt, 0, 2 * sizeof(unsigned int), m->stream);
+        (void)hipMemsetAsync(m->attn_words, 0,
+                             attn_span_words(m->cfg.max_seq, m->cfg.n_heads, m->cfg.head_dim) * sizeof(unsigned long long),
+                             m->stream);
         throw Error(K2T_E_INTERNAL, e == 2   ? "MoE route selection: router wait timed out"
                                     : e == 3 ? "span attention: span wait timed out"
                                              : "persistent decode kernel: dependency wait timed out");
@@ -983,6 +984,8 @@ int32_t k2t_model_create(k2t_ctx *ctx, const k2t_model_config *cfg, int32_t max_
             m->max_batch = max_batch;
             m->layers.resize(c.n_layers);
             hip_check(hipStreamCreateWithFlags(&m->stream, hipStreamNonBlocking), "stream create");
+            // (what is cleared is cleared on this stream: a plain hipMemset returns before it is done, on a stream that
+            // this one does not wait for and that other work may hold up)
             const size_t slots = (size_t)c.n_layers * c.n_kv_heads * c.max_seq;
             m->kq = (int8_t *)dalloc(m, slots * c.head_dim);
             m->vq = (int8_t *)dalloc(m, slots * c.head_dim);
@@ -993,7 +996,7 @@ int32_t k2t_model_create(k2t_ctx *ctx, const k2t_model_config *cfg, int32_t max_
             hip_check(hipMemcpy(m->rope, rt.data(), rt.size() * sizeof(float), hipMemcpyHostToDevice), "rope upload");
             m->pos_dev = (int *)dalloc(m, (size_t)(max_batch + 1) * sizeof(int));
             m->tokens = m->pos_dev + 1;
-            hip_check(hipMemset(m->pos_dev, 0, (size_t)(max_batch + 1) * sizeof(int)), "pos clear");
+            hip_check(hipMemsetAsync(m->pos_dev, 0, (size_t)(max_batch + 1) * sizeof(int), m->stream), "pos clear");
             const size_t qkv_w = (size_t)(c.n_heads + 2 * c.n_kv_heads) * c.head_dim;
             const size_t kmax = std::max({c.hidden, c.intermediate, c.n_heads * c.head_dim});
             m->hidden = (float *)dalloc(m, (size_t)max_batch * c.hidden * sizeof(float));
@@ -1006,9 +1009,9 @@ int32_t k2t_model_create(k2t_ctx *ctx, const k2t_model_config *cfg, int32_t max_
             // zeroed once (epochs only grow, so no launch clears them)
             const size_t gw = attn_span_words(c.max_seq, c.n_heads, c.head_dim);
             m->attn_words = (unsigned long long *)dalloc(m, gw * sizeof(unsigned long long));
-            hip_check(hipMemset(m->attn_words, 0, gw * sizeof(unsigned long long)), "span words clear");
+            hip_check(hipMemsetAsync(m->attn_words, 0, gw * sizeof(unsigned long long), m->stream), "span words clear");
             m->attn_cnt = (unsigned int *)dalloc(m, 2 * sizeof(unsigned int));
-            hip_check(hipMemset(m->attn_cnt, 0, 2 * sizeof(unsigned int)), "counter clear");
+            hip_check(hipMemsetAsync(m->attn_cnt, 0, 2 * sizeof(unsigned int), m->stream), "counter clear");
             m->rms_x86 = (float *)dalloc(m, (size_t)max_batch * sizeof(float));
             m->attn_f = (float *)dalloc(m, (size_t)max_batch * c.n_heads * c.head_dim * sizeof(float));
             m->xq = (int8_t *)dalloc(m, (size_t)max_batch * kmax);
@@ -1035,7 +1038,7 @@ int32_t k2t_model_create(k2t_ctx *ctx, const k2t_model_config *cfg, int32_t max_
             const size_t words =
                 kMkRep * (2 * (size_t)c.hidden + oact + gact) + qkv_w + 2 * (size_t)ctx->num_cus + apart;
             m->ll_ha = (unsigned long long *)dalloc(m, words * 8);
-            hip_check(hipMemset(m->ll_ha, 0, words * 8), "hand-off clear");
+            hip_check(hipMemsetAsync(m->ll_ha, 0, words * 8, m->stream), "hand-off clear");
             m->ll_hb = m->ll_ha + kMkRep * (size_t)c.hidden;
             m->ll_oact = m->ll_hb + kMkRep * (size_t)c.hidden;
             m->ll_gact = m->ll_oact + kMkRep * oact;
@@ -1165,7 +1168,7 @@ int32_t k2t_model_set_moe(k2t_model *m, int32_t layer, const k2t_experts *bank, 
         if (need > m->moe_ws_floats) {
             float *ws = (float *)dalloc(m, need * sizeof(float));
             // the route hand-off words and the call counter start at epoch 0
-            hip_check(hipMemset(ws, 0, need * sizeof(float)), "moe workspace clear");
+            hip_check(hipMemsetAsync(ws, 0, need * sizeof(float), m->stream), "moe workspace clear");
             m->moe_ws = ws;
             m->moe_ws_floats = need;
         }
@@ -1293,7 +1296,7 @@ int32_t k2t_model_set_kv_window(k2t_model *m, int32_t window, int32_t sink_token
             m->ring = KvRing{c.max_seq, 0, 0, 0, m->ring.bits};
         }
         // set_kv_sliding_window starts a new context (real_llm.rs:1764-1790)
-        hip_check(hipMemset(m->pos_dev, 0, sizeof(int)), "pos reset");
+        hip_check(hipMemsetAsync(m->pos_dev, 0, sizeof(int), m->stream), "pos reset");
         m->pos = 0;
         drop_graph(m);
     });
@@ -1308,7 +1311,7 @@ int32_t k2t_model_set_kv_bits(k2t_model *m, int32_t bits) {
         // set_kv_bits (real_llm.rs:1732-1752): a new cache, position 0.  The NF4 nibbles
         // and BF16 block scales fit in the int8 buffers (hd/2 <= hd bytes, hd/64 BF16 <= one f32).
         m->ring.bits = bits;
-        hip_check(hipMemset(m->pos_dev, 0, sizeof(int)), "pos reset");
+        hip_check(hipMemsetAsync(m->pos_dev, 0, sizeof(int), m->stream), "pos reset");
         m->pos = 0;
         drop_graph(m);
     });
@@ -1349,7 +1352,7 @@ int32_t k2t_model_reset(k2t_model *m) {
         arg(m != nullptr, "model is NULL");
         hip_check(hipSetDevice(m->ctx->device), "hipSetDevice");
         hip_check(hipStreamSynchronize(m->stream), "sync");
-        hip_check(hipMemset(m->pos_dev, 0, sizeof(int)), "pos reset");
+        hip_check(hipMemsetAsync(m->pos_dev, 0, sizeof(int), m->stream), "pos reset");
         m->pos = 0;
     });
 }

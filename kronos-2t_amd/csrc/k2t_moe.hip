@@ -944,7 +944,7 @@ int32_t k2t_moe_ffn(k2t_ctx *ctx, const k2t_experts *bank, int32_t shard_layer, 
             hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
             if (hipStreamIsCapturing(ctx->stream, &cap) == hipSuccess && cap == hipStreamCaptureStatusNone &&
                 hipStreamSynchronize(ctx->stream) == hipSuccess)
-                (void)hipMemset(ctx->moe_state, 0, kMoeStateWords * sizeof(unsigned long long));
+                (void)hipMemsetAsync(ctx->moe_state, 0, kMoeStateWords * sizeof(unsigned long long), ctx->stream);
             throw;
         }
     });

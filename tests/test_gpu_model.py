@@ -325,3 +325,46 @@ def test_persistent_kernel_with_large_max_seq(gpu_ctx):
     for t in (7, 123, 400):
         ok, info = _close(gm.decode(t), ref.forward_token(t), 0.9999)
         assert ok, info
+
+
+@pytest.mark.parametrize("fmt,planes", [("nf4", None), ("n4", {"qkv": 5, "o": 5, "gu": 4, "down": 5, "head": 4})])
+def test_new_contexts_beside_work_of_other_streams(gpu_ctx, fmt, planes):
+    """A model that starts a new context (reset, set_kv_bits) or is made while another stream is busy, whichever of the
+    device's queues that one has: the position is cleared before the model's next step."""
+    import torch
+    cfg = dict(n_layers=2, hidden=256, n_heads=4, n_kv_heads=2, head_dim=64, intermediate=512, vocab=520, max_seq=24, rms_eps=1e-5,
+               rope_theta=10000.0)
+    layers, head, fn = random_model(cfg, seed=5, fmt=fmt, planes=planes)
+
+    def steps(m):
+        m.prefill(np.array([3, 9, 250], np.int32), want_logits=False)
+        return np.stack([m.decode(77), m.decode(5)])
+
+    gm, mats = _gpu_model(gpu_ctx, cfg, layers, head, fn)
+    want = steps(gm)
+    x = torch.zeros(1 << 26, device="cuda")
+    for i in range(8):
+        s = torch.cuda.Stream()
+        torch.cuda.synchronize()
+
+        def busy():
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    x.add_(1.0)
+        busy()
+        gm.reset()
+        assert np.array_equal(steps(gm), want), i
+        busy()
+        gm.set_kv_bits(8)
+        assert np.array_equal(steps(gm), want), i
+        if i % 2 == 0:
+            busy()
+            other, more = _gpu_model(gpu_ctx, cfg, layers, head, fn)
+            assert np.array_equal(steps(other), want), i
+            other.close()
+            for m in more:
+                m.close()
+        torch.cuda.synchronize()
+    gm.close()
+    for m in mats:
+        m.close()
