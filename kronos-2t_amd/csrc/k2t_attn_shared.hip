@@ -42,7 +42,7 @@ struct SharedArgs : ColumnArgs {
 };
 
 template <int HD, int BITS, int NQ>
-__global__ __launch_bounds__(64 * kWaves, 2) void shared_part_kernel(SharedArgs A) {
+__global__ __launch_bounds__(64 * kWaves, HD * NQ <= 128 ? 3 : 2) void shared_part_kernel(SharedArgs A) {
     __shared__ union U {
         Shared<HD, NQ> prefix;
         Shared<HD, 1> tail;
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_part_kernel(SharedArgs 
 // Few positions: one workgroup per (row, KV head, 16 q heads) takes the prefix and the tail and writes
 // the output; the prefix is read once per row, by so few bytes that a second launch costs more.
 template <int HD, int BITS>
-__global__ __launch_bounds__(64 * kWaves, 2) void shared_whole_kernel(SharedArgs A) {
+__global__ __launch_bounds__(64 * kWaves, 3) void shared_whole_kernel(SharedArgs A) {
     __shared__ Shared<HD, 1> sh;
     int t = (int)blockIdx.x;
     const int cg = t % A.tgroups;

@@ -35,11 +35,13 @@ constexpr float kTop = 9.0f, kLimit = 15.0f, kLift = 256.0f, kLog2Lift = 8.0f;
 // size), but a weight refers to the first, which therefore counts as 2^-60 of the second at least.
 constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f;
 // Scores so far from zero that fp32 does not tell whole numbers apart.  An exact product less the reference would
-// be up to half a step of the score off then, which may be any power of two: in a column that has met one, scores
-// are rounded before the reference, a rounded one itself, is taken off.  The largest score's weight is then a power of two that
-// its scale asks for where a step of the score leaves it, else one: a reference that took in the scale before it was
-// rounded could lie a whole step above every score.
+// be up to half a step of the score off then, which may be any power of two: in a column whose reference is so far, scores
+// are rounded before the reference, the largest rounded one, is taken off.  What V scales ask for cannot be part of such a
+// reference, whose steps may be larger than that, and whose rounding would put it a step above every score: it is a
+// second number (State::beside), taken off after.  Waves and parts are joined by the first one alone, in sums of V
+// that such columns' scales may take to 2^100.
 constexpr float kFar = 0x1p24f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m > -FLT_MAX; }
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // What the kernels' argument structs share: the columns' queries and outputs.
@@ -211,6 +213,13 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_
     lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
 }
 
+// The lane's column, counted anew: as a value kept over the loop it would cost a register where none is left.
+__device__ __forceinline__ uint32_t own_column() {
+    uint32_t all = ~0u;
+    asm volatile("" : "+s"(all));
+    return __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u)) & 15u;
+}
+
 // What a wave carries from tile to tile for NQ tiles of 16 columns: lane li is a column.  SN: V scales of a
 // slot (NF4 heads of two blocks have one each).
 template <int HD, int NQ, int SN>
@@ -218,9 +227,13 @@ struct State {
     v4f o[NQ][HD / 16];  // output tile b of column li: sums of 2^(s - m) V, times kLift (block 1: and 2^(m - m1))
     float m[NQ], l[NQ];  // reference (a whole number; -FLT_MAX: no score yet); this lane's share of the sum of 2^(s - m)
     float m1[SN > 1 ? NQ : 1], up1[SN > 1 ? NQ : 1];  // block 1's own reference, and 2^(m - m1) kLift
-    bool far;            // some column of the wave has a reference beyond kFar
+    // Columns whose reference is far (is_far): it is m + beside, and block 1's m + m1 (up1: 2^(beside - m1) kLift).  In LDS, for
+    // such columns alone; far: the wave has met one.
+    float *beside;
+    bool far;
 
-    __device__ __forceinline__ void clear() {
+    __device__ __forceinline__ void clear(float *lds) {
+        beside = lds;
         far = false;
 #pragma unroll
         for (int a = 0; a < NQ; a++) {
@@ -234,12 +247,12 @@ struct State {
             for (int b = 0; b < HD / 16; b++) o[a][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
-    // What takes output tile b of column tile a back to sums of 2^(s - m) V.
+    // The wave's lane's place of column tile a.
+    __device__ __forceinline__ float &beside_of(int a) const { return beside[16 * a + own_column()]; }
+    // What takes output tiles of 64-block b of column tile a back to sums of 2^(s - m) V; block 0's times kLift, its sum.
     __device__ __forceinline__ float back(int a, int b) const {
-        if constexpr (SN > 1) {
-            if (b >= 4) return __builtin_amdgcn_exp2f(m1[a] - m[a]) * (1.0f / kLift);
-        }
-        return 1.0f / kLift;
+        if (SN > 1 && b) return __builtin_amdgcn_exp2f(far && is_far(m[a]) ? m1[SN > 1 ? a : 0] : m1[SN > 1 ? a : 0] - m[a]) * (1.0f / kLift);
+        return far && is_far(m[a]) ? __builtin_amdgcn_exp2f(beside_of(a)) * (1.0f / kLift) : 1.0f / kLift;
     }
 };
 
@@ -267,6 +280,11 @@ __device__ __forceinline__ float column_max(float v) {  // over a column's four 
     return fmaxf(v, xor_lane(v, 32));
 }
 
+__device__ __forceinline__ bool column_any(bool b) {
+    const uint64_t lanes = __ballot(b), two = lanes | lanes >> 32;
+    return ((uint32_t)two | (uint32_t)two >> 16) >> own_column() & 1u;
+}
+
 // The largest of three: fmaxf's result, without the instructions that quiet each operand first.
 __device__ __forceinline__ float max3(float a, float b, float c) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -279,6 +297,54 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ float max8(const float (&t)[2][4]) {
     return max3(max3(t[0][0], t[0][1], t[0][2]), max3(t[0][3], t[1][0], t[1][1]), fmaxf(t[1][2], t[1][3]));
+}
+
+// What weights() does to the references of column tile a where a column of the wave is far, in it or in another.  mn: the
+// column's new reference but for that; u1: log2 of its block 1's largest product, asks1: whether the column asks for a change by that.
+template <int HD, int NQ, int SN>
+__device__ __forceinline__ void far_references(State<HD, NQ, SN> &S, int a, const float (&t)[2][4], float qas, const float (&vs)[2][4][SN],
+                                               float top, float u1, bool asks1, float mn, float to_lift, float &down, float &down1) {
+    const bool was = is_far(S.m[a]);
+    const float best = column_max(top * qas);
+    // (near kFar the scale may ask for a far reference where the score is none)
+    const float at = fmaxf(S.m[a], fabsf(best) >= kFar ? best : copysignf(kFar, mn));
+    const bool now = is_far(mn) && is_far(at);
+    mn = now ? at : mn;
+    float v[SN];
+    // (as if not known: the scales' logarithms, kept from the caller's loop, would not fit the registers)
+    uint32_t magnitude = 0x7FFFFFFFu;
+    asm volatile("" : "+s"(magnitude));
+#pragma unroll
+    for (int k = 0; k < SN; k++) {
+        v[k] = top * qas - mn + (kLog2Lift - 100.0f);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                v[k] = fmaxf(v[k], (t[j][i] * qas - mn) + log2_bits(__float_as_uint(vs[j][i][k]) & magnitude, to_lift));
+    }
+    if constexpr (SN > 1) v[0] = fmaxf(v[0], v[1] - kApart);
+    // the blocks' references, counted from m: before, and after
+    const float shift = S.m[a] - mn;
+    const float at0 = (was ? S.beside_of(a) : 0.0f) + shift, most0 = column_max(v[0]);
+    const float to0 = !now ? 0.0f : most0 > at0 + kLimit ? ceilf(most0) - kTop : at0;
+    down = at0 == to0 ? 1.0f : __builtin_amdgcn_exp2f(at0 - to0);
+    down1 = down;
+    if constexpr (SN > 1) {
+        const float at1 = (was ? S.m1[a] : S.m1[a] - S.m[a]) + shift, most1 = column_max(v[SN - 1]);
+        float to1;
+        if (now) {
+            to1 = fmaxf(most1 > at1 + kLimit ? ceilf(most1) - kTop : at1, to0 - 120.0f);
+        } else {
+            const float m1 = was ? S.m[a] + S.m1[a] : S.m1[a], most = column_max(u1);
+            to1 = fmaxf((was || asks1) && most > m1 + kLimit ? ceilf(most) - kTop : m1, mn - 120.0f) - mn;
+        }
+        down1 = at1 == to1 ? 1.0f : __builtin_amdgcn_exp2f(at1 - to1);
+        S.m1[a] = now ? to1 : mn + to1;
+        S.up1[a] = __builtin_amdgcn_exp2f(to0 - to1) * kLift;
+    }
+    S.m[a] = mn;
+    if (now) S.beside_of(a) = to0;
 }
 
 // Weights of a tile from its scores: t = dots * K scales of positions 16 j + 4 lg + i of the columns
@@ -309,11 +375,7 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
         news |= fmaf(top[a], qas[a], lv[0]) > S.m[a];
         if constexpr (SN > 1) news |= fmaf(top[a], qas[a], lv[1]) > S.m1[a];
     }
-    if (S.far) {  // (a step of the score may be more than the limit)
-#pragma unroll
-        for (int a = 0; a < NQ; a++) news |= fabsf(S.m[a]) >= kFar && top[a] * qas[a] > S.m[a];
-    }
-    if (__any(news)) {
+    if (S.far || __any(news)) {
 #pragma unroll
         for (int a = 0; a < NQ; a++) {
             float u[SN];
@@ -327,30 +389,29 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                         u[k] = fmaxf(u[k], fmaf(t[a][j][i], qas[a], log2_bits(__float_as_uint(vs[j][i][k]) & 0x7FFFFFFFu, kToLift)));
             }
             if constexpr (SN > 1) u[0] = fmaxf(u[0], u[1] - kApart);
+            // (only where the column asks for it by itself: another one's scores change nothing)
+            const bool asks = column_any(fmaf(top[a], qas[a], lv[0]) > S.m[a]) || is_far(S.m[a]);
+            const bool asks1 = SN > 1 && column_any(fmaf(top[a], qas[a], lv[SN - 1]) > S.m1[SN > 1 ? a : 0]);
             const float most = column_max(u[0]);
-            float mn = most > S.m[a] + kLimit ? ceilf(most) - kTop : S.m[a];
-            if (fabsf(most) >= kFar) {
-                const float rounded = column_max(top[a] * qas[a]);
-                float scale = lv[0];
-                if constexpr (SN > 1) scale = fmaxf(scale, lv[1]);
-                scale = fminf(column_max(scale) + kLimit, 100.0f);  // log2 of the largest V scale times kLift
-                const float with = rounded + scale;
-                mn = fmaxf(fabsf((with - rounded) - scale) <= 4.0f ? with : rounded, S.m[a]);
+            float mn = asks && most > S.m[a] + kLimit ? ceilf(most) - kTop : S.m[a];
+            S.far |= __any(is_far(mn)) != 0;
+            float down, down1;
+            if (__builtin_expect(!S.far, 1)) {
+                down = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
+                down1 = down;
+                if constexpr (SN > 1) {
+                    // (no lower than 2^-120 of the first block's: 2^(m - m1) stays finite)
+                    const float most1 = column_max(u[SN - 1]);
+                    const float m1 = fmaxf(asks1 && most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - 120.0f);
+                    down1 = m1 == S.m1[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m1[a] - m1);
+                    S.m1[a] = m1;
+                    S.up1[a] = __builtin_amdgcn_exp2f(mn - m1) * kLift;
+                }
+                S.m[a] = mn;
+            } else {
+                far_references(S, a, t[a], qas[a], vs, top[a], u[SN - 1], asks1, mn, kToLift, down, down1);
             }
-            S.far |= __any(fabsf(mn) >= kFar && mn > -FLT_MAX) != 0;
-            const float down = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
-            float down1 = down;
-            S.m[a] = mn;
             S.l[a] *= down;
-            if constexpr (SN > 1) {
-                // (no lower than 2^-120 of the first block's: 2^(m - m1) stays finite)
-                const float most1 = column_max(u[SN - 1]);
-                float m1 = fmaxf(most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - 120.0f);
-                if (fabsf(mn) >= kFar) m1 = mn;
-                down1 = m1 == S.m1[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m1[a] - m1);
-                S.m1[a] = m1;
-                S.up1[a] = __builtin_amdgcn_exp2f(mn - m1) * kLift;
-            }
 #pragma unroll
             for (int b = 0; b < HD / 16; b++) S.o[a][b] = S.o[a][b] * (SN > 1 && b >= 4 ? down1 : down);
         }
@@ -361,15 +422,15 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
         by[a] = qas[a];
         from[a] = S.m[a];
     }
-    if (S.far) {
+    if (__builtin_expect(S.far, 0)) {
 #pragma unroll
         for (int a = 0; a < NQ; a++) {
-            const bool far = fabsf(S.m[a]) >= kFar;  // (the other columns: t * 1 - 0)
-            const float by0 = far ? qas[a] : 1.0f, from0 = far ? S.m[a] : 0.0f;
+            const bool far = is_far(S.m[a]);  // (the other columns: t * 1 - 0)
+            const float by0 = far ? qas[a] : 1.0f, from0 = far ? S.m[a] : 0.0f, beside = far ? S.beside_of(a) : 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) t[a][j][i] = t[a][j][i] * by0 - from0;
+                for (int i = 0; i < 4; i++) t[a][j][i] = (t[a][j][i] * by0 - from0) - beside;
             by[a] = far ? 1.0f : qas[a];
             from[a] = far ? 0.0f : S.m[a];
         }
@@ -560,7 +621,8 @@ __device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const S
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
         if (16 * a >= I.n) break;
-        float l = S.l[a];
+        const float back[2] = {S.back(a, 0), S.back(a, SN - 1)};
+        float l = S.l[a] * (back[0] * kLift);
         l += xor_lane(l, 16);
         l += xor_lane(l, 32);
         if (lg == 0) {
@@ -570,7 +632,7 @@ __device__ __forceinline__ void join(const ColumnArgs &A, const Item &I, const S
 #pragma unroll
         for (int b = 0; b < HD / 16; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) J.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * S.back(a, b);
+            for (int i = 0; i < 4; i++) J.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * back[b >= 4];
         __syncthreads();
         // column, sixteenth of a 64-block's dimensions, and the first such block (four waves take one at a time)
         const int x = (int)(tid >> 4 & 15u), sl = (int)(tid & 15u), d0 = 64 * (wave >> 2);
@@ -622,6 +684,7 @@ template <int HD, int NQ, int WAVES = kWaves>
 struct Shared {
     Queries<HD, 16 * NQ> q;
     Join<HD, WAVES> j;
+    float beside[WAVES][16 * NQ];
 };
 // hide(i, t, vs): takes out of tile i what a column does not see (Hidden); NoMask: columns see all positions of the item.
 struct NoMask {};
@@ -669,7 +732,7 @@ __device__ __forceinline__ void attend(const ColumnArgs &A, const Item &I, const
         if constexpr (!std::is_same<Hide, NoMask>::value) above_zero(qas[a], qb[a]);
     }
     State<HD, NQ, SN> S;
-    S.clear();
+    S.clear(sh.beside[wave]);
     for (int i = wave; i < tiles; i += WAVES) {
         const int left = i < first ? I.len[0] - kTile * i : I.len[1] - kTile * (i - first);
         float s[NQ][2][4], vs[2][4][SN];

@@ -112,7 +112,7 @@ struct Seen {
 
 // Few columns: an item is (row, KV head, part, 16 NQ columns).
 template <int HD, int BITS, int NQ, bool WHOLE, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void tokens_few_kernel(const TokensArgs A) {
+__global__ __launch_bounds__(64 * WAVES, HD * NQ <= 128 ? 3 : 2) void tokens_few_kernel(const TokensArgs A) {
     __shared__ Shared<HD, NQ, WAVES> sh;
     const uint32_t lane = threadIdx.x & 63u;
     const int unit = (int)blockIdx.x % A.units, cg = A.cgs - 1 - (int)blockIdx.x / A.units;
@@ -254,6 +254,7 @@ struct BlockShared {
         Queries<HD, 16> q[kBlockWaves];
         float o[kBlockWaves][16][HD + 4];
     };
+    float beside[kBlockWaves][16];
     __device__ BlockShared() {}
 };
 
@@ -317,7 +318,7 @@ __device__ __forceinline__ void block_item(const TokensArgs &A, int item, int pa
         above_zero(qas[a], qb[a]);
     }
     State<HD, NQ, SN> S;
-    S.clear();
+    S.clear(sh.beside[wave]);
     __syncthreads();
     const int tiles = none ? 0 : (end - t0 + T::P - 1) / T::P;
     if (!none) {
@@ -381,13 +382,14 @@ __device__ __forceinline__ void block_item(const TokensArgs &A, int item, int pa
     // outputs: 16 columns of every wave at a time, four of them by sixteen lanes each
 #pragma unroll
     for (int a = 0; a < NQ; a++) {
-        float l = S.l[a];
+        const float back[2] = {S.back(a, 0), S.back(a, SN - 1)};
+        float l = S.l[a] * (back[0] * kLift);
         l += xor_lane(l, 16);
         l += xor_lane(l, 32);
 #pragma unroll
         for (int b = 0; b < DB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) sh.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * S.back(a, b);
+            for (int i = 0; i < 4; i++) sh.o[wave][li][out_dim<HD, BITS>(b, 4 * (int)lg + i)] = S.o[a][b][i] * back[b >= 4];
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 4; k++) {

@@ -845,3 +845,92 @@ def test_contexts_on_two_streams_do_not_meet(bits, hd, nq, nkv, ntok, start):
             assert torch.equal(o, run[6][0])
     for c in ctxs:
         c.close()
+
+
+# ---------------------------------------------------------------- scores past whole numbers, with V scales apart
+def exponents(bits, rng, shape, lo, hi):
+    """Scales 2^lo .. 2^hi of the cache's type."""
+    f = np.exp2(rng.uniform(lo, hi, shape)).astype(np.float32)
+    return f if bits == 8 else (f.view(np.uint32) >> 16).astype(np.uint16)
+
+
+def check_best(got, bits, q, cache, pos, counts, sees, nq, nkv, hd, scale, length):
+    """Where a token's best visible position leads by more than rounding leaves open, and by enough for the others to
+    weigh nothing next to their V scales, its output is that position's V.  A score is off by 5 roundings of the largest.
+    Returns the share of (token, head) that are told apart."""
+    import oracle as O
+    batch, ntok = q.shape[:2]
+    g, told, every = nq // nkv, 0, 0
+    for r in range(batch):
+        n = int(max(0, min(ntok, counts[r])))
+        end = int(max(0, min(length, pos[r] + n)))
+        if n == 0 or end == 0:
+            continue
+        see = R.visible(ntok, int(pos[r]), n, end, None if sees is None else [int(x) for x in sees[r]])[:n]
+        see_h, rows = np.repeat(see, g, 0), np.repeat(see.any(1), g)
+        for h in range(nkv):
+            k, v = (B.values(bits, cache[i][r, h, :end], cache[i + 1][r, h, :end]) for i in (0, 2))
+            vs = cache[3][r, h, :end] if bits == 8 else B.bf16(cache[3][r, h, :end])
+            lv = np.log2(vs.astype(np.float64)).reshape(end, -1)
+            heads = q[r, :n, h * g:(h + 1) * g].reshape(n * g, hd)
+            x = np.stack([c.astype(np.float64) * np.float64(s) for c, s in (O.kv_quant_head(a) for a in heads)])
+            z = np.where(see_h, (x @ k.T) * float(np.float32(scale)), -np.inf)
+            best = z.argmax(1)
+            size = np.abs(np.where(see_h, z, 0)).max(1, keepdims=True)
+            apart = (lv[None] - lv[best][:, None]).max(-1)
+            gap = z[np.arange(n * g), best][:, None] - z - 10 * R.U * size - np.log(2) * (45 + np.maximum(apart, 0))
+            gap[np.arange(n * g), best] = np.inf
+            ok = (gap.min(1) >= 0) & rows
+            out = got[r, :n, h * g:(h + 1) * g].reshape(n * g, hd)
+            assert np.isfinite(out).all()
+            want = B.unrotate(v[best])
+            # pieces of 2^-21, a sum of one term, the rotation's 8 roundings, all others together 2^-30
+            bound = (2.0 ** -21 + 8 * R.U + 2.0 ** -30) * B.block_sums(np.abs(v[best])) / 8
+            off = np.abs(out - want) > bound
+            assert not off[ok].any(), (r, h, np.argwhere(off & ok[:, None])[:4], out[ok][off[ok]][:4], want[ok][off[ok]][:4])
+            told += int(ok.sum())
+            every += int(rows.sum())
+    return told / max(1, every)
+
+
+# few columns of one tile and of two, in one part and in several; many columns, whole and cut; one token
+FAR = [(3, 9, 3, 5, 300, 0, True), (1, 8, 1, 3, 700, 0, False), (2, 4, 2, 64, 100, 0, True), (1, 64, 8, 40, 30, 0, False), (2, 32, 4, 64, 700, 20000, True),
+       (3, 96, 48, 130, 70, 0, False), (3, 16, 2, 300, 10, 12000, False), (7, 1, 1, 1, 200, 0, False)]
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch,nq,nkv,ntok,start,room,with_tree", FAR)
+@pytest.mark.parametrize("size", [1.1e7, 3e7, 1e9, 1e13])
+def test_attention_of_far_scores_and_scales_far_apart(gpu_ctx, bits, hd, batch, nq, nkv, ntok, start, room, with_tree, size):
+    """Scores of 1.1e7 (where steps pass one) to 1e13 and V scales 2^-30 .. 2^30: a large scale of small weight, or of a
+    position that the token does not see, takes nothing from the best position's V."""
+    print(f"far bits={bits} hd={hd} heads={nq}/{nkv} batch={batch} ntok={ntok} start={start} room={room} size={size}", flush=True)
+    rng = np.random.default_rng(hd + ntok + nq)
+    q, cache, pos, counts, sees, cap = case(rng, bits, batch, ntok, nq, nkv, hd, start, False, with_tree, spare=3 + room)
+    shape = cache[3].shape
+    cache[3][:] = exponents(bits, rng, shape, -30, 30)
+    for r in range(batch):  # what lies behind a row's block: any scale
+        cache[1][r, :, pos[r] + ntok:] = exponents(bits, rng, cache[1][r, :, pos[r] + ntok:].shape, -60, 60)
+        cache[3][r, :, pos[r] + ntok:] = exponents(bits, rng, cache[3][r, :, pos[r] + ntok:].shape, 60, 100)
+    # |q . k| of these is about sqrt(hd) * 2 at one standard deviation
+    scale = np.float32(size / (4 * 2 * hd ** 0.5))
+    got = attend(gpu_ctx, bits, q, cache, pos, counts, sees, nq, nkv, hd, float(scale), cap)
+    assert check_best(got, bits, q, cache, pos, np.full(batch, ntok), sees, nq, nkv, hd, scale, cap) >= 0.6
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("nq,nkv,ntok,start,with_tree", [(4, 2, 12, 60, True), (8, 1, 40, 20, False), (8, 8, 200, 0, False), (48, 1, 300, 100, False)])
+def test_attention_of_a_far_query_leaves_the_others_bits(gpu_ctx, bits, hd, nq, nkv, ntok, start, with_tree):
+    """Heads whose scores are far, between heads whose scores are not: the others' outputs keep their bits."""
+    rng = np.random.default_rng(hd + ntok)
+    q, cache, pos, counts, sees, cap = case(rng, bits, 2, ntok, nq, nkv, hd, start, False, with_tree)
+    cache[3][:] = exponents(bits, rng, cache[3].shape, -12, 12)
+    for r in range(2):
+        cache[3][r, :, pos[r] + ntok:] = np.nan if bits == 8 else 0x7FC0
+    far = rng.random((2, ntok, nq)) < 0.2
+    both = np.where(far[..., None], np.float32(2.0 ** 26) * q, q)
+    plain = attend(gpu_ctx, bits, q, cache, pos, counts, sees, nq, nkv, hd, 0.17, cap)
+    got = attend(gpu_ctx, bits, both, cache, pos, counts, sees, nq, nkv, hd, 0.17, cap)
+    assert got[~far].tobytes() == plain[~far].tobytes()
+    assert np.isfinite(got).all()

@@ -775,3 +775,47 @@ def test_the_most_rows(gpu_ctx):
     chosen = cand[o[2].long(), o[1].long()]  # and the token and row named have that score
     assert (chosen - want).abs().max() <= 2.0 ** -18
     assert (o[2] // beams == torch.arange(n_seq, device="cuda")[:, None]).all()
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
+@pytest.mark.parametrize("beams,prefix,tail", [(3, 60, 9), (8, 1500, 40), (64, 900, 300)])
+@pytest.mark.parametrize("size", [1.1e7, 3e7, 1e9, 1e13])
+def test_attention_of_far_scores_with_v_scales_far_apart(gpu_ctx, bits, hd, beams, prefix, tail, size):
+    """Scores of 1.1e7 (where their steps pass one) to 1e13 and V scales 2^-30 .. 2^30: a large scale of small weight takes
+    nothing from the best position's V."""
+    nq, nkv = 8, 2
+    g = nq // nkv
+    rng = np.random.default_rng(hd + bits + prefix)
+    pre, tl = R.new_cache(bits, 1, nkv, prefix, hd, rng), R.new_cache(bits, beams, nkv, tail, hd, rng)
+    for c in (pre, tl):
+        f = np.exp2(rng.uniform(-30, 30, c[3].shape)).astype(np.float32)
+        c[3][:] = f if bits == 8 else (f.view(np.uint32) >> 16).astype(np.uint16)
+    q = rng.standard_normal((beams, nq, hd)).astype(np.float32)
+    scale = np.float32(size / (4 * 2 * hd ** 0.5))  # (|q . k| is about 2 sqrt(hd) at one standard deviation)
+    out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+    _, p = rows_of(pre, prefix)
+    _, t = rows_of(tl, tail)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(bits, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, t, float(scale), out, ws)
+    gpu_ctx.sync()
+    got = out.cpu().numpy()
+    assert np.isfinite(got).all()
+    import oracle as O
+    told = 0
+    for r in range(beams):
+        for h in range(nkv):
+            k, v, s = (np.concatenate((f(pre)[0, h], f(tl)[r, h])) for f in (
+                lambda c: R.values(bits, c[0], c[1]), lambda c: R.values(bits, c[2], c[3]),
+                lambda c: np.log2((c[3] if bits == 8 else R.bf16(c[3])).astype(np.float64)).reshape(c[3].shape[:3] + (-1,))))
+            x = np.stack([c.astype(np.float64) * np.float64(e) for c, e in (O.kv_quant_head(a) for a in q[r, h * g:(h + 1) * g])])
+            z = (x @ k.T) * float(scale)
+            best = z.argmax(1)
+            # a score is off by 5 roundings of the largest; the others weigh 2^-45 at most, next to their V scales
+            gap = z.max(1, keepdims=True) - z - 10 * R.U * np.abs(z).max(1, keepdims=True)
+            gap -= np.log(2) * (45 + np.maximum((s[None] - s[best][:, None]).max(-1), 0))
+            gap[np.arange(g), best] = np.inf
+            ok = gap.min(1) >= 0
+            bound = (2.0 ** -21 + 8 * R.U + 2.0 ** -30) * R.block_sums(np.abs(v[best])) / 8
+            assert (np.abs(got[r, h * g:(h + 1) * g] - R.unrotate(v[best])) <= bound)[ok].all(), (r, h)
+            told += int(ok.sum())
+    assert told >= 0.6 * beams * nq
