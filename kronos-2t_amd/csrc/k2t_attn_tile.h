@@ -33,7 +33,8 @@ constexpr float kTop = 9.0f, kLimit = 15.0f, kLift = 256.0f, kLog2Lift = 8.0f;
 // Scales below 2^-100 count as that much in the reference, so that a weight is at most 2^107 and a sum of
 // 2^16 of them finite (from 2^120 on, half of the largest scale that a head has, kLift overflows); an NF4 head's second block has a reference of its own (its scales may be of another
 // size), but a weight refers to the first, which therefore counts as 2^-60 of the second at least.
-constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f;
+// Nor is that block's reference lower than 2^-119 of the first one's: up1, 2^(m - m1) times kLift, stays finite.
+constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f, kWidest = 119.0f;
 // Scores so far from zero that fp32 does not tell whole numbers apart.  An exact product less the reference would
 // be up to half a step of the score off then, which may be any power of two: in a column whose reference is so far, scores
 // are rounded before the reference, the largest rounded one, is taken off.  What V scales ask for cannot be part of such a
@@ -334,10 +335,10 @@ __device__ __forceinline__ void far_references(State<HD, NQ, SN> &S, int a, cons
         const float at1 = (was ? S.m1[a] : S.m1[a] - S.m[a]) + shift, most1 = column_max(v[SN - 1]);
         float to1;
         if (now) {
-            to1 = fmaxf(most1 > at1 + kLimit ? ceilf(most1) - kTop : at1, to0 - 120.0f);
+            to1 = fmaxf(most1 > at1 + kLimit ? ceilf(most1) - kTop : at1, to0 - kWidest);
         } else {
             const float m1 = was ? S.m[a] + S.m1[a] : S.m1[a], most = column_max(u1);
-            to1 = fmaxf((was || asks1) && most > m1 + kLimit ? ceilf(most) - kTop : m1, mn - 120.0f) - mn;
+            to1 = fmaxf((was || asks1) && most > m1 + kLimit ? ceilf(most) - kTop : m1, mn - kWidest) - mn;
         }
         down1 = at1 == to1 ? 1.0f : __builtin_amdgcn_exp2f(at1 - to1);
         S.m1[a] = now ? to1 : mn + to1;
@@ -400,9 +401,8 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                 down = mn == S.m[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m[a] - mn);
                 down1 = down;
                 if constexpr (SN > 1) {
-                    // (no lower than 2^-120 of the first block's: 2^(m - m1) stays finite)
                     const float most1 = column_max(u[SN - 1]);
-                    const float m1 = fmaxf(asks1 && most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - 120.0f);
+                    const float m1 = fmaxf(asks1 && most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - kWidest);
                     down1 = m1 == S.m1[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m1[a] - m1);
                     S.m1[a] = m1;
                     S.up1[a] = __builtin_amdgcn_exp2f(mn - m1) * kLift;

@@ -934,3 +934,16 @@ def test_attention_of_a_far_query_leaves_the_others_bits(gpu_ctx, bits, hd, nq, 
     got = attend(gpu_ctx, bits, both, cache, pos, counts, sees, nq, nkv, hd, 0.17, cap)
     assert got[~far].tobytes() == plain[~far].tobytes()
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("nq,nkv,ntok,start", [(2, 1, 3, 40), (8, 2, 40, 300), (32, 8, 200, 100), (64, 32, 130, 0)])
+@pytest.mark.parametrize("first,second", [(2.0 ** 20, 0.0), (2.0 ** 60, 0.0), (0.0, 2.0 ** 60), (2.0 ** 25, 2.0 ** -80), (0.0, 0.0)])
+def test_attention_of_nf4_blocks_of_scales_far_apart(gpu_ctx, nq, nkv, ntok, start, first, second):
+    """The two V blocks of a head of 128: one of zeros, or one 2^105 times the other."""
+    rng = np.random.default_rng(ntok)
+    q, cache, pos, counts, sees, cap = case(rng, 4, 2, ntok, nq, nkv, 128, start, False, False)
+    for b, size in ((0, first), (1, second)):
+        f = (rng.uniform(1, 2, cache[3].shape[:3]) * size).astype(np.float32)
+        cache[3][..., b] = (f.view(np.uint32) >> 16).astype(np.uint16)
+    want, bound = attention_on_gpu(4, q, cache, pos, np.full(2, ntok), sees, nq, nkv, 128, 0.17, cap)
+    check(attend(gpu_ctx, 4, q, cache, pos, counts, sees, nq, nkv, 128, 0.17, cap), want, bound)

@@ -819,3 +819,25 @@ def test_attention_of_far_scores_with_v_scales_far_apart(gpu_ctx, bits, hd, beam
             assert (np.abs(got[r, h * g:(h + 1) * g] - R.unrotate(v[best])) <= bound)[ok].all(), (r, h)
             told += int(ok.sum())
     assert told >= 0.6 * beams * nq
+
+
+@pytest.mark.parametrize("beams,prefix,tail", [(3, 60, 9), (8, 1500, 40)])
+@pytest.mark.parametrize("first,second", [(2.0 ** 20, 0.0), (2.0 ** 60, 0.0), (0.0, 2.0 ** 60), (2.0 ** 25, 2.0 ** -80), (0.0, 0.0)])
+def test_attention_of_nf4_blocks_of_scales_far_apart(gpu_ctx, beams, prefix, tail, first, second):
+    """The two V blocks of a head of 128: one of zeros, or one 2^105 times the other."""
+    nq, nkv, hd = 8, 2, 128
+    rng = np.random.default_rng(prefix)
+    pre, tl = R.new_cache(4, 1, nkv, prefix, hd, rng), R.new_cache(4, beams, nkv, tail, hd, rng)
+    for c in (pre, tl):
+        for b, size in ((0, first), (1, second)):
+            f = (rng.uniform(1, 2, c[3].shape[:3]) * size).astype(np.float32)
+            c[3][..., b] = (f.view(np.uint32) >> 16).astype(np.uint16)
+    q = rng.standard_normal((beams, nq, hd)).astype(np.float32)
+    out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+    _, p = rows_of(pre, prefix)
+    _, t = rows_of(tl, tail)
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, prefix, tail))
+    gpu_ctx.attn_shared(4, dev(q.reshape(beams, -1)), nq * hd, 1, beams, nq, nkv, hd, p, t, 0.17, out, ws)
+    gpu_ctx.sync()
+    want, bound = R.attention(4, q, pre, tl, [prefix], [tail] * beams, beams, nq, nkv, hd, 0.17)
+    assert (np.abs(out.cpu().numpy() - want) <= bound).all()
