@@ -473,9 +473,9 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
 
 // Takes out of a tile what its columns do not see: bit 4 j + i of counts(a), the lane's column of tile a, is set for what it
 // sees.  A score of -inf weighs nothing (the columns' qas are positive).  What is not seen may have any V scale, and a
-// weight of zero times NaN is NaN: a scale that is not finite counts as zero, and the columns that do see its position get
-// a NaN score, so that their outputs are NaN.
-template <int NQ, int SN, typename Counts>
+// weight of zero times NaN is NaN: a scale that is not finite, or would not be once times kLift, counts as zero, and the
+// columns that do see its position get a NaN score, so that their outputs are NaN.
+template <bool LIFTED, int NQ, int SN, typename Counts>
 __device__ __forceinline__ void hide_tile(float (&t)[NQ][2][4], float (&vs)[2][4][SN], const Counts &counts) {
     bool bad[2][4];
 #pragma unroll
@@ -485,7 +485,7 @@ __device__ __forceinline__ void hide_tile(float (&t)[NQ][2][4], float (&vs)[2][4
             bad[j][i] = false;
 #pragma unroll
             for (int k = 0; k < SN; k++) {
-                const bool b = !(fabsf(vs[j][i][k]) <= FLT_MAX);
+                const bool b = !(fabsf(vs[j][i][k]) <= FLT_MAX / (LIFTED ? 1.0f : kLift));
                 vs[j][i][k] = b ? 0.0f : vs[j][i][k];
                 bad[j][i] |= b;
             }

@@ -144,7 +144,7 @@ __global__ __launch_bounds__(64 * WAVES, HD * NQ <= 128 ? 3 : 2) void tokens_few
     seen.lg = (int)(lane >> 4);
     const auto hide = [&](int i, auto &t, auto &vs) {
         seen.p0 = t0 + kTile * i;
-        if (!seen.whole()) hide_tile(t, vs, [&](int a) { return seen.counts(a); });
+        if (!seen.whole()) hide_tile<false>(t, vs, [&](int a) { return seen.counts(a); });
     };
     const auto any = [&](int c) {
         const Sees s = sees_of(A, R, row, (int)column(A, c).row);
@@ -359,7 +359,7 @@ __device__ __forceinline__ void block_item(const TokensArgs &A, int item, int pa
                 for (int a = 0; a < NQ; a++) scores<BITS>(kf, qb[a], [&](int e, int b) { return ks[e][SN > 1 ? b : 0]; }, t[a][j]);
             }
             uint32_t ph[NQ][SN][4], pl[NQ][SN][4];
-            if (!seen.whole()) hide_tile(t, vs, [&](int a) { return seen.counts(a); });
+            if (!seen.whole()) hide_tile<true>(t, vs, [&](int a) { return seen.counts(a); });
             weights<HD, NQ, SN, true>(S, t, qas, vs, kTile, lg, ph, pl);
 #pragma unroll
             for (int g = 0; g < DB / 4; g++) {

@@ -947,3 +947,22 @@ def test_attention_of_nf4_blocks_of_scales_far_apart(gpu_ctx, nq, nkv, ntok, sta
         cache[3][..., b] = (f.view(np.uint32) >> 16).astype(np.uint16)
     want, bound = attention_on_gpu(4, q, cache, pos, np.full(2, ntok), sees, nq, nkv, 128, 0.17, cap)
     check(attend(gpu_ctx, 4, q, cache, pos, counts, sees, nq, nkv, 128, 0.17, cap), want, bound)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd,nq,nkv,ntok,start", [(64, 2, 2, 12, 50), (128, 8, 2, 40, 200), (128, 16, 2, 64, 1500), (64, 40, 8, 150, 0)])
+def test_attention_beside_the_largest_scales(gpu_ctx, bits, hd, nq, nkv, ntok, start):
+    """A token's V scale, or K scale, of up to the largest finite number reaches no token that does not see it."""
+    rng = np.random.default_rng(ntok + hd)
+    q, cache, pos, counts, sees, cap = case(rng, bits, 2, ntok, nq, nkv, hd, start, False, ntok <= 64)
+    clean, bound = attention_on_gpu(bits, q, cache, pos, np.full(2, ntok), sees, nq, nkv, hd, 0.2, cap)
+    bad = ntok // 2
+    see = R.visible(ntok, int(pos[0]), ntok, cap, None if sees is None else [int(x) for x in sees[0]])[:, pos[0] + bad]
+    for which in (1, 3):
+        for size in (2.0 ** 100, 2.0 ** 119, 2.0 ** 120.5, 3.3e38):
+            c = [a.copy() for a in cache]
+            f = np.float32(size)
+            c[which][0, :, pos[0] + bad] = f if bits == 8 else f.view(np.uint32) >> 16
+            got = attend(gpu_ctx, bits, q, c, pos, counts, sees, nq, nkv, hd, 0.2, cap)
+            assert (np.abs(got - clean)[1] <= bound[1]).all()
+            assert (np.abs(got - clean)[0, ~see] <= bound[0, ~see]).all(), (which, size)
