@@ -2,7 +2,7 @@
 // cache's K and V (k2t_attn_shared.hip, k2t_attn_tokens.hip): tiles of 32 positions, the running softmax, queries, joins.
 //
 // Scores S^T = K Q^T by the int8 MFMA, whose sums are exact, and outputs O^T = V^T W^T by the f16 MFMA. V's codes are
-// exact in f16; a weight times its V scale is split into two f16 pieces that hold 21 bits of it (24 in an fp32 product,
+// exact in f16; a weight times its V scale is split into two f16 pieces that hold it to 2^-23 (an fp32 product to 2^-24,
 // at several times the MFMAs). f16's range decides what the running softmax refers to: not a column's largest score, but
 // its largest product of weight and V scale, so that a large scale of small weight takes no bits from the others.
 // References are raised lazily, sums and outputs are fp32 and joined in a fixed order.
@@ -200,9 +200,14 @@ __device__ __forceinline__ uint32_t v_word(uint32_t w, const Nf4 &c) {
     return nf4_xlut((w & 0x0F0Fu) | ((w & 0xF0F0u) << 12), c.t0, c.t1, c.u0, c.u1);
 }
 
-// Two floats as f16 pairs hi + lo: x = hi + lo within 2^-21 |x|.
+// Two floats as f16 pairs hi + lo, each rounded to nearest: x = hi + lo within 2^-23 |x| (what is left of x has 2^-11 of it at
+// most, and a sign).  Cut off instead, pieces were off by up to 2^-21.4, always towards zero, which the sum that
+// outputs are divided by is not.
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    const auto pack = [](float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2h)); };
+    hi = pack(x0, x1);
     float r0, r1;  // x - hi, exact: one mixed-precision fma each (the compiler converts and subtracts)
 #if defined(__HIP_DEVICE_COMPILE__)
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(x0));
@@ -211,7 +216,7 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_
     r0 = x0;
     r1 = x1;
 #endif
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+    lo = pack(r0, r1);
 }
 
 // The lane's column, counted anew: as a value kept over the loop it would cost a register where none is left.

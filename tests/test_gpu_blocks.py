@@ -966,3 +966,24 @@ def test_attention_beside_the_largest_scales(gpu_ctx, bits, hd, nq, nkv, ntok, s
             got = attend(gpu_ctx, bits, q, c, pos, counts, sees, nq, nkv, hd, 0.2, cap)
             assert (np.abs(got - clean)[1] <= bound[1]).all()
             assert (np.abs(got - clean)[0, ~see] <= bound[0, ~see]).all(), (which, size)
+
+
+@pytest.mark.parametrize("hd,nq,nkv,batch", [(64, 2, 2, 1), (128, 8, 2, 2), (64, 32, 32, 12), (128, 48, 24, 16)])
+@pytest.mark.parametrize("room", [0, 3000])
+def test_attention_of_one_position_rounds_its_v_to_nearest(gpu_ctx, hd, nq, nkv, batch, room):
+    """Zero queries, one visible position, and a V head of a single code 1: what comes out is the V scale over 8, every
+    step exact but for the scale's two pieces, 2^-23 of it, and their sum, a step at most."""
+    rng = np.random.default_rng(hd + nq)
+    ntok = 64
+    cache = B.new_cache(8, batch, nkv, ntok + room, hd, rng)
+    cache[2][:] = 0
+    at = rng.integers(0, hd, cache[3].shape)
+    np.put_along_axis(cache[2], at[..., None], 1, -1)
+    cache[3][:] = rng.uniform(2.0 ** -6, 2.0 ** -3, cache[3].shape)
+    sees = np.tile(np.uint64(1) << np.arange(ntok, dtype=np.uint64), (batch, 1))
+    got = attend(gpu_ctx, 8, np.zeros((batch, ntok, nq, hd), np.float32), cache, np.zeros(batch, np.int32), None, sees, nq, nkv, hd, 0.17, ntok + room)
+    vs = np.repeat(cache[3][:, :, :ntok].astype(np.float64), nq // nkv, 1).transpose(0, 2, 1)[..., None]  # [batch][ntok][nq][1]
+    where = np.repeat(at[:, :, :ntok], nq // nkv, 1).transpose(0, 2, 1)[..., None] // 64 == np.arange(hd) // 64
+    assert (got[~where] == 0).all()
+    off = (np.abs(np.abs(got) * 8 - vs) / vs)[where]
+    assert off.max() <= 2.0 ** -23 + 2.0 ** -23, off.max()

@@ -841,3 +841,27 @@ def test_attention_of_nf4_blocks_of_scales_far_apart(gpu_ctx, beams, prefix, tai
     gpu_ctx.sync()
     want, bound = R.attention(4, q, pre, tl, [prefix], [tail] * beams, beams, nq, nkv, hd, 0.17)
     assert (np.abs(out.cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("hd,nq,nkv,tail", [(64, 2, 2, 1), (128, 8, 2, 1), (64, 32, 8, 900)])
+def test_attention_of_one_position_rounds_its_v_to_nearest(gpu_ctx, hd, nq, nkv, tail):
+    """Zero queries, one position, and a V head of a single code 1: what comes out is the V scale over 8, every step exact
+    but for the scale's two pieces, 2^-23 of it, and their sum, a step at most."""
+    beams = 60
+    rng = np.random.default_rng(hd + nq)
+    tl = R.new_cache(8, beams, nkv, tail, hd, rng)
+    tl[2][:] = 0
+    at = rng.integers(0, hd, (beams, nkv, 1))
+    np.put_along_axis(tl[2], np.broadcast_to(at, tl[3].shape)[..., None], 1, -1)
+    tl[3][:] = rng.uniform(2.0 ** -6, 2.0 ** -3, (beams, nkv, 1))
+    out = torch.full((beams, nq, hd), float("nan"), device="cuda")
+    _, t = rows_of(tl, tail, d_len=ints([1] * beams))
+    ws = workspace(gpu_ctx.attn_shared_workspace(1, beams, nq, nkv, hd, 0, tail))
+    gpu_ctx.attn_shared(8, torch.zeros(beams, nq * hd, device="cuda"), nq * hd, 1, beams, nq, nkv, hd, None, t, 0.17, out, ws)
+    gpu_ctx.sync()
+    got = out.cpu().numpy()
+    vs = np.repeat(tl[3][:, :, 0].astype(np.float64), nq // nkv, 1)[..., None]
+    where = np.repeat(at[..., 0], nq // nkv, 1)[..., None] // 64 == np.arange(hd) // 64
+    assert (got[~where] == 0).all()
+    off = (np.abs(np.abs(got) * 8 - vs) / vs)[where]
+    assert off.max() <= 2.0 ** -23 + 2.0 ** -23, off.max()
