@@ -25,23 +25,26 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = 4, kTile = 32;  // waves of a workgroup (where none is given); positions of a wave's tile
 // A column's reference m is a power of two such that its products 2^(s - m) * V scale * kLift have reached 2^8
-// and stay below 2^15: pieces below f16's smallest step, 2^-24, are then 2^-32 of the largest product. It is
+// and stay below 2^15.8: pieces below f16's smallest step, 2^-24, are then 2^-32 of the largest product. It is
 // raised (a rescaling of the outputs, which some column of a tile would nearly always ask for) only where a
-// product would pass 2^15, and then to bring that one to 2^8 .. 2^9.  kLift makes s - m, which fp32 rounds by
+// product would pass 2^15.5, and then to bring that one to 2^8 .. 2^9.  kLift makes s - m, which fp32 rounds by
 // 2^-24 of itself, a small number for scales of the usual size (2^-8 .. 1).
-constexpr float kTop = 9.0f, kLimit = 15.0f, kLift = 256.0f, kLog2Lift = 8.0f;
+// A wave looks at its references where a bound of some column's products passes kLimit, and raises those whose
+// products pass kRaise: so much later that a column's own bound has passed then, however the two were rounded
+// (by 2^-3 each below kFar), and another column's products change nothing in it.
+constexpr float kTop = 9.0f, kLimit = 15.0f, kRaise = 15.5f, kLift = 256.0f, kLog2Lift = 8.0f;
 // Scales below 2^-100 count as that much in the reference, so that a weight is at most 2^107 and a sum of
 // 2^16 of them finite (from 2^120 on, half of the largest scale that a head has, kLift overflows); an NF4 head's second block has a reference of its own (its scales may be of another
 // size), but a weight refers to the first, which therefore counts as 2^-60 of the second at least.
 // Nor is that block's reference lower than 2^-119 of the first one's: up1, 2^(m - m1) times kLift, stays finite.
 constexpr float kLeastScale = 7.888609052210118e-31f, kApart = 60.0f, kWidest = 119.0f;
-// Scores so far from zero that fp32 does not tell whole numbers apart.  An exact product less the reference would
+// Scores so far from zero that fp32 hardly tells whole numbers apart, or not at all.  An exact product less the reference would
 // be up to half a step of the score off then, which may be any power of two: in a column whose reference is so far, scores
 // are rounded before the reference, the largest rounded one, is taken off.  What V scales ask for cannot be part of such a
 // reference, whose steps may be larger than that, and whose rounding would put it a step above every score: it is a
 // second number (State::beside), taken off after.  Waves and parts are joined by the first one alone, in sums of V
 // that such columns' scales may take to 2^100.
-constexpr float kFar = 0x1p24f;
+constexpr float kFar = 0x1p22f;
 __device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m > -FLT_MAX; }
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -286,11 +289,6 @@ __device__ __forceinline__ float column_max(float v) {  // over a column's four 
     return fmaxf(v, xor_lane(v, 32));
 }
 
-__device__ __forceinline__ bool column_any(bool b) {
-    const uint64_t lanes = __ballot(b), two = lanes | lanes >> 32;
-    return ((uint32_t)two | (uint32_t)two >> 16) >> own_column() & 1u;
-}
-
 // The largest of three: fmaxf's result, without the instructions that quiet each operand first.
 __device__ __forceinline__ float max3(float a, float b, float c) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -306,10 +304,10 @@ __device__ __forceinline__ float max8(const float (&t)[2][4]) {
 }
 
 // What weights() does to the references of column tile a where a column of the wave is far, in it or in another.  mn: the
-// column's new reference but for that; u1: log2 of its block 1's largest product, asks1: whether the column asks for a change by that.
+// column's new reference but for that; u1: log2 of its block 1's largest product.
 template <int HD, int NQ, int SN>
 __device__ __forceinline__ void far_references(State<HD, NQ, SN> &S, int a, const float (&t)[2][4], float qas, const float (&vs)[2][4][SN],
-                                               float top, float u1, bool asks1, float mn, float to_lift, float &down, float &down1) {
+                                               float top, float u1, float mn, float to_lift, float &down, float &down1) {
     const bool was = is_far(S.m[a]);
     const float best = column_max(top * qas);
     // (near kFar the scale may ask for a far reference where the score is none)
@@ -333,17 +331,17 @@ __device__ __forceinline__ void far_references(State<HD, NQ, SN> &S, int a, cons
     // the blocks' references, counted from m: before, and after
     const float shift = S.m[a] - mn;
     const float at0 = (was ? S.beside_of(a) : 0.0f) + shift, most0 = column_max(v[0]);
-    const float to0 = !now ? 0.0f : most0 > at0 + kLimit ? ceilf(most0) - kTop : at0;
+    const float to0 = !now ? 0.0f : most0 > at0 + kRaise ? ceilf(most0) - kTop : at0;
     down = at0 == to0 ? 1.0f : __builtin_amdgcn_exp2f(at0 - to0);
     down1 = down;
     if constexpr (SN > 1) {
         const float at1 = (was ? S.m1[a] : S.m1[a] - S.m[a]) + shift, most1 = column_max(v[SN - 1]);
         float to1;
         if (now) {
-            to1 = fmaxf(most1 > at1 + kLimit ? ceilf(most1) - kTop : at1, to0 - kWidest);
+            to1 = fmaxf(most1 > at1 + kRaise ? ceilf(most1) - kTop : at1, to0 - kWidest);
         } else {
             const float m1 = was ? S.m[a] + S.m1[a] : S.m1[a], most = column_max(u1);
-            to1 = fmaxf((was || asks1) && most > m1 + kLimit ? ceilf(most) - kTop : m1, mn - kWidest) - mn;
+            to1 = fmaxf(most > m1 + kRaise ? ceilf(most) - kTop : m1, mn - kWidest) - mn;
         }
         down1 = at1 == to1 ? 1.0f : __builtin_amdgcn_exp2f(at1 - to1);
         S.m1[a] = now ? to1 : mn + to1;
@@ -395,11 +393,8 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                         u[k] = fmaxf(u[k], fmaf(t[a][j][i], qas[a], log2_bits(__float_as_uint(vs[j][i][k]) & 0x7FFFFFFFu, kToLift)));
             }
             if constexpr (SN > 1) u[0] = fmaxf(u[0], u[1] - kApart);
-            // (only where the column asks for it by itself: another one's scores change nothing)
-            const bool asks = column_any(fmaf(top[a], qas[a], lv[0]) > S.m[a]) || is_far(S.m[a]);
-            const bool asks1 = SN > 1 && column_any(fmaf(top[a], qas[a], lv[SN - 1]) > S.m1[SN > 1 ? a : 0]);
             const float most = column_max(u[0]);
-            float mn = asks && most > S.m[a] + kLimit ? ceilf(most) - kTop : S.m[a];
+            float mn = most > S.m[a] + kRaise ? ceilf(most) - kTop : S.m[a];
             S.far |= __any(is_far(mn)) != 0;
             float down, down1;
             if (__builtin_expect(!S.far, 1)) {
@@ -407,14 +402,14 @@ __device__ __forceinline__ void weights(State<HD, NQ, SN> &S, float (&t)[NQ][2][
                 down1 = down;
                 if constexpr (SN > 1) {
                     const float most1 = column_max(u[SN - 1]);
-                    const float m1 = fmaxf(asks1 && most1 > S.m1[a] + kLimit ? ceilf(most1) - kTop : S.m1[a], mn - kWidest);
+                    const float m1 = fmaxf(most1 > S.m1[a] + kRaise ? ceilf(most1) - kTop : S.m1[a], mn - kWidest);
                     down1 = m1 == S.m1[a] ? 1.0f : __builtin_amdgcn_exp2f(S.m1[a] - m1);
                     S.m1[a] = m1;
                     S.up1[a] = __builtin_amdgcn_exp2f(mn - m1) * kLift;
                 }
                 S.m[a] = mn;
             } else {
-                far_references(S, a, t[a], qas[a], vs, top[a], u[SN - 1], asks1, mn, kToLift, down, down1);
+                far_references(S, a, t[a], qas[a], vs, top[a], u[SN - 1], mn, kToLift, down, down1);
             }
             S.l[a] *= down;
 #pragma unroll

@@ -901,9 +901,9 @@ FAR = [(3, 9, 3, 5, 300, 0, True), (1, 8, 1, 3, 700, 0, False), (2, 4, 2, 64, 10
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("batch,nq,nkv,ntok,start,room,with_tree", FAR)
-@pytest.mark.parametrize("size", [1.1e7, 3e7, 1e9, 1e13])
+@pytest.mark.parametrize("size", [2.9e6, 1.1e7, 3e7, 1e9, 1e13])
 def test_attention_of_far_scores_and_scales_far_apart(gpu_ctx, bits, hd, batch, nq, nkv, ntok, start, room, with_tree, size):
-    """Scores of 1.1e7 (where steps pass one) to 1e13 and V scales 2^-30 .. 2^30: a large scale of small weight, or of a
+    """Scores of 2.9e6 (2^22 powers of two) to 1e13 and V scales 2^-30 .. 2^30: a large scale of small weight, or of a
     position that the token does not see, takes nothing from the best position's V."""
     print(f"far bits={bits} hd={hd} heads={nq}/{nkv} batch={batch} ntok={ntok} start={start} room={room} size={size}", flush=True)
     rng = np.random.default_rng(hd + ntok + nq)

@@ -779,9 +779,9 @@ def test_the_most_rows(gpu_ctx):
 
 @pytest.mark.parametrize("bits,hd", [(8, 64), (8, 128), (4, 64), (4, 128)])
 @pytest.mark.parametrize("beams,prefix,tail", [(3, 60, 9), (8, 1500, 40), (64, 900, 300)])
-@pytest.mark.parametrize("size", [1.1e7, 3e7, 1e9, 1e13])
+@pytest.mark.parametrize("size", [2.9e6, 1.1e7, 3e7, 1e9, 1e13])
 def test_attention_of_far_scores_with_v_scales_far_apart(gpu_ctx, bits, hd, beams, prefix, tail, size):
-    """Scores of 1.1e7 (where their steps pass one) to 1e13 and V scales 2^-30 .. 2^30: a large scale of small weight takes
+    """Scores of 2.9e6 (2^22 powers of two) to 1e13 and V scales 2^-30 .. 2^30: a large scale of small weight takes
     nothing from the best position's V."""
     nq, nkv = 8, 2
     g = nq // nkv
