@@ -497,8 +497,9 @@ void launch_kv_keep(int cus, hipStream_t st, int bits, const k2t_kv_rows &kv, co
     const dim3 grid((unsigned)(2 * (size_t)n_layers * rows * nkv), 2);
     // Sixteen waves, and chunks four times as long, where there are few workgroups or long lists (us, four waves and sixteen: 204
     // workgroups of heads x 128, 6027 entries 98 and 54; 384 of 3000 59 and 40; 768 of 3000 121 and 110; 1536 of heads x
-    // 64 124 both; 256 of 150 to 400 the same; but 960 of 293 9.8 and 13.1, some 3000 of 400 46 and 52).
-    if (grid.x <= 2 * (unsigned)cus || n_keep >= 1024) launch_keep<1024>(grid, st, A);
+    // 64 124 both; 256 of 150 to 400 the same; but 960 of 293 9.8 and 13.1, some 3000 of 400 46 and 52).  (A launch has fewer
+    // than 2^32 threads in a direction: four million workgroups are of four waves.)
+    if ((grid.x <= 2 * (unsigned)cus || n_keep >= 1024) && grid.x < 1u << 22) launch_keep<1024>(grid, st, A);
     else launch_keep<256>(grid, st, A);
     hip_check(hipGetLastError(), "kv_keep launch");
 }

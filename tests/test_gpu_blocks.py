@@ -987,3 +987,27 @@ def test_attention_of_one_position_rounds_its_v_to_nearest(gpu_ctx, hd, nq, nkv,
     assert (got[~where] == 0).all()
     off = (np.abs(np.abs(got) * 8 - vs) / vs)[where]
     assert off.max() <= 2.0 ** -23 + 2.0 ** -23, off.max()
+
+
+def test_keep_of_millions_of_heads_and_long_lists(gpu_ctx):
+    """More than 2^21 (layer, row, head) triples, lists of 1024 entries: first positions that take the second one's codes and scales."""
+    layers, rows, nkv, cap, n_keep = 3, 1000, 1024, 2, 1024
+    g = torch.Generator(device="cuda").manual_seed(4)
+    heads = layers * rows * nkv
+    assert heads > 1 << 21
+    c = [torch.randint(0, 256, (heads * cap, 32), generator=g, device="cuda", dtype=torch.uint8) for _ in range(2)]
+    s = [torch.randint(0, 1 << 14, (heads * cap,), generator=g, device="cuda", dtype=torch.int16) for _ in range(2)]
+    old = [t.clone() for t in (c[0], s[0], c[1], s[1])]
+    keep = torch.full((rows, n_keep), -1, dtype=torch.int32, device="cuda")
+    keep[:, 0] = 1
+    keep[:, 1] = 1023  # (outside the cache)
+    counts = torch.full((rows,), n_keep, dtype=torch.int32, device="cuda")
+    counts[::7] = 0
+    gpu_ctx.kv_keep(4, k2t.KVRows(c[0], s[0], c[1], s[1], cap=cap), torch.zeros(rows, dtype=torch.int32, device="cuda"), keep, n_keep, counts,
+                    n_keep, layers, rows, nkv, 64)
+    gpu_ctx.sync()
+    moved = (counts > 0).view(1, rows, 1, 1)
+    for got, was in zip((c[0], s[0], c[1], s[1]), old):
+        got, was = (t.view(layers, rows, nkv, cap, -1) for t in (got, was))
+        assert torch.equal(got[:, :, :, 1], was[:, :, :, 1])
+        assert torch.equal(got[:, :, :, 0], torch.where(moved, was[:, :, :, 1], was[:, :, :, 0]))
