@@ -566,7 +566,8 @@ int32_t k2t_attn_tokens_workspace(k2t_ctx *ctx, int32_t batch, int32_t ntok, int
  *     a token that is listed twice gets both.
  *   d_mask [mask_rows][mask_stride] words: bit t % 32 of word t / 32 allows token t; row r is ruled by mask row
  *     d_mask_row[r] (d_mask_row NULL: r), and by none if that is outside 0 .. mask_rows - 1.
- * Tokens outside the vocabulary are passed over.  history_len <= 2^20, bias_len <= 4096. */
+ * Tokens outside the vocabulary are passed over.  history_len <= 2^20, bias_len <= 4096; a list of length 0, and masks of 0
+ * rows, may be NULL beside what goes with them (penalties of a history that has no tokens yet apply to nothing). */
 typedef struct k2t_logits_rules {
     const int32_t *d_history, *d_history_len, *d_prompt_len;
     const float *d_repeat, *d_presence, *d_frequency;

@@ -232,8 +232,8 @@ int32_t k2t_logits_adjust(k2t_ctx *ctx, const float *d_logits, int32_t vocab, si
             branch_arg(R.history_len >= 0 && R.history_len <= kMaxHistory && R.history_stride >= (size_t)R.history_len &&
                            R.history_stride < (size_t)1 << 40,
                        "history_len must be 0 .. 2^20, history_stride no smaller");
-        else
-            branch_arg(!R.d_repeat && !R.d_presence && !R.d_frequency, "penalties without a history");
+        else  // (a list without entries has no address)
+            branch_arg(R.history_len == 0 || (!R.d_repeat && !R.d_presence && !R.d_frequency), "penalties without a history");
         branch_arg((R.d_bias_tokens != nullptr) == (R.d_bias != nullptr), "biases need both their tokens and their values");
         if (R.d_bias)
             branch_arg(R.bias_len >= 0 && R.bias_len <= kMaxBias && R.bias_stride >= (size_t)R.bias_len &&
@@ -244,7 +244,7 @@ int32_t k2t_logits_adjust(k2t_ctx *ctx, const float *d_logits, int32_t vocab, si
                            R.mask_stride < (size_t)1 << 40,
                        "mask_rows or mask_stride too small");
         else
-            branch_arg(!R.d_mask_row, "mask rows without masks");
+            branch_arg(R.mask_rows == 0 || !R.d_mask_row, "mask rows without masks");
         if (rows == 0) return;
         branch_arg(d_logits && d_out, "NULL argument");
         const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p); };

@@ -188,7 +188,7 @@ class RopePlan(C.Structure):
 
 class LogitsRules(C.Structure):
     """k2t_logits_rules: int32 / float32 tensors, one row of each per row of logits (mask: rows of int32
-    words); None: not applied."""
+    words); None, or without entries: not applied."""
     _fields_ = [(n, VP) for n in ("history", "history_len", "prompt_len", "repeat", "presence", "frequency",
                                   "bias_tokens", "bias", "bias_len", "mask", "mask_row")] + \
         [("history_stride", SZ), ("bias_stride", SZ), ("mask_stride", SZ), ("history_max", I32), ("bias_max", I32),
@@ -199,9 +199,13 @@ class LogitsRules(C.Structure):
         def shape(t):
             if t is None:
                 return 0, 0, 0
+            if t.numel() == 0:  # (no entries, and no address)
+                return 0, 0, 0
             if t.shape[1] > 1 and t.stride(1) != 1:
                 raise ValueError("lists and masks are rows of consecutive words")
             return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        if mask is not None and mask.shape[0] > 0 and mask.shape[1] == 0:
+            raise ValueError("masks without words")
         _, hn, hs = shape(history)
         _, bn, bs = shape(bias_tokens)
         if bias_tokens is not None and (bias is None or bias.shape != bias_tokens.shape or shape(bias)[2] != bs):

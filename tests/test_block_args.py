@@ -184,3 +184,26 @@ def test_the_reference_itself():
     assert z.tolist() == [[1.0, -5.0, 4.0, -np.inf]]
     a = np.arange(6).reshape(1, 1, 1, 6, 1)
     assert R.keep([a], [1], np.array([[0, 2, 1, 9]]), None, 4)[0].ravel().tolist() == [0, 1, 3, 3, 4, 5]
+
+
+def test_logits_of_lists_without_entries():
+    """A history that has no tokens yet, no biases, no masks this time: lists of length zero, which have no address."""
+    import torch
+    keep = []
+
+    def at(r):
+        keep.append(r)
+        return C.addressof(r)
+    good = [CTX, P, 1000, 1000, 3, at(rules(history=None, history_max=0, bias_tokens=None, bias=None, bias_max=0, mask=None, mask_rows=0)), 2 * P, 1000]
+    refused("k2t_logits_adjust", good, [{5: at(rules(history=None, history_max=1))}, {5: at(rules(mask=None, mask_rows=1))},
+                                        {5: at(rules(bias=None, bias_max=0))}])
+    if no_gpu():
+        assert call("k2t_logits_adjust", *good) == HIP
+    i, f = dict(dtype=torch.int32), dict(dtype=torch.float32)
+    for rows in (0, 3):
+        r = k2t.LogitsRules(history=torch.zeros(rows, 0, **i), repeat=torch.ones(3, **f), bias_tokens=torch.zeros(rows, 0, **i),
+                            bias=torch.zeros(rows, 0, **f), mask=torch.zeros(0, 40, **i), mask_row=torch.zeros(3, **i))
+        assert (r.history, r.history_max, r.bias, r.bias_max, r.mask, r.mask_rows) == (None, 0, None, 0, None, 0) and r.repeat
+    assert k2t.LogitsRules(history=torch.zeros(0, 5, **i)).history_max == 0
+    with pytest.raises(ValueError):
+        k2t.LogitsRules(mask=torch.zeros(3, 0, **i))

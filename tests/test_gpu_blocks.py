@@ -1011,3 +1011,20 @@ def test_keep_of_millions_of_heads_and_long_lists(gpu_ctx):
         got, was = (t.view(layers, rows, nkv, cap, -1) for t in (got, was))
         assert torch.equal(got[:, :, :, 1], was[:, :, :, 1])
         assert torch.equal(got[:, :, :, 0], torch.where(moved, was[:, :, :, 1], was[:, :, :, 0]))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_logits_of_lists_without_entries(gpu_ctx, in_place):
+    """Penalties of a history without tokens, beside no biases or some, and mask rows without masks."""
+    rng = np.random.default_rng(9)
+    rows, vocab = 3, 5001
+    x = rng.standard_normal((rows, vocab + 3)).astype(np.float32)
+    none = dict(history=np.zeros((rows, 0), np.int32), repeat=np.full(rows, 1.5, np.float32), presence=np.full(rows, 2.0, np.float32),
+                history_len=np.full(rows, 4, np.int32), prompt_len=np.zeros(rows, np.int32),
+                bias_tokens=np.zeros((rows, 0), np.int32), bias=np.zeros((rows, 0), np.float32),
+                mask=np.zeros((0, 157), np.int32), mask_row=np.zeros(rows, np.int32))
+    got = adjust(gpu_ctx, x, vocab, none, in_place)
+    assert got[:, :vocab].tobytes() == x[:, :vocab].tobytes()
+    some = dict(none, bias_tokens=np.array([[7, 5000], [1, 1], [-1, 6000]], np.int32), bias=rng.standard_normal((rows, 2)).astype(np.float32))
+    want = R.logits(x, vocab, {k: some[k] for k in ("bias_tokens", "bias")})
+    assert np.array_equal(adjust(gpu_ctx, x, vocab, some, in_place)[:, :vocab], want[:, :vocab])
