@@ -553,8 +553,8 @@ int32_t k2t_attn_tokens(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const int32_t *d_pos,
                         const int32_t *d_counts, const uint64_t *d_sees, const k2t_kv_rows *kv, float attn_scale,
                         float *d_out, void *d_ws, size_t ws_bytes);
-/* Its workspace for blocks of up to ntok tokens over caches of up to len positions (their `len`): what serves these
- * serves every smaller block and shorter cache. */
+/* Its workspace for blocks of up to ntok tokens of up to batch rows over caches of up to len positions (their `len`): what serves
+ * these serves fewer rows, smaller blocks and shorter caches. */
 int32_t k2t_attn_tokens_workspace(k2t_ctx *ctx, int32_t batch, int32_t ntok, int32_t n_heads, int32_t n_kv_heads,
                                   int32_t head_dim, int32_t len, size_t *bytes);
 

@@ -567,17 +567,22 @@ Plan plan_of(const k2t_ctx *ctx, const TokensShape &s, int bits, bool tree, int 
 size_t part_slots(const TokensShape &s, int parts) { return (size_t)s.batch * s.ntok * s.nq * parts; }
 size_t slot_bytes(int hd) { return hd * sizeof(float) + sizeof(float2); }
 size_t ws_bytes_of(const TokensShape &s, int parts) { return parts == 1 ? 16 : part_slots(s, parts) * slot_bytes(s.hd); }
-// At least that of every plan of up to so many tokens and positions: for every kind of item and number of column groups, as
-// many columns as it has and as many parts as it may be cut into (fewer where there are more groups).
+// At least that of every plan of up to so many rows, tokens and positions: for every kind of item, number of rows and of column
+// groups, as many columns as they have and as many parts as they may be cut into (fewer where there are more items).
 size_t most_ws_bytes(const k2t_ctx *ctx, const TokensShape &s, int len) {
-    const int cols = s.ntok * (s.nq / s.nkv);
-    const size_t heads = (size_t)s.batch * s.nkv;
     size_t most = 16;
+    if (s.batch == 0) return most;
+    const int cols = s.ntok * (s.nq / s.nkv);
     for (int item : {16, 32, 16 * kBlockWaves}) {
-        for (int cgs = 1; (cgs - 1) * item < cols; cgs++) {
-            const int parts = most_parts(ctx, item == 16 * kBlockWaves, heads * cgs, len);
-            if (parts <= 1) break;
-            most = std::max(most, heads * std::min(cols, cgs * item) * parts * slot_bytes(s.hd));
+        const auto parts = [&](size_t items) { return most_parts(ctx, item == 16 * kBlockWaves, items, len); };
+        for (int rows = 1; rows <= s.batch; rows++) {
+            const size_t heads = (size_t)rows * s.nkv;
+            if (parts(heads) <= 1) break;
+            for (int cgs = 1; (cgs - 1) * item < cols; cgs++) {
+                const int n = parts(heads * cgs);
+                if (n <= 1) break;
+                most = std::max(most, heads * std::min(cols, cgs * item) * n * slot_bytes(s.hd));
+            }
         }
     }
     return most;

@@ -207,3 +207,34 @@ def test_logits_of_lists_without_entries():
     assert k2t.LogitsRules(history=torch.zeros(0, 5, **i)).history_max == 0
     with pytest.raises(ValueError):
         k2t.LogitsRules(mask=torch.zeros(3, 0, **i))
+
+
+@pytest.mark.parametrize("heads", [(32, 32, 64), (32, 8, 128), (9, 3, 64), (16, 1, 128), (1, 1, 64)])
+def test_attention_workspace_serves_fewer_rows(heads):
+    """Requests of a batch that end leave fewer rows, whose positions are cut into more parts: the batch's workspace is
+    enough for them."""
+    ctx = (C.c_int32 * 1024)(*[256] * 1024)  # a context of 256 CUs, on a device that no machine has
+
+    def workspace(batch, ntok, length):
+        n = C.c_size_t()
+        assert call("k2t_attn_tokens_workspace", ctx, batch, ntok, *heads, length, C.byref(n)) == 0
+        return n.value
+
+    for batch in (4, 16, 17, 64, 200):
+        for ntok, length in [(1, 2000), (13, 2113), (64, 12064), (515, 4613), (40, 100)]:
+            if batch * ntok * heads[0] > 1 << 22:
+                continue
+            ws = workspace(batch, ntok, length)
+            for b in [x for x in (1, 2, 3, 5, 8, 11, 16, 31, 32, 33, 64, 100, 128, 199) if x < batch]:
+                assert workspace(b, ntok, length) <= ws
+                for t in {1, min(ntok, 16), ntok}:
+                    for n in (1, 300, length):
+                        rc = call("k2t_attn_tokens", ctx, 8, P, heads[0] * heads[2], b, t, *heads, P, None, None,
+                                  rows(cap=1 << 24, length=min(n, length)), 0.125, P, P, ws)
+                        assert rc == HIP, (batch, ntok, length, b, t, n)
+
+
+def test_attention_workspace_of_no_rows():
+    n = C.c_size_t()
+    assert call("k2t_attn_tokens_workspace", CTX, 0, 2 ** 31 - 1, 16, 1, 64, 1 << 24, C.byref(n)) == 0 and n.value == 16
+    assert call("k2t_attn_tokens_workspace", CTX, 5, 0, 16, 1, 64, 1 << 24, C.byref(n)) == 0 and n.value == 16
