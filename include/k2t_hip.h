@@ -464,7 +464,7 @@ int32_t k2t_attn_shared(k2t_ctx *ctx, int32_t bits, const float *d_q, size_t q_s
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const k2t_kv_rows *prefix,
                         const k2t_kv_rows *tail, float attn_scale, float *d_out, void *d_ws, size_t ws_bytes);
 /* Its workspace for caches of up to prefix_len and tail_len positions (their `len`): what serves these
- * lengths serves every shorter one, and a missing cache. */
+ * lengths serves every shorter one, and a missing cache, of as many sequences and rows (fewer are cut into more parts). */
 int32_t k2t_attn_shared_workspace(k2t_ctx *ctx, int32_t n_seq, int32_t beams, int32_t n_heads, int32_t n_kv_heads,
                                   int32_t head_dim, int32_t prefix_len, int32_t tail_len, size_t *bytes);
 /* Beam search's choice: the k best continuations of every sequence over its `beams` rows and
@@ -544,7 +544,8 @@ int32_t k2t_rope(k2t_ctx *ctx, const float *d_x, size_t x_stride, int32_t batch,
  * below d_pos[b] and, within the block, d_sees = NULL: to tokens 0 .. t (causal); else (ntok <= 64) to the tokens j whose
  * bit j of d_sees[b * ntok + t] is set; in both cases only to tokens that the row has and to positions 0 .. kv->len - 1
  * (d_len is not used).  A token that sees nothing gets zeros.  What the cache holds at positions that a token does not
- * see (infinities and NaN among scales) does not reach its output, nor do other tokens' queries.  d_q: token's n_heads post-RoPE
+ * see (infinities and NaN among scales) does not reach its output, nor do other tokens' queries; the V scales of positions that
+ * it sees are below 2^120 (2^100 where its scores are beyond 2^22 ln 2).  d_q: token's n_heads post-RoPE
  * query heads at d_q + (b * ntok + t) * q_stride floats; d_out [batch * ntok][n_heads][hd].  attn_scale is finite and
  * not negative.  d_ws: device workspace of k2t_attn_tokens_workspace bytes, of this call alone while it runs (two
  * graphs that may run at once need one each); it needs no initial value.  d_q, d_out and d_ws are 16-byte aligned,

@@ -16,7 +16,7 @@
 // instructions (weights and their pieces, V's codes to f16, scales) next to 40 MFMAs, two waves to a
 // SIMD; a part has few tiles, so its queries' transform and its join count too. Measured (passes in a row):
 // 8 rows x 32 heads x 64, 1500 positions 9.5 us (0.9 TB/s of cache bytes); 64 rows x 32 / 4 heads x 128,
-// 12000 + 333 positions 35.3 us (365 TFLOP/s); 3 sequences of 8 rows x 32 / 8 heads x 128, NF4, 4100 positions
+// 12000 + 333 positions 35.3 to 36.5 us by the card (365 TFLOP/s); 3 sequences of 8 rows x 32 / 8 heads x 128, NF4, 4100 positions
 // 19.0 us, a third of whose instructions look codes up; 4 rows x 9 / 3 heads x 64, 52 positions 5.2 us, a launch.
 // References by products instead of scores cost NF4 heads of two blocks 2 to 3 % (a reference each: 19.9 and
 // 20.3 us, 47.2 and 48.4 us with 64 rows), the others nothing where V scales are alike; with scales anywhere within

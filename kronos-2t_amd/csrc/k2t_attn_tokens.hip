@@ -13,15 +13,17 @@
 // too (tokens_block_kernel).  Where that leaves CUs without a workgroup (tokens_block_kernel: without a second one),
 // positions are cut into parts, which a second kernel joins.
 //
-// What bounds it.  8192 tokens from the start, 32 / 4 heads x 128, int8: 780 to 865 us by the card, 0.55 PFLOP that count at
-// 0.7 PFLOP/s.  The matrix cores and the power they draw (the core's clock is down at 2.0 GHz): outputs are done twice, for
-// a weight's two pieces, and all products would take 555 us at the rate of a large one (1.24 PFLOP/s f16, int8 twice
-// that).  68 us are the ends of items, queries and outputs (268 MB).  6 prompts of 389 to 777 tokens, 32 heads x 64: 39 us,
-// the ends half of them.
-// Chunks of a prompt behind a context: NF4's lookups, the ends, the join (515 tokens behind 4100, 32 / 8 x 128, NF4: 107 to
-// 118 us, 15 and 12 of them).  Drafts behind a context: latencies at two waves per SIMD, and what one CU loads at a time (64 tokens
-// behind 12000, 32 / 4 x 128: 35 us, 4.6 of them the join; 8 x 13 behind 2100, 32 / 8 x 128, NF4: 24).  Short drafts: a launch,
-// a few tiles and the transforms (10 tokens behind 300, 9 / 3 x 64: 5.9 us).
+// What bounds it (passes in a row, by events; kernels are longer under the profiler).
+// 8192 tokens from the start, 32 / 4 heads x 128, int8: 780 to 865 us by the card, 0.55 TFLOP that count at 0.7 PFLOP/s.  The
+// matrix cores and the power they draw (the core's clock is down at 2.0 GHz): outputs are done twice, for a weight's two
+// pieces, and all products would take 555 us at the rate of a large one (1.24 PFLOP/s f16, int8 twice that).  68 us are the
+// ends of items, queries and outputs (268 MB).  6 prompts of 389 to 777 tokens, 32 heads x 64: 38 to 41 us, the ends half of them;
+// 6 of 777, 32 / 8 x 128, NF4: 96 to 102.  Chunks of a prompt behind a context: NF4's lookups, the ends, the join (515 tokens behind
+// 4100, 32 / 8 x 128, NF4: 107 to 111 us; under the profiler 113 and 15 of join).  Drafts behind a context: latencies at two
+// waves per SIMD, and what one CU loads at a time (64 tokens behind 12000, 32 / 4 x 128: 34 to 37 us, under the profiler 35
+// and 5 of join; 8 x 13 behind 2100, 32 / 8 x 128, NF4: 24).  Short drafts: a launch, a few tiles and the transforms (10
+// tokens behind 300, 9 / 3 x 64: 5.9 us).  Work is cut by the cache's len, not by what rows hold: with len 32768, 64 single tokens
+// behind 2000 take 51 us for 45.5, the 8 x 13 39.5 for 24.5, prompts of 777 the same 84 to 88.
 #include <float.h>
 #include <math.h>
 
@@ -110,7 +112,8 @@ struct Seen {
     }
 };
 
-// Few columns: an item is (row, KV head, part, 16 NQ columns).
+// Few columns: an item is (row, KV head, part, 16 NQ columns).  Launch bounds: three waves to a SIMD where one tile of columns of
+// 128 or two of 64 leave the registers for it (by itself the compiler takes 2 to 10 more for some and leaves two).
 template <int HD, int BITS, int NQ, bool WHOLE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, HD * NQ <= 128 ? 3 : 2) void tokens_few_kernel(const TokensArgs A) {
     __shared__ Shared<HD, NQ, WAVES> sh;
@@ -431,6 +434,7 @@ __device__ __forceinline__ void block_item(const TokensArgs &A, int item, int pa
 // that a few long items fill the card evenly (515 tokens behind 4100, 32 / 8 heads x 128 NF4, 136 items for 512 workgroups:
 // 119.5 us, 130 in three equal parts of every item); an item has a part for every workgroup that comes to it.  Else a
 // workgroup has an item.
+// (128-dimensional NF4 heads spill three registers, before the loop over tiles and behind it.)
 template <int HD, int BITS, bool CUT>
 __global__ __launch_bounds__(64 * kBlockWaves, 4) void tokens_block_kernel(const TokensArgs A) {
     constexpr int P = BlockTile<HD, BITS>::P;

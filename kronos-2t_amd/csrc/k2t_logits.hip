@@ -14,7 +14,7 @@
 // What bounds it: bytes, and every slice's pass over the row's lists. 64 rows of 151936, histories of 2000, 40 biases and a
 // mask (78 MB read and written): 18.8 us, 4.2 TB/s; slices of 1024, 4096 and 8192 logits 22.8, 23.7 and 32 us (more passes
 // over the lists; fewer loads in flight), one load of the history at a time and cached stores 26.8. 4 rows of 49152: 4.1 us, a launch
-// and the lists. Tokens that are named twice (4 rows of 10536, 213 biases: 8.1 us; 128 rows of 32000, 300: 14.8): 17.0 and
+// and the lists. Rows that do not begin at multiples of 16 bytes, a logit at a time: 64 of 50257 (contiguous) 12.5 us, of 50260 9.7. Tokens that are named twice (4 rows of 10536, 213 biases: 8.1 us; 128 rows of 32000, 300: 14.8): 17.0 and
 // 33.4 with a search through the row's whole list. (4000 biases in 5 slices, most named twice: 356 us, 1890.)
 #include <math.h>
 

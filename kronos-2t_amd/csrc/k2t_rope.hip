@@ -9,9 +9,10 @@
 // under way, then rotate eight elements (four pairs) at a time.
 //
 // What bounds it: bytes. 6 rows of 389 to 777 tokens, 36 heads x 128 (129 MB read and written): 21 to 23 us, 5.5 to 6 TB/s (the
-// inputs partly from the Infinity Cache); 34.7 with one piece in flight per thread and cached stores. 6 rows of 777, 168 MB: 28.5,
-// interleaved 28.9 (49.9 with a thread's two pieces side by side), rot_dim 98, halves, a pair at a time, 54. One token of 4
-// rows, 12 heads x 64: 3.6 us, a launch and the chain from position to angle to output.
+// inputs partly from the Infinity Cache); 34.7 with one piece in flight per thread and cached stores. 6 rows of 777, 168 MB: 28.5 to
+// 30.7, interleaved 28.9 to 31.8 (49.9 with a thread's two pieces side by side), rot_dim 98, halves, a pair at a time, 54 (4 bytes
+// per lane and access, since the halves of such a head do not begin at the same alignment).
+// One token of 4 rows, 12 heads x 64: 3.6 us, a launch and the chain from position to angle to output.
 #include <math.h>
 
 #include <algorithm>
